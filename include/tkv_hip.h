@@ -543,6 +543,116 @@ int32_t tkv_hip_dev_matmul_q8_0(int64_t ctx, const int8_t* a, const int8_t* code
                                 const float* scale_a, int64_t scale_a_stride, const float* bias,
                                 float* y);
 
+/* ======================================================================== */
+/* Attention beside the quantized linears (extension): rotary positions, a   */
+/* paged key / value cache, attention of whole prompts and of new tokens     */
+/* over the cache.  No counterpart on the reference's quantization path,     */
+/* which ends at the linears.                                                */
+/* ======================================================================== */
+
+/* Element types of queries, keys, values and outputs; I8 is for caches only:
+ * int8 codes with one f32 scale per (token, head), value = code * scale. */
+#define TKV_HIP_F32 0
+#define TKV_HIP_F16 1
+#define TKV_HIP_BF16 2
+#define TKV_HIP_I8 3
+
+/* A device tensor [tokens, heads, head_dim] inside a larger one, such as the
+ * query part of a fused projection's output: strides in elements, the
+ * innermost dimension contiguous. */
+typedef struct {
+    void* data;
+    int64_t stride_token;
+    int64_t stride_head;
+} tkv_hip_rows;
+
+/* A paged cache: K and V [num_pages, heads, page_size, head_dim] of `type`,
+ * and for I8 f32 scales [num_pages, heads, page_size] each.  Slot s of the
+ * pool is (s / page_size, s % page_size).  k == NULL: the handle allocates
+ * (zeroed) and frees the memory; otherwise the four device pointers are the
+ * caller's (scales NULL unless I8) and have to outlive the handle.
+ * num_pages * page_size < 2^31; head_dim <= 256. */
+int32_t tkv_hip_kv_create(int64_t ctx, int32_t type, int64_t num_pages, int64_t page_size,
+                          int64_t heads, int64_t head_dim, void* k, void* v, float* k_scales,
+                          float* v_scales, int64_t* handle_out);
+int32_t tkv_hip_kv_free(int64_t handle);
+/* The cache's device pointers (any output may be NULL). */
+int32_t tkv_hip_kv_info(int64_t handle, void** k, void** v, float** k_scales, float** v_scales);
+
+/* The rotation table of positions 0 .. positions - 1, f32 [positions,
+ * rot_dim / 2, 2]: amplitude * (cos, sin)(p * inv_freq[i]), computed in f64.
+ * inv_freq: rot_dim / 2 doubles in host memory, so a scaling for long contexts
+ * is a choice of frequencies (and amplitude) made by the caller.  rot_dim even,
+ * 2 .. 256. */
+int32_t tkv_hip_dev_rope_table(int64_t ctx, int64_t positions, int64_t rot_dim,
+                               const double* inv_freq, double amplitude, float* table);
+/* The new tokens' rows on their way to the attention: q and k rotated, all
+ * three converted to type_out, k and v appended to the cache.
+ *   rotation (table != NULL): pair i of the head's first rot_dim elements,
+ *     (a, b) = (x[i], x[i + rot_dim / 2]) (ROPE_HALF) or (x[2i], x[2i + 1])
+ *     (ROPE_PAIRS), becomes (a c - b s, b c + a s) with (c, s) the entry of the
+ *     token's position, each product and sum rounded to f32; other elements
+ *     and v pass through.  table == NULL: nothing is rotated (positions unused).
+ *   q_out, k_out (each may be NULL): the rows of q and k in type_out; they may
+ *     be the inputs themselves where the types agree and heads do not overlap.
+ *   cache (0: none): token t's k and v go to pool slot slots[t]; a slot outside
+ *     the pool appends nothing.  Cache types: type_out, or I8, whose rows are
+ *     coded from the f32 values as scale = fl32(max(max|x|, 1e-8) / 127),
+ *     code = clamp(rne(fl32(x * fl32(1 / scale))), -127, 127), NaN 0.
+ * A position outside [0, table_len) marks a padding token: its q_out and k_out
+ * rows are zeros and it is not appended.  q, k, v may be NULL with their head
+ * count 0 (k and v go together where there is a cache).  positions and slots
+ * are device arrays of `tokens` entries; head_dim <= 256. */
+#define TKV_HIP_ROPE_HALF 0
+#define TKV_HIP_ROPE_PAIRS 1
+int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, int64_t heads_q,
+                                int64_t heads_kv, int64_t head_dim, const tkv_hip_rows* q,
+                                const tkv_hip_rows* k, const tkv_hip_rows* v,
+                                const int32_t* positions, const float* table, int64_t table_len,
+                                int64_t rot_dim, int32_t layout, const tkv_hip_rows* q_out,
+                                const tkv_hip_rows* k_out, int32_t type_out, int64_t cache,
+                                const int64_t* slots);
+
+/* Attention.  For every query row i of a sequence of n query and t key rows,
+ * at position pos = t - n + i,
+ *   out_i = sum_j exp(a_ij - m_i) v_j / sum_j exp(a_ij - m_i),
+ *   a_ij = scale * q_i . k_j, m_i = max_j a_ij,
+ * over the keys j in [0, t) that it sees: all of them, only j <= pos where
+ * causal != 0, and only j > pos - window where window > 0.  A row that sees no
+ * key gives zeros; what a row does not see (NaN and infinities included) does
+ * not touch it.  Query head h reads key / value head h / (heads_q / heads_kv).
+ * Statistics and sums are f32.  For f16 and bf16 the products run on the
+ * matrix units from values of that type, the weights exp(a - m) rounded to it
+ * for the second product; f32 stays f32 throughout.  type_out: `type`, or F32
+ * (the unrounded sums of the same computation).  head_dim <= 256; sizes that
+ * are multiples of 16 bytes with 16-byte aligned rows take the fast kernels.
+ * Length arrays are read on the device and clamped to the tokens and pages
+ * that there are, page ids outside the pool read page 0; query rows that no
+ * sequence covers are not written.
+ *
+ * Whole prompts, packed: sequence s has the query rows cu_q[s] .. cu_q[s + 1]
+ * and the key rows cu_k[s] .. cu_k[s + 1] (cu_k NULL: cu_q's), device arrays of
+ * `sequences` + 1 rising entries. */
+int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, int64_t tokens_k,
+                                     int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                                     int64_t sequences, const tkv_hip_rows* q,
+                                     const tkv_hip_rows* k, const tkv_hip_rows* v,
+                                     const tkv_hip_rows* out, int32_t type_out,
+                                     const int32_t* cu_q, const int32_t* cu_k, float scale,
+                                     int32_t causal, int64_t window);
+/* New tokens over a paged cache: sequence s has the query rows cu_q[s] ..
+ * cu_q[s + 1] (cu_q NULL: the one row s) and the first kv_lens[s] tokens of the
+ * pages page_table[s * table_stride ..], its new tokens (already appended) the
+ * last of them.  The cache's type is `type` or I8.  max_q and max_kv (0: not
+ * known): the longest of the sequences' query rows and cache lengths, which
+ * choose the launch shape alone: longer sequences are still right. */
+int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, int64_t heads_q,
+                                    int64_t cache, int64_t sequences, const tkv_hip_rows* q,
+                                    const tkv_hip_rows* out, int32_t type_out,
+                                    const int32_t* page_table, int64_t table_stride,
+                                    const int32_t* cu_q, const int32_t* kv_lens, int64_t max_q,
+                                    int64_t max_kv, float scale, int32_t causal, int64_t window);
+
 #ifdef __cplusplus
 }
 #endif
