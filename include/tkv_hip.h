@@ -618,8 +618,8 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
  *   out_i = sum_j exp(a_ij - m_i) v_j / sum_j exp(a_ij - m_i),
  *   a_ij = scale * q_i . k_j, m_i = max_j a_ij,
  * over the keys j in [0, t) that it sees: all of them, only j <= pos where
- * causal != 0, and only j > pos - window where window > 0.  A row that sees no
- * key gives zeros; what a row does not see (NaN and infinities included) does
+ * causal != 0, and only j > pos - window where window > 0; scale >= 0.  A row
+ * that sees no key (or whose logits are all -inf) gives zeros; what a row does not see (NaN and infinities included) does
  * not touch it.  Query head h reads key / value head h / (heads_q / heads_kv).
  * Statistics and sums are f32.  For f16 and bf16 the products run on the
  * matrix units from values of that type, the weights exp(a - m) rounded to it

@@ -70,8 +70,13 @@ struct AttnArgs {
     int32_t seqs, hq, hkv, g, d;
     int32_t causal;
     int64_t window;    // 0: none
-    float scale_log2;  // scale * log2(e): weights are exp2(s * scale_log2 - m)
+    float scale_log2;  // scale * log2(e) > 0: weights are exp2(s * scale_log2 - m)
     int32_t out_f32;
+    // split over the keys: sums [splits][tokens][hq][d] and (m, l) of each
+    FastDiv gdiv;      // g
+    int32_t splits, units;
+    float* part_o;
+    float2* part_ml;
 };
 
 // The rows of sequence i, clamped to what there is.
@@ -119,7 +124,94 @@ __device__ __forceinline__ int seen_begin(const AttnArgs& a, int pos) {
     return b > 0 ? (b > 0x7fffffff ? 0x7fffffff : (int)b) : 0;
 }
 
+// The last sequence that begins at or before query row `row`, which is the one
+// that has it if any does.
+__device__ __forceinline__ int seq_at(const AttnArgs& a, int64_t row) {
+    if (!a.cu_q) return (int)row;
+    int lo = 0, hi = a.seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu_q[mid] <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+__device__ __forceinline__ bool covered(const AttnArgs& a, int64_t row) {
+    if (!a.cu_q) return true;
+    const int i = seq_at(a, row);
+    const int q0 = clamp_to(a.cu_q[i], a.tokens);
+    return row >= q0 && row < clamp_to(a.cu_q[i + 1], a.tokens);
+}
+
+// Element offset of key (or value) row j of a sequence; *srow, where paged, the
+// row of its scale.
+template <bool PAGED>
+__device__ __forceinline__ int64_t kv_row(const AttnArgs& a, const Seq& s, const int32_t* table,
+                                          int kvh, int j, int64_t st, int64_t sh, int64_t* srow) {
+    if (!PAGED) return (s.k0 + j) * st + kvh * sh;
+    const uint32_t pg = div_by(a.page, (uint32_t)j), slot = (uint32_t)j - pg * a.page.d;
+    uint32_t id = (uint32_t)table[pg];
+    id = (int64_t)id < a.pool_pages ? id : 0;
+    const int64_t row = ((int64_t)id * a.hkv + kvh) * a.page.d + slot;
+    *srow = row;
+    return row * a.d;
+}
+
+// One query row (qr) over the keys [j0, j1) by one wave: a key per lane for the
+// logits, an element of the head per lane for the sums (lane + 64 e in acc[e]).
+// Keys outside the range are not read.  *m in log2 units.
+template <typename T, typename C, bool PAGED>
+__device__ __forceinline__ void attend_row(const AttnArgs& a, const Seq& s, const int32_t* table,
+                                           int kvh, const T* qr, int j0, int j1, float* mo,
+                                           float* lo, float (&acc)[4]) {
+    const int lane = threadIdx.x & 63;
+    const C* kp = static_cast<const C*>(a.k);
+    const C* vp = static_cast<const C*>(a.v);
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int e = 0; e < 4; e++) acc[e] = 0.0f;
+    for (int j = j0; j < j1; j += 64) {
+        const bool seen = j + lane < j1;
+        float x = -__builtin_inff(), vs = 1.0f;
+        if (seen) {
+            int64_t sr = 0;
+            const C* kr = kp + kv_row<PAGED>(a, s, table, kvh, j + lane, a.k_st, a.k_sh, &sr);
+            float dot = 0.0f;
+            for (int e = 0; e < a.d; e++) dot = fmaf(to_f32(qr[e]), to_f32(kr[e]), dot);
+            if (sizeof(C) == 1) {
+                dot *= a.ks[sr];
+                vs = a.vs[sr];
+            }
+            x = dot * a.scale_log2;
+        }
+        float top = x;
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.0f : mn;
+        const float p = seen ? exp2f(x - base) : 0.0f, fix = exp2f(m - base);
+        float sum = p;
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        l = l * fix + sum;
+        for (int e = 0; e < 4; e++) acc[e] *= fix;
+        m = mn;
+        const int n = j1 - j < 64 ? j1 - j : 64;
+        for (int t = 0; t < n; t++) {
+            int64_t sr = 0;
+            const float w = __shfl(p * vs, t);
+            const C* vr = vp + kv_row<PAGED>(a, s, table, kvh, j + t, a.v_st, a.v_sh, &sr);
+            for (int e = 0; e < 4; e++)
+                if (lane + 64 * e < a.d) acc[e] = fmaf(w, to_f32(vr[lane + 64 * e]), acc[e]);
+        }
+    }
+    *mo = m;
+    *lo = l;
+}
+
 // attn_any.hip: any head size up to 256, any strides and alignment.
 int launch_attn_any(Ctx* c, const AttnArgs& a, int type, int kv_type);
+// attn_tile_*.hip: many query rows per sequence and head, on the matrix units.
+// 16-byte rows; `splits` > 1 leaves partial sums in a.part_o and a.part_ml.
+int launch_attn_tile_bf16(Ctx* c, const AttnArgs& a, bool i8);
+int launch_attn_tile_f16(Ctx* c, const AttnArgs& a, bool i8);
+int launch_attn_tile_f32(Ctx* c, const AttnArgs& a, bool i8);
+// Query rows (of all heads of one key / value head) that a workgroup takes.
+constexpr int kTileRows = 128;
 
 }  // namespace tkv

@@ -1,5 +1,7 @@
 // attn.hip -- entry points of the attention operators: argument checks and the
 // choice of kernel.
+#include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "attn.h"
@@ -8,7 +10,8 @@ namespace tkv {
 
 static int check_attention(const char* who, int32_t type, int32_t type_out, int64_t tokens,
                            int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t sequences,
-                           const tkv_hip_rows* q, const tkv_hip_rows* out, int64_t window) {
+                           const tkv_hip_rows* q, const tkv_hip_rows* out, float scale,
+                           int64_t window) {
     const std::string w(who);
     if (!float_type(type) || (type_out != type && type_out != TKV_HIP_F32))
         return set_error(TKV_HIP_BAD_ARG, w + ": type is F32, F16 or BF16, type_out the same or F32");
@@ -18,6 +21,8 @@ static int check_attention(const char* who, int32_t type, int32_t type_out, int6
     if (heads_q % heads_kv)
         return set_error(TKV_HIP_BAD_ARG, w + ": heads_q is not a multiple of heads_kv");
     if (window < 0) return set_error(TKV_HIP_BAD_ARG, w + ": negative window");
+    if (!(scale >= 0.0f) || !std::isfinite(scale))
+        return set_error(TKV_HIP_BAD_ARG, w + ": scale is negative or not finite");
     if (!q || !out || (tokens > 0 && (!q->data || !out->data)))
         return set_error(TKV_HIP_BAD_ARG, w + ": NULL rows");
     return TKV_HIP_OK;
@@ -41,8 +46,92 @@ static void common_args(AttnArgs* a, int32_t type, int32_t type_out, int64_t tok
     a->d = (int32_t)head_dim;
     a->causal = causal != 0;
     a->window = window;
-    a->scale_log2 = (float)((double)scale * 1.4426950408889634);
+    // a scale of zero (equal weights) as one that no finite logit notices, so
+    // that hidden logits of -inf stay -inf
+    a->scale_log2 = std::max((float)((double)scale * 1.4426950408889634), 1e-30f);
     a->out_f32 = type_out == TKV_HIP_F32;
+}
+
+// Joins the splits of a query row and head: O = sum_s 2^(m_s - m) O_s / sum_s
+// 2^(m_s - m) l_s, in the order of the splits.  One wave per row and head; reads
+// d + 2 floats per split.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t rows = a.tokens * a.hq;
+    if (unit >= rows) return;
+    const int64_t row = unit / a.hq;
+    const int h = (int)(unit - row * a.hq);
+    if (!covered(a, row)) return;  // its partial sums were not written either
+    float m = -__builtin_inff();
+    for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.part_ml[s * rows + unit].x);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; s++) {
+        const float2 ml = a.part_ml[s * rows + unit];
+        const float w = __builtin_amdgcn_exp2f(ml.x - base);
+        l = fmaf(w, ml.y, l);
+        const float* po = a.part_o + (s * rows + unit) * a.d;
+        if (w != 0.0f)
+            for (int e = 0; e < 4; e++)
+                if (lane + 64 * e < a.d) acc[e] = fmaf(w, po[lane + 64 * e], acc[e]);
+    }
+    const int64_t at = row * a.o_st + h * a.o_sh;
+    for (int e = 0; e < 4; e++) {
+        const int x = lane + 64 * e;
+        if (x >= a.d) continue;
+        const float y = l == 0.0f ? 0.0f : acc[e] / l;
+        if (a.out_f32) static_cast<float*>(a.out)[at + x] = y;
+        else static_cast<T*>(a.out)[at + x] = from_f32<T>(y);
+    }
+}
+
+static bool rows_of_16(const void* p, int64_t st, int64_t sh, int64_t bytes) {
+    return aligned(p, 16) && st * bytes % 16 == 0 && sh * bytes % 16 == 0;
+}
+
+// keys: the most that a sequence can have, as far as the host knows.
+static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t max_q, int64_t keys) {
+    const bool i8 = kv_type == TKV_HIP_I8;
+    const int64_t b = type_bytes(type), kb = type_bytes(kv_type), ob = a.out_f32 ? 4 : b;
+    const int64_t chunk = i8 ? 8 : 16 / b;
+    if (a.d % chunk || !rows_of_16(a.q, a.q_st, a.q_sh, b) || !rows_of_16(a.out, a.o_st, a.o_sh, ob) ||
+        !rows_of_16(a.k, a.k_st, a.k_sh, kb) || !rows_of_16(a.v, a.v_st, a.v_sh, kb))
+        return launch_attn_any(c, a, type, kv_type);
+    a.gdiv = fast_div((uint32_t)a.g);
+    const int64_t units = a.tokens * a.g / kTileRows + a.seqs;
+    if (a.tokens * a.g >= (1ll << 31) || units >= (1ll << 31))
+        return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
+    a.units = (int32_t)units;
+    // too few tiles for two workgroups per CU: the keys are split, 256 of them
+    // at least to a split
+    const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, kTileRows), a.seqs) * a.hkv;
+    const int64_t want = std::min<int64_t>(2 * c->num_cus / tiles, keys / 256);
+    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), 64);
+    if (a.splits > 1) {
+        const int64_t rows = a.tokens * a.hq * a.splits;
+        void* ws;
+        const int rc = ctx_workspace(c, 16, (size_t)(rows * (a.d + 2) * 4), &ws);
+        if (no_room(rc)) {
+            a.splits = 1;
+        } else {
+            TKV_RC_TRY(rc);
+            a.part_ml = static_cast<float2*>(ws);
+            a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
+        }
+    }
+    TKV_RC_TRY(type == TKV_HIP_F32   ? launch_attn_tile_f32(c, a, i8)
+               : type == TKV_HIP_F16 ? launch_attn_tile_f16(c, a, i8)
+                                     : launch_attn_tile_bf16(c, a, i8));
+    if (a.splits > 1) {
+        const dim3 grid((unsigned)ceil_div(a.tokens * a.hq, 4));
+        if (type == TKV_HIP_F32) k_attn_join<float><<<grid, 256, 0, c->stream>>>(a);
+        else if (type == TKV_HIP_F16) k_attn_join<_Float16><<<grid, 256, 0, c->stream>>>(a);
+        else k_attn_join<__bf16><<<grid, 256, 0, c->stream>>>(a);
+        TKV_LAUNCH_CHECK();
+    }
+    return TKV_HIP_OK;
 }
 
 }  // namespace tkv
@@ -59,7 +148,7 @@ int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, 
                                      const int32_t* cu_q, const int32_t* cu_k, float scale,
                                      int32_t causal, int64_t window) {
     TKV_RC_TRY(check_attention("attention_prompt", type, type_out, tokens, heads_q, heads_kv,
-                               head_dim, sequences, q, out, window));
+                               head_dim, sequences, q, out, scale, window));
     if (tokens_k < 0 || tokens_k >= (1ll << 31) || !k || !v || (tokens_k > 0 && (!k->data || !v->data)) ||
         (sequences > 0 && !cu_q))
         return set_error(TKV_HIP_BAD_ARG, "attention_prompt: bad keys, values or cu_q");
@@ -79,7 +168,7 @@ int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, 
     a.cu_k = cu_k;
     a.tokens_k = tokens_k;
     a.page = fast_div(1);
-    return launch_attn_any(c, a, type, type);
+    return launch_attention(c, a, type, type, tokens, tokens_k);
 }
 
 int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, int64_t heads_q,
@@ -91,7 +180,7 @@ int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, i
     const KvCache* kv = reinterpret_cast<const KvCache*>(cache);
     if (!kv) return set_error(TKV_HIP_BAD_ARG, "attention_paged: NULL cache");
     TKV_RC_TRY(check_attention("attention_paged", type, type_out, tokens, heads_q, kv->heads, kv->d,
-                               sequences, q, out, window));
+                               sequences, q, out, scale, window));
     if (kv->type != type && kv->type != TKV_HIP_I8)
         return set_error(TKV_HIP_BAD_ARG, "attention_paged: the cache's type is neither type nor I8");
     if (table_stride < 0 || max_q < 0 || max_kv < 0 ||
@@ -119,7 +208,8 @@ int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, i
     a.page = fast_div((uint32_t)kv->page);
     a.cu_q = cu_q;
     a.kv_lens = kv_lens;
-    return launch_attn_any(c, a, type, kv->type);
+    const int64_t held = table_stride * kv->page;
+    return launch_attention(c, a, type, kv->type, max_q, max_kv ? std::min(max_kv, held) : held);
 }
 
 }  // extern "C"

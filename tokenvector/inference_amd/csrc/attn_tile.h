@@ -1,0 +1,562 @@
+// attn_tile.h -- attention of many query rows on the matrix units (MFMA).
+//
+// Softmax in one pass over the keys: per query row a running maximum m, a sum l
+// and the unnormalised output O, all f32.  A workgroup of four waves takes 128
+// rows of one key / value head; a row is a (token, query head of the group)
+// pair, token-major, so grouped heads share every key tile and a causal tile's
+// rows span few positions.  Each wave owns 32 rows, all waves share the key and
+// value tiles in LDS, which global_load_lds copies a tile ahead (two buffers,
+// one barrier per tile).
+//
+// Both products are computed transposed, so that a lane owns one query row
+// (column lane & 31 of the 32 x 32 accumulators; lanes l and l + 32 share it):
+//   S^T = K Q^T     A = key rows from LDS, B = the wave's queries in registers
+//   O^T = V^T P^T   A = value columns, B = the weights in registers
+// The maximum, the sum and the rescaling of O are then lane-local (one
+// permlane32_swap joins the halves), and the accumulator layout of S^T (lane
+// half h holds keys 8 i + 4 h .. + 3) is a B operand's layout up to the order
+// of the keys in the contraction: the values are read in that order
+// (ds_read_b64_tr_b16: four keys of one column per lane), and P never leaves
+// its registers.  f32 uses the 32x32x2 product, whose two-key steps take the
+// same registers as they are.
+#pragma once
+
+#include "attn.h"
+
+namespace tkv {
+namespace attn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_void;
+
+template <typename T>
+struct Vec {  // 16 bytes
+    static constexpr int N = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(N)));
+};
+
+__device__ __forceinline__ f32x16 mfma32(Vec<__bf16>::type a, Vec<__bf16>::type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(Vec<_Float16>::type a, Vec<_Float16>::type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// 16 bytes per lane from global memory to LDS at `dst` (wave-uniform) + 16 lane.
+// In asm, since the compiler would put a wait for every copy in flight before
+// each LDS read it cannot tell apart from the copy's destination; the waits
+// here are the callers' own (wait_vm below, before a barrier).  No register is
+// written; the s_nop is the wait state between a scalar write of m0 and the
+// copy that uses it.
+__device__ __forceinline__ void copy16_to_lds(const void* src, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(src), "s"(dst)
+                 : "memory");
+}
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ unsigned lds_at(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The other half's value: lanes l and l + 32 exchange.
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
+}
+
+// LDS rows of CPR 16-byte chunks.  Key rows are read 16 lanes = 16 rows at one
+// chunk at a time: the chunk is XORed so that the 16 land in different banks.
+template <int CPR>
+__device__ __forceinline__ int swz_k(int row) {
+    if constexpr (CPR % 16 == 0) return row & 15;
+    else if constexpr (CPR % 8 == 0) return (row >> 1) & 7;
+    else return (row >> 2) & 3;
+}
+// Value rows are read four rows (16-bit types; two rows 4 apart for f32) at a
+// 64-byte (128-byte) window at a time: the window is XORed.
+template <int CPR, int SIZE>
+__device__ __forceinline__ int swz_v(int row) {
+    if constexpr (SIZE == 4) return CPR % 16 == 0 ? ((row >> 2) & 1) << 3 : 0;
+    else if constexpr (CPR % 16 == 0) return (row & 3) << 2;
+    else if constexpr (CPR % 8 == 0) return ((row >> 1) & 1) << 2;
+    else return 0;
+}
+
+enum { KV_PACKED = 0, KV_PAGED = 1, KV_I8 = 2 };
+
+// DP: head size, padded (64, 96, 128, 192, 256; f32 96 only as 128).
+template <typename T, int DP>
+struct TileShape {
+    static constexpr int E = sizeof(T);
+    static constexpr int BN = (E == 4 || DP >= 192) ? 32 : 64;  // keys of a tile
+    static constexpr int CPR = DP * E / 16;
+    static constexpr int CE = 16 / E;                           // elements of a chunk
+    static constexpr int TILE = BN * DP * E;                    // bytes
+    static constexpr int NT = 256;
+    static constexpr int N = BN * CPR / NT;                     // chunks a thread copies
+    static_assert(BN * CPR % NT == 0, "chunks per thread");
+    static constexpr int LDS = 4 * TILE + 4 * BN * 4;           // two buffers of K and V, scales
+};
+
+// Sequence and tile of a unit.  Sequence i's tiles begin at
+// floor(cu[i] g / 128) + i, which leaves each sequence room for all of its
+// tiles (and up to one unit without rows).  Lanes look at 64 sequences at a
+// time: the last one that begins at or before the unit.
+template <bool PAGED>
+__device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first) {
+    const int lane = threadIdx.x & 63;
+    int found = 0, begin = 0;
+    for (int b = 0; b < a.seqs; b += 64) {
+        const int i = b + lane;
+        int at = 0x7fffffff;
+        if (i < a.seqs) {
+            const int q0 = (PAGED && !a.cu_q) ? i : clamp_to(a.cu_q[i], a.tokens);
+            at = (int)((int64_t)q0 * a.g / kTileRows) + i;
+        }
+        const unsigned long long before = __ballot(at <= unit);
+        if (!before) break;
+        const int last = 63 - __builtin_clzll(before);
+        found = b + last;
+        begin = __shfl(at, last);
+        if (last < 63) break;
+    }
+    *first = uniform(begin);
+    return uniform(found);
+}
+
+template <typename T, int DP, int KV>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_attn_tile(AttnArgs a) {
+    using S = TileShape<T, DP>;
+    using V8 = typename Vec<T>::type;
+    constexpr bool PAGED = KV != KV_PACKED, I8 = KV == KV_I8, F32 = sizeof(T) == 4;
+    constexpr int BN = S::BN, NKB = BN / 32, NDB = DP / 32, CPR = S::CPR, N = S::N;
+    constexpr float kInf = __builtin_inff();
+    using C = typename std::conditional<I8, int8_t, T>::type;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* lds_ks = reinterpret_cast<float*>(lds + 4 * S::TILE);  // [2][BN] keys' and values' scales
+    float* lds_vs = lds_ks + 2 * BN;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int l31 = lane & 31, half = lane >> 5;
+    // heads vary fastest: one head's tiles stay on few XCDs, whose L2 then holds
+    // its keys; later tiles, the longest ones where causal, start first
+    const int kvh = blockIdx.x % a.hkv;
+    const int unit = a.units - 1 - (int)(blockIdx.x / a.hkv);
+    int first;
+    const int seq = tile_seq<PAGED>(a, unit, &first);
+    Seq s = seq_of<PAGED>(a, seq);
+    s.q0 = uniform(s.q0), s.n = uniform(s.n), s.len = uniform(s.len);
+    const int rows = s.n * a.g;
+    const int row0 = (unit - first) * kTileRows;
+    if (row0 >= rows) return;
+    const int32_t* table = PAGED ? a.pages + seq * a.pages_st : nullptr;
+
+    // positions of the workgroup's and the wave's rows, and what they see
+    const int shift = s.len - s.n;
+    const int last_row = min(row0 + kTileRows, rows) - 1;
+    int kb = seen_begin(a, shift + (int)div_by(a.gdiv, row0));
+    int ke = seen_end(a, shift + (int)div_by(a.gdiv, last_row), s.len);
+    const int wrow = row0 + 32 * wave, wlast = min(wrow + 31, rows - 1);
+    const bool live = wrow < rows;
+    const int pos_lo = shift + (int)div_by(a.gdiv, live ? wrow : 0);
+    const int pos_hi = shift + (int)div_by(a.gdiv, live ? wlast : 0);
+    const int w_begin = uniform(seen_begin(a, pos_lo)), w_end = uniform(live ? seen_end(a, pos_hi, s.len) : 0);
+    const int f_begin = uniform(seen_begin(a, pos_hi)), f_end = uniform(seen_end(a, pos_lo, s.len));
+    // this lane's row
+    const int row = wrow + l31;
+    const bool mine = row < rows;
+    const int tok = (int)div_by(a.gdiv, mine ? row : 0), head = kvh * a.g + (mine ? row : 0) - tok * a.g;
+    const int my_begin = seen_begin(a, shift + tok), my_end = mine ? seen_end(a, shift + tok, s.len) : 0;
+
+    // tiles of this split
+    int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
+    if (a.splits > 1) {
+        const int per = (t1 - t0 + a.splits - 1) / a.splits;
+        t0 = min(t0 + (int)blockIdx.y * per, t1);
+        t1 = min(t0 + per, t1);
+    }
+    t0 = uniform(t0), t1 = uniform(t1);
+
+    // queries: element order of a B operand, chunk 2 i + half of the row
+    V8 q[CPR / 2];
+    {
+        const T* qr = static_cast<const T*>(a.q) + (int64_t)(s.q0 + tok) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < CPR / 2; i++) {
+            const int e = (2 * i + half) * S::CE;
+            q[i] = V8{};
+            if (mine && e < a.d) q[i] = *reinterpret_cast<const V8*>(qr + e);
+        }
+    }
+    if (a.d < DP) {
+        // the chunks past the head's end are never copied: zeros, as the queries there
+        for (int i = tid; i < 4 * S::TILE / 16; i += 256)
+            reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+        barrier();
+    }
+
+    // ---- copies: thread's chunk i is position i * 256 + tid of the tile ----
+    uint32_t page_of[PAGED ? N : 1], slot_of[PAGED ? N : 1];
+    const auto row_of = [&](int i) { return (i * 256 + tid) / CPR; };
+    const auto find_pages = [&](int t) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int j = min(t * BN + row_of(i), s.len - 1);  // past the end: the last key again, masked
+                const uint32_t pg = div_by(a.page, (uint32_t)j);
+                slot_of[i] = (uint32_t)j - pg * a.page.d;
+                page_of[i] = (uint32_t)table[pg];
+            }
+        }
+    };
+    constexpr int NR = I8 ? BN * (DP / 8) / 256 : 1;  // 8 codes per thread and trip
+    uint2 kc[NR], vc[NR];
+    float sc = 0.0f;
+    const auto copy_tile = [&](int t, int buf) {
+        if constexpr (!I8) {
+            const unsigned base = lds_at(lds) + buf * 2 * S::TILE;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int pos = (i * 256 + tid) % CPR, r = row_of(i);
+                const int ck = pos ^ swz_k<CPR>(r), cv = pos ^ swz_v<CPR, S::E>(r);
+                const T *kr, *vr;
+                if constexpr (PAGED) {
+                    const uint32_t id = (int64_t)page_of[i] < a.pool_pages ? page_of[i] : 0;
+                    const int64_t at = (((int64_t)id * a.hkv + kvh) * a.page.d + slot_of[i]) * a.d;
+                    kr = static_cast<const T*>(a.k) + at;
+                    vr = static_cast<const T*>(a.v) + at;
+                } else {
+                    const int64_t j = s.k0 + min(t * BN + r, s.len - 1);
+                    kr = static_cast<const T*>(a.k) + j * a.k_st + (int64_t)kvh * a.k_sh;
+                    vr = static_cast<const T*>(a.v) + j * a.v_st + (int64_t)kvh * a.v_sh;
+                }
+                const unsigned dst = uniform(base + (i * 4 + wave) * 1024);
+                if (ck * S::CE < a.d) copy16_to_lds(kr + ck * S::CE, dst);
+                if (cv * S::CE < a.d) copy16_to_lds(vr + cv * S::CE, dst + S::TILE);
+            }
+        } else {
+            // codes through registers: converted on their way to LDS, below
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const int x = i * 256 + tid, r = x / (DP / 8), e = 8 * (x % (DP / 8));
+                const int j = min(t * BN + r, s.len - 1);
+                int64_t sr;
+                const int64_t at = kv_row<true>(a, s, table, kvh, j, 0, 0, &sr) + e;
+                kc[i] = vc[i] = uint2{0, 0};
+                if (e < a.d) {
+                    kc[i] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.k) + at);
+                    vc[i] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.v) + at);
+                }
+            }
+            if (tid < 2 * BN) {
+                const int j = min(t * BN + (tid & (BN - 1)), s.len - 1);
+                int64_t sr;
+                kv_row<true>(a, s, table, kvh, j, 0, 0, &sr);
+                sc = (tid < BN ? a.ks : a.vs)[sr];
+            }
+        }
+    };
+    const auto put_codes = [&](int buf) {
+        if constexpr (I8) {
+            char* base = lds + buf * 2 * S::TILE;
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const int x = i * 256 + tid, r = x / (DP / 8), e = 8 * (x % (DP / 8));
+                const auto put = [&](char* to, uint2 w, int swz) {
+#pragma unroll
+                    for (int h = 0; h < 8 / S::CE; h++) {
+                        V8 y;
+#pragma unroll
+                        for (int j = 0; j < S::CE; j++) {
+                            const int at = h * S::CE + j;
+                            y[j] = (T)(float)(int8_t)((at < 4 ? w.x : w.y) >> (8 * (at & 3)));
+                        }
+                        *reinterpret_cast<V8*>(to + r * (CPR * 16) + (((e / S::CE + h) ^ swz) << 4)) = y;
+                    }
+                };
+                put(base, kc[i], swz_k<CPR>(r));
+                put(base + S::TILE, vc[i], swz_v<CPR, S::E>(r));
+            }
+            if (tid < 2 * BN) (tid < BN ? lds_ks : lds_vs)[buf * BN + (tid & (BN - 1))] = sc;
+        }
+    };
+
+    f32x16 o[NDB];
+#pragma unroll
+    for (int b = 0; b < NDB; b++) o[b] = f32x16{};
+    float m = -kInf, l = 0.0f;
+    constexpr bool SCALED = I8 && std::is_same<T, _Float16>::value;
+    float vexp = SCALED ? 0.0f : 1.0f;  // SCALED: O is in units of vexp, 0 or a power of two
+
+    // LDS offsets of this lane's reads
+    const int k_row = l31 * (CPR * 16), k_swz = swz_k<CPR>(l31);
+    const int vr = half * 4 + ((lane & 15) >> 2);
+    const int v_swz = swz_v<CPR, S::E>(vr);
+    const int v_col = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);  // chunk of the lane's column block
+
+    if (t0 < t1) {
+        find_pages(t0);
+        copy_tile(t0, 0);
+        put_codes(0);
+        if (t0 + 1 < t1) find_pages(t0 + 1);
+    }
+    for (int t = t0; t < t1; t++) {
+        const int buf = (t - t0) & 1;
+        if constexpr (!I8) wait_vm();
+        barrier();  // tile t is in LDS, and nobody reads the other buffer any more
+        if (t + 1 < t1) {
+            copy_tile(t + 1, buf ^ 1);
+            if (t + 2 < t1) find_pages(t + 2);
+        }
+        const int j0 = t * BN;
+        if (j0 < w_end && j0 + BN > w_begin) {
+            const char* kt = lds + buf * 2 * S::TILE;
+            const char* vt = kt + S::TILE;
+            f32x16 x[NKB];
+#pragma unroll
+            for (int b = 0; b < NKB; b++) {
+                x[b] = f32x16{};
+#pragma unroll
+                for (int i = 0; i < CPR / 2; i++) {
+                    const V8 k = *reinterpret_cast<const V8*>(kt + b * 32 * (CPR * 16) + k_row +
+                                                              (((2 * i + half) ^ k_swz) << 4));
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            x[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[i][j], x[b], 0, 0, 0);
+                    } else {
+                        x[b] = mfma32(k, q[i], x[b]);
+                    }
+                }
+            }
+            const bool full = j0 >= f_begin && j0 + BN <= f_end;
+            float vs[I8 ? NKB * 16 : 1];
+            if constexpr (I8) {
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = b * 32 + 8 * i + 4 * half;
+                        const f32x4 ks4 = *reinterpret_cast<const f32x4*>(lds_ks + buf * BN + key);
+                        const f32x4 vs4 = *reinterpret_cast<const f32x4*>(lds_vs + buf * BN + key);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            x[b][4 * i + j] *= ks4[j];
+                            vs[b * 16 + 4 * i + j] = vs4[j];
+                        }
+                    }
+            }
+            if (!full) {
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int j = j0 + b * 32 + (e & 3) + 8 * (e >> 2) + 4 * half;
+                        const bool seen = j >= my_begin && j < my_end;
+                        x[b][e] = seen ? x[b][e] : -kInf;
+                        if constexpr (I8) vs[b * 16 + e] = seen ? vs[b * 16 + e] : 0.0f;
+                    }
+            }
+            float mx = -kInf;
+#pragma unroll
+            for (int b = 0; b < NKB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, x[b][e]);
+            mx = fmaxf(mx, other_half(mx)) * a.scale_log2;
+            // O and l are rescaled only once the maximum has grown by 2^8: the
+            // weights stay below that, far inside every type's range, and most
+            // tiles skip 4 * DP multiplications per row
+            if (__any(mx > m + 8.0f || (m == -kInf && mx > -kInf))) {
+                const float mn = fmaxf(m, mx);
+                const float fix = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= fix;
+#pragma unroll
+                for (int b = 0; b < NDB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[b][e] *= fix;
+            }
+            const float base = m == -kInf ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NKB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    x[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], a.scale_log2, -base));
+                    sum += x[b][e];
+                }
+            l += sum;
+            if constexpr (I8) {
+                if constexpr (SCALED) {
+                    // f16 weights times scales of any size: O is kept in units of
+                    // the largest scale's power of two so far
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NKB * 16; i++) top = fmaxf(top, vs[i]);
+                    top = fmaxf(top, other_half(top));
+                    const float unit2 = top > 0.0f && top < kInf
+                                            ? __builtin_ldexpf(1.0f, max(ilogbf(top), -100)) : 0.0f;
+                    if (__any(unit2 > vexp)) {
+                        const float nu = fmaxf(unit2, vexp), fix = nu > 0.0f ? vexp / nu : 1.0f;
+                        vexp = nu;
+#pragma unroll
+                        for (int b = 0; b < NDB; b++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[b][e] *= fix;
+                    }
+                    const float inv = vexp > 0.0f ? 1.0f / vexp : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NKB * 16; i++) vs[i] *= inv;
+                }
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[b][e] *= vs[b * 16 + e];
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int key = (e & 3) + 8 * (e >> 2) + 4 * half;
+                    const char* row_at = vt + key * (CPR * 16);
+                    const int swz = swz_v<CPR, 4>(key);
+#pragma unroll
+                    for (int b = 0; b < NDB; b++) {
+                        const int col = b * 32 + l31;
+                        const float v = *reinterpret_cast<const float*>(
+                            row_at + (((col >> 2) ^ swz) << 4) + ((col & 3) << 2));
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[0][e], o[b], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int st = 0; st < BN / 16; st++) {
+                    V8 p;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) p[j] = (T)x[st >> 1][(st & 1) * 8 + j];
+#pragma unroll
+                    for (int b = 0; b < NDB; b++) {
+                        const char* at = vt + (st * 16 + vr) * (CPR * 16) + (((b * 4 + v_col) ^ v_swz) << 4) +
+                                         ((lane & 1) << 3);
+                        typedef __attribute__((address_space(3))) s16x4* lds4;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * (CPR * 16)));
+                        typedef short s16x8 __attribute__((ext_vector_type(8)));
+                        const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[b] = mfma32(__builtin_bit_cast(V8, v), p, o[b]);
+                    }
+                }
+            }
+        }
+        if (t + 1 < t1) put_codes(buf ^ 1);
+    }
+    l += other_half(l);
+    if (!live) return;
+
+    // A value that no row of a wave's tile may see still meets a weight of zero
+    // in the product; where that left something that is not finite, those rows
+    // are computed again, key by key.  Rows that see such values end up the same.
+    bool bad = !(fabsf(l) < kInf);
+#pragma unroll
+    for (int b = 0; b < NDB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) bad |= !(fabsf(o[b][e]) < kInf);
+    unsigned long long ball = __ballot(bad && mine);
+    unsigned again = uniform((unsigned)ball | (unsigned)(ball >> 32));
+    const bool split = a.splits > 1;
+    const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
+
+    if (mine && !((again >> l31) & 1)) {
+        const int64_t t_at = s.q0 + tok;
+        const float scale = (split || l == 0.0f ? 1.0f : 1.0f / l) * vexp;
+        if (split && half == 0) a.part_ml[(part + t_at) * a.hq + head] = make_float2(m, l);
+        float* po = a.part_o + ((part + t_at) * a.hq + head) * a.d;
+        char* out = static_cast<char*>(a.out) +
+                    (t_at * a.o_st + (int64_t)head * a.o_sh) * (a.out_f32 ? 4 : sizeof(T));
+#pragma unroll
+        for (int b = 0; b < NDB; b++) {
+            if (split || a.out_f32) {
+                float* to = split ? po : reinterpret_cast<float*>(out);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = b * 32 + 8 * i + 4 * half;
+                    const f32x4 y = {o[b][4 * i] * scale, o[b][4 * i + 1] * scale, o[b][4 * i + 2] * scale,
+                                     o[b][4 * i + 3] * scale};
+                    if (e < a.d) *reinterpret_cast<f32x4*>(to + e) = y;
+                }
+            } else if constexpr (!F32) {
+                // halves exchange groups of four: 8 elements, 16 bytes, per store
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    T y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) y[j] = (T)(o[b][8 * i + j] * scale);
+                    uint2 lo, hi;
+                    __builtin_memcpy(&lo, y, 8);
+                    __builtin_memcpy(&hi, y + 4, 8);
+                    const auto sx = __builtin_amdgcn_permlane32_swap(lo.x, hi.x, false, false);
+                    const auto sy = __builtin_amdgcn_permlane32_swap(lo.y, hi.y, false, false);
+                    const int e = b * 32 + 16 * i + 8 * half;
+                    if (e < a.d) *reinterpret_cast<u32x4*>(out + e * 2) = u32x4{sx[0], sy[0], sx[1], sy[1]};
+                }
+            }
+        }
+    }
+    while (again) {
+        const int i = __builtin_ctz(again);
+        again &= again - 1;
+        const int r = wrow + i, tk = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tk * a.g;
+        const int64_t t_at = s.q0 + tk;
+        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
+        float mm, ll, acc[4];
+        attend_row<T, C, PAGED>(a, s, table, kvh, qr, max(seen_begin(a, shift + tk), t0 * BN),
+                                min(seen_end(a, shift + tk, s.len), t1 * BN), &mm, &ll, acc);
+        if (split && lane == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
+        for (int e = 0; e < 4; e++) {
+            const int x = lane + 64 * e;
+            if (x >= a.d) continue;
+            const float y = split || ll == 0.0f ? acc[e] : acc[e] / ll;
+            if (split) a.part_o[((part + t_at) * a.hq + h) * a.d + x] = y;
+            else if (a.out_f32) static_cast<float*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = y;
+            else static_cast<T*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = from_f32<T>(y);
+        }
+    }
+}
+
+template <typename T, int DP, int KV>
+int launch_tile_dp(Ctx* c, const AttnArgs& a) {
+    using S = TileShape<T, DP>;
+    static_assert(S::LDS <= 163840, "LDS of a workgroup");
+    if ((size_t)S::LDS > c->max_lds) return set_error(TKV_HIP_UNSUPPORTED, "attention: not enough LDS");
+    const int64_t blocks = (int64_t)a.units * a.hkv;
+    if (blocks >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many tiles");
+    k_attn_tile<T, DP, KV><<<dim3((unsigned)blocks, (unsigned)a.splits), 256, S::LDS, c->stream>>>(a);
+    TKV_LAUNCH_CHECK();
+    return TKV_HIP_OK;
+}
+
+template <typename T, int KV>
+int launch_tile_kv(Ctx* c, const AttnArgs& a) {
+    if (a.d <= 64) return launch_tile_dp<T, 64, KV>(c, a);
+    if constexpr (sizeof(T) == 2)
+        if (a.d <= 96) return launch_tile_dp<T, 96, KV>(c, a);
+    if (a.d <= 128) return launch_tile_dp<T, 128, KV>(c, a);
+    if (a.d <= 192) return launch_tile_dp<T, 192, KV>(c, a);
+    return launch_tile_dp<T, 256, KV>(c, a);
+}
+
+template <typename T>
+int launch_tile(Ctx* c, const AttnArgs& a, bool i8) {
+    if (!a.pages) return launch_tile_kv<T, KV_PACKED>(c, a);
+    return i8 ? launch_tile_kv<T, KV_I8>(c, a) : launch_tile_kv<T, KV_PAGED>(c, a);
+}
+
+}  // namespace attn
+}  // namespace tkv

@@ -99,7 +99,8 @@ struct Ctx {
     // grow-only workspaces
     // 10, 11: f16-decoded FP8 operands; 12: INT4 split-K partials (any kernel);
     // 13, 14, 15: INT4 digit planes, retiled weight codes, permuted activations
-    static constexpr int kSlots = 16;
+    // 16: partial sums of the attention's splits over the keys
+    static constexpr int kSlots = 17;
     void* ws[kSlots] = {};
     size_t ws_bytes[kSlots] = {};
     // Staging of the INT8 GEMM's host mirror (codes on their way to the device):
