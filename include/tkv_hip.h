@@ -571,7 +571,7 @@ typedef struct {
  * pool is (s / page_size, s % page_size).  k == NULL: the handle allocates
  * (zeroed) and frees the memory; otherwise the four device pointers are the
  * caller's (scales NULL unless I8) and have to outlive the handle.
- * num_pages * page_size < 2^31; head_dim <= 256. */
+ * num_pages * page_size < 2^31, times heads < 2^32; head_dim <= 256. */
 int32_t tkv_hip_kv_create(int64_t ctx, int32_t type, int64_t num_pages, int64_t page_size,
                           int64_t heads, int64_t head_dim, void* k, void* v, float* k_scales,
                           float* v_scales, int64_t* handle_out);

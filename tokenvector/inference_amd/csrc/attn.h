@@ -211,6 +211,11 @@ int launch_attn_any(Ctx* c, const AttnArgs& a, int type, int kv_type);
 int launch_attn_tile_bf16(Ctx* c, const AttnArgs& a, bool i8);
 int launch_attn_tile_f16(Ctx* c, const AttnArgs& a, bool i8);
 int launch_attn_tile_f32(Ctx* c, const AttnArgs& a, bool i8);
+// attn_few_*.hip: up to 32 query rows per sequence and key / value head, over a
+// cache (int8 ones with d a multiple of 16).
+int launch_attn_few_bf16(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
+int launch_attn_few_f16(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
+int launch_attn_few_f32(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
 // Query rows (of all heads of one key / value head) that a workgroup takes.
 constexpr int kTileRows = 128;
 

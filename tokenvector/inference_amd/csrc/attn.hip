@@ -100,15 +100,29 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
         !rows_of_16(a.k, a.k_st, a.k_sh, kb) || !rows_of_16(a.v, a.v_st, a.v_sh, kb))
         return launch_attn_any(c, a, type, kv_type);
     a.gdiv = fast_div((uint32_t)a.g);
-    const int64_t units = a.tokens * a.g / kTileRows + a.seqs;
-    if (a.tokens * a.g >= (1ll << 31) || units >= (1ll << 31))
+    if (a.tokens * a.g >= (1ll << 31))
         return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
+    // up to 32 rows per sequence take the streaming kernel, blocks of 16 rows
+    const int64_t longest = a.pages ? (a.cu_q ? max_q : 1) * a.g : 0;
+    const bool few = longest > 0 && longest <= 32 && !(i8 && a.d % 16);
+    const int blocks16 = longest <= 16 ? 1 : 2;
+    const int64_t block = few ? 16 * blocks16 : kTileRows;
+    const int64_t units = few && !a.cu_q ? a.seqs : a.tokens * a.g / block + a.seqs;
+    if (units >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     a.units = (int32_t)units;
-    // too few tiles for two workgroups per CU: the keys are split, 256 of them
-    // at least to a split
-    const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, kTileRows), a.seqs) * a.hkv;
-    const int64_t want = std::min<int64_t>(2 * c->num_cus / tiles, keys / 256);
-    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), 64);
+    const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs) * a.hkv;
+    int64_t want;
+    if (few) {
+        // streaming: four rounds of the workgroups that fit, so that caches of
+        // different lengths even out
+        const int64_t slots = (a.d <= 128 ? 2 : 1) * c->num_cus;
+        want = std::min<int64_t>(4 * slots / tiles, keys / 256);
+    } else {
+        // too few tiles for two workgroups per CU: the keys are split, 256 of
+        // them at least to a split
+        want = std::min<int64_t>(2 * c->num_cus / tiles, keys / 256);
+    }
+    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), 128);
     if (a.splits > 1) {
         const int64_t rows = a.tokens * a.hq * a.splits;
         void* ws;
@@ -121,9 +135,14 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
             a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
         }
     }
-    TKV_RC_TRY(type == TKV_HIP_F32   ? launch_attn_tile_f32(c, a, i8)
-               : type == TKV_HIP_F16 ? launch_attn_tile_f16(c, a, i8)
-                                     : launch_attn_tile_bf16(c, a, i8));
+    if (few)
+        TKV_RC_TRY(type == TKV_HIP_F32   ? launch_attn_few_f32(c, a, i8, blocks16)
+                   : type == TKV_HIP_F16 ? launch_attn_few_f16(c, a, i8, blocks16)
+                                         : launch_attn_few_bf16(c, a, i8, blocks16));
+    else
+        TKV_RC_TRY(type == TKV_HIP_F32   ? launch_attn_tile_f32(c, a, i8)
+                   : type == TKV_HIP_F16 ? launch_attn_tile_f16(c, a, i8)
+                                         : launch_attn_tile_bf16(c, a, i8));
     if (a.splits > 1) {
         const dim3 grid((unsigned)ceil_div(a.tokens * a.hq, 4));
         if (type == TKV_HIP_F32) k_attn_join<float><<<grid, 256, 0, c->stream>>>(a);

@@ -1,0 +1,471 @@
+// attn_few.h -- attention of few query rows over a paged cache: decoding, and
+// chunks of up to 32 (token, query head of the group) rows.  HBM bound: the
+// cache's bytes, read once for all heads of a group.
+//
+// Each wave streams tiles of its own, without barriers: K and V rows are copied
+// to the wave's part of LDS (global_load_lds, two buffers), page ids two tiles
+// further ahead (four small buffers), so that between one and two tiles per
+// wave, 64 to 128 KB per CU, are always on their way.  Every vector memory
+// operation of the loop is such a copy, so the waits count them exactly.
+//
+// The products are transposed as in the 128-row kernel, with 16 x 16
+// accumulators: a lane owns query row lane & 15 of each block of 16 rows, and
+// its group g = lane >> 4 holds keys 16 b + 4 g .. + 3 of key block b, which is
+// again the weights' layout as a B operand.  int8 caches are copied as codes:
+// converted when read (V by a byte transpose read), the keys' scales multiply
+// the logits, the values' scales the weights.
+//
+// At the end the workgroup's waves are joined through LDS, in order, and the
+// splits of the keys over workgroups by the join kernel, in order.
+#pragma once
+
+#include "attn_mfma.h"
+
+namespace tkv {
+namespace attn {
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// Value rows of one transposed read: 16-bit, 8 rows x 32 bytes per half wave;
+// f32, rows 4 apart x 64 bytes; int8, 16 rows x 16 bytes per half wave.
+template <int CPR, int E>
+__device__ __forceinline__ int swz_few_v(int row) {
+    if constexpr (E == 4) return ((row >> 2) & 3) << 2;
+    else if constexpr (E == 2) {
+        if constexpr (CPR % 16 == 0) return (row & 7) << 1;
+        else if constexpr (CPR % 8 == 0) return ((row >> 1) & 3) << 1;
+        else return ((row >> 2) & 1) << 1;
+    } else {
+        if constexpr (CPR % 16 == 0) return (row & 7) | ((row >> 4) & 1) << 3;
+        else if constexpr (CPR % 8 == 0) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
+        else if constexpr (CPR % 4 == 0) return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
+        else return (row >> 2) & 1;
+    }
+}
+
+template <typename T, int DP, bool I8>
+struct FewShape {
+    static constexpr int E = I8 ? 1 : sizeof(T);             // bytes of a cached element
+    static constexpr int BN = 64 / E;                        // keys of a tile
+    static constexpr int TILE = 64 * DP;                     // bytes, K or V
+    static constexpr int CPR = DP * E / 16;
+    static constexpr int IDS = 4 * 256;
+    static constexpr int WAVE = 4 * TILE + IDS + (I8 ? 2 * 512 : 0);
+    // as many waves as two (up to DP = 128) or one workgroup per CU leave room for
+    static constexpr int NW = DP <= 64 ? 4 : DP <= 96 ? 3 : DP <= 128 ? 2 : DP <= 192 ? 3 : 2;
+    static constexpr int COPIES = 2 * TILE / 1024 + (I8 ? 2 : 0);  // memory operations of a tile
+};
+
+template <typename T, int DP, bool I8, int NB>
+__global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(AttnArgs a) {
+    using S = FewShape<T, DP, I8>;
+    using V8 = typename Vec<T>::type;
+    using C = typename std::conditional<I8, int8_t, T>::type;
+    constexpr bool F32 = sizeof(T) == 4, SCALED = I8 && std::is_same<T, _Float16>::value;
+    constexpr int BN = S::BN, CPR = S::CPR, NW = S::NW, ROWS = 16 * NB;
+    constexpr int CE = Vec<T>::N, QC = DP / (4 * CE);  // 16-byte chunks of a lane's query
+    constexpr int NKB = BN / 16, NDB = DP / 16;
+    constexpr float kInf = __builtin_inff();
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float2 row_ml[NW][ROWS];
+    __shared__ int row_bad[ROWS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int l15 = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % a.hkv, unit = blockIdx.x / a.hkv;
+    int first;
+    const int seq = tile_seq<true, ROWS>(a, unit, &first);
+    Seq s = seq_of<true>(a, seq);
+    s.q0 = uniform(s.q0), s.n = uniform(s.n), s.len = uniform(s.len);
+    const int rows = s.n * a.g, row0 = (unit - first) * ROWS;
+    if (row0 >= rows) return;
+    const int32_t* table = a.pages + seq * a.pages_st;
+    const int shift = s.len - s.n;
+    const int pos_lo = shift + (int)div_by(a.gdiv, row0);
+    const int pos_hi = shift + (int)div_by(a.gdiv, min(row0 + ROWS, rows) - 1);
+    const int kb = seen_begin(a, pos_lo), ke = seen_end(a, pos_hi, s.len);
+    const int f_begin = uniform(seen_begin(a, pos_hi)), f_end = uniform(seen_end(a, pos_lo, s.len));
+    int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
+    if (a.splits > 1) {
+        const int per = (t1 - t0 + a.splits - 1) / a.splits;
+        t0 = min(t0 + (int)blockIdx.y * per, t1);
+        t1 = min(t0 + per, t1);
+    }
+    t0 = uniform(t0), t1 = uniform(t1);
+
+    char* mem = lds + wave * S::WAVE;
+    int* ids = reinterpret_cast<int*>(mem + 4 * S::TILE);
+    float* scales = reinterpret_cast<float*>(mem + 4 * S::TILE + S::IDS);  // [2][K, V][64]
+    if (tid < ROWS) row_bad[tid] = 0;
+    if (a.d < DP) {
+        // the chunks past the head's end are never copied: zeros, as the queries there
+        for (int i = lane; i < 4 * S::TILE / 16; i += 64)
+            reinterpret_cast<u32x4*>(mem)[i] = u32x4{0, 0, 0, 0};
+        wait_lds();
+    }
+
+    const int count = t1 - t0 > wave ? (t1 - t0 - wave + NW - 1) / NW : 0;
+    const auto tile = [&](int k) { return t0 + wave + k * NW; };
+    const auto key_of = [&](int k) {  // this lane's key of the k-th tile; past the end the last one, masked
+        return min(min(tile(k), t1 - 1) * BN + (lane & (BN - 1)), s.len - 1);
+    };
+    const auto copy_ids = [&](int k) {
+        copy4_to_lds(table + div_by(a.page, (uint32_t)key_of(k)), uniform(lds_at(ids + 64 * (k & 3))));
+    };
+    const auto copy_tile = [&](int k) {
+        // pool row of this lane's key, handed to the lanes that copy its chunks
+        const uint32_t j = (uint32_t)key_of(k), pg = div_by(a.page, j);
+        uint32_t id = (uint32_t)ids[64 * (k & 3) + lane];
+        id = (int64_t)id < a.pool_pages ? id : 0;
+        const uint32_t my_row = (id * (uint32_t)a.hkv + kvh) * a.page.d + (j - pg * a.page.d);
+        const unsigned dst = uniform(lds_at(mem) + (k & 1) * 2 * S::TILE);
+        const int64_t row_bytes = (int64_t)a.d * S::E;
+#pragma unroll
+        for (int i = 0; i < S::TILE / 1024; i++) {
+            const int r = (i * 64 + lane) / CPR, c = (i * 64 + lane) % CPR;
+            const int64_t at = (int64_t)(uint32_t)__shfl((int)my_row, r) * row_bytes;
+            const int ck = c ^ swz_k<CPR>(r), cv = c ^ swz_few_v<CPR, S::E>(r);
+            if (ck * 16 < row_bytes) copy16_to_lds(static_cast<const char*>(a.k) + at + ck * 16, dst + i * 1024);
+            if (cv * 16 < row_bytes)
+                copy16_to_lds(static_cast<const char*>(a.v) + at + cv * 16, dst + S::TILE + i * 1024);
+        }
+        if constexpr (I8) {
+            const unsigned to = uniform(lds_at(scales + 128 * (k & 1)));
+            copy4_to_lds(a.ks + my_row, to);
+            copy4_to_lds(a.vs + my_row, to + 256);
+        }
+    };
+
+    if (count > 0) {
+        copy_ids(0);
+        copy_ids(1);
+    }
+    // queries, B operand: row l15, chunk 4 i + g
+    V8 q[NB][QC];
+    int my_begin[NB], my_end[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int row = row0 + 16 * b + l15;
+        const bool mine = row < rows;
+        const int tok = (int)div_by(a.gdiv, mine ? row : 0), h = kvh * a.g + (mine ? row : 0) - tok * a.g;
+        const T* qr = static_cast<const T*>(a.q) + (int64_t)(s.q0 + tok) * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < QC; i++) {
+            const int e = (4 * i + g) * CE;
+            q[b][i] = V8{};
+            if (mine && e < a.d) q[b][i] = *reinterpret_cast<const V8*>(qr + e);
+        }
+        my_begin[b] = seen_begin(a, shift + tok);
+        my_end[b] = mine ? seen_end(a, shift + tok, s.len) : 0;
+    }
+    if (count > 0) {
+        wait_vm();
+        copy_tile(0);
+        copy_ids(2);
+        if (count > 1) copy_tile(1);
+        copy_ids(3);
+    }
+
+    f32x4 o[NB][NDB];
+    float m[NB], l[NB], vexp[NB];  // SCALED: O is in units of vexp, 0 or a power of two
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        m[b] = -kInf, l[b] = 0.0f, vexp[b] = SCALED ? 0.0f : 1.0f;
+#pragma unroll
+        for (int n = 0; n < NDB; n++) o[b][n] = f32x4{};
+    }
+    const auto join_max = [](float x) {  // over the four key groups of a row
+        x = fmaxf(x, other_row(x));
+        return fmaxf(x, other_half(x));
+    };
+    const int k_swz = swz_k<CPR>(l15);  // rows 16 apart are swizzled alike
+    // value rows of a transposed read: 4 g + i of a block (and + 16)
+    const int v_row16 = 4 * g + (l15 >> 2), v_row8 = (l15 >> 1) < 4 ? 4 * g + (l15 >> 1) : 12 + 4 * g + (l15 >> 1);
+
+    for (int k = 0; k < count; k++) {
+        if (k + 1 < count) wait_vm_but<S::COPIES + 1>();  // all but the next tile and its ids' successor
+        else wait_vm();
+        const int j0 = tile(k) * BN;
+        const char* kt = mem + (k & 1) * 2 * S::TILE;
+        const char* vt = kt + S::TILE;
+        const float* sk = scales + 128 * (k & 1);
+        f32x4 x[NB][NKB];
+#pragma unroll
+        for (int b = 0; b < NKB; b++) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) x[n][b] = f32x4{};
+            const char* kr = kt + (b * 16 + l15) * (CPR * 16);
+#pragma unroll
+            for (int i = 0; i < QC; i++) {
+                V8 kf;
+                if constexpr (I8) {
+                    const int at = (4 * i + g) * CE;  // first element, CE bytes
+                    const char* p = kr + (((at >> 4) ^ k_swz) << 4) + (at & 15);
+                    if constexpr (F32) {
+                        const int w = *reinterpret_cast<const int*>(p);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) kf[j] = (float)(int8_t)(w >> (8 * j));
+                    } else {
+                        const i32x2 w = *reinterpret_cast<const i32x2*>(p);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) kf[j] = (T)(float)(int8_t)(w[j >> 2] >> (8 * (j & 3)));
+                    }
+                } else {
+                    kf = *reinterpret_cast<const V8*>(kr + (((4 * i + g) ^ k_swz) << 4));
+                }
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            x[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], q[n][i][j], x[n][b], 0, 0, 0);
+                    } else {
+                        x[n][b] = mfma16(kf, q[n][i], x[n][b]);
+                    }
+                }
+            }
+        }
+        const bool full = j0 >= f_begin && j0 + BN <= f_end;
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            float vs[I8 ? BN / 4 : 1];
+            float mx = -kInf;
+#pragma unroll
+            for (int b = 0; b < NKB; b++) {
+                if constexpr (I8) {
+                    const f32x4 ks4 = *reinterpret_cast<const f32x4*>(sk + b * 16 + 4 * g);
+                    const f32x4 vs4 = *reinterpret_cast<const f32x4*>(sk + 64 + b * 16 + 4 * g);
+                    x[n][b] *= ks4;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) vs[b * 4 + j] = vs4[j];
+                }
+                if (!full) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int key = j0 + b * 16 + 4 * g + j;
+                        const bool seen = key >= my_begin[n] && key < my_end[n];
+                        x[n][b][j] = seen ? x[n][b][j] : -kInf;
+                        if constexpr (I8) vs[b * 4 + j] = seen ? vs[b * 4 + j] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) mx = fmaxf(mx, x[n][b][j]);
+            }
+            mx = join_max(mx) * a.scale_log2;
+            // rescaled only once the maximum has grown by 2^8, as in the 128-row kernel
+            if (__any(mx > m[n] + 8.0f || (m[n] == -kInf && mx > -kInf))) {
+                const float mn = fmaxf(m[n], mx);
+                const float fix = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+                m[n] = mn;
+                l[n] *= fix;
+#pragma unroll
+                for (int d = 0; d < NDB; d++) o[n][d] *= fix;
+            }
+            const float base = m[n] == -kInf ? 0.0f : m[n];
+#pragma unroll
+            for (int b = 0; b < NKB; b++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[n][b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][b][j], a.scale_log2, -base));
+                    l[n] += x[n][b][j];
+                }
+            if constexpr (I8) {
+                if constexpr (SCALED) {
+                    // f16 weights times scales of any size: O is kept in units of
+                    // the largest scale's power of two so far
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < BN / 4; i++) top = fmaxf(top, vs[i]);
+                    top = join_max(top);
+                    const float unit2 = top > 0.0f && top < kInf
+                                            ? __builtin_ldexpf(1.0f, max(ilogbf(top), -100)) : 0.0f;
+                    if (__any(unit2 > vexp[n])) {
+                        const float nu = fmaxf(unit2, vexp[n]), fix = nu > 0.0f ? vexp[n] / nu : 1.0f;
+                        vexp[n] = nu;
+#pragma unroll
+                        for (int d = 0; d < NDB; d++) o[n][d] *= fix;
+                    }
+                    const float inv = vexp[n] > 0.0f ? 1.0f / vexp[n] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < BN / 4; i++) vs[i] *= inv;
+                }
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[n][b][j] *= vs[b * 4 + j];
+            }
+        }
+        // values: steps of 32 keys (blocks 2 st and 2 st + 1), f32 without codes one block
+        constexpr int STEP = F32 && !I8 ? 1 : 2;
+#pragma unroll
+        for (int st = 0; st < NKB / STEP; st++) {
+            V8 p[NB];
+            if constexpr (!F32) {
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) p[n][j] = (T)x[n][2 * st + (j >> 2)][j & 3];
+            }
+#pragma unroll
+            for (int d = 0; d < NDB; d++) {
+                if constexpr (I8) {
+                    const int r = st * 32 + v_row8;
+                    const char* at = vt + r * (CPR * 16) + ((d ^ swz_few_v<CPR, 1>(v_row8)) << 4) + ((lane & 1) << 3);
+                    typedef __attribute__((address_space(3))) i32x2* lds2;
+                    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)at);
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) y[j] = (float)(int8_t)(w[j >> 2] >> (8 * (j & 3)));
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                o[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    y[j], x[n][2 * st + (j >> 2)][j & 3], o[n][d], 0, 0, 0);
+                    } else {
+                        V8 v;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[j] = (T)y[j];
+#pragma unroll
+                        for (int n = 0; n < NB; n++) o[n][d] = mfma16(v, p[n], o[n][d]);
+                    }
+                } else if constexpr (F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int r = st * 16 + 4 * g + j, col = d * 16 + l15;
+                        const float v = *reinterpret_cast<const float*>(
+                            vt + r * (CPR * 16) + (((col >> 2) ^ swz_few_v<CPR, 4>(4 * g)) << 4) + ((col & 3) << 2));
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+                            o[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[n][st][j], o[n][d], 0, 0, 0);
+                    }
+                } else {
+                    const int c = d * 2 + ((l15 & 3) >> 1);
+                    const char* at = vt + (st * 32 + v_row16) * (CPR * 16) +
+                                     ((c ^ swz_few_v<CPR, 2>(v_row16)) << 4) + ((lane & 1) << 3);
+                    typedef __attribute__((address_space(3))) s16x4* lds4;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 16 * (CPR * 16)));
+                    typedef short s16x8 __attribute__((ext_vector_type(8)));
+                    const V8 v = __builtin_bit_cast(V8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int n = 0; n < NB; n++) o[n][d] = mfma16(v, p[n], o[n][d]);
+                }
+            }
+        }
+        wait_lds();  // this tile is read: its buffer is free
+        if (k + 2 < count) copy_tile(k + 2);
+        copy_ids(k + 4);
+    }
+    wait_vm();
+
+    // the waves' sums, joined in their order: rows of DP f32 per wave in LDS
+    barrier();
+    float* sums = reinterpret_cast<float*>(lds) + wave * ROWS * DP;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        l[n] += other_row(l[n]);
+        l[n] += other_half(l[n]);
+        // what a masked key's values left behind: such rows are computed again,
+        // as in the 128-row kernel
+        bool bad = !(fabsf(l[n]) < kInf);
+#pragma unroll
+        for (int d = 0; d < NDB; d++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) bad |= !(fabsf(o[n][d][j]) < kInf);
+            *reinterpret_cast<f32x4*>(sums + (n * 16 + l15) * DP + d * 16 + 4 * g) = o[n][d] * vexp[n];
+        }
+        if (bad) row_bad[n * 16 + l15] = 1;
+        if (g == 0) row_ml[wave][n * 16 + l15] = make_float2(m[n], l[n]);
+    }
+    barrier();
+    const bool split = a.splits > 1;
+    const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
+    for (int i = tid; i < ROWS * (DP / 4); i += 64 * NW) {
+        const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
+        if (row >= rows || e >= a.d || row_bad[r]) continue;
+        float mm = -kInf;
+#pragma unroll
+        for (int w = 0; w < NW; w++) mm = fmaxf(mm, row_ml[w][r].x);
+        const float base = mm == -kInf ? 0.0f : mm;
+        float ll = 0.0f;
+        f32x4 y = {};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(row_ml[w][r].x - base);
+            ll = __builtin_fmaf(f, row_ml[w][r].y, ll);
+            y += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * ROWS + r) * DP + e);
+        }
+        const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+        const int64_t t_at = s.q0 + tok;
+        if (split) {
+            if (e == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
+            *reinterpret_cast<f32x4*>(a.part_o + ((part + t_at) * a.hq + h) * a.d + e) = y;
+        } else {
+            y *= ll == 0.0f ? 1.0f : 1.0f / ll;
+            const int64_t at = t_at * a.o_st + (int64_t)h * a.o_sh + e;
+            if (a.out_f32) {
+                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
+            } else {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                T4 z;
+#pragma unroll
+                for (int j = 0; j < 4; j++) z[j] = (T)y[j];
+                *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = z;
+            }
+        }
+    }
+    for (int r = wave; r < ROWS; r += NW) {
+        const int row = row0 + r;
+        if (row >= rows || !uniform(row_bad[r])) continue;
+        const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+        const int64_t t_at = s.q0 + tok;
+        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
+        float mm, ll, acc[4];
+        attend_row<T, C, true>(a, s, table, kvh, qr, max(seen_begin(a, shift + tok), t0 * BN),
+                               min(seen_end(a, shift + tok, s.len), t1 * BN), &mm, &ll, acc);
+        if (split && lane == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
+        for (int e = 0; e < 4; e++) {
+            const int x = lane + 64 * e;
+            if (x >= a.d) continue;
+            const float y = split || ll == 0.0f ? acc[e] : acc[e] / ll;
+            if (split) a.part_o[((part + t_at) * a.hq + h) * a.d + x] = y;
+            else if (a.out_f32) static_cast<float*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = y;
+            else static_cast<T*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = from_f32<T>(y);
+        }
+    }
+}
+
+template <typename T, int DP, bool I8>
+int launch_few_dp(Ctx* c, const AttnArgs& a, int blocks_of_16) {
+    using S = FewShape<T, DP, I8>;
+    constexpr int LDS = S::NW * S::WAVE;
+    static_assert(LDS <= 163840 - 4096 && S::NW * 32 * DP * 4 <= LDS, "LDS of a workgroup");
+    if ((size_t)LDS + 4096 > c->max_lds) return set_error(TKV_HIP_UNSUPPORTED, "attention: not enough LDS");
+    const int64_t blocks = (int64_t)a.units * a.hkv;
+    if (blocks >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
+    const dim3 grid((unsigned)blocks, (unsigned)a.splits);
+    if (blocks_of_16 == 1) k_attn_few<T, DP, I8, 1><<<grid, 64 * S::NW, LDS, c->stream>>>(a);
+    else k_attn_few<T, DP, I8, 2><<<grid, 64 * S::NW, LDS, c->stream>>>(a);
+    TKV_LAUNCH_CHECK();
+    return TKV_HIP_OK;
+}
+
+template <typename T, bool I8>
+int launch_few_kv(Ctx* c, const AttnArgs& a, int blocks_of_16) {
+    if (a.d <= 64) return launch_few_dp<T, 64, I8>(c, a, blocks_of_16);
+    if constexpr (sizeof(T) == 2)
+        if (a.d <= 96) return launch_few_dp<T, 96, I8>(c, a, blocks_of_16);
+    if (a.d <= 128) return launch_few_dp<T, 128, I8>(c, a, blocks_of_16);
+    if (a.d <= 192) return launch_few_dp<T, 192, I8>(c, a, blocks_of_16);
+    return launch_few_dp<T, 256, I8>(c, a, blocks_of_16);
+}
+
+template <typename T>
+int launch_few(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16) {
+    return i8 ? launch_few_kv<T, true>(c, a, blocks_of_16) : launch_few_kv<T, false>(c, a, blocks_of_16);
+}
+
+}  // namespace attn
+}  // namespace tkv

@@ -1,0 +1,10 @@
+// attn_few_bf16.hip -- the matrix kernels of attn_few.h for bf16.
+#include "attn_few.h"
+
+namespace tkv {
+
+int launch_attn_few_bf16(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16) {
+    return attn::launch_few<__bf16>(c, a, i8, blocks_of_16);
+}
+
+}  // namespace tkv

@@ -21,76 +21,11 @@
 // same registers as they are.
 #pragma once
 
-#include "attn.h"
+#include "attn_mfma.h"
 
 namespace tkv {
 namespace attn {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* lds_void;
-
-template <typename T>
-struct Vec {  // 16 bytes
-    static constexpr int N = 16 / sizeof(T);
-    typedef T type __attribute__((ext_vector_type(N)));
-};
-
-__device__ __forceinline__ f32x16 mfma32(Vec<__bf16>::type a, Vec<__bf16>::type b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma32(Vec<_Float16>::type a, Vec<_Float16>::type b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// 16 bytes per lane from global memory to LDS at `dst` (wave-uniform) + 16 lane.
-// In asm, since the compiler would put a wait for every copy in flight before
-// each LDS read it cannot tell apart from the copy's destination; the waits
-// here are the callers' own (wait_vm below, before a barrier).  No register is
-// written; the s_nop is the wait state between a scalar write of m0 and the
-// copy that uses it.
-__device__ __forceinline__ void copy16_to_lds(const void* src, unsigned dst) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                 :
-                 : "v"(src), "s"(dst)
-                 : "memory");
-}
-__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-__device__ __forceinline__ unsigned lds_at(const void* p) {
-    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// The other half's value: lanes l and l + 32 exchange.
-__device__ __forceinline__ float other_half(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
-}
-
-// LDS rows of CPR 16-byte chunks.  Key rows are read 16 lanes = 16 rows at one
-// chunk at a time: the chunk is XORed so that the 16 land in different banks.
-template <int CPR>
-__device__ __forceinline__ int swz_k(int row) {
-    if constexpr (CPR % 16 == 0) return row & 15;
-    else if constexpr (CPR % 8 == 0) return (row >> 1) & 7;
-    else return (row >> 2) & 3;
-}
-// Value rows are read four rows (16-bit types; two rows 4 apart for f32) at a
-// 64-byte (128-byte) window at a time: the window is XORed.
-template <int CPR, int SIZE>
-__device__ __forceinline__ int swz_v(int row) {
-    if constexpr (SIZE == 4) return CPR % 16 == 0 ? ((row >> 2) & 1) << 3 : 0;
-    else if constexpr (CPR % 16 == 0) return (row & 3) << 2;
-    else if constexpr (CPR % 8 == 0) return ((row >> 1) & 1) << 2;
-    else return 0;
-}
-
-enum { KV_PACKED = 0, KV_PAGED = 1, KV_I8 = 2 };
 
 // DP: head size, padded (64, 96, 128, 192, 256; f32 96 only as 128).
 template <typename T, int DP>
@@ -105,32 +40,6 @@ struct TileShape {
     static_assert(BN * CPR % NT == 0, "chunks per thread");
     static constexpr int LDS = 4 * TILE + 4 * BN * 4;           // two buffers of K and V, scales
 };
-
-// Sequence and tile of a unit.  Sequence i's tiles begin at
-// floor(cu[i] g / 128) + i, which leaves each sequence room for all of its
-// tiles (and up to one unit without rows).  Lanes look at 64 sequences at a
-// time: the last one that begins at or before the unit.
-template <bool PAGED>
-__device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first) {
-    const int lane = threadIdx.x & 63;
-    int found = 0, begin = 0;
-    for (int b = 0; b < a.seqs; b += 64) {
-        const int i = b + lane;
-        int at = 0x7fffffff;
-        if (i < a.seqs) {
-            const int q0 = (PAGED && !a.cu_q) ? i : clamp_to(a.cu_q[i], a.tokens);
-            at = (int)((int64_t)q0 * a.g / kTileRows) + i;
-        }
-        const unsigned long long before = __ballot(at <= unit);
-        if (!before) break;
-        const int last = 63 - __builtin_clzll(before);
-        found = b + last;
-        begin = __shfl(at, last);
-        if (last < 63) break;
-    }
-    *first = uniform(begin);
-    return uniform(found);
-}
 
 template <typename T, int DP, int KV>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_attn_tile(AttnArgs a) {
@@ -151,7 +60,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
     const int kvh = blockIdx.x % a.hkv;
     const int unit = a.units - 1 - (int)(blockIdx.x / a.hkv);
     int first;
-    const int seq = tile_seq<PAGED>(a, unit, &first);
+    const int seq = tile_seq<PAGED, kTileRows>(a, unit, &first);
     Seq s = seq_of<PAGED>(a, seq);
     s.q0 = uniform(s.q0), s.n = uniform(s.n), s.len = uniform(s.len);
     const int rows = s.n * a.g;

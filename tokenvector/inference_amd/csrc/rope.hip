@@ -236,8 +236,9 @@ int32_t tkv_hip_kv_create(int64_t ctx, int32_t type, int64_t num_pages, int64_t 
         return set_error(TKV_HIP_BAD_ARG, "kv_create: sizes out of range or NULL output");
     if (!i8 && !float_type(type)) return set_error(TKV_HIP_BAD_ARG, "kv_create: unknown type");
     if (page_size >= (1ll << 31) || num_pages >= (1ll << 31) ||
-        num_pages * page_size >= (1ll << 31))
-        return set_error(TKV_HIP_BAD_ARG, "kv_create: num_pages * page_size >= 2^31");
+        num_pages * page_size >= (1ll << 31) || num_pages * page_size * heads >= (1ll << 32))
+        return set_error(TKV_HIP_BAD_ARG,
+                         "kv_create: num_pages * page_size >= 2^31, or 2^32 with the heads");
     if (!!k != !!v || (k && i8) != !!k_scales || (k && i8) != !!v_scales)
         return set_error(TKV_HIP_BAD_ARG,
                          "kv_create: give both pools or none, and scales with int8 pools only");
