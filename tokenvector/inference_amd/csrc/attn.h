@@ -72,11 +72,13 @@ struct AttnArgs {
     int64_t window;    // 0: none
     float scale_log2;  // scale * log2(e) > 0: weights are exp2(s * scale_log2 - m)
     int32_t out_f32;
-    // split over the keys: sums [splits][tokens][hq][d] and (m, l) of each
     FastDiv gdiv;      // g
+    // split over the keys: sums [splits][tokens][hq][d] and (m, l) of each, and
+    // the arrival counts [units][hkv]
     int32_t splits, units;
     float* part_o;
     float2* part_ml;
+    unsigned* arrivals;
 };
 
 // The rows of sequence i, clamped to what there is.
@@ -135,13 +137,6 @@ __device__ __forceinline__ int seq_at(const AttnArgs& a, int64_t row) {
     }
     return lo;
 }
-__device__ __forceinline__ bool covered(const AttnArgs& a, int64_t row) {
-    if (!a.cu_q) return true;
-    const int i = seq_at(a, row);
-    const int q0 = clamp_to(a.cu_q[i], a.tokens);
-    return row >= q0 && row < clamp_to(a.cu_q[i + 1], a.tokens);
-}
-
 // Element offset of key (or value) row j of a sequence; *srow, where paged, the
 // row of its scale.
 template <bool PAGED>

@@ -52,41 +52,6 @@ static void common_args(AttnArgs* a, int32_t type, int32_t type_out, int64_t tok
     a->out_f32 = type_out == TKV_HIP_F32;
 }
 
-// Joins the splits of a query row and head: O = sum_s 2^(m_s - m) O_s / sum_s
-// 2^(m_s - m) l_s, in the order of the splits.  One wave per row and head; reads
-// d + 2 floats per split.
-template <typename T>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t rows = a.tokens * a.hq;
-    if (unit >= rows) return;
-    const int64_t row = unit / a.hq;
-    const int h = (int)(unit - row * a.hq);
-    if (!covered(a, row)) return;  // its partial sums were not written either
-    float m = -__builtin_inff();
-    for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.part_ml[s * rows + unit].x);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; s++) {
-        const float2 ml = a.part_ml[s * rows + unit];
-        const float w = __builtin_amdgcn_exp2f(ml.x - base);
-        l = fmaf(w, ml.y, l);
-        const float* po = a.part_o + (s * rows + unit) * a.d;
-        if (w != 0.0f)
-            for (int e = 0; e < 4; e++)
-                if (lane + 64 * e < a.d) acc[e] = fmaf(w, po[lane + 64 * e], acc[e]);
-    }
-    const int64_t at = row * a.o_st + h * a.o_sh;
-    for (int e = 0; e < 4; e++) {
-        const int x = lane + 64 * e;
-        if (x >= a.d) continue;
-        const float y = l == 0.0f ? 0.0f : acc[e] / l;
-        if (a.out_f32) static_cast<float*>(a.out)[at + x] = y;
-        else static_cast<T*>(a.out)[at + x] = from_f32<T>(y);
-    }
-}
-
 static bool rows_of_16(const void* p, int64_t st, int64_t sh, int64_t bytes) {
     return aligned(p, 16) && st * bytes % 16 == 0 && sh * bytes % 16 == 0;
 }
@@ -111,18 +76,14 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     if (units >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     a.units = (int32_t)units;
     const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs) * a.hkv;
-    int64_t want;
-    if (few) {
-        // streaming: four rounds of the workgroups that fit, so that caches of
-        // different lengths even out
-        const int64_t slots = (a.d <= 128 ? 2 : 1) * c->num_cus;
-        want = std::min<int64_t>(4 * slots / tiles, keys / 256);
-    } else {
-        // too few tiles for two workgroups per CU: the keys are split, 256 of
-        // them at least to a split
-        want = std::min<int64_t>(2 * c->num_cus / tiles, keys / 256);
-    }
-    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), 128);
+    // Splits over the keys.  Streaming: four rounds of the workgroups that fit, so
+    // that caches of different lengths even out, 128 keys at least to a split.
+    // 128-row tiles: two workgroups per CU, 256 keys at least.
+    const int64_t slots = (!few || a.d <= 128 ? 2 : 1) * c->num_cus;
+    const int64_t want = std::min<int64_t>((few ? 4 : 1) * slots / tiles, keys / (few ? 128 : 256));
+    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kArriveFlat);
+    if (units * a.hkv > kAttnCounters) a.splits = 1;
+    a.arrivals = c->attn_arrivals;
     if (a.splits > 1) {
         const int64_t rows = a.tokens * a.hq * a.splits;
         void* ws;
@@ -143,13 +104,6 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
         TKV_RC_TRY(type == TKV_HIP_F32   ? launch_attn_tile_f32(c, a, i8)
                    : type == TKV_HIP_F16 ? launch_attn_tile_f16(c, a, i8)
                                          : launch_attn_tile_bf16(c, a, i8));
-    if (a.splits > 1) {
-        const dim3 grid((unsigned)ceil_div(a.tokens * a.hq, 4));
-        if (type == TKV_HIP_F32) k_attn_join<float><<<grid, 256, 0, c->stream>>>(a);
-        else if (type == TKV_HIP_F16) k_attn_join<_Float16><<<grid, 256, 0, c->stream>>>(a);
-        else k_attn_join<__bf16><<<grid, 256, 0, c->stream>>>(a);
-        TKV_LAUNCH_CHECK();
-    }
     return TKV_HIP_OK;
 }
 

@@ -16,7 +16,7 @@
 // the logits, the values' scales the weights.
 //
 // At the end the workgroup's waves are joined through LDS, in order, and the
-// splits of the keys over workgroups by the join kernel, in order.
+// splits of the keys over workgroups by the unit's last workgroup, in order.
 #pragma once
 
 #include "attn_mfma.h"
@@ -86,11 +86,14 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     const int kb = seen_begin(a, pos_lo), ke = seen_end(a, pos_hi, s.len);
     const int f_begin = uniform(seen_begin(a, pos_hi)), f_end = uniform(seen_end(a, pos_lo, s.len));
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
-    if (a.splits > 1) {
+    int splits = 1;  // that have tiles
+    if (a.splits > 1 && t1 > t0) {
         const int per = (t1 - t0 + a.splits - 1) / a.splits;
-        t0 = min(t0 + (int)blockIdx.y * per, t1);
+        splits = (t1 - t0 + per - 1) / per;
+        t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
     }
+    if ((int)blockIdx.y >= splits) return;
     t0 = uniform(t0), t1 = uniform(t1);
 
     char* mem = lds + wave * S::WAVE;
@@ -380,7 +383,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         if (g == 0) row_ml[wave][n * 16 + l15] = make_float2(m[n], l[n]);
     }
     barrier();
-    const bool split = a.splits > 1;
+    const bool split = splits > 1;
     const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
     for (int i = tid; i < ROWS * (DP / 4); i += 64 * NW) {
         const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
@@ -400,40 +403,25 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
         const int64_t t_at = s.q0 + tok;
         if (split) {
-            if (e == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
-            *reinterpret_cast<f32x4*>(a.part_o + ((part + t_at) * a.hq + h) * a.d + e) = y;
+            const int64_t p_at = (part + t_at) * a.hq + h;
+            if (e == 0) put_part_ml(a.part_ml + p_at, mm, ll);
+            put_part4(a.part_o + p_at * a.d + e, y);
         } else {
-            y *= ll == 0.0f ? 1.0f : 1.0f / ll;
-            const int64_t at = t_at * a.o_st + (int64_t)h * a.o_sh + e;
-            if (a.out_f32) {
-                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
-            } else {
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                T4 z;
-#pragma unroll
-                for (int j = 0; j < 4; j++) z[j] = (T)y[j];
-                *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = z;
-            }
+            put_out4<T>(a, t_at, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
         }
     }
     for (int r = wave; r < ROWS; r += NW) {
         const int row = row0 + r;
         if (row >= rows || !uniform(row_bad[r])) continue;
         const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
-        const int64_t t_at = s.q0 + tok;
-        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
-        float mm, ll, acc[4];
-        attend_row<T, C, true>(a, s, table, kvh, qr, max(seen_begin(a, shift + tok), t0 * BN),
-                               min(seen_end(a, shift + tok, s.len), t1 * BN), &mm, &ll, acc);
-        if (split && lane == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
-        for (int e = 0; e < 4; e++) {
-            const int x = lane + 64 * e;
-            if (x >= a.d) continue;
-            const float y = split || ll == 0.0f ? acc[e] : acc[e] / ll;
-            if (split) a.part_o[((part + t_at) * a.hq + h) * a.d + x] = y;
-            else if (a.out_f32) static_cast<float*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = y;
-            else static_cast<T*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = from_f32<T>(y);
-        }
+        row_again<T, C, true>(a, s, table, kvh, tok, h, max(seen_begin(a, shift + tok), t0 * BN),
+                              min(seen_end(a, shift + tok, s.len), t1 * BN), split);
+    }
+    if (split) {
+        unsigned* counter = a.arrivals + blockIdx.x;
+        if (!arrive_last(counter, splits)) return;
+        join_splits<T>(a, s, kvh, row0, min(rows - row0, ROWS), splits);
+        arrive_clear(counter, splits);
     }
 }
 

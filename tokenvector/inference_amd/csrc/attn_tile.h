@@ -87,12 +87,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
 
     // tiles of this split
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
-    if (a.splits > 1) {
+    int splits = 1;  // that have tiles
+    if (a.splits > 1 && t1 > t0) {
         const int per = (t1 - t0 + a.splits - 1) / a.splits;
-        t0 = min(t0 + (int)blockIdx.y * per, t1);
+        splits = (t1 - t0 + per - 1) / per;
+        t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
     }
+    if ((int)blockIdx.y >= splits) return;
     t0 = uniform(t0), t1 = uniform(t1);
+    const bool split = splits > 1;
 
     // queries: element order of a B operand, chunk 2 i + half of the row
     V8 q[CPR / 2];
@@ -367,7 +371,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
         if (t + 1 < t1) put_codes(buf ^ 1);
     }
     l += other_half(l);
-    if (!live) return;
 
     // A value that no row of a wave's tile may see still meets a weight of zero
     // in the product; where that left something that is not finite, those rows
@@ -377,31 +380,30 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
     for (int b = 0; b < NDB; b++)
 #pragma unroll
         for (int e = 0; e < 16; e++) bad |= !(fabsf(o[b][e]) < kInf);
-    unsigned long long ball = __ballot(bad && mine);
+    const unsigned long long ball = __ballot(bad && mine);
     unsigned again = uniform((unsigned)ball | (unsigned)(ball >> 32));
-    const bool split = a.splits > 1;
     const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
 
     if (mine && !((again >> l31) & 1)) {
         const int64_t t_at = s.q0 + tok;
         const float scale = (split || l == 0.0f ? 1.0f : 1.0f / l) * vexp;
-        if (split && half == 0) a.part_ml[(part + t_at) * a.hq + head] = make_float2(m, l);
-        float* po = a.part_o + ((part + t_at) * a.hq + head) * a.d;
-        char* out = static_cast<char*>(a.out) +
-                    (t_at * a.o_st + (int64_t)head * a.o_sh) * (a.out_f32 ? 4 : sizeof(T));
+        const int64_t p_at = (part + t_at) * a.hq + head;
+        if (split && half == 0) put_part_ml(a.part_ml + p_at, m, l);
 #pragma unroll
         for (int b = 0; b < NDB; b++) {
-            if (split || a.out_f32) {
-                float* to = split ? po : reinterpret_cast<float*>(out);
+            if (F32 || split || a.out_f32) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int e = b * 32 + 8 * i + 4 * half;
                     const f32x4 y = {o[b][4 * i] * scale, o[b][4 * i + 1] * scale, o[b][4 * i + 2] * scale,
                                      o[b][4 * i + 3] * scale};
-                    if (e < a.d) *reinterpret_cast<f32x4*>(to + e) = y;
+                    if (e >= a.d) continue;
+                    if (split) put_part4(a.part_o + p_at * a.d + e, y);
+                    else put_out4<float>(a, t_at, head, e, y);
                 }
             } else if constexpr (!F32) {
                 // halves exchange groups of four: 8 elements, 16 bytes, per store
+                T* out = static_cast<T*>(a.out) + t_at * a.o_st + (int64_t)head * a.o_sh;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     T y[8];
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
                     const auto sx = __builtin_amdgcn_permlane32_swap(lo.x, hi.x, false, false);
                     const auto sy = __builtin_amdgcn_permlane32_swap(lo.y, hi.y, false, false);
                     const int e = b * 32 + 16 * i + 8 * half;
-                    if (e < a.d) *reinterpret_cast<u32x4*>(out + e * 2) = u32x4{sx[0], sy[0], sx[1], sy[1]};
+                    if (e < a.d) *reinterpret_cast<u32x4*>(out + e) = u32x4{sx[0], sy[0], sx[1], sy[1]};
                 }
             }
         }
@@ -422,20 +424,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
         const int i = __builtin_ctz(again);
         again &= again - 1;
         const int r = wrow + i, tk = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tk * a.g;
-        const int64_t t_at = s.q0 + tk;
-        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
-        float mm, ll, acc[4];
-        attend_row<T, C, PAGED>(a, s, table, kvh, qr, max(seen_begin(a, shift + tk), t0 * BN),
-                                min(seen_end(a, shift + tk, s.len), t1 * BN), &mm, &ll, acc);
-        if (split && lane == 0) a.part_ml[(part + t_at) * a.hq + h] = make_float2(mm, ll);
-        for (int e = 0; e < 4; e++) {
-            const int x = lane + 64 * e;
-            if (x >= a.d) continue;
-            const float y = split || ll == 0.0f ? acc[e] : acc[e] / ll;
-            if (split) a.part_o[((part + t_at) * a.hq + h) * a.d + x] = y;
-            else if (a.out_f32) static_cast<float*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = y;
-            else static_cast<T*>(a.out)[t_at * a.o_st + h * a.o_sh + x] = from_f32<T>(y);
-        }
+        row_again<T, C, PAGED>(a, s, table, kvh, tk, h, max(seen_begin(a, shift + tk), t0 * BN),
+                               min(seen_end(a, shift + tk, s.len), t1 * BN), split);
+    }
+    if (split) {
+        unsigned* counter = a.arrivals + blockIdx.x;
+        if (!arrive_last(counter, splits)) return;
+        join_splits<T>(a, s, kvh, row0, min(rows - row0, kTileRows), splits);
+        arrive_clear(counter, splits);
     }
 }
 

@@ -76,7 +76,7 @@ int ctx_create(int device, Ctx** out) {
     size_t red_bytes = sizeof(RedPartial) * kMaxReduceBlocks + 256 + sizeof(tkv_hip_qparams_dev) * 64 +
                        256 + gemv_bytes + (size_t)kGemvSplitBlocks * sizeof(unsigned) + 256 +
                        (size_t)kMaxGridSlots * 8 + (size_t)kCalHistBins * 8 +
-                       (size_t)kCalCounters * kArriveWords * sizeof(unsigned);
+                       (size_t)(kCalCounters * kArriveWords + kAttnCounters) * sizeof(unsigned);
     void* red = nullptr;
     e = hipMalloc(&red, red_bytes);
     if (e != hipSuccess) {
@@ -95,6 +95,7 @@ int ctx_create(int device, Ctx** out) {
     }
     c->cal_hist = c->grid_slots + kMaxGridSlots;
     c->cal_arrivals = reinterpret_cast<unsigned*>(c->cal_hist + kCalHistBins);
+    c->attn_arrivals = c->cal_arrivals + kCalCounters * kArriveWords;
     // One-time zeroing at creation, so params read before any calibration
     // are defined (never inside a caller's stream capture).
     e = hipMemset(red, 0, red_bytes);

@@ -60,6 +60,8 @@ constexpr unsigned kArriveGroups = 16;
 constexpr unsigned kArriveStride = 64;
 constexpr unsigned kArriveFlat = 64;  // up to so many workgroups use the first word alone
 constexpr unsigned kArriveWords = (1 + kArriveGroups) * kArriveStride;
+// Arrival counts of the attention's splits: one per unit of rows and key / value head.
+constexpr int kAttnCounters = 4096;
 constexpr int64_t kCalHistBins = 4096;  // the largest KL histogram
 
 struct Graph;
@@ -96,6 +98,9 @@ struct Ctx {
     // Contexts that do not run the calibrators leave them null.
     unsigned long long* cal_hist = nullptr;
     unsigned* cal_arrivals = nullptr;
+    // kAttnCounters arrival counts, zero at creation; the last workgroup of a
+    // unit clears its own.  Null as above.
+    unsigned* attn_arrivals = nullptr;
     // grow-only workspaces
     // 10, 11: f16-decoded FP8 operands; 12: INT4 split-K partials (any kernel);
     // 13, 14, 15: INT4 digit planes, retiled weight codes, permuted activations
