@@ -76,11 +76,14 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     if (units >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     a.units = (int32_t)units;
     const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs) * a.hkv;
-    // Splits over the keys.  Streaming: four rounds of the workgroups that fit, so
-    // that caches of different lengths even out, 128 keys at least to a split.
-    // 128-row tiles: two workgroups per CU, 256 keys at least.
-    const int64_t slots = (!few || a.d <= 128 ? 2 : 1) * c->num_cus;
-    const int64_t want = std::min<int64_t>((few ? 4 : 1) * slots / tiles, keys / (few ? 128 : 256));
+    // Splits over the keys: as many as fill the chip once, 128 keys (streaming) or
+    // 256 (tiles) at least to each.  Streaming, up to four times as many where each
+    // still has 512 KB to read, so that caches of different lengths even out: a
+    // workgroup's start and end take as long as reading about 100 KB.
+    const int64_t slots = 2 * c->num_cus;
+    int64_t want = std::min<int64_t>(slots / tiles, keys / (few ? 128 : 256));
+    if (few)
+        want = std::max(want, std::min<int64_t>(4 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
     a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kArriveFlat);
     if (units * a.hkv > kAttnCounters) a.splits = 1;
     a.arrivals = c->attn_arrivals;

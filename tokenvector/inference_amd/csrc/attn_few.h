@@ -5,7 +5,8 @@
 // Each wave streams tiles of its own, without barriers: K and V rows are copied
 // to the wave's part of LDS (global_load_lds, two buffers), page ids two tiles
 // further ahead (four small buffers), so that between one and two tiles per
-// wave, 64 to 128 KB per CU, are always on their way.  Every vector memory
+// wave, 64 to 128 KB per CU, are always on their way.  Tiles are small, so that
+// two workgroups fit a CU and one's start and end run beside the other's stream.  Every vector memory
 // operation of the loop is such a copy, so the waits count them exactly.
 //
 // The products are transposed as in the 128-row kernel, with 16 x 16
@@ -46,13 +47,15 @@ __device__ __forceinline__ int swz_few_v(int row) {
 template <typename T, int DP, bool I8>
 struct FewShape {
     static constexpr int E = I8 ? 1 : sizeof(T);             // bytes of a cached element
-    static constexpr int BN = 64 / E;                        // keys of a tile
-    static constexpr int TILE = 64 * DP;                     // bytes, K or V
+    // keys of a tile: 4 to 8 KB of K and of V (f32 to 16 KB)
+    static constexpr int BN = E == 4 ? 16 : (DP <= 96 ? 64 : 32) / E;
+    static constexpr int TILE = BN * DP * E;                 // bytes, K or V
     static constexpr int CPR = DP * E / 16;
     static constexpr int IDS = 4 * 256;
     static constexpr int WAVE = 4 * TILE + IDS + (I8 ? 2 * 512 : 0);
-    // as many waves as two (up to DP = 128) or one workgroup per CU leave room for
-    static constexpr int NW = DP <= 64 ? 4 : DP <= 96 ? 3 : DP <= 128 ? 2 : DP <= 192 ? 3 : 2;
+    // as many waves, up to four, as let two workgroups share a CU's LDS
+    static constexpr int FIT = 80 * 1024 / WAVE;
+    static constexpr int NW = FIT < 1 ? 1 : FIT > 4 ? 4 : FIT;
     static constexpr int COPIES = 2 * TILE / 1024 + (I8 ? 2 : 0);  // memory operations of a tile
 };
 
@@ -298,16 +301,17 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                     for (int j = 0; j < 4; j++) x[n][b][j] *= vs[b * 4 + j];
             }
         }
-        // values: steps of 32 keys (blocks 2 st and 2 st + 1), f32 without codes one block
-        constexpr int STEP = F32 && !I8 ? 1 : 2;
+        // values: steps of 32 keys (blocks 2 st and 2 st + 1) or of 16
+        constexpr int STEP = NKB == 1 ? 1 : 2;
 #pragma unroll
         for (int st = 0; st < NKB / STEP; st++) {
-            V8 p[NB];
+            typedef T P __attribute__((ext_vector_type(4 * STEP)));
+            P p[NB];
             if constexpr (!F32) {
 #pragma unroll
                 for (int n = 0; n < NB; n++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) p[n][j] = (T)x[n][2 * st + (j >> 2)][j & 3];
+                    for (int j = 0; j < 4 * STEP; j++) p[n][j] = (T)x[n][STEP * st + (j >> 2)][j & 3];
             }
 #pragma unroll
             for (int d = 0; d < NDB; d++) {
@@ -336,6 +340,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                 } else if constexpr (F32) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
+                        static_assert(STEP == 1 || !F32 || I8, "f32 tiles are one block");
                         const int r = st * 16 + 4 * g + j, col = d * 16 + l15;
                         const float v = *reinterpret_cast<const float*>(
                             vt + r * (CPR * 16) + (((col >> 2) ^ swz_few_v<CPR, 4>(4 * g)) << 4) + ((col & 3) << 2));
@@ -345,15 +350,22 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                     }
                 } else {
                     const int c = d * 2 + ((l15 & 3) >> 1);
-                    const char* at = vt + (st * 32 + v_row16) * (CPR * 16) +
+                    const char* at = vt + (st * 16 * STEP + v_row16) * (CPR * 16) +
                                      ((c ^ swz_few_v<CPR, 2>(v_row16)) << 4) + ((lane & 1) << 3);
                     typedef __attribute__((address_space(3))) s16x4* lds4;
                     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                    if constexpr (STEP == 1) {
+#pragma unroll
+                        for (int n = 0; n < NB; n++) o[n][d] = mfma16(__builtin_bit_cast(P, lo), p[n], o[n][d]);
+                        continue;
+                    }
                     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 16 * (CPR * 16)));
                     typedef short s16x8 __attribute__((ext_vector_type(8)));
                     const V8 v = __builtin_bit_cast(V8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    if constexpr (STEP == 2) {
 #pragma unroll
-                    for (int n = 0; n < NB; n++) o[n][d] = mfma16(v, p[n], o[n][d]);
+                        for (int n = 0; n < NB; n++) o[n][d] = mfma16(v, p[n], o[n][d]);
+                    }
                 }
             }
         }

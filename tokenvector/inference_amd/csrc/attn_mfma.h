@@ -10,6 +10,8 @@ namespace attn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_void;
@@ -25,6 +27,13 @@ __device__ __forceinline__ f32x4 mfma16(Vec<__bf16>::type a, Vec<__bf16>::type b
 }
 __device__ __forceinline__ f32x4 mfma16(Vec<_Float16>::type a, Vec<_Float16>::type b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16x4 a, bf16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                                                     __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(f16x4 a, f16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x16 mfma32(Vec<__bf16>::type a, Vec<__bf16>::type b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -201,7 +210,7 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, const Seq& s, const
 // The rows row0 .. row0 + count of a unit from its `splits` partial sums,
 //   O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, in the splits' order,
 // by the whole workgroup; a split without visible keys has l = 0, O = 0.  The
-// loads of eight splits are in flight together.
+// loads of sixteen splits are in flight together.
 template <typename T>
 __device__ void join_splits(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int splits) {
     const int quads = a.d >> 2;
@@ -212,25 +221,25 @@ __device__ void join_splits(const AttnArgs& a, const Seq& s, int kvh, int row0, 
         const int64_t t_at = s.q0 + tok, at = t_at * a.hq + h;
         float m = -__builtin_inff(), l = 0.0f;
         f32x4 y = {};
-        for (int b = 0; b < splits; b += 8) {
-            float2 ml[8];
-            f32x4 o[8];
+        for (int b = 0; b < splits; b += 16) {
+            float2 ml[16];
+            f32x4 o[16];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
+            for (int k = 0; k < 16; k++) {
                 const int64_t p = min(b + k, splits - 1) * rows + at;
                 ml[k] = get_part_ml(a.part_ml + p);
                 o[k] = get_part4(a.part_o + p * a.d + e);
             }
             float top = m;
 #pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, ml[k].x);
+            for (int k = 0; k < 16; k++) top = fmaxf(top, ml[k].x);
             const float base = top == -__builtin_inff() ? 0.0f : top;
             const float fix = __builtin_amdgcn_exp2f(m - base);
             l *= fix;
             y *= fix;
             m = top;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
+            for (int k = 0; k < 16; k++) {
                 const float w = b + k < splits ? __builtin_amdgcn_exp2f(ml[k].x - base) : 0.0f;
                 l = __builtin_fmaf(w, ml[k].y, l);
                 if (w != 0.0f) y += w * o[k];
