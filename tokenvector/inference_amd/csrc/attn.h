@@ -73,8 +73,8 @@ struct AttnArgs {
     float scale_log2;  // scale * log2(e) > 0: weights are exp2(s * scale_log2 - m)
     int32_t out_f32;
     FastDiv gdiv;      // g
-    // split over the keys: sums [splits][tokens][hq][d] and (m, l) of each, and
-    // the arrival counts [units][hkv]
+    // split over the keys: sums [splits + groups][tokens][hq][d] and (m, l) of
+    // each, and the arrival counts [units][hkv][1 + kJoin]
     int32_t splits, units;
     float* part_o;
     float2* part_ml;
@@ -211,6 +211,9 @@ int launch_attn_tile_f32(Ctx* c, const AttnArgs& a, bool i8);
 int launch_attn_few_bf16(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
 int launch_attn_few_f16(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
 int launch_attn_few_f32(Ctx* c, const AttnArgs& a, bool i8, int blocks_of_16);
+// Sums that one level of the splits' join reads; the most splits.
+constexpr int kJoin = 16;
+constexpr int kMaxSplits = kJoin * kJoin;
 // Query rows (of all heads of one key / value head) that a workgroup takes.
 constexpr int kTileRows = 128;
 

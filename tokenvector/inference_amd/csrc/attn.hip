@@ -84,11 +84,12 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     int64_t want = std::min<int64_t>(slots / tiles, keys / (few ? 128 : 256));
     if (few)
         want = std::max(want, std::min<int64_t>(4 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
-    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kArriveFlat);
-    if (units * a.hkv > kAttnCounters) a.splits = 1;
+    a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kMaxSplits);
+    if (units * a.hkv * (1 + kJoin) > kAttnCounters) a.splits = 1;
     a.arrivals = c->attn_arrivals;
     if (a.splits > 1) {
-        const int64_t rows = a.tokens * a.hq * a.splits;
+        const int64_t sums = a.splits + (a.splits > kJoin ? ceil_div(a.splits, kJoin) : 0);
+        const int64_t rows = a.tokens * a.hq * sums;
         void* ws;
         const int rc = ctx_workspace(c, 16, (size_t)(rows * (a.d + 2) * 4), &ws);
         if (no_room(rc)) {

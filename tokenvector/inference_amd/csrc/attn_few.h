@@ -429,12 +429,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         row_again<T, C, true>(a, s, table, kvh, tok, h, max(seen_begin(a, shift + tok), t0 * BN),
                               min(seen_end(a, shift + tok, s.len), t1 * BN), split);
     }
-    if (split) {
-        unsigned* counter = a.arrivals + blockIdx.x;
-        if (!arrive_last(counter, splits)) return;
-        join_splits<T>(a, s, kvh, row0, min(rows - row0, ROWS), splits);
-        arrive_clear(counter, splits);
-    }
+    if (split) join_splits<T>(a, s, kvh, row0, min(rows - row0, ROWS), splits);
 }
 
 template <typename T, int DP, bool I8>

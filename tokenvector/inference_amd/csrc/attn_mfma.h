@@ -207,46 +207,70 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, const Seq& s, const
     }
 }
 
-// The rows row0 .. row0 + count of a unit from its `splits` partial sums,
-//   O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, in the splits' order,
-// by the whole workgroup; a split without visible keys has l = 0, O = 0.  The
-// loads of sixteen splits are in flight together.
+// The rows row0 .. row0 + count of a unit from `n` sums of its splits, the
+// `first`-th on (n <= kJoin),
+//   O = sum_s 2^(m_s - m) O_s,  l = sum_s 2^(m_s - m) l_s,
+// in the splits' order, by the whole workgroup, with all loads of a row in flight
+// together: into the output (to < 0), as O / l, or into the `to`-th sum.  A split
+// without visible keys has l = 0, O = 0.
 template <typename T>
-__device__ void join_splits(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int splits) {
+__device__ void join_sums(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int first, int n,
+                          int to) {
     const int quads = a.d >> 2;
     const int64_t rows = a.tokens * a.hq;
     for (int i = threadIdx.x; i < count * quads; i += blockDim.x) {
         const int r = i / quads, e = 4 * (i - r * quads), row = row0 + r;
         const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
         const int64_t t_at = s.q0 + tok, at = t_at * a.hq + h;
-        float m = -__builtin_inff(), l = 0.0f;
-        f32x4 y = {};
-        for (int b = 0; b < splits; b += 16) {
-            float2 ml[16];
-            f32x4 o[16];
+        float2 ml[kJoin];
+        f32x4 o[kJoin];
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const int64_t p = min(b + k, splits - 1) * rows + at;
-                ml[k] = get_part_ml(a.part_ml + p);
-                o[k] = get_part4(a.part_o + p * a.d + e);
-            }
-            float top = m;
-#pragma unroll
-            for (int k = 0; k < 16; k++) top = fmaxf(top, ml[k].x);
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            const float fix = __builtin_amdgcn_exp2f(m - base);
-            l *= fix;
-            y *= fix;
-            m = top;
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const float w = b + k < splits ? __builtin_amdgcn_exp2f(ml[k].x - base) : 0.0f;
-                l = __builtin_fmaf(w, ml[k].y, l);
-                if (w != 0.0f) y += w * o[k];
-            }
+        for (int k = 0; k < kJoin; k++) {
+            const int64_t p = (first + min(k, n - 1)) * rows + at;
+            ml[k] = get_part_ml(a.part_ml + p);
+            o[k] = get_part4(a.part_o + p * a.d + e);
         }
-        put_out4<T>(a, t_at, h, e, l == 0.0f ? f32x4{} : y * (1.0f / l));
+        float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoin; k++) m = fmaxf(m, ml[k].x);
+        const float base = m == -__builtin_inff() ? 0.0f : m;
+        f32x4 y = {};
+#pragma unroll
+        for (int k = 0; k < kJoin; k++) {
+            const float w = k < n ? __builtin_amdgcn_exp2f(ml[k].x - base) : 0.0f;
+            l = __builtin_fmaf(w, ml[k].y, l);
+            if (w != 0.0f) y += w * o[k];
+        }
+        if (to < 0) {
+            put_out4<T>(a, t_at, h, e, l == 0.0f ? f32x4{} : y * (1.0f / l));
+        } else {
+            const int64_t p = to * rows + at;
+            if (e == 0) put_part_ml(a.part_ml + p, m, l);
+            put_part4(a.part_o + p * a.d + e, y);
+        }
     }
+}
+
+// Joins a unit's `splits` sums, by its last workgroup; above kJoin of them the
+// last workgroup of each kJoin joins those first (into the sums a.splits on), so
+// that no workgroup reads more than kJoin sums per level.
+template <typename T>
+__device__ void join_splits(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int splits) {
+    unsigned* counter = a.arrivals + blockIdx.x * (1 + kJoin);
+    const int groups = (splits + kJoin - 1) / kJoin;
+    int first = 0, n = splits;
+    if (groups > 1) {
+        const int group = blockIdx.y / kJoin;
+        const int members = min(kJoin, splits - group * kJoin);
+        if (!arrive_last(counter + 1 + group, members)) return;
+        join_sums<T>(a, s, kvh, row0, count, group * kJoin, members, a.splits + group);
+        arrive_clear(counter + 1 + group, members);
+        first = a.splits;
+        n = groups;
+    }
+    if (!arrive_last(counter, n)) return;
+    join_sums<T>(a, s, kvh, row0, count, first, n, -1);
+    arrive_clear(counter, n);
 }
 
 }  // namespace attn

@@ -427,12 +427,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
         row_again<T, C, PAGED>(a, s, table, kvh, tk, h, max(seen_begin(a, shift + tk), t0 * BN),
                                min(seen_end(a, shift + tk, s.len), t1 * BN), split);
     }
-    if (split) {
-        unsigned* counter = a.arrivals + blockIdx.x;
-        if (!arrive_last(counter, splits)) return;
-        join_splits<T>(a, s, kvh, row0, min(rows - row0, kTileRows), splits);
-        arrive_clear(counter, splits);
-    }
+    if (split) join_splits<T>(a, s, kvh, row0, min(rows - row0, kTileRows), splits);
 }
 
 template <typename T, int DP, int KV>

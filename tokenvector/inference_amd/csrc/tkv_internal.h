@@ -60,8 +60,8 @@ constexpr unsigned kArriveGroups = 16;
 constexpr unsigned kArriveStride = 64;
 constexpr unsigned kArriveFlat = 64;  // up to so many workgroups use the first word alone
 constexpr unsigned kArriveWords = (1 + kArriveGroups) * kArriveStride;
-// Arrival counts of the attention's splits: one per unit of rows and key / value head.
-constexpr int kAttnCounters = 4096;
+// Arrival counts of the attention's splits: 17 per unit of rows and key / value head.
+constexpr int kAttnCounters = 17 * 1024;
 constexpr int64_t kCalHistBins = 4096;  // the largest KL histogram
 
 struct Graph;
