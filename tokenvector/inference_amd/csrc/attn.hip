@@ -62,7 +62,8 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     const int64_t b = type_bytes(type), kb = type_bytes(kv_type), ob = a.out_f32 ? 4 : b;
     const int64_t chunk = i8 ? 8 : 16 / b;
     if (a.d % chunk || !rows_of_16(a.q, a.q_st, a.q_sh, b) || !rows_of_16(a.out, a.o_st, a.o_sh, ob) ||
-        !rows_of_16(a.k, a.k_st, a.k_sh, kb) || !rows_of_16(a.v, a.v_st, a.v_sh, kb))
+        !rows_of_16(a.k, a.k_st, a.k_sh, kb) || !rows_of_16(a.v, a.v_st, a.v_sh, kb) ||
+        std::min(a.k_st, a.v_st) < 0 || std::max(a.k_st, a.v_st) >= (1ll << 22))
         return launch_attn_any(c, a, type, kv_type);
     a.gdiv = fast_div((uint32_t)a.g);
     if (a.tokens * a.g >= (1ll << 31))

@@ -54,6 +54,13 @@ __device__ __forceinline__ void copy16_to_lds(const void* src, unsigned dst) {
                  : "v"(src), "s"(dst)
                  : "memory");
 }
+// The same from a wave-uniform base and a byte offset per lane.
+__device__ __forceinline__ void copy16_to_lds(const char* base, uint32_t offset, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(dst)
+                 : "memory");
+}
 // 4 bytes per lane, to `dst` + 4 lane.
 __device__ __forceinline__ void copy4_to_lds(const void* src, unsigned dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
@@ -76,6 +83,15 @@ __device__ __forceinline__ unsigned lds_at(const void* p) {
     return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const char* uniform(const char* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const char*>((uint64_t)(uint32_t)uniform((int)v) |
+                                         (uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32);
+}
+// A wave-uniform element of read-only memory, through the scalar cache.
+__device__ __forceinline__ int load_uniform(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)p;
+}
 
 // The other half's value: lanes l and l + 32 exchange.
 __device__ __forceinline__ float other_half(float x) {

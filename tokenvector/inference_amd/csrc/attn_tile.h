@@ -117,16 +117,41 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
     }
 
     // ---- copies: thread's chunk i is position i * 256 + tid of the tile ----
-    uint32_t page_of[PAGED ? N : 1], slot_of[PAGED ? N : 1];
-    const auto row_of = [&](int i) { return (i * 256 + tid) / CPR; };
-    const auto find_pages = [&](int t) {
-        if constexpr (PAGED) {
+    // Addresses are a wave-uniform base per 1 KB copy and an offset per lane that
+    // stays the same from tile to tile (only the sequence's last tile clamps rows
+    // past its end to the last key, masked later).  Paged, a copy's rows lie in one
+    // page where the page size is a multiple of them; else each lane looks one
+    // key's row up and the lanes that copy its chunks get it by shuffle.
+    constexpr int RPC = CPR <= 64 && 64 % CPR == 0 ? 64 / CPR : 0;  // rows of a copy, 0: not whole
+    constexpr bool ALIKE = RPC > 0 && 4 * RPC % 16 == 0;  // all of a thread's chunks are swizzled alike
+    constexpr int NO = ALIKE ? 1 : N;
+    const bool whole = !PAGED || (RPC > 0 && a.page.d % (RPC > 0 ? RPC : 1) == 0);
+    const uint32_t row_bytes = (uint32_t)a.d * S::E;  // of a cached row
+    const uint32_t k_step = PAGED ? row_bytes : (uint32_t)a.k_st * S::E;
+    const uint32_t v_step = PAGED ? row_bytes : (uint32_t)a.v_st * S::E;
+    uint32_t k_off[NO], v_off[NO];  // of a thread's chunks (from the copy's first row where paged)
+    bool k_in[NO], v_in[NO];
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int j = min(t * BN + row_of(i), s.len - 1);  // past the end: the last key again, masked
-                const uint32_t pg = div_by(a.page, (uint32_t)j);
-                slot_of[i] = (uint32_t)j - pg * a.page.d;
-                page_of[i] = (uint32_t)table[pg];
+    for (int i = 0; i < NO; i++) {
+        const int pos = (i * 256 + tid) % CPR, r = (i * 256 + tid) / CPR;
+        const int ck = pos ^ swz_k<CPR>(r), cv = pos ^ swz_v<CPR, S::E>(r);
+        const int from = PAGED ? (RPC > 0 ? r % (RPC > 0 ? RPC : 1) : 0) : r;
+        k_off[i] = from * k_step + ck * 16;
+        v_off[i] = from * v_step + cv * 16;
+        k_in[i] = ck * S::CE < a.d;
+        v_in[i] = cv * S::CE < a.d;
+    }
+    const char* const k_head = static_cast<const char*>(a.k) + (PAGED ? 0 : (s.k0 * a.k_st + kvh * a.k_sh) * S::E);
+    const char* const v_head = static_cast<const char*>(a.v) + (PAGED ? 0 : (s.k0 * a.v_st + kvh * a.v_sh) * S::E);
+    int ids[PAGED ? N : 1], lane_id = 0;  // pages of the next tile's copies, or of the lane's key
+    const auto copy_first = [&](int t, int i) { return min(t * BN + (i * 4 + wave) * RPC, s.len - 1); };
+    const auto find_pages = [&](int t) {
+        if constexpr (PAGED && !I8) {
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < N; i++) ids[i] = load_uniform(table + div_by(a.page, copy_first(t, i)));
+            } else {
+                lane_id = table[div_by(a.page, min(t * BN + (lane & (BN - 1)), s.len - 1))];
             }
         }
     };
@@ -135,25 +160,67 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
     float sc = 0.0f;
     const auto copy_tile = [&](int t, int buf) {
         if constexpr (!I8) {
-            const unsigned base = lds_at(lds) + buf * 2 * S::TILE;
+            const unsigned dst0 = lds_at(lds) + buf * 2 * S::TILE + wave * 1024;
+            const bool last = (t + 1) * BN > s.len;
+            if (PAGED && !whole) {
+                const uint32_t j = min(t * BN + (lane & (BN - 1)), s.len - 1), pg = div_by(a.page, j);
+                const uint32_t id = lane_id < a.pool_pages && lane_id >= 0 ? lane_id : 0;
+                const uint32_t my_row = (id * (uint32_t)a.hkv + kvh) * a.page.d + (j - pg * a.page.d);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int pos = (i * 256 + tid) % CPR, r = (i * 256 + tid) / CPR;
+                    const int ck = pos ^ swz_k<CPR>(r), cv = pos ^ swz_v<CPR, S::E>(r);
+                    const int64_t at = (int64_t)(uint32_t)__shfl((int)my_row, r) * row_bytes;
+                    const unsigned dst = uniform(dst0 + i * 4096);
+                    if (ck * S::CE < a.d) copy16_to_lds(k_head + at + ck * 16, dst);
+                    if (cv * S::CE < a.d) copy16_to_lds(v_head + at + cv * 16, dst + S::TILE);
+                }
+                return;
+            }
+            const char *kt = k_head, *vt = v_head;
+            if constexpr (!PAGED) {
+                kt += (int64_t)t * BN * k_step;
+                vt += (int64_t)t * BN * v_step;
+            }
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int pos = (i * 256 + tid) % CPR, r = row_of(i);
-                const int ck = pos ^ swz_k<CPR>(r), cv = pos ^ swz_v<CPR, S::E>(r);
-                const T *kr, *vr;
+                const int o = ALIKE ? 0 : i;
+                const char *kr = kt, *vr = vt;
+                int rows_in;  // rows of the copy (or tile) that the sequence has
                 if constexpr (PAGED) {
-                    const uint32_t id = (int64_t)page_of[i] < a.pool_pages ? page_of[i] : 0;
-                    const int64_t at = (((int64_t)id * a.hkv + kvh) * a.page.d + slot_of[i]) * a.d;
-                    kr = static_cast<const T*>(a.k) + at;
-                    vr = static_cast<const T*>(a.v) + at;
+                    const int j = copy_first(t, i);
+                    const uint32_t slot = j - div_by(a.page, j) * a.page.d;
+                    const uint32_t id = ids[i] < a.pool_pages && ids[i] >= 0 ? ids[i] : 0;
+                    const int64_t at = (int64_t)((id * (uint32_t)a.hkv + kvh) * a.page.d + slot) * row_bytes;
+                    kr += at;
+                    vr += at;
+                    rows_in = s.len - j;
                 } else {
-                    const int64_t j = s.k0 + min(t * BN + r, s.len - 1);
-                    kr = static_cast<const T*>(a.k) + j * a.k_st + (int64_t)kvh * a.k_sh;
-                    vr = static_cast<const T*>(a.v) + j * a.v_st + (int64_t)kvh * a.v_sh;
+                    if (ALIKE) {
+                        kr += (int64_t)(i * 4 * RPC) * k_step;
+                        vr += (int64_t)(i * 4 * RPC) * v_step;
+                    }
+                    rows_in = s.len - t * BN - (ALIKE ? i * 4 * RPC : 0);
                 }
-                const unsigned dst = uniform(base + (i * 4 + wave) * 1024);
-                if (ck * S::CE < a.d) copy16_to_lds(kr + ck * S::CE, dst);
-                if (cv * S::CE < a.d) copy16_to_lds(vr + cv * S::CE, dst + S::TILE);
+                uint32_t ko = k_off[o], vo = v_off[o];
+                if (last) {
+                    // rows past the end: back to the last one, wherever it lies
+                    const int r = PAGED ? (RPC > 0 ? lane / CPR : 0)
+                                        : ((ALIKE ? 0 : i * 256) + tid) / CPR;
+                    const int past = max(r - (rows_in - 1), 0);
+                    if constexpr (PAGED) {
+                        ko -= past * k_step;
+                        vo -= past * v_step;
+                    } else {
+                        const int64_t back_k = (int64_t)past * k_step, back_v = (int64_t)past * v_step;
+                        if (k_in[o]) copy16_to_lds(kr + ko - back_k, uniform(dst0 + i * 4096));
+                        if (v_in[o]) copy16_to_lds(vr + vo - back_v, uniform(dst0 + i * 4096) + S::TILE);
+                        continue;
+                    }
+                }
+                const unsigned dst = uniform(dst0 + i * 4096);
+                if (k_in[o]) copy16_to_lds(uniform(kr), ko, dst);
+                if (v_in[o]) copy16_to_lds(uniform(vr), vo, dst + S::TILE);
             }
         } else {
             // codes through registers: converted on their way to LDS, below
