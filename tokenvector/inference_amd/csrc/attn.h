@@ -73,11 +73,13 @@ struct AttnArgs {
     float scale_log2;  // scale * log2(e) > 0: weights are exp2(s * scale_log2 - m)
     int32_t out_f32;
     FastDiv gdiv;      // g
-    // split over the keys: sums [splits + groups][tokens][hq][d] and (m, l) of
-    // each, and the arrival counts [units][hkv][1 + kJoin]
+    // split over the keys: arrival counts [units][hkv][1 + kJoin], and the sums,
+    // sum_bytes for every workgroup of the grid (and, above kJoin splits, for
+    // every kJoin of them)
     int32_t splits, units;
-    float* part_o;
-    float2* part_ml;
+    int32_t split_tiles;  // key tiles of a split; more where there would be more splits
+    char* sums;
+    int64_t sum_bytes;
     unsigned* arrivals;
 };
 
@@ -199,10 +201,15 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, const Seq& s, cons
     *lo = l;
 }
 
+// The head size that a matrix kernel is built for.
+inline int64_t padded_head(int64_t d, bool f32) {
+    return d <= 64 ? 64 : d <= 96 && !f32 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
+}
+
 // attn_any.hip: any head size up to 256, any strides and alignment.
 int launch_attn_any(Ctx* c, const AttnArgs& a, int type, int kv_type);
 // attn_tile_*.hip: many query rows per sequence and head, on the matrix units.
-// 16-byte rows; `splits` > 1 leaves partial sums in a.part_o and a.part_ml.
+// 16-byte rows.
 int launch_attn_tile_bf16(Ctx* c, const AttnArgs& a, bool i8);
 int launch_attn_tile_f16(Ctx* c, const AttnArgs& a, bool i8);
 int launch_attn_tile_f32(Ctx* c, const AttnArgs& a, bool i8);

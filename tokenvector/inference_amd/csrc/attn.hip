@@ -81,7 +81,8 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     // 256 (tiles) at least to each.  Streaming, up to four times as many where each
     // still has 512 KB to read, so that caches of different lengths even out: a
     // workgroup's start and end take as long as reading about 100 KB.
-    const int64_t slots = 2 * c->num_cus;
+    // f32 products take 16 times as long: twice as many there.
+    const int64_t slots = (!few && type == TKV_HIP_F32 ? 4 : 2) * c->num_cus;
     int64_t want = std::min<int64_t>(slots / tiles, keys / (few ? 128 : 256));
     if (few)
         want = std::max(want, std::min<int64_t>(4 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
@@ -89,16 +90,16 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     if (units * a.hkv * (1 + kJoin) > kAttnCounters) a.splits = 1;
     a.arrivals = c->attn_arrivals;
     if (a.splits > 1) {
-        const int64_t sums = a.splits + (a.splits > kJoin ? ceil_div(a.splits, kJoin) : 0);
-        const int64_t rows = a.tokens * a.hq * sums;
+        const int64_t groups = a.splits > kJoin ? ceil_div(a.splits, kJoin) : 0;
+        // (m, l) and O of a workgroup's rows
+        a.sum_bytes = block * (8 + 4 * padded_head(a.d, type == TKV_HIP_F32));
         void* ws;
-        const int rc = ctx_workspace(c, 16, (size_t)(rows * (a.d + 2) * 4), &ws);
+        const int rc = ctx_workspace(c, 16, (size_t)(units * a.hkv * (a.splits + groups) * a.sum_bytes), &ws);
         if (no_room(rc)) {
             a.splits = 1;
         } else {
             TKV_RC_TRY(rc);
-            a.part_ml = static_cast<float2*>(ws);
-            a.part_o = reinterpret_cast<float*>(a.part_ml + rows);
+            a.sums = static_cast<char*>(ws);
         }
     }
     if (few)

@@ -91,7 +91,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
     int splits = 1;  // that have tiles
     if (a.splits > 1 && t1 > t0) {
-        const int per = (t1 - t0 + a.splits - 1) / a.splits;
+        const int per = max(a.split_tiles, (t1 - t0 + a.splits - 1) / a.splits);
         splits = (t1 - t0 + per - 1) / per;
         t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
@@ -396,8 +396,16 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     }
     barrier();
     const bool split = splits > 1;
-    const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
-    for (int i = tid; i < ROWS * (DP / 4); i += 64 * NW) {
+    // sums of a split: (m, l) of the rows, then two planes of 8 bytes per four elements
+    constexpr int QUADS = ROWS * (DP / 4);
+    const auto sum_of = [&](int i) {
+        return reinterpret_cast<u64*>(a.sums + ((int64_t)i * gridDim.x + blockIdx.x) * a.sum_bytes);
+    };
+    const auto put_quad = [&](u64* sum, int i, f32x4 y) {
+        put_sum(sum + ROWS + i, y[0], y[1]);
+        put_sum(sum + ROWS + QUADS + i, y[2], y[3]);
+    };
+    for (int i = tid; i < QUADS; i += 64 * NW) {
         const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
         if (row >= rows || e >= a.d || row_bad[r]) continue;
         float mm = -kInf;
@@ -412,24 +420,94 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
             ll = __builtin_fmaf(f, row_ml[w][r].y, ll);
             y += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * ROWS + r) * DP + e);
         }
-        const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
-        const int64_t t_at = s.q0 + tok;
         if (split) {
-            const int64_t p_at = (part + t_at) * a.hq + h;
-            if (e == 0) put_part_ml(a.part_ml + p_at, mm, ll);
-            put_part4(a.part_o + p_at * a.d + e, y);
+            u64* sum = sum_of(blockIdx.y);
+            if (e == 0) put_sum(sum + r, mm, ll);
+            put_quad(sum, i, y);
         } else {
-            put_out4<T>(a, t_at, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
+            const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+            put_out4<T>(a, s.q0 + tok, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
         }
     }
     for (int r = wave; r < ROWS; r += NW) {
         const int row = row0 + r;
         if (row >= rows || !uniform(row_bad[r])) continue;
         const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
-        row_again<T, C, true>(a, s, table, kvh, tok, h, max(seen_begin(a, shift + tok), t0 * BN),
-                              min(seen_end(a, shift + tok, s.len), t1 * BN), split);
+        const int64_t t_at = s.q0 + tok;
+        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
+        float mm, ll, acc[4];
+        attend_row<T, C, true>(a, s, table, kvh, qr, max(seen_begin(a, shift + tok), t0 * BN),
+                               min(seen_end(a, shift + tok, s.len), t1 * BN), &mm, &ll, acc);
+        if (!split) {
+            put_row<T>(a, t_at, h, ll, acc);
+            continue;
+        }
+        u64* sum = sum_of(blockIdx.y);
+        if (lane == 0) put_sum(sum + r, mm, ll);
+        for (int x4 = 0; x4 < 4; x4++) {
+            const int x = lane + 64 * x4;
+            const float v = acc[x4], next = __shfl_down(v, 1);
+            if (x < a.d && !(x & 1)) put_sum(sum + ROWS + (x & 2 ? QUADS : 0) + r * (DP / 4) + x / 4, v, next);
+        }
     }
-    if (split) join_splits<T>(a, s, kvh, row0, min(rows - row0, ROWS), splits);
+    if (!split) return;
+
+    // The unit's last workgroup joins its splits, in their order,
+    //   O = sum_s 2^(m_s - m) O_s,  l = sum_s 2^(m_s - m) l_s;
+    // above kJoin of them the last workgroup of each kJoin joins those first, so
+    // that none reads more than kJoin sums per level, all of them in flight
+    // together.
+    const auto join = [&](auto most, int from, int n, int to) __attribute__((always_inline)) {
+        constexpr int MOST = decltype(most)::value;
+        for (int i = tid; i < QUADS; i += 64 * NW) {
+            const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
+            if (row >= rows || e >= a.d) continue;
+            float2 ml[MOST], lo[MOST], hi[MOST];
+#pragma unroll
+            for (int k = 0; k < MOST; k++) {
+                const u64* sum = sum_of(from + min(k, n - 1));
+                ml[k] = get_sum(sum + r);
+                lo[k] = get_sum(sum + ROWS + i);
+                hi[k] = get_sum(sum + ROWS + QUADS + i);
+            }
+            float mm = -kInf, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < MOST; k++) mm = fmaxf(mm, ml[k].x);
+            const float base = mm == -kInf ? 0.0f : mm;
+            f32x4 y = {};
+#pragma unroll
+            for (int k = 0; k < MOST; k++) {
+                const float w = k < n ? __builtin_amdgcn_exp2f(ml[k].x - base) : 0.0f;
+                ll = __builtin_fmaf(w, ml[k].y, ll);
+                if (w != 0.0f) y += w * f32x4{lo[k].x, lo[k].y, hi[k].x, hi[k].y};
+            }
+            if (to >= 0) {
+                if (e == 0) put_sum(sum_of(to) + r, mm, ll);
+                put_quad(sum_of(to), i, y);
+            } else {
+                const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+                put_out4<T>(a, s.q0 + tok, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
+            }
+        }
+    };
+    const auto join_all = [&](int from, int n, int to) __attribute__((always_inline)) {
+        if (n <= 4) join(std::integral_constant<int, 4>{}, from, n, to);
+        else if (n <= 8) join(std::integral_constant<int, 8>{}, from, n, to);
+        else join(std::integral_constant<int, kJoin>{}, from, n, to);
+    };
+    unsigned* counter = a.arrivals + blockIdx.x * (1 + kJoin);
+    int from = 0, n = splits;
+    if (splits > kJoin) {
+        const int group = blockIdx.y / kJoin, members = min(kJoin, splits - group * kJoin);
+        if (!arrive_last(counter + 1 + group, members)) return;
+        arrive_clear(counter + 1 + group, members);
+        join_all(group * kJoin, members, a.splits + group);
+        from = a.splits;
+        n = (splits + kJoin - 1) / kJoin;
+    }
+    if (!arrive_last(counter, n)) return;
+    arrive_clear(counter, n);
+    join_all(from, n, -1);
 }
 
 template <typename T, int DP, bool I8>

@@ -157,28 +157,17 @@ __device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first)
 }
 
 // Partial sums of a split, written where the unit's last workgroup, on whatever
-// XCD, reads them (agent scope: past this XCD's L2; see arrive_last).
-__device__ __forceinline__ void put_part4(float* p, f32x4 v) {
-    unsigned long long w[2];
-    __builtin_memcpy(w, &v, 16);
-    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p) + 1, w[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// XCD, reads them (agent scope: past this XCD's L2; see arrive_last).  8 bytes is
+// the widest such access, so sums are laid out for lanes to be 8 bytes apart: a
+// wave writes and reads whole lines.  (16 bytes apart, in rows of the output, the
+// same traffic took twice as long as the whole attention of 8 x 1024 tokens.)
+typedef unsigned long long u64;
+__device__ __forceinline__ void put_sum(u64* p, float x, float y) {
+    __hip_atomic_store(p, (u64)__float_as_uint(x) | ((u64)__float_as_uint(y) << 32), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ f32x4 get_part4(const float* p) {
-    unsigned long long w[2];
-    w[0] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    w[1] = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    f32x4 v;
-    __builtin_memcpy(&v, w, 16);
-    return v;
-}
-__device__ __forceinline__ void put_part_ml(float2* p, float m, float l) {
-    const unsigned long long w = (unsigned long long)__float_as_uint(m) | ((unsigned long long)__float_as_uint(l) << 32);
-    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 get_part_ml(const float2* p) {
-    const unsigned long long w =
-        __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ float2 get_sum(const u64* p) {
+    const u64 w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
 }
 
@@ -197,96 +186,18 @@ __device__ __forceinline__ void put_out4(const AttnArgs& a, int64_t token, int h
     }
 }
 
-// A row computed key by key (attend_row) over [j0, j1), by one wave, into the
-// output or this split's partial sums.
-template <typename T, typename C, bool PAGED>
-__device__ __forceinline__ void row_again(const AttnArgs& a, const Seq& s, const int32_t* table, int kvh,
-                                          int tok, int h, int j0, int j1, bool split) {
+// An output row from the sums of attend_row, by one wave.
+template <typename T>
+__device__ __forceinline__ void put_row(const AttnArgs& a, int64_t token, int head, float l, const float (&acc)[4]) {
     const int lane = threadIdx.x & 63;
-    const int64_t t_at = s.q0 + tok;
-    const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
-    float m, l, acc[4];
-    attend_row<T, C, PAGED>(a, s, table, kvh, qr, j0, j1, &m, &l, acc);
-    const int64_t p_at = ((int64_t)blockIdx.y * a.tokens + t_at) * a.hq + h;
-    if (split && lane == 0) put_part_ml(a.part_ml + p_at, m, l);
+    const int64_t at = token * a.o_st + (int64_t)head * a.o_sh;
     for (int e = 0; e < 4; e++) {
         const int x = lane + 64 * e;
         if (x >= a.d) continue;
-        if (split) {
-            __hip_atomic_store(a.part_o + p_at * a.d + x, acc[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            continue;
-        }
         const float y = l == 0.0f ? 0.0f : acc[e] / l;
-        const int64_t at = t_at * a.o_st + (int64_t)h * a.o_sh + x;
-        if (a.out_f32) static_cast<float*>(a.out)[at] = y;
-        else static_cast<T*>(a.out)[at] = from_f32<T>(y);
+        if (a.out_f32) static_cast<float*>(a.out)[at + x] = y;
+        else static_cast<T*>(a.out)[at + x] = from_f32<T>(y);
     }
-}
-
-// The rows row0 .. row0 + count of a unit from `n` sums of its splits, the
-// `first`-th on (n <= kJoin),
-//   O = sum_s 2^(m_s - m) O_s,  l = sum_s 2^(m_s - m) l_s,
-// in the splits' order, by the whole workgroup, with all loads of a row in flight
-// together: into the output (to < 0), as O / l, or into the `to`-th sum.  A split
-// without visible keys has l = 0, O = 0.
-template <typename T>
-__device__ void join_sums(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int first, int n,
-                          int to) {
-    const int quads = a.d >> 2;
-    const int64_t rows = a.tokens * a.hq;
-    for (int i = threadIdx.x; i < count * quads; i += blockDim.x) {
-        const int r = i / quads, e = 4 * (i - r * quads), row = row0 + r;
-        const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
-        const int64_t t_at = s.q0 + tok, at = t_at * a.hq + h;
-        float2 ml[kJoin];
-        f32x4 o[kJoin];
-#pragma unroll
-        for (int k = 0; k < kJoin; k++) {
-            const int64_t p = (first + min(k, n - 1)) * rows + at;
-            ml[k] = get_part_ml(a.part_ml + p);
-            o[k] = get_part4(a.part_o + p * a.d + e);
-        }
-        float m = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kJoin; k++) m = fmaxf(m, ml[k].x);
-        const float base = m == -__builtin_inff() ? 0.0f : m;
-        f32x4 y = {};
-#pragma unroll
-        for (int k = 0; k < kJoin; k++) {
-            const float w = k < n ? __builtin_amdgcn_exp2f(ml[k].x - base) : 0.0f;
-            l = __builtin_fmaf(w, ml[k].y, l);
-            if (w != 0.0f) y += w * o[k];
-        }
-        if (to < 0) {
-            put_out4<T>(a, t_at, h, e, l == 0.0f ? f32x4{} : y * (1.0f / l));
-        } else {
-            const int64_t p = to * rows + at;
-            if (e == 0) put_part_ml(a.part_ml + p, m, l);
-            put_part4(a.part_o + p * a.d + e, y);
-        }
-    }
-}
-
-// Joins a unit's `splits` sums, by its last workgroup; above kJoin of them the
-// last workgroup of each kJoin joins those first (into the sums a.splits on), so
-// that no workgroup reads more than kJoin sums per level.
-template <typename T>
-__device__ void join_splits(const AttnArgs& a, const Seq& s, int kvh, int row0, int count, int splits) {
-    unsigned* counter = a.arrivals + blockIdx.x * (1 + kJoin);
-    const int groups = (splits + kJoin - 1) / kJoin;
-    int first = 0, n = splits;
-    if (groups > 1) {
-        const int group = blockIdx.y / kJoin;
-        const int members = min(kJoin, splits - group * kJoin);
-        if (!arrive_last(counter + 1 + group, members)) return;
-        join_sums<T>(a, s, kvh, row0, count, group * kJoin, members, a.splits + group);
-        arrive_clear(counter + 1 + group, members);
-        first = a.splits;
-        n = groups;
-    }
-    if (!arrive_last(counter, n)) return;
-    join_sums<T>(a, s, kvh, row0, count, first, n, -1);
-    arrive_clear(counter, n);
 }
 
 }  // namespace attn

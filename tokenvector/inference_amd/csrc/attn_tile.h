@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
     int splits = 1;  // that have tiles
     if (a.splits > 1 && t1 > t0) {
-        const int per = (t1 - t0 + a.splits - 1) / a.splits;
+        const int per = max(a.split_tiles, (t1 - t0 + a.splits - 1) / a.splits);
         splits = (t1 - t0 + per - 1) / per;
         t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
@@ -449,52 +449,101 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
         for (int e = 0; e < 16; e++) bad |= !(fabsf(o[b][e]) < kInf);
     const unsigned long long ball = __ballot(bad && mine);
     unsigned again = uniform((unsigned)ball | (unsigned)(ball >> 32));
-    const int64_t part = split ? (int64_t)blockIdx.y * a.tokens : 0;
 
-    if (mine && !((again >> l31) & 1)) {
-        const int64_t t_at = s.q0 + tok;
-        const float scale = (split || l == 0.0f ? 1.0f : 1.0f / l) * vexp;
-        const int64_t p_at = (part + t_at) * a.hq + head;
-        if (split && half == 0) put_part_ml(a.part_ml + p_at, m, l);
+    // a split's sums, in this kernel's register layout
+    u64* const mine_sum = split ? reinterpret_cast<u64*>(a.sums + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) *
+                                                                      a.sum_bytes) : nullptr;
+    if (split && !((again >> l31) & 1)) {
+        if (half == 0) put_sum(mine_sum + wave * 32 + l31, m, l);
 #pragma unroll
-        for (int b = 0; b < NDB; b++) {
-            if (F32 || split || a.out_f32) {
+        for (int b = 0; b < NDB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e = b * 32 + 8 * i + 4 * half;
-                    const f32x4 y = {o[b][4 * i] * scale, o[b][4 * i + 1] * scale, o[b][4 * i + 2] * scale,
-                                     o[b][4 * i + 3] * scale};
-                    if (e >= a.d) continue;
-                    if (split) put_part4(a.part_o + p_at * a.d + e, y);
-                    else put_out4<float>(a, t_at, head, e, y);
+            for (int e = 0; e < 16; e += 2)
+                put_sum(mine_sum + kTileRows + (b * 8 + e / 2) * 256 + tid, o[b][e] * vexp, o[b][e + 1] * vexp);
+    }
+    for (unsigned todo = again; todo; todo &= todo - 1) {
+        const int i = __builtin_ctz(todo);
+        const int r = wrow + i, tk = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tk * a.g;
+        const int64_t t_at = s.q0 + tk;
+        const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
+        float mm, ll, acc[4];
+        attend_row<T, C, PAGED>(a, s, table, kvh, qr, max(seen_begin(a, shift + tk), t0 * BN),
+                                min(seen_end(a, shift + tk, s.len), t1 * BN), &mm, &ll, acc);
+        if (!split) {
+            put_row<T>(a, t_at, h, ll, acc);
+            continue;
+        }
+        if (lane == 0) put_sum(mine_sum + wave * 32 + i, mm, ll);
+        for (int x4 = 0; x4 < 4; x4++) {
+            const int x = lane + 64 * x4, y = x & 31;  // register 4 (y / 8) + y % 4 of lane half y / 4 % 2
+            if (x >= DP) continue;
+            const float v = x < a.d ? acc[x4] : 0.0f, next = __shfl_down(v, 1);
+            if (!(x & 1))
+                put_sum(mine_sum + kTileRows + ((x >> 5) * 8 + 2 * (y >> 3) + ((y & 3) >> 1)) * 256 + wave * 64 +
+                            32 * ((y >> 2) & 1) + i,
+                        v, next);
+        }
+    }
+    if (split) {
+        unsigned* counter = a.arrivals + blockIdx.x * (1 + kJoin);
+        if (!arrive_last(counter, splits)) return;
+        arrive_clear(counter, splits);
+        // the unit's last workgroup joins its splits, in their order:
+        //   O = sum_s 2^(m_s - m) O_s,  l = sum_s 2^(m_s - m) l_s
+        m = -kInf, l = 0.0f, vexp = 1.0f;
+        for (int k = 0; k < splits; k++) {
+            const u64* sum = reinterpret_cast<const u64*>(a.sums + ((int64_t)k * gridDim.x + blockIdx.x) * a.sum_bytes);
+            const float2 ml = get_sum(sum + wave * 32 + l31);
+            float2 y[NDB * 8];
+#pragma unroll
+            for (int e = 0; e < NDB * 8; e++) y[e] = get_sum(sum + kTileRows + e * 256 + tid);
+            const float mn = fmaxf(m, ml.x), base = mn == -kInf ? 0.0f : mn;
+            const float fix = __builtin_amdgcn_exp2f(m - base), w = __builtin_amdgcn_exp2f(ml.x - base);
+            m = mn;
+            l = l * fix + ml.y * w;
+#pragma unroll
+            for (int b = 0; b < NDB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float v = e & 1 ? y[b * 8 + e / 2].y : y[b * 8 + e / 2].x;
+                    // a sum that nothing was added to may follow one that is not finite
+                    o[b][e] = (k == 0 ? 0.0f : o[b][e] * fix) + (w == 0.0f ? 0.0f : v * w);
                 }
-            } else if constexpr (!F32) {
-                // halves exchange groups of four: 8 elements, 16 bytes, per store
-                T* out = static_cast<T*>(a.out) + t_at * a.o_st + (int64_t)head * a.o_sh;
+        }
+        again = 0;
+    }
+
+    if (!mine || ((again >> l31) & 1)) return;
+    const int64_t t_at = s.q0 + tok;
+    const float scale = (l == 0.0f ? 1.0f : 1.0f / l) * vexp;
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    T y[8];
+    for (int b = 0; b < NDB; b++) {
+        if (F32 || a.out_f32) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) y[j] = (T)(o[b][8 * i + j] * scale);
-                    uint2 lo, hi;
-                    __builtin_memcpy(&lo, y, 8);
-                    __builtin_memcpy(&hi, y + 4, 8);
-                    const auto sx = __builtin_amdgcn_permlane32_swap(lo.x, hi.x, false, false);
-                    const auto sy = __builtin_amdgcn_permlane32_swap(lo.y, hi.y, false, false);
-                    const int e = b * 32 + 16 * i + 8 * half;
-                    if (e < a.d) *reinterpret_cast<u32x4*>(out + e) = u32x4{sx[0], sy[0], sx[1], sy[1]};
-                }
+            for (int i = 0; i < 4; i++) {
+                const int e = b * 32 + 8 * i + 4 * half;
+                const f32x4 y = {o[b][4 * i] * scale, o[b][4 * i + 1] * scale, o[b][4 * i + 2] * scale,
+                                 o[b][4 * i + 3] * scale};
+                if (e < a.d) put_out4<float>(a, t_at, head, e, y);
+            }
+        } else if constexpr (!F32) {
+            // halves exchange groups of four: 8 elements, 16 bytes, per store
+            T* out = static_cast<T*>(a.out) + t_at * a.o_st + (int64_t)head * a.o_sh;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                T y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = (T)(o[b][8 * i + j] * scale);
+                uint2 lo, hi;
+                __builtin_memcpy(&lo, y, 8);
+                __builtin_memcpy(&hi, y + 4, 8);
+                const auto sx = __builtin_amdgcn_permlane32_swap(lo.x, hi.x, false, false);
+                const auto sy = __builtin_amdgcn_permlane32_swap(lo.y, hi.y, false, false);
+                const int e = b * 32 + 16 * i + 8 * half;
+                if (e < a.d) *reinterpret_cast<u32x4*>(out + e) = u32x4{sx[0], sy[0], sx[1], sy[1]};
             }
         }
     }
-    while (again) {
-        const int i = __builtin_ctz(again);
-        again &= again - 1;
-        const int r = wrow + i, tk = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tk * a.g;
-        row_again<T, C, PAGED>(a, s, table, kvh, tk, h, max(seen_begin(a, shift + tk), t0 * BN),
-                               min(seen_end(a, shift + tk, s.len), t1 * BN), split);
-    }
-    if (split) join_splits<T>(a, s, kvh, row0, min(rows - row0, kTileRows), splits);
 }
 
 template <typename T, int DP, int KV>
