@@ -42,7 +42,7 @@ struct TileShape {
 };
 
 template <typename T, int DP, int KV>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_attn_tile(AttnArgs a) {
+__global__ __launch_bounds__(256, (DP == 256 || (sizeof(T) == 4 && DP > 128)) ? 1 : 2) void k_attn_tile(AttnArgs a) {
     using S = TileShape<T, DP>;
     using V8 = typename Vec<T>::type;
     constexpr bool PAGED = KV != KV_PACKED, I8 = KV == KV_I8, F32 = sizeof(T) == 4;
@@ -335,12 +335,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP > 128) ? 1 : 2) void k_a
                     }
             }
             if (!full) {
+                // what this lane's row sees: keys [lo, hi) counted from the lane's first
+                const int lo = my_begin - j0 - 4 * half, hi = my_end - j0 - 4 * half;
 #pragma unroll
                 for (int b = 0; b < NKB; b++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const int j = j0 + b * 32 + (e & 3) + 8 * (e >> 2) + 4 * half;
-                        const bool seen = j >= my_begin && j < my_end;
+                        const int j = b * 32 + (e & 3) + 8 * (e >> 2);
+                        const bool seen = j >= lo && j < hi;
                         x[b][e] = seen ? x[b][e] : -kInf;
                         if constexpr (I8) vs[b * 16 + e] = seen ? vs[b * 16 + e] : 0.0f;
                     }
