@@ -41,9 +41,9 @@ struct RopeArgs {
     const int32_t* positions;
     const float2* table;
     int64_t table_len;
-    int64_t rows;        // tokens * heads
+    int64_t tokens;
     int32_t hq, hkv, d, rot, pairs;
-    int32_t lanes_log2;  // lanes of a head row, 8 elements each
+    int32_t lanes_log2;  // lanes of a head row
 };
 
 template <typename T>
@@ -51,54 +51,167 @@ struct alignas(16) Vec8 {
     T e[8];
 };
 
-// 8 elements of a row from e0 on: one or two 16-byte loads (VEC), else those
-// below d one by one.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int e0, int d, float (&x)[8]) {
-    if constexpr (VEC) {
-        const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(row + e0);
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(p);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32(v.e[i]);
+    for (int i = 0; i < 8; i++) x[i] = to_f32(v.e[i]);
+}
+// 16-bit chunks are stored past the L2's reuse: the lanes of a row write whole
+// lines (8192 tokens of 48 heads of 128: 50.6 -> 45.1 us).  f32 chunks are half
+// lines per store and lose by it.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v.e[i] = from_f32<T>(x[i]);
+    if constexpr (sizeof(T) == 2) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 w;
+        __builtin_memcpy(&w, &v, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
     } else {
+        *reinterpret_cast<Vec8<T>*>(p) = v;
+    }
+}
+// codes of a row from its max |x| (over 1 << lanes lanes)
+__device__ __forceinline__ float row_max(float m, int lanes) {
+    for (int o = 1 << lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m;
+}
+__device__ __forceinline__ int8_t code_of(float x, float inv) {
+    const float y = __builtin_rintf(x * inv);
+    return y != y ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(y, -127.0f), 127.0f);
+}
+
+// Chunks of 8 elements: a lane takes two of a head row's, in the half layout those
+// that are rotated with each other, so that neighbouring lanes have neighbouring
+// chunks; 2^lanes lanes per head row, and
+// `HEADS` heads of its token in turn, all their loads in flight together, so that
+// each element is read once and a table entry once per HEADS heads.  HBM bound.
+// Head index and with it the role (q, k or v) are the workgroup's.
+template <typename TI, typename TO, typename C, int HEADS>
+__global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
+    const int64_t t64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
+    if (t64 >= a.tokens) return;  // whole groups: the rows' lanes stay together
+    const int tok = (int)t64, i = (int)threadIdx.x & ((1 << a.lanes_log2) - 1);
+    const int chunks = a.d >> 3;
+    const int turns = a.pairs ? 0 : a.rot >> 4;  // chunk pairs rotated with each other
+    const int rest = chunks - 2 * turns, j = i - turns;
+    const int c0 = i < turns ? i : j < (rest + 1) / 2 ? 2 * turns + j : chunks;
+    const int c1 = i < turns ? i + turns : c0 < chunks ? c0 + (rest + 1) / 2 : chunks;
+    const bool in0 = c0 < chunks, in1 = c1 < chunks;
+    const int pos = a.table ? a.positions[tok] : 0;
+    const bool pad = a.table && (pos < 0 || pos >= a.table_len);
+    int64_t slot = -1;
+    if (a.kc && !pad) slot = a.slots[tok];
+    const bool put = slot >= 0 && slot < a.n_slots;
+    const uint32_t s32 = put ? (uint32_t)slot : 0, pg = div_by(a.page, s32);
+    // (cos, sin): of the 8 pairs of a chunk pair, or the 4 of either chunk
+    const bool turn0 = a.pairs ? c0 < a.rot >> 3 : i < turns, turn1 = a.pairs ? c1 < a.rot >> 3 : i < turns;
+    float2 w[8];
+    const auto entries = [&](int at, float2* to) {
+        const float4* cs = reinterpret_cast<const float4*>(a.table + (int64_t)pos * (a.rot >> 1) + at);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = e0 + i < d ? to_f32(row[e0 + i]) : 0.0f;
+        for (int k = 0; k < 2; k++) {
+            const float4 v = cs[k];
+            to[2 * k] = make_float2(v.x, v.y);
+            to[2 * k + 1] = make_float2(v.z, v.w);
+        }
+    };
+    if (turn0 && !pad) entries(a.pairs ? 4 * c0 : 8 * i, w);
+    if (turn1 && !pad) entries(a.pairs ? 4 * c1 : 8 * i + 4, w + 4);
+    const int first = blockIdx.y * HEADS;
+    float x0[HEADS][8], x1[HEADS][8];
+#pragma unroll
+    for (int u = 0; u < HEADS; u++) {
+        const int row = min(first + u, (int)a.heads.d - 1);
+        const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
+        const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
+        const TI* src = static_cast<const TI*>(isq ? a.q : isv ? a.v : a.k) +
+                        (int64_t)h * (isq ? a.q_sh : isv ? a.v_sh : a.k_sh) +
+                        (int64_t)tok * (isq ? a.q_st : isv ? a.v_st : a.k_st);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x0[u][k] = x1[u][k] = 0.0f;
+        if (in0 && !pad) load8(src + 8 * c0, x0[u]);
+        if (in1 && !pad) load8(src + 8 * c1, x1[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < HEADS; u++) {
+        const int row = first + u;
+        if (row >= (int)a.heads.d) break;
+        const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
+        const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
+        if (!isv && !pad) {
+            // each product and sum is rounded by itself (no contraction in this
+            // library): the same bits as separate elementwise operations
+            if (a.pairs) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (!(k < 4 ? turn0 : turn1)) continue;
+                    float* x = k < 4 ? x0[u] : x1[u];
+                    const int e = 2 * (k & 3);
+                    const float p = x[e], q = x[e + 1];
+                    x[e] = p * w[k].x - q * w[k].y;
+                    x[e + 1] = q * w[k].x + p * w[k].y;
+                }
+            } else if (turn0) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float p = x0[u][k], q = x1[u][k];
+                    x0[u][k] = p * w[k].x - q * w[k].y;
+                    x1[u][k] = q * w[k].x + p * w[k].y;
+                }
+            }
+        }
+        if (!isv && (isq ? a.qo : a.ko)) {
+            TO* dst = static_cast<TO*>(isq ? a.qo : a.ko) + (int64_t)tok * (isq ? a.qo_st : a.ko_st) +
+                      (int64_t)h * (isq ? a.qo_sh : a.ko_sh);
+            if (in0) store8(dst + 8 * c0, x0[u]);
+            if (in1) store8(dst + 8 * c1, x1[u]);
+        }
+        if (isq || !a.kc) continue;
+        const int64_t at = ((int64_t)pg * a.hkv + h) * a.page.d + (s32 - pg * a.page.d);
+        if constexpr (sizeof(C) == 1) {
+            float m = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = fmaxf(m, fmaxf(fabsf(x0[u][k]), fabsf(x1[u][k])));
+            m = row_max(m, a.lanes_log2);
+            if (!put) continue;
+            const float scale = fmaxf(m, 1e-8f) / 127.0f, inv = 1.0f / scale;
+            if (i == 0) (isv ? a.vs : a.ks)[at] = scale;
+            int8_t* dst = static_cast<int8_t*>(isv ? a.vc : a.kc) + at * a.d;
+            int8_t z[8];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) z[k] = code_of(half ? x1[u][k] : x0[u][k], inv);
+                uint2 v;
+                __builtin_memcpy(&v, z, 8);
+                if (half ? in1 : in0) *reinterpret_cast<uint2*>(dst + 8 * (half ? c1 : c0)) = v;
+            }
+        } else if (put) {
+            C* dst = static_cast<C*>(isv ? a.vc : a.kc) + at * a.d;
+            if (in0) store8(dst + 8 * c0, x0[u]);
+            if (in1) store8(dst + 8 * c1, x1[u]);
+        }
     }
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int e0, int d, const float (&x)[8]) {
-    if constexpr (VEC) {
-        Vec8<T> v;
-#pragma unroll
-        for (int i = 0; i < 8; i++) v.e[i] = from_f32<T>(x[i]);
-        *reinterpret_cast<Vec8<T>*>(row + e0) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (e0 + i < d) row[e0 + i] = from_f32<T>(x[i]);
-    }
-}
-
-// One head row (of q, k or v) per 2^lanes_log2 lanes, 8 elements per lane, one
-// row per thread group and no loop: HBM bound, each input element read from it
-// once.  A lane also loads the 8 elements that its own are rotated with (they
-// are another lane's, so the second load hits the cache; a shuffle of 8 f32
-// through LDS costs more) and the 8 or 4 table entries, which the token's other
-// heads read too.
-//
-// VEC: 16-byte aligned rows, d and rot / 2 multiples of 8.
-template <typename TI, typename TO, typename C, bool VEC>
-__global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
+// Any head size, rotation and alignment: one head row per 2^lanes lanes, 8
+// elements a lane, one by one; the element that one is rotated with is loaded
+// again.
+template <typename TI, typename TO, typename C>
+__global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t r64 = t >> a.lanes_log2;
-    if (r64 >= a.rows) return;  // whole groups: the rows' lanes stay together
+    if (r64 >= a.tokens * a.heads.d) return;  // whole groups: the rows' lanes stay together
     const uint32_t r = (uint32_t)r64;
     const int e0 = 8 * ((int)threadIdx.x & ((1 << a.lanes_log2) - 1));
     const uint32_t tok = div_by(a.heads, r);
     int h = (int)(r - tok * a.heads.d);
     const bool isq = h < a.hq, isv = h >= a.hq + a.hkv;
     h -= isq ? 0 : isv ? a.hq + a.hkv : a.hq;
-
     const TI* src = static_cast<const TI*>(isq ? a.q : isv ? a.v : a.k) +
                     (int64_t)tok * (isq ? a.q_st : isv ? a.v_st : a.k_st) +
                     (int64_t)h * (isq ? a.q_sh : isv ? a.v_sh : a.k_sh);
@@ -106,100 +219,80 @@ __global__ __launch_bounds__(256) void k_rope_append(RopeArgs a) {
     const bool pad = a.table && (pos < 0 || pos >= a.table_len);
     int64_t slot = -1;
     if (!isq && a.kc && !pad) slot = a.slots[tok];
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    const bool live = e0 < a.d;
-    if (live && !pad) {
-        load8<TI, VEC>(src, e0, a.d, x);
-        if (a.table && !isv && e0 < a.rot) {
-            const int half = a.rot >> 1;
-            const float2* cs = a.table + (int64_t)pos * half;
-            // each product and sum is rounded by itself (no contraction in
-            // this library): the same bits as separate elementwise operations
-            if (VEC && a.pairs) {
+    const int half = a.rot >> 1;
+    const float2* cs = a.table + (int64_t)pos * half;
+    float x[8];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 w = cs[(e0 >> 1) + i];
-                    const float u = x[2 * i], y = x[2 * i + 1];
-                    x[2 * i] = u * w.x - y * w.y;
-                    x[2 * i + 1] = y * w.x + u * w.y;
-                }
-            } else if (VEC) {
-                const bool low = e0 < half;
-                float o[8];
-                load8<TI, VEC>(src, low ? e0 + half : e0 - half, a.d, o);
-                const float2* w = cs + (low ? e0 : e0 - half);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float c = w[i].x, s = w[i].y;
-                    x[i] = low ? x[i] * c - o[i] * s : x[i] * c + o[i] * s;
-                }
-            } else {
-                for (int i = 0; i < 8; i++) {
-                    const int e = e0 + i;
-                    if (e >= a.rot) break;
-                    const bool low = a.pairs ? !(e & 1) : e < half;
-                    const int mate = a.pairs ? e ^ 1 : low ? e + half : e - half;
-                    const float2 w = cs[a.pairs ? e >> 1 : low ? e : e - half];
-                    const float o = to_f32(src[mate]);
-                    x[i] = low ? x[i] * w.x - o * w.y : x[i] * w.x + o * w.y;
-                }
-            }
+    for (int i = 0; i < 8; i++) {
+        const int e = e0 + i;
+        x[i] = e < a.d && !pad ? to_f32(src[e]) : 0.0f;
+        if (e < a.rot && !isv && !pad) {
+            const bool low = a.pairs ? !(e & 1) : e < half;
+            const int mate = a.pairs ? e ^ 1 : low ? e + half : e - half;
+            const float2 w = cs[a.pairs ? e >> 1 : low ? e : e - half];
+            const float o = to_f32(src[mate]);
+            x[i] = low ? x[i] * w.x - o * w.y : x[i] * w.x + o * w.y;
         }
     }
-    if (live && isq && a.qo)
-        store8<TO, VEC>(static_cast<TO*>(a.qo) + (int64_t)tok * a.qo_st + (int64_t)h * a.qo_sh, e0, a.d, x);
-    if (live && !isq && !isv && a.ko)
-        store8<TO, VEC>(static_cast<TO*>(a.ko) + (int64_t)tok * a.ko_st + (int64_t)h * a.ko_sh, e0, a.d, x);
+    if (!isv && (isq ? a.qo : a.ko)) {
+        // a row may be rotated in place: its lanes are one wave's, and all have
+        // loaded before the first stores
+        __builtin_amdgcn_wave_barrier();
+        TO* dst = static_cast<TO*>(isq ? a.qo : a.ko) + (int64_t)tok * (isq ? a.qo_st : a.ko_st) +
+                  (int64_t)h * (isq ? a.qo_sh : a.ko_sh);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (e0 + i < a.d) dst[e0 + i] = from_f32<TO>(x[i]);
+    }
     const bool put = slot >= 0 && slot < a.n_slots;
     const uint32_t s32 = put ? (uint32_t)slot : 0, pg = div_by(a.page, s32);
     const int64_t at = ((int64_t)pg * a.hkv + h) * a.page.d + (s32 - pg * a.page.d);
     if constexpr (sizeof(C) == 1) {
-        // max |x| of the row over its lanes (NaN skipped), then its codes
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-        for (int o = 1 << a.lanes_log2 >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = row_max(m, a.lanes_log2);
         if (!put) return;
         const float scale = fmaxf(m, 1e-8f) / 127.0f, inv = 1.0f / scale;
         if (e0 == 0) (isv ? a.vs : a.ks)[at] = scale;
-        if (!live) return;
-        int8_t* dst = static_cast<int8_t*>(isv ? a.vc : a.kc) + at * a.d + e0;
-        int8_t q[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float y = __builtin_rintf(x[i] * inv);
-            q[i] = y != y ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(y, -127.0f), 127.0f);
-        }
-        if constexpr (VEC) {
-            uint2 w;
-            __builtin_memcpy(&w, q, 8);
-            *reinterpret_cast<uint2*>(dst) = w;
-        } else {
-            for (int i = 0; i < 8; i++)
-                if (e0 + i < a.d) dst[i] = q[i];
-        }
-    } else if (put && live) {
-        store8<C, VEC>(static_cast<C*>(isv ? a.vc : a.kc) + at * a.d, e0, a.d, x);
+        int8_t* dst = static_cast<int8_t*>(isv ? a.vc : a.kc) + at * a.d;
+        for (int i = 0; i < 8; i++)
+            if (e0 + i < a.d) dst[e0 + i] = code_of(x[i], inv);
+    } else if (put) {
+        C* dst = static_cast<C*>(isv ? a.vc : a.kc) + at * a.d;
+        for (int i = 0; i < 8; i++)
+            if (e0 + i < a.d) dst[e0 + i] = from_f32<C>(x[i]);
     }
+}
+
+template <typename TI, typename TO, typename C>
+static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
+    const int64_t heads = a.heads.d;
+    if (!vec) {
+        while (8 << a.lanes_log2 < a.d) a.lanes_log2++;
+        k_rope_any<TI, TO, C><<<(unsigned)ceil_div(a.tokens * heads << a.lanes_log2, 256), 256, 0, c->stream>>>(a);
+        return;
+    }
+    while (16 << a.lanes_log2 < a.d) a.lanes_log2++;
+    const int64_t blocks = ceil_div(a.tokens << a.lanes_log2, 256);
+    // four heads per lane where that still leaves eight workgroups per CU
+    if (blocks * ceil_div(heads, 4) >= 8 * c->num_cus)
+        k_rope_rows<TI, TO, C, 4><<<dim3((unsigned)blocks, (unsigned)ceil_div(heads, 4)), 256, 0, c->stream>>>(a);
+    else
+        k_rope_rows<TI, TO, C, 1><<<dim3((unsigned)blocks, (unsigned)heads), 256, 0, c->stream>>>(a);
 }
 
 template <typename TI, typename TO>
-static void launch_rope(Ctx* c, const RopeArgs& a, bool i8, bool vec) {
-    const dim3 grid((unsigned)ceil_div(a.rows << a.lanes_log2, 256));
-    if (i8) {
-        if (vec) k_rope_append<TI, TO, int8_t, true><<<grid, 256, 0, c->stream>>>(a);
-        else k_rope_append<TI, TO, int8_t, false><<<grid, 256, 0, c->stream>>>(a);
-    } else {
-        if (vec) k_rope_append<TI, TO, TO, true><<<grid, 256, 0, c->stream>>>(a);
-        else k_rope_append<TI, TO, TO, false><<<grid, 256, 0, c->stream>>>(a);
-    }
+static void launch_rope_to(Ctx* c, const RopeArgs& a, bool i8, bool vec) {
+    if (i8) launch_rope<TI, TO, int8_t>(c, a, vec);
+    else launch_rope<TI, TO, TO>(c, a, vec);
 }
 
 template <typename TI>
-static void launch_rope_to(Ctx* c, const RopeArgs& a, int type_out, bool i8, bool vec) {
-    if (type_out == TKV_HIP_F32) launch_rope<TI, float>(c, a, i8, vec);
-    else if (type_out == TKV_HIP_F16) launch_rope<TI, _Float16>(c, a, i8, vec);
-    else launch_rope<TI, __bf16>(c, a, i8, vec);
+static void launch_rope_from(Ctx* c, const RopeArgs& a, int type_out, bool i8, bool vec) {
+    if (type_out == TKV_HIP_F32) launch_rope_to<TI, float>(c, a, i8, vec);
+    else if (type_out == TKV_HIP_F16) launch_rope_to<TI, _Float16>(c, a, i8, vec);
+    else launch_rope_to<TI, __bf16>(c, a, i8, vec);
 }
 
 static bool rows_aligned(const tkv_hip_rows* r, int64_t bytes) {
@@ -376,22 +469,21 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
     a.positions = positions;
     a.table = reinterpret_cast<const float2*>(table);
     a.table_len = table_len;
-    a.rows = tokens * heads;
+    a.tokens = tokens;
     a.hq = (int32_t)heads_q;
     a.hkv = (int32_t)heads_kv;
     a.d = (int32_t)head_dim;
     a.rot = table ? (int32_t)rot_dim : 0;
     a.pairs = layout == TKV_HIP_ROPE_PAIRS;
-    while (8 << a.lanes_log2 < head_dim) a.lanes_log2++;
     const int64_t bi = type_bytes(type_in), bo = type_bytes(type_out);
-    const bool vec = head_dim % 8 == 0 && (a.rot / 2) % 8 == 0 && rows_aligned(has_q ? q : nullptr, bi) &&
+    const bool vec = head_dim % 8 == 0 && a.rot % (a.pairs ? 8 : 16) == 0 && aligned(table, 16) && heads < 65536 && rows_aligned(has_q ? q : nullptr, bi) &&
                      rows_aligned(has_k ? k : nullptr, bi) && rows_aligned(has_v ? v : nullptr, bi) &&
                      rows_aligned(q_out, bo) && rows_aligned(k_out, bo) &&
                      (!kv || (aligned(kv->k, 16) && aligned(kv->v, 16)));
     const bool i8 = kv && kv->type == TKV_HIP_I8;
-    if (type_in == TKV_HIP_F32) launch_rope_to<float>(c, a, type_out, i8, vec);
-    else if (type_in == TKV_HIP_F16) launch_rope_to<_Float16>(c, a, type_out, i8, vec);
-    else launch_rope_to<__bf16>(c, a, type_out, i8, vec);
+    if (type_in == TKV_HIP_F32) launch_rope_from<float>(c, a, type_out, i8, vec);
+    else if (type_in == TKV_HIP_F16) launch_rope_from<_Float16>(c, a, type_out, i8, vec);
+    else launch_rope_from<__bf16>(c, a, type_out, i8, vec);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
