@@ -68,24 +68,26 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     a.gdiv = fast_div((uint32_t)a.g);
     if (a.tokens * a.g >= (1ll << 31))
         return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
-    // up to 32 rows per sequence take the streaming kernel, blocks of 16 rows
+    // up to 32 rows per sequence take the streaming kernel, blocks of 16 rows, a
+    // unit per sequence; else units of 128 rows (see tile_seq)
     const int64_t longest = a.pages ? (a.cu_q ? max_q : 1) * a.g : 0;
     const bool few = longest > 0 && longest <= 32 && !(i8 && a.d % 16);
     const int blocks16 = longest <= 16 ? 1 : 2;
     const int64_t block = few ? 16 * blocks16 : kTileRows;
-    const int64_t units = few && !a.cu_q ? a.seqs : a.tokens * a.g / block + a.seqs;
+    const int64_t units = few ? a.seqs : a.tokens * a.g / block + a.seqs;
     if (units >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     a.units = (int32_t)units;
-    const int64_t tiles = std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs) * a.hkv;
+    const int64_t tiles = (few ? a.seqs : std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs)) * a.hkv;
     // Splits over the keys: as many as fill the chip once, 128 keys (streaming) or
-    // 256 (tiles) at least to each.  Streaming, up to four times as many where each
+    // 256 (tiles) at least to each.  Streaming, up to eight times as many where each
     // still has 512 KB to read, so that caches of different lengths even out: a
     // workgroup's start and end take as long as reading about 100 KB.
-    // f32 products take 16 times as long: twice as many there.
-    const int64_t slots = (!few && type == TKV_HIP_F32 ? 4 : 2) * c->num_cus;
+    // f32 products take 16 times as long: twice as many there.  Heads of 64 let
+    // three workgroups share a CU.
+    const int64_t slots = (few ? 2 : type == TKV_HIP_F32 ? 4 : a.d <= 64 ? 3 : 2) * c->num_cus;
     int64_t want = std::min<int64_t>(slots / tiles, keys / (few ? 128 : 256));
     if (few)
-        want = std::max(want, std::min<int64_t>(4 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
+        want = std::max(want, std::min<int64_t>(8 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
     a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kMaxSplits);
     if (units * a.hkv * (1 + kJoin) > kAttnCounters) a.splits = 1;
     a.arrivals = c->attn_arrivals;

@@ -75,17 +75,31 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int l15 = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % a.hkv, unit = blockIdx.x / a.hkv;
-    int first;
-    const int seq = tile_seq<true, ROWS>(a, unit, &first);
+    const int kvh = blockIdx.x % a.hkv, seq = blockIdx.x / a.hkv;
     Seq s = seq_of<true>(a, seq);
     s.q0 = uniform(s.q0), s.n = uniform(s.n), s.len = uniform(s.len);
-    const int rows = s.n * a.g, row0 = (unit - first) * ROWS;
-    if (row0 >= rows) return;
+    const int rows = s.n * a.g;
     const int32_t* table = a.pages + seq * a.pages_st;
     const int shift = s.len - s.n;
-    const int pos_lo = shift + (int)div_by(a.gdiv, row0);
-    const int pos_hi = shift + (int)div_by(a.gdiv, min(row0 + ROWS, rows) - 1);
+    char* mem = lds + wave * S::WAVE;
+    int* ids = reinterpret_cast<int*>(mem + 4 * S::TILE);
+    float* scales = reinterpret_cast<float*>(mem + 4 * S::TILE + S::IDS);  // [2][K, V][64]
+
+    if (rows == 0) return;
+    // A sequence of more rows than the caller's max_q said is still right, if
+    // slow: its first split's workgroup takes those past the block key by key.
+    if (rows > ROWS && blockIdx.y == 0) {
+        for (int row = ROWS + wave; row < rows; row += NW) {
+            const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+            const T* qr = static_cast<const T*>(a.q) + (int64_t)(s.q0 + tok) * a.q_st + (int64_t)h * a.q_sh;
+            float mm, ll, acc[4];
+            attend_row<T, C, true>(a, s, table, kvh, qr, seen_begin(a, shift + tok),
+                                   seen_end(a, shift + tok, s.len), &mm, &ll, acc);
+            put_row<T>(a, s.q0 + tok, h, ll, acc);
+        }
+    }
+    const int pos_lo = shift;
+    const int pos_hi = shift + (int)div_by(a.gdiv, min(ROWS, rows) - 1);
     const int kb = seen_begin(a, pos_lo), ke = seen_end(a, pos_hi, s.len);
     const int f_begin = uniform(seen_begin(a, pos_hi)), f_end = uniform(seen_end(a, pos_lo, s.len));
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
@@ -99,9 +113,6 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     if ((int)blockIdx.y >= splits) return;
     t0 = uniform(t0), t1 = uniform(t1);
 
-    char* mem = lds + wave * S::WAVE;
-    int* ids = reinterpret_cast<int*>(mem + 4 * S::TILE);
-    float* scales = reinterpret_cast<float*>(mem + 4 * S::TILE + S::IDS);  // [2][K, V][64]
     if (tid < ROWS) row_bad[tid] = 0;
     if (a.d < DP) {
         // the chunks past the head's end are never copied: zeros, as the queries there
@@ -151,7 +162,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     int my_begin[NB], my_end[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        const int row = row0 + 16 * b + l15;
+        const int row = 16 * b + l15;
         const bool mine = row < rows;
         const int tok = (int)div_by(a.gdiv, mine ? row : 0), h = kvh * a.g + (mine ? row : 0) - tok * a.g;
         const T* qr = static_cast<const T*>(a.q) + (int64_t)(s.q0 + tok) * a.q_st + (int64_t)h * a.q_sh;
@@ -406,7 +417,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         put_sum(sum + ROWS + QUADS + i, y[2], y[3]);
     };
     for (int i = tid; i < QUADS; i += 64 * NW) {
-        const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
+        const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = r;
         if (row >= rows || e >= a.d || row_bad[r]) continue;
         float mm = -kInf;
 #pragma unroll
@@ -430,7 +441,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         }
     }
     for (int r = wave; r < ROWS; r += NW) {
-        const int row = row0 + r;
+        const int row = r;
         if (row >= rows || !uniform(row_bad[r])) continue;
         const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
         const int64_t t_at = s.q0 + tok;
@@ -460,7 +471,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     const auto join = [&](auto most, int from, int n, int to) __attribute__((always_inline)) {
         constexpr int MOST = decltype(most)::value;
         for (int i = tid; i < QUADS; i += 64 * NW) {
-            const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = row0 + r;
+            const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = r;
             if (row >= rows || e >= a.d) continue;
             float2 ml[MOST], lo[MOST], hi[MOST];
 #pragma unroll

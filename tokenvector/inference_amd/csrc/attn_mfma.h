@@ -133,10 +133,6 @@ enum { KV_PACKED = 0, KV_PAGED = 1, KV_I8 = 2 };
 template <bool PAGED, int ROWS>
 __device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first) {
     const int lane = threadIdx.x & 63;
-    if (PAGED && !a.cu_q && a.g <= ROWS) {  // a unit per sequence
-        *first = unit;
-        return unit;
-    }
     int found = 0, begin = 0;
     for (int b = 0; b < a.seqs; b += 64) {
         const int i = b + lane;
