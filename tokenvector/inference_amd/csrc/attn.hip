@@ -89,6 +89,11 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     if (few)
         want = std::max(want, std::min<int64_t>(8 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
     a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kMaxSplits);
+    // many short rows (see TileShape): clearly over two workgroups per CU, up to 4096
+    // keys each as far as the host knows
+    int64_t per_row = a.pages ? keys : a.tokens_k / a.seqs;
+    if (a.window > 0) per_row = std::min(per_row, a.window + kTileRows);
+    a.narrow = 10 * tiles > 23 * c->num_cus && per_row <= 4096;
     if (units * a.hkv * (1 + kJoin) > kAttnCounters) a.splits = 1;
     a.arrivals = c->attn_arrivals;
     if (a.splits > 1) {

@@ -27,11 +27,17 @@ namespace tkv {
 namespace attn {
 
 
-// DP: head size, padded (64, 96, 128, 192, 256; f32 96 only as 128).
-template <typename T, int DP>
+// DP: head size, padded (64, 96, 128, 192, 256; f32 96 only as 128).  Keys of a
+// tile: as many as two workgroups per CU have registers and LDS for, 64 where the
+// maximum, the rescaling test and the barrier of a tile spread over more of them.
+// NARROW: 32 keys, and three workgroups per CU (heads of 128), which pays where
+// many short rows make starts and ends weigh: 17 prompts of 12001 tokens 149 ->
+// 136 us, 13 chunks under a window of 1024 88 -> 71; one prompt of 16384 tokens
+// 1139 -> 1175, 4 of 1024 in exactly two workgroups per CU 38 -> 45.
+template <typename T, int DP, bool NARROW>
 struct TileShape {
     static constexpr int E = sizeof(T);
-    static constexpr int BN = (E == 4 || DP >= 192) ? 32 : 64;  // keys of a tile
+    static constexpr int BN = (NARROW || E == 4 || DP >= 192) ? 32 : 64;
     static constexpr int CPR = DP * E / 16;
     static constexpr int CE = 16 / E;                           // elements of a chunk
     static constexpr int TILE = BN * DP * E;                    // bytes
@@ -41,9 +47,10 @@ struct TileShape {
     static constexpr int LDS = 4 * TILE + 4 * BN * 4;           // two buffers of K and V, scales
 };
 
-template <typename T, int DP, int KV>
-__global__ __launch_bounds__(256, (DP == 256 || (sizeof(T) == 4 && DP > 128)) ? 1 : 2) void k_attn_tile(AttnArgs a) {
-    using S = TileShape<T, DP>;
+template <typename T, int DP, int KV, bool NARROW>
+__global__ __launch_bounds__(256, NARROW ? 3 : (DP == 256 || (sizeof(T) == 4 && DP > 128)) ? 1 : 2)
+void k_attn_tile(AttnArgs a) {
+    using S = TileShape<T, DP, NARROW>;
     using V8 = typename Vec<T>::type;
     constexpr bool PAGED = KV != KV_PACKED, I8 = KV == KV_I8, F32 = sizeof(T) == 4;
     constexpr int BN = S::BN, NKB = BN / 32, NDB = DP / 32, CPR = S::CPR, N = S::N;
@@ -548,14 +555,15 @@ __global__ __launch_bounds__(256, (DP == 256 || (sizeof(T) == 4 && DP > 128)) ? 
     }
 }
 
-template <typename T, int DP, int KV>
+template <typename T, int DP, int KV, bool NARROW = false>
 int launch_tile_dp(Ctx* c, const AttnArgs& a) {
-    using S = TileShape<T, DP>;
+    using S = TileShape<T, DP, NARROW>;
     static_assert(S::LDS <= 163840, "LDS of a workgroup");
     if ((size_t)S::LDS > c->max_lds) return set_error(TKV_HIP_UNSUPPORTED, "attention: not enough LDS");
     const int64_t blocks = (int64_t)a.units * a.hkv;
     if (blocks >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many tiles");
-    k_attn_tile<T, DP, KV><<<dim3((unsigned)blocks, (unsigned)a.splits), 256, S::LDS, c->stream>>>(a);
+    k_attn_tile<T, DP, KV, NARROW>
+        <<<dim3((unsigned)blocks, (unsigned)a.splits), 256, S::LDS, c->stream>>>(a);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
@@ -565,6 +573,8 @@ int launch_tile_kv(Ctx* c, const AttnArgs& a) {
     if (a.d <= 64) return launch_tile_dp<T, 64, KV>(c, a);
     if constexpr (sizeof(T) == 2)
         if (a.d <= 96) return launch_tile_dp<T, 96, KV>(c, a);
+    if constexpr (sizeof(T) == 2 && KV != KV_I8)
+        if (a.d <= 128 && a.narrow) return launch_tile_dp<T, 128, KV, true>(c, a);
     if (a.d <= 128) return launch_tile_dp<T, 128, KV>(c, a);
     if (a.d <= 192) return launch_tile_dp<T, 192, KV>(c, a);
     return launch_tile_dp<T, 256, KV>(c, a);
