@@ -132,7 +132,7 @@ void k_attn_tile(AttnArgs a) {
     constexpr int RPC = CPR <= 64 && 64 % CPR == 0 ? 64 / CPR : 0;  // rows of a copy, 0: not whole
     constexpr bool ALIKE = RPC > 0 && 4 * RPC % 16 == 0;  // all of a thread's chunks are swizzled alike
     constexpr int NO = ALIKE ? 1 : N;
-    const bool whole = !PAGED || (RPC > 0 && a.page.d % (RPC > 0 ? RPC : 1) == 0);
+    const bool whole = !PAGED || (!I8 && RPC > 0 && a.page.d % (RPC > 0 ? RPC : 1) == 0);
     const uint32_t row_bytes = (uint32_t)a.d * S::E;  // of a cached row
     const uint32_t k_step = PAGED ? row_bytes : (uint32_t)a.k_st * S::E;
     const uint32_t v_step = PAGED ? row_bytes : (uint32_t)a.v_st * S::E;
@@ -153,7 +153,7 @@ void k_attn_tile(AttnArgs a) {
     int ids[PAGED ? N : 1], lane_id = 0;  // pages of the next tile's copies, or of the lane's key
     const auto copy_first = [&](int t, int i) { return min(t * BN + (i * 4 + wave) * RPC, s.len - 1); };
     const auto find_pages = [&](int t) {
-        if constexpr (PAGED && !I8) {
+        if constexpr (PAGED) {
             if (whole) {
 #pragma unroll
                 for (int i = 0; i < N; i++) ids[i] = load_uniform(table + div_by(a.page, copy_first(t, i)));
@@ -161,6 +161,12 @@ void k_attn_tile(AttnArgs a) {
                 lane_id = table[div_by(a.page, min(t * BN + (lane & (BN - 1)), s.len - 1))];
             }
         }
+    };
+    // pool row of the lane's key of tile t, whose page find_pages(t) has looked up
+    const auto lane_row = [&](int t) {
+        const uint32_t j = min(t * BN + (lane & (BN - 1)), s.len - 1), pg = div_by(a.page, j);
+        const uint32_t id = lane_id < a.pool_pages && lane_id >= 0 ? lane_id : 0;
+        return (id * (uint32_t)a.hkv + kvh) * a.page.d + (j - pg * a.page.d);
     };
     constexpr int NR = I8 ? BN * (DP / 8) / 256 : 1;  // 8 codes per thread and trip
     uint2 kc[NR], vc[NR];
@@ -170,9 +176,7 @@ void k_attn_tile(AttnArgs a) {
             const unsigned dst0 = lds_at(lds) + buf * 2 * S::TILE + wave * 1024;
             const bool last = (t + 1) * BN > s.len;
             if (PAGED && !whole) {
-                const uint32_t j = min(t * BN + (lane & (BN - 1)), s.len - 1), pg = div_by(a.page, j);
-                const uint32_t id = lane_id < a.pool_pages && lane_id >= 0 ? lane_id : 0;
-                const uint32_t my_row = (id * (uint32_t)a.hkv + kvh) * a.page.d + (j - pg * a.page.d);
+                const uint32_t my_row = lane_row(t);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const int pos = (i * 256 + tid) % CPR, r = (i * 256 + tid) / CPR;
@@ -231,24 +235,18 @@ void k_attn_tile(AttnArgs a) {
             }
         } else {
             // codes through registers: converted on their way to LDS, below
+            const uint32_t my_row = lane_row(t);
 #pragma unroll
             for (int i = 0; i < NR; i++) {
-                const int x = i * 256 + tid, r = x / (DP / 8), e = 8 * (x % (DP / 8));
-                const int j = min(t * BN + r, s.len - 1);
-                int64_t sr;
-                const int64_t at = kv_row<true>(a, s, table, kvh, j, 0, 0, &sr) + e;
+                const int x = i * 256 + tid, e = 8 * (x % (DP / 8));
+                const int64_t at = (int64_t)(uint32_t)__shfl((int)my_row, x / (DP / 8)) * a.d + e;
                 kc[i] = vc[i] = uint2{0, 0};
                 if (e < a.d) {
                     kc[i] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.k) + at);
                     vc[i] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.v) + at);
                 }
             }
-            if (tid < 2 * BN) {
-                const int j = min(t * BN + (tid & (BN - 1)), s.len - 1);
-                int64_t sr;
-                kv_row<true>(a, s, table, kvh, j, 0, 0, &sr);
-                sc = (tid < BN ? a.ks : a.vs)[sr];
-            }
+            if (tid < 2 * BN) sc = (tid < BN ? a.ks : a.vs)[my_row];
         }
     };
     const auto put_codes = [&](int buf) {
