@@ -287,6 +287,39 @@ def test_prompt_infinite_value_behind_a_finite_key(ctx, typ):
     assert np.all(np.abs(got[:at, 0] - whole[0][:at]) <= bound[:at])
 
 
+@pytest.mark.parametrize("typ", [A.BF16, A.F16], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("d", [104, 128])
+def test_prompt_many_short_sequences(ctx, typ, d):
+    """Hundreds of tiles: the kernel with 32 keys a tile."""
+    r = np.random.default_rng(8)
+    lens = r.integers(0, 12, 200).tolist() + [70, 33, 200]
+    p = Prompt(ctx, typ, 8, 4, d, lens)
+    p.call()
+    p.check("many short sequences")
+
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F16, A.F32], ids=lambda t: NAME[t])
+def test_prompt_scale_zero_and_infinite_logits(ctx, typ):
+    """Equal weights at scale 0; a key whose logits are -inf has no weight; rows that
+    see nothing else are zeros."""
+    p = Prompt(ctx, typ, 2, 2, 64, [90], scale=0.0)
+    p.call()
+    p.check("scale zero")
+    p = Prompt(ctx, typ, 1, 1, 64, [90])
+    x = p.x.reshape(-1, 3, 64)
+    x[:90, 0] = np.abs(x[:90, 0]) + 0.5              # queries all positive
+    x[0, 1] = -np.inf
+    x[5, 1] = -np.inf
+    p.xd.upload(_bytes(p.x.reshape(-1), typ))
+    p.call()
+    got = p.result()[:90]
+    assert not got[0].any(), "the first row's only logit is -inf"
+    mask = _seen(90, 90, True, 0)
+    mask[:, [0, 5]] = False
+    k = np.where(np.isfinite(x[:90, 1:2]), x[:90, 1:2], 0)
+    _check(got[1:], x[1:90, :1], k, x[:90, 2:], mask[1:], p.scale, typ, typ, "keys of -inf logits")
+
+
 # ---- the paged cache --------------------------------------------------------------
 
 class Paged:
@@ -363,7 +396,7 @@ class Paged:
 
 
 LAYOUTS = [(2, 2, 64), (8, 2, 128), (4, 1, 128), (3, 3, 80), (5, 1, 96), (16, 2, 64), (4, 2, 192),
-           (8, 1, 256), (2, 2, 16), (20, 1, 64)]
+           (8, 1, 256), (2, 2, 16), (20, 1, 64), (4, 2, 72), (33, 1, 64), (40, 1, 128)]
 TYPES = [(A.BF16, A.BF16), (A.F16, A.F16), (A.F32, A.F32), (A.BF16, A.I8), (A.F16, A.I8), (A.F32, A.I8)]
 TYPE_IDS = [f"{NAME[a]}-{NAME[b]}" for a, b in TYPES]
 
@@ -434,6 +467,132 @@ def test_chunk_masks(ctx, typ, cache, causal, window):
     p = Paged(ctx, typ, cache, 4, 2, 64, [40, 100, 2], [400, 100, 90], causal=causal, window=window)
     p.call()
     p.check("chunk masks")
+
+
+class Poisoned(Paged):
+    """A windowed cache whose tokens before the earliest query's window hold NaN and
+    infinities (int8: such scales)."""
+
+    def __init__(self, ctx, typ, cache, hq, hkv, d, new, total, page, window):
+        super().__init__(ctx, typ, cache, hq, hkv, d, new, total, page=page, window=window)
+        kp, vp = (b.download() for b in self.bufs)
+        raw = _bytes(POISON, typ) if cache != A.I8 else None
+        tab = self.tab.download()
+        for s, (n, t) in enumerate(zip(new, total)):
+            for j in range(max(0, t - n + 1 - window)):
+                pg, slot = tab[s, j // page], j % page
+                if cache == A.I8:
+                    self.ks[pg, :, slot] = self.vs[pg, :, slot] = POISON[j % 3]
+                else:
+                    kp[pg, :, slot] = vp[pg, :, slot] = raw[j % 3]
+        if cache == A.I8:
+            self.pool._kept[2].upload(self.ks)
+            self.pool._kept[3].upload(self.vs)
+        else:
+            self.bufs[0].upload(kp)
+            self.bufs[1].upload(vp)
+
+
+@pytest.mark.parametrize("typ,cache", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("new,total,window", [([1, 1], [700, 90], 37), ([1], [6000], 3000), ([40, 3], [300, 500], 21),
+                                              ([150], [5000], 2900)])
+def test_window_hides_what_is_not_finite(ctx, typ, cache, new, total, window):
+    p = Poisoned(ctx, typ, cache, 4, 2, 64, new, total, 16, window)
+    p.call()
+    p.check("poison before the window")
+
+
+@pytest.mark.parametrize("typ,cache", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("total", [60, 5000])
+def test_chunk_hides_later_keys_that_are_not_finite(ctx, typ, cache, total):
+    """The last new token's key and value are poison: the rows before it do not see it."""
+    for new in (2, 50):
+        p = Paged(ctx, typ, cache, 4, 2, 64, [new], [total], page=16)
+        tab, j = p.tab.download(), total - 1
+        pg, slot = tab[0, j // 16], j % 16
+        if cache == A.I8:
+            p.ks[pg, :, slot] = p.vs[pg, :, slot] = np.inf
+            p.pool._kept[2].upload(p.ks)
+            p.pool._kept[3].upload(p.vs)
+        else:
+            for b in p.bufs:
+                x = b.download()
+                x[pg, :, slot] = _bytes(POISON[1:2], typ)[0]
+                b.upload(x)
+        p.call()
+        got = p.result()
+        k, v = p.kv[0]
+        mask = _seen(new, total, True, 0)[:-1]
+        _check(got[:-1], p.q[:-1], k, v, mask, p.scale, typ, typ, "rows before the poisoned key")
+        assert not np.isfinite(got[-1]).any()
+
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F16, A.F32], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lo,hi", [(1e-7, 1e-5), (1e-6, 4.0), (0.0, 0.01)])
+@pytest.mark.parametrize("new", [1, 60])
+def test_int8_scales_of_any_size(ctx, typ, lo, hi, new):
+    p = Paged(ctx, typ, A.I8, 4, 2, 64, [new], [400], page=16)
+    r = np.random.default_rng(4)
+    tab = p.tab.download()
+    k, v = p.kv[0]
+    codes = p.bufs[1].download()
+    for j in range(400):
+        pg, slot = tab[0, j // 16], j % 16
+        s = (np.exp(r.uniform(np.log(max(lo, 1e-7)), np.log(hi), 2)) * (lo > 0 or j % 3 > 0)).astype(np.float32)
+        p.vs[pg, :, slot] = s
+        v[j] = codes[pg, :, slot] * s[:, None].astype(np.float64)
+    p.pool._kept[3].upload(p.vs)
+    p.call()
+    p.check(f"scales {lo} to {hi}")
+
+
+def test_paged_uncovered_rows_stay(ctx):
+    """Query rows before the first sequence and after the last are nobody's."""
+    p = Paged(ctx, A.BF16, A.BF16, 4, 2, 64, [5, 40, 6], [100, 200, 30])
+    p.cu.upload(np.array([5, 45, 45, 45], np.int32))
+    p.lens.upload(np.array([200, 0, 0], np.int32))
+    tab = p.tab.download()
+    tab[0] = tab[1]
+    p.tab.upload(tab)
+    p.call()
+    got = p.result()
+    assert np.array_equal(got[:5], p.out0[:5]) and np.array_equal(got[45:], p.out0[45:])
+    k, v = p.kv[1]
+    _check(got[5:45], p.q[5:45], k, v, _seen(40, 200, True, 0), p.scale, A.BF16, A.BF16, "covered rows")
+
+
+def test_paged_many_chunks(ctx):
+    """Hundreds of tiles over a cache."""
+    r = np.random.default_rng(9)
+    new = r.integers(9, 30, 160).tolist()
+    total = [n + int(x) for n, x in zip(new, r.integers(0, 60, 160))]
+    p = Paged(ctx, A.BF16, A.BF16, 16, 4, 128, new, total, page=8)
+    p.call()
+    p.check("many chunks")
+
+
+def test_on_another_stream(ctx):
+    """A context on the caller's stream: inputs written there just before the call."""
+    p = Paged(ctx, A.BF16, A.BF16, 4, 2, 64, [1, 1], [900, 50])
+    p.call()
+    want = p.od.download()
+    q = torch.from_numpy(p.qd.download().copy()).cuda()
+    out = torch.empty_like(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    _lib.check(_lib.lib().tkv_hip_ctx_set_stream(ctx.handle, stream.cuda_stream))
+    try:
+        call = A.AttentionPaged(ctx, A.BF16, 2, 4, p.pool, 2, A.Rows(out.data_ptr() , 256, 64),
+                                A.Rows(out.data_ptr(), 256, 64), p.tab, p.tab.shape[1], p.lens, None, 1, 900,
+                                p.scale)
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                out.copy_(q)
+                call()                               # in place: each row is read before it is written
+        stream.synchronize()
+        assert np.array_equal(out.cpu().numpy().reshape(want.shape), want)
+    finally:
+        _lib.check(_lib.lib().tkv_hip_ctx_set_stream(ctx.handle, None))
 
 
 @pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F32, A.F32), (A.BF16, A.I8)])
@@ -678,6 +837,8 @@ def test_refusals(ctx):
     refused(A.AttentionPrompt, ctx, A.F32, 1, 1, 1, 64, 1, rows, rows, rows, rows, None)
     refused(A.AttentionPrompt, ctx, A.F32, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, window=-1)
     refused(A.AttentionPrompt, ctx, A.F16, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, type_out=A.BF16)
+    refused(A.AttentionPrompt, ctx, A.F32, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, scale=-1.0)
+    refused(A.AttentionPrompt, ctx, A.F32, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, scale=float("nan"))
     refused(A.AttentionPrompt, ctx, A.F32, -1, 1, 1, 64, 1, rows, rows, rows, rows, cu)
     refused(A.AttentionPrompt, ctx, A.F32, 1, 1, 1, 64, 1, A.Rows(None, 64, 64), rows, rows, rows, cu)
     refused(A.AttentionPaged, ctx, A.F16, 1, 1, pool, 1, rows, rows, cu, 1, cu)      # the cache is bf16
