@@ -26,6 +26,7 @@ namespace tkv {
 namespace attn {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Value rows of one transposed read: 16-bit, 8 rows x 32 bytes per half wave;
 // f32, rows 4 apart x 64 bytes; int8, 16 rows x 16 bytes per half wave.
@@ -68,6 +69,8 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     constexpr int BN = S::BN, CPR = S::CPR, NW = S::NW, ROWS = 16 * NB;
     constexpr int CE = Vec<T>::N, QC = DP / (4 * CE);  // 16-byte chunks of a lane's query
     constexpr int NKB = BN / 16, NDB = DP / 16;
+    // int8: the queries in digits, 24 bits from a row's largest element on (f32: 32)
+    constexpr int STEPS = (DP + 63) / 64, DIGITS = F32 ? 4 : 3;
     constexpr float kInf = __builtin_inff();
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float2 row_ml[NW][ROWS];
@@ -157,8 +160,13 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         copy_ids(0);
         copy_ids(1);
     }
-    // queries, B operand: row l15, chunk 4 i + g
-    V8 q[NB][QC];
+    const auto join_max = [](float x) {  // over the four key groups of a row
+        x = fmaxf(x, other_row(x));
+        return fmaxf(x, other_half(x));
+    };
+    // queries, B operand: row l15, chunk 4 i + g (int8: 16 elements from 64 i + 16 g on)
+    constexpr int QN = I8 ? STEPS * (16 / CE) : QC;
+    V8 q[NB][QN];
     int my_begin[NB], my_end[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
@@ -167,8 +175,8 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         const int tok = (int)div_by(a.gdiv, mine ? row : 0), h = kvh * a.g + (mine ? row : 0) - tok * a.g;
         const T* qr = static_cast<const T*>(a.q) + (int64_t)(s.q0 + tok) * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
-        for (int i = 0; i < QC; i++) {
-            const int e = (4 * i + g) * CE;
+        for (int i = 0; i < QN; i++) {
+            const int e = I8 ? 64 * (i / (16 / CE)) + 16 * g + i % (16 / CE) * CE : (4 * i + g) * CE;
             q[b][i] = V8{};
             if (mine && e < a.d) q[b][i] = *reinterpret_cast<const V8*>(qr + e);
         }
@@ -182,6 +190,50 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         if (count > 1) copy_tile(1);
         copy_ids(3);
     }
+    // int8: the elements in units of the row's largest power of two /
+    // 2^(8 DIGITS - 2), in digits of base 256 from -128 to 127
+    i32x4 qd[I8 ? NB : 1][I8 ? STEPS : 1][DIGITS];
+    float qunit[NB];  // of the lowest digit
+    if constexpr (I8) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            // NaN where the row is not finite: so are then its logits
+            float top = 0.0f, sick = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QN; i++)
+#pragma unroll
+                for (int k = 0; k < CE; k++) {
+                    const float x = fabsf(to_f32(q[b][i][k]));
+                    top = fmaxf(top, x);
+                    sick = x < kInf ? sick : 1.0f;
+                }
+            top = join_max(top);
+            const bool finite = join_max(sick) == 0.0f;
+            const int e2 = finite && top > 0.0f ? ilogbf(top) + 1 : 0;  // |x| < 2^e2
+            qunit[b] = finite ? __builtin_ldexpf(1.0f, e2 - (8 * DIGITS - 2)) : __builtin_nanf("");
+#pragma unroll
+            for (int i = 0; i < STEPS; i++)
+#pragma unroll
+                for (int j4 = 0; j4 < 4; j4++) {
+                    // v + 0x80 in every byte: its bytes are the digits + 128
+                    unsigned v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int at = 4 * j4 + k;
+                        const float x = to_f32(q[b][i * (16 / CE) + at / CE][at % CE]);
+                        const float y = __builtin_rintf(__builtin_ldexpf(x, 8 * DIGITS - 2 - e2));
+                        v[k] = (unsigned)(finite ? (int)y : 0) + 0x80808080u;
+                    }
+#pragma unroll
+                    for (int n = 0; n < DIGITS; n++) {
+                        const unsigned at = n | (4 + n) << 8;  // bytes n of two words
+                        const unsigned lo = __builtin_amdgcn_perm(v[1], v[0], at | 0x0c0c0000u);
+                        const unsigned hi = __builtin_amdgcn_perm(v[3], v[2], at << 16 | 0x0c0cu);
+                        qd[b][i][n][j4] = (int)((lo | hi) ^ 0x80808080u);
+                    }
+                }
+        }
+    }
 
     f32x4 o[NB][NDB];
     float m[NB], l[NB], vexp[NB];  // SCALED: O is in units of vexp, 0 or a power of two
@@ -191,10 +243,6 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
 #pragma unroll
         for (int n = 0; n < NDB; n++) o[b][n] = f32x4{};
     }
-    const auto join_max = [](float x) {  // over the four key groups of a row
-        x = fmaxf(x, other_row(x));
-        return fmaxf(x, other_half(x));
-    };
     const int k_swz = swz_k<CPR>(l15);  // rows 16 apart are swizzled alike
     // value rows of a transposed read: 4 g + i of a block (and + 16)
     const int v_row16 = 4 * g + (l15 >> 2), v_row8 = (l15 >> 1) < 4 ? 4 * g + (l15 >> 1) : 12 + 4 * g + (l15 >> 1);
@@ -209,35 +257,49 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         f32x4 x[NB][NKB];
 #pragma unroll
         for (int b = 0; b < NKB; b++) {
-#pragma unroll
-            for (int n = 0; n < NB; n++) x[n][b] = f32x4{};
             const char* kr = kt + (b * 16 + l15) * (CPR * 16);
+            if constexpr (I8) {
+                // the codes as they are against the queries' digits: exact sums, one
+                // rounding when they are joined (a chunk past the row's end meets
+                // digits of zero)
+                i32x4 sum[NB][DIGITS];
 #pragma unroll
-            for (int i = 0; i < QC; i++) {
-                V8 kf;
-                if constexpr (I8) {
-                    const int at = (4 * i + g) * CE;  // first element, CE bytes
-                    const char* p = kr + (((at >> 4) ^ k_swz) << 4) + (at & 15);
-                    if constexpr (F32) {
-                        const int w = *reinterpret_cast<const int*>(p);
+                for (int n = 0; n < NB; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) kf[j] = (float)(int8_t)(w >> (8 * j));
-                    } else {
-                        const i32x2 w = *reinterpret_cast<const i32x2*>(p);
+                    for (int k = 0; k < DIGITS; k++) sum[n][k] = i32x4{};
 #pragma unroll
-                        for (int j = 0; j < 8; j++) kf[j] = (T)(float)(int8_t)(w[j >> 2] >> (8 * (j & 3)));
-                    }
-                } else {
-                    kf = *reinterpret_cast<const V8*>(kr + (((4 * i + g) ^ k_swz) << 4));
+                for (int i = 0; i < STEPS; i++) {
+                    const i32x4 kf = *reinterpret_cast<const i32x4*>(kr + (((4 * i + g) ^ k_swz) << 4));
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+#pragma unroll
+                        for (int k = 0; k < DIGITS; k++)
+                            sum[n][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[n][i][k], sum[n][k], 0, 0, 0);
                 }
 #pragma unroll
-                for (int n = 0; n < NB; n++) {
-                    if constexpr (F32) {
+                for (int n = 0; n < NB; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            x[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], q[n][i][j], x[n][b], 0, 0, 0);
-                    } else {
-                        x[n][b] = mfma16(kf, q[n][i], x[n][b]);
+                    for (int j = 0; j < 4; j++) {
+                        float y = (float)sum[n][DIGITS - 1][j];
+#pragma unroll
+                        for (int k = DIGITS - 2; k >= 0; k--) y = __builtin_fmaf(y, 256.0f, (float)sum[n][k][j]);
+                        x[n][b][j] = y;
+                    }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NB; n++) x[n][b] = f32x4{};
+#pragma unroll
+                for (int i = 0; i < QC; i++) {
+                    const V8 kf = *reinterpret_cast<const V8*>(kr + (((4 * i + g) ^ k_swz) << 4));
+#pragma unroll
+                    for (int n = 0; n < NB; n++) {
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                x[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], q[n][i][j], x[n][b], 0, 0, 0);
+                        } else {
+                            x[n][b] = mfma16(kf, q[n][i], x[n][b]);
+                        }
                     }
                 }
             }
@@ -252,7 +314,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                 if constexpr (I8) {
                     const f32x4 ks4 = *reinterpret_cast<const f32x4*>(sk + b * 16 + 4 * g);
                     const f32x4 vs4 = *reinterpret_cast<const f32x4*>(sk + 64 + b * 16 + 4 * g);
-                    x[n][b] *= ks4;
+                    x[n][b] *= ks4 * qunit[n];
 #pragma unroll
                     for (int j = 0; j < 4; j++) vs[b * 4 + j] = vs4[j];
                 }
