@@ -461,6 +461,18 @@ def test_chunk_long(ctx, typ, cache, new, total):
     assert np.array_equal(first, p.od.download()), "two runs differ"
 
 
+@pytest.mark.parametrize("typ,cache", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("new,total", [([5], [20000]), ([17, 6], [20000, 9000])])
+def test_chunk_over_many_splits(ctx, typ, cache, new, total):
+    """Over 16 (and over 64) splits of the keys, joined in two levels."""
+    p = Paged(ctx, typ, cache, 8, 1, 64, new, total, page=256)
+    p.call()
+    p.check("chunk of many splits")
+    first = p.od.download()
+    p.call()
+    assert np.array_equal(first, p.od.download()), "two runs differ"
+
+
 @pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F32, A.F32), (A.F16, A.I8)])
 @pytest.mark.parametrize("causal,window", [(True, 64), (False, 0)])
 def test_chunk_masks(ctx, typ, cache, causal, window):

@@ -77,8 +77,7 @@ struct AttnArgs {
     // sum_bytes for every workgroup of the grid (and, above kJoin splits, for
     // every kJoin of them)
     int32_t splits, units;
-    int32_t narrow;       // 128-row tiles: the kernel with 32 keys a tile, where there is one
-    int32_t split_tiles;  // key tiles of a split; more where there would be more splits
+    int32_t narrow;  // 128-row tiles: the kernel with 32 keys a tile, where there is one
     char* sums;
     int64_t sum_bytes;
     unsigned* arrivals;

@@ -108,7 +108,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
     int splits = 1;  // that have tiles
     if (a.splits > 1 && t1 > t0) {
-        const int per = max(a.split_tiles, (t1 - t0 + a.splits - 1) / a.splits);
+        const int per = (t1 - t0 + a.splits - 1) / a.splits;
         splits = (t1 - t0 + per - 1) / per;
         t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
@@ -479,8 +479,8 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
         put_sum(sum + ROWS + QUADS + i, y[2], y[3]);
     };
     for (int i = tid; i < QUADS; i += 64 * NW) {
-        const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = r;
-        if (row >= rows || e >= a.d || row_bad[r]) continue;
+        const int r = i / (DP / 4), e = 4 * (i % (DP / 4));
+        if (r >= rows || e >= a.d || row_bad[r]) continue;
         float mm = -kInf;
 #pragma unroll
         for (int w = 0; w < NW; w++) mm = fmaxf(mm, row_ml[w][r].x);
@@ -498,14 +498,13 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
             if (e == 0) put_sum(sum + r, mm, ll);
             put_quad(sum, i, y);
         } else {
-            const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+            const int tok = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tok * a.g;
             put_out4<T>(a, s.q0 + tok, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
         }
     }
     for (int r = wave; r < ROWS; r += NW) {
-        const int row = r;
-        if (row >= rows || !uniform(row_bad[r])) continue;
-        const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+        if (r >= rows || !uniform(row_bad[r])) continue;
+        const int tok = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tok * a.g;
         const int64_t t_at = s.q0 + tok;
         const T* qr = static_cast<const T*>(a.q) + t_at * a.q_st + (int64_t)h * a.q_sh;
         float mm, ll, acc[4];
@@ -533,8 +532,8 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     const auto join = [&](auto most, int from, int n, int to) __attribute__((always_inline)) {
         constexpr int MOST = decltype(most)::value;
         for (int i = tid; i < QUADS; i += 64 * NW) {
-            const int r = i / (DP / 4), e = 4 * (i % (DP / 4)), row = r;
-            if (row >= rows || e >= a.d) continue;
+            const int r = i / (DP / 4), e = 4 * (i % (DP / 4));
+            if (r >= rows || e >= a.d) continue;
             float2 ml[MOST], lo[MOST], hi[MOST];
 #pragma unroll
             for (int k = 0; k < MOST; k++) {
@@ -558,7 +557,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                 if (e == 0) put_sum(sum_of(to) + r, mm, ll);
                 put_quad(sum_of(to), i, y);
             } else {
-                const int tok = (int)div_by(a.gdiv, (uint32_t)row), h = kvh * a.g + row - tok * a.g;
+                const int tok = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tok * a.g;
                 put_out4<T>(a, s.q0 + tok, h, e, y * (ll == 0.0f ? 1.0f : 1.0f / ll));
             }
         }

@@ -26,7 +26,6 @@
 namespace tkv {
 namespace attn {
 
-
 // DP: head size, padded (64, 96, 128, 192, 256; f32 96 only as 128).  Keys of a
 // tile: as many as two workgroups per CU have registers and LDS for, 64 where the
 // maximum, the rescaling test and the barrier of a tile spread over more of them.
@@ -96,7 +95,7 @@ void k_attn_tile(AttnArgs a) {
     int t0 = kb / BN, t1 = ke > kb ? (ke + BN - 1) / BN : t0;
     int splits = 1;  // that have tiles
     if (a.splits > 1 && t1 > t0) {
-        const int per = max(a.split_tiles, (t1 - t0 + a.splits - 1) / a.splits);
+        const int per = (t1 - t0 + a.splits - 1) / a.splits;
         splits = (t1 - t0 + per - 1) / per;
         t0 += (int)blockIdx.y * per;
         t1 = min(t0 + per, t1);
@@ -458,16 +457,19 @@ void k_attn_tile(AttnArgs a) {
     unsigned again = uniform((unsigned)ball | (unsigned)(ball >> 32));
 
     // a split's sums, in this kernel's register layout
-    u64* const mine_sum = split ? reinterpret_cast<u64*>(a.sums + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) *
-                                                                      a.sum_bytes) : nullptr;
-    if (split && !((again >> l31) & 1)) {
-        if (half == 0) put_sum(mine_sum + wave * 32 + l31, m, l);
+    const auto sum_of = [&](int i) {
+        return reinterpret_cast<u64*>(a.sums + ((int64_t)i * gridDim.x + blockIdx.x) * a.sum_bytes);
+    };
+    const auto put_sums = [&](u64* sum) __attribute__((always_inline)) {
+        if (half == 0) put_sum(sum + wave * 32 + l31, m, l);
 #pragma unroll
         for (int b = 0; b < NDB; b++)
 #pragma unroll
             for (int e = 0; e < 16; e += 2)
-                put_sum(mine_sum + kTileRows + (b * 8 + e / 2) * 256 + tid, o[b][e] * vexp, o[b][e + 1] * vexp);
-    }
+                put_sum(sum + kTileRows + (b * 8 + e / 2) * 256 + tid, o[b][e] * vexp, o[b][e + 1] * vexp);
+    };
+    u64* const mine_sum = split ? sum_of(blockIdx.y) : nullptr;
+    if (split && !((again >> l31) & 1)) put_sums(mine_sum);
     for (unsigned todo = again; todo; todo &= todo - 1) {
         const int i = __builtin_ctz(todo);
         const int r = wrow + i, tk = (int)div_by(a.gdiv, (uint32_t)r), h = kvh * a.g + r - tk * a.g;
@@ -492,30 +494,42 @@ void k_attn_tile(AttnArgs a) {
         }
     }
     if (split) {
-        unsigned* counter = a.arrivals + blockIdx.x * (1 + kJoin);
-        if (!arrive_last(counter, splits)) return;
-        arrive_clear(counter, splits);
         // the unit's last workgroup joins its splits, in their order:
         //   O = sum_s 2^(m_s - m) O_s,  l = sum_s 2^(m_s - m) l_s
-        m = -kInf, l = 0.0f, vexp = 1.0f;
-        for (int k = 0; k < splits; k++) {
-            const u64* sum = reinterpret_cast<const u64*>(a.sums + ((int64_t)k * gridDim.x + blockIdx.x) * a.sum_bytes);
-            const float2 ml = get_sum(sum + wave * 32 + l31);
-            float2 y[NDB * 8];
+        // Above kJoin of them the last workgroup of each kJoin joins those first.
+        unsigned* const counter = a.arrivals + blockIdx.x * (1 + kJoin);
+        const int group = blockIdx.y / kJoin;
+        bool top = splits <= kJoin;
+        int from = top ? 0 : group * kJoin, n = top ? splits : min(kJoin, splits - from);
+        for (;;) {
+            unsigned* const count = counter + (top ? 0 : 1 + group);
+            if (!arrive_last(count, n)) return;
+            arrive_clear(count, n);
+            m = -kInf, l = 0.0f, vexp = 1.0f;
+            for (int k = 0; k < n; k++) {
+                const u64* sum = sum_of(from + k);
+                const float2 ml = get_sum(sum + wave * 32 + l31);
+                float2 y[NDB * 8];
 #pragma unroll
-            for (int e = 0; e < NDB * 8; e++) y[e] = get_sum(sum + kTileRows + e * 256 + tid);
-            const float mn = fmaxf(m, ml.x), base = mn == -kInf ? 0.0f : mn;
-            const float fix = __builtin_amdgcn_exp2f(m - base), w = __builtin_amdgcn_exp2f(ml.x - base);
-            m = mn;
-            l = l * fix + ml.y * w;
+                for (int e = 0; e < NDB * 8; e++) y[e] = get_sum(sum + kTileRows + e * 256 + tid);
+                const float mn = fmaxf(m, ml.x), base = mn == -kInf ? 0.0f : mn;
+                const float fix = __builtin_amdgcn_exp2f(m - base), w = __builtin_amdgcn_exp2f(ml.x - base);
+                m = mn;
+                l = l * fix + ml.y * w;
 #pragma unroll
-            for (int b = 0; b < NDB; b++)
+                for (int b = 0; b < NDB; b++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float v = e & 1 ? y[b * 8 + e / 2].y : y[b * 8 + e / 2].x;
-                    // a sum that nothing was added to may follow one that is not finite
-                    o[b][e] = (k == 0 ? 0.0f : o[b][e] * fix) + (w == 0.0f ? 0.0f : v * w);
-                }
+                    for (int e = 0; e < 16; e++) {
+                        const float v = e & 1 ? y[b * 8 + e / 2].y : y[b * 8 + e / 2].x;
+                        // a sum that nothing was added to may follow one that is not finite
+                        o[b][e] = (k == 0 ? 0.0f : o[b][e] * fix) + (w == 0.0f ? 0.0f : v * w);
+                    }
+            }
+            if (top) break;
+            put_sums(sum_of(a.splits + group));
+            top = true;
+            from = a.splits;
+            n = (splits + kJoin - 1) / kJoin;
         }
         again = 0;
     }
