@@ -79,13 +79,21 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     a.units = (int32_t)units;
     const int64_t tiles = (few ? a.seqs : std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs)) * a.hkv;
     // Splits over the keys: as many as fill the chip once, 128 keys (streaming) or
-    // 256 (tiles) at least to each.  Streaming, up to eight times as many where each
-    // still has 512 KB to read, so that caches of different lengths even out: a
-    // workgroup's start and end take as long as reading about 100 KB.
-    // f32 products take 16 times as long: twice as many there.  Heads of 64 let
-    // three workgroups share a CU.
-    const int64_t slots = (few ? 2 : type == TKV_HIP_F32 ? 4 : a.d <= 64 ? 3 : 2) * c->num_cus;
-    int64_t want = std::min<int64_t>(slots / tiles, keys / (few ? 128 : 256));
+    // 256 (tiles) at least to each; a split of fewer costs more in the join than it
+    // saves (200 tokens of 12 heads over 2200 keys in 8 splits 19.1 us, in 17 25.7).
+    // f32 products take eight times as long: there 64 keys are enough as long as no
+    // CU gets a second workgroup (12 heads of 64, 256 tokens 24.1 -> 14.5 us, 512
+    // 28.9 -> 20.7; 768 tokens in 4 splits, 288 workgroups, 39 us, in 3 30).
+    // Workgroups that fill the chip: two per CU; three with heads of 64 (2048 tokens
+    // of 12 heads 26.6 -> 23.7 us, f32 127 -> 86; in four 95); four f32 ones with
+    // larger heads, which even out (2048 tokens of 32 heads of 128: 376 -> 331 us).
+    // Streaming, up to eight times as many splits where each still has 512 KB to
+    // read, so that caches of different lengths even out: a workgroup's start and
+    // end take as long as reading about 100 KB.
+    const int64_t slots = (few ? 2 : a.d <= 64 ? 3 : type == TKV_HIP_F32 ? 4 : 2) * c->num_cus;
+    int64_t want = keys / (few ? 128 : 256);
+    if (!few && type == TKV_HIP_F32) want = std::max(want, std::min<int64_t>(keys / 64, c->num_cus / tiles));
+    want = std::min(want, slots / tiles);
     if (few)
         want = std::max(want, std::min<int64_t>(8 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
     a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kMaxSplits);
