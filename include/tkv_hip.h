@@ -597,7 +597,7 @@ int32_t tkv_hip_dev_rope_table(int64_t ctx, int64_t positions, int64_t rot_dim,
  *     be the inputs themselves where the types agree and heads do not overlap.
  *   cache (0: none): token t's k and v go to pool slot slots[t]; a slot outside
  *     the pool appends nothing.  Cache types: type_out, or I8, whose rows are
- *     coded from the f32 values as scale = fl32(max(max|x|, 1e-8) / 127),
+ *     coded from the f32 values as scale = fl32(max(max|x|, 1e-8) * fl32(1 / 127)),
  *     code = clamp(rne(fl32(x * fl32(1 / scale))), -127, 127), NaN 0.
  * A position outside [0, table_len) marks a padding token: its q_out and k_out
  * rows are zeros and it is not appended.  q, k, v may be NULL with their head
@@ -619,11 +619,14 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
  *   a_ij = scale * q_i . k_j, m_i = max_j a_ij,
  * over the keys j in [0, t) that it sees: all of them, only j <= pos where
  * causal != 0, and only j > pos - window where window > 0; scale >= 0.  A row
- * that sees no key (or whose logits are all -inf) gives zeros; what a row does not see (NaN and infinities included) does
- * not touch it.  Query head h reads key / value head h / (heads_q / heads_kv).
+ * that sees no key (or whose logits are all -inf) gives zeros; what a row does
+ * not see (NaN and infinities included) does not touch it.  Query head h reads key / value head h / (heads_q / heads_kv).
  * Statistics and sums are f32.  For f16 and bf16 the products run on the
  * matrix units from values of that type, the weights exp(a - m) rounded to it
- * for the second product; f32 stays f32 throughout.  type_out: `type`, or F32
+ * for the second product; f32 stays f32 throughout.  An int8 cache's codes are
+ * exact in every type; its keys' scales multiply the logits, its values' scales
+ * the weights before that rounding.  out may be q itself where the types agree.
+ * Results do not depend on timing: splits are joined in their order.  type_out: `type`, or F32
  * (the unrounded sums of the same computation).  head_dim <= 256; sizes that
  * are multiples of 16 bytes with 16-byte aligned rows take the fast kernels.
  * Length arrays are read on the device and clamped to the tokens and pages

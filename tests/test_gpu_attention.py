@@ -784,7 +784,7 @@ def test_rope_append(ctx, tin, tout, cache, layout, hq, hkv, d, rot, tokens):
     for buf, scales, y in ((kb, sc[0], turned[put, hq:]), (vb, sc[1], x[put, hq + hkv:])):
         want = old.copy()
         if cache == A.I8:
-            scale = (np.maximum(np.abs(y).max(-1), np.float32(1e-8)) / np.float32(127)).astype(np.float32)
+            scale = np.maximum(np.abs(y).max(-1), np.float32(1e-8)) * (np.float32(1) / np.float32(127))
             inv_s = np.float32(1) / scale
             want[at, :, slot] = np.clip(np.rint(y * inv_s[..., None]), -127, 127).astype(np.int8)
             ws = np.full((pages, hkv, page), 9.0, np.float32)

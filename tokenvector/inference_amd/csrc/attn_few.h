@@ -6,18 +6,32 @@
 // to the wave's part of LDS (global_load_lds, two buffers), page ids two tiles
 // further ahead (four small buffers), so that between one and two tiles per
 // wave, 64 to 128 KB per CU, are always on their way.  Tiles are small, so that
-// two workgroups fit a CU and one's start and end run beside the other's stream.  Every vector memory
-// operation of the loop is such a copy, so the waits count them exactly.
+// two workgroups fit a CU and one's start and end run beside the other's stream.
+// Every vector memory operation of the loop is such a copy, so the waits count
+// them exactly.
 //
 // The products are transposed as in the 128-row kernel, with 16 x 16
 // accumulators: a lane owns query row lane & 15 of each block of 16 rows, and
 // its group g = lane >> 4 holds keys 16 b + 4 g .. + 3 of key block b, which is
-// again the weights' layout as a B operand.  int8 caches are copied as codes:
-// converted when read (V by a byte transpose read), the keys' scales multiply
-// the logits, the values' scales the weights.
+// again the weights' layout as a B operand.
+//
+// int8 caches are copied as codes, and converting them would take more of the
+// vector unit than everything else (64 sequences of 8000 keys at most: 153 us).
+// So the keys' codes are multiplied as they are, on the INT8 matrix units, with
+// the queries split into digits of base 256: q = u (d0 + 256 d1 + 65536 d2), u the
+// power of two that gives the row's largest element 22 bits and a sign (f32 rows:
+// four digits, 30 bits).  bf16 and f16 elements down to 2^-14 and 2^-11 of the
+// largest are exact; smaller ones are off by 2^-23 of it at most, as a sum in f32
+// would be.  The digits' sums are exact in INT32, and three roundings join them.
+// The values' codes are converted after a byte transpose read; the keys' scales
+// multiply the logits, the values' scales the weights.
 //
 // At the end the workgroup's waves are joined through LDS, in order, and the
 // splits of the keys over workgroups by the unit's last workgroup, in order.
+//
+// Measured: 32 sequences of up to 32768 keys, 8 heads of 128, bf16: 355 us, 5.45
+// TB/s; 64 of up to 8000, int8: 133 us, 4.4 TB/s; one token over 1000 keys of 12
+// heads of 64: 7.1 us, of which launch, first loads and join are all but one.
 #pragma once
 
 #include "attn_mfma.h"
