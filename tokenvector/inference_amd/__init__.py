@@ -8,6 +8,8 @@ Submodules:
                   for graphs of quantized nodes
     device        device-pointer API: contexts, buffers, packed kernels,
                   resident quantized weights and the W8A8 linear
+    attention     rotary positions, paged caches, attention of prompts and of
+                  new tokens over a cache
     _lib          ctypes binding of libtkv_hip.so (C ABI in include/tkv_hip.h)
 """
 from . import _lib

@@ -31,7 +31,7 @@
 //
 // Measured: 32 sequences of up to 32768 keys, 8 heads of 128, bf16: 355 us, 5.45
 // TB/s; 64 of up to 8000, int8: 133 us, 4.4 TB/s; one token over 1000 keys of 12
-// heads of 64: 7.1 us, of which launch, first loads and join are all but one.
+// heads of 64: 7.1 us, most of it launch, first loads and join.
 #pragma once
 
 #include "attn_mfma.h"

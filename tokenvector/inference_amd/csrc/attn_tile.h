@@ -23,15 +23,16 @@
 // Measured: 16384 f16 tokens of 16 / 4 heads of 128 in 1.18 ms, 933 TFLOP/s (a
 // library product of 8192^3: 1160); 4 x 512 new tokens over 16384 cached ones, 32 /
 // 8 heads, 0.61 ms, 911; f32, 4096 tokens of 12 heads of 64, 283 us, 91 (library:
-// 154).  There the matrix units and the LDS reads that feed them (a 32-row wave
-// needs one for every product) bound it.  Short rows are bound by latency: a wave
-// alone takes 0.9 us (heads of 64) to 1.6 us (128) for a tile of 64 keys, LDS reads,
-// products and exponentials after each other, and 5 us to start and end: 8 x 1024
-// tokens of 12 heads of 64 30 us, 434 TFLOP/s.  What did not help: 64 rows per wave
-// (half the LDS reads, half the waves: 16384 tokens of heads of 64 467 -> 515 us, 8
-// x 1024 30 -> 42), two teams of four waves with every other tile each (30 -> 36),
-// three buffers (no change: the copies are there in time), products of the next
-// tile between the exponentials of this one (registers: 1.14 -> 2.36 ms).
+// 154).  There the matrix units are busy in 50 % of the cycles and the vector units
+// in 47 %, LDS in 25 % (no bank conflicts): the two waves of a SIMD rarely have one
+// multiply while the other takes exponentials.  Short rows are bound by latency: a
+// wave alone takes 0.9 us (heads of 64) to 1.6 us (128) for a tile of 64 keys, LDS
+// reads, products and exponentials after each other, and 5 us to start and end: 8 x
+// 1024 tokens of 12 heads of 64 30 us, 434 TFLOP/s.  What did not help: 64 rows
+// per wave (half the LDS reads, half the waves: 16384 tokens of heads of 64 467 ->
+// 515 us, 8 x 1024 30 -> 42), two teams of four waves with every other tile each (30
+// -> 36), three buffers (no change: the copies are there in time), products of the
+// next tile between the exponentials of this one (registers: 1.14 -> 2.36 ms).
 #pragma once
 
 #include "attn_mfma.h"
