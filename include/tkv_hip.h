@@ -645,8 +645,8 @@ int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, 
                                      int32_t causal, int64_t window);
 /* New tokens over a paged cache: sequence s has the query rows cu_q[s] ..
  * cu_q[s + 1] (cu_q NULL: the one row s) and the first kv_lens[s] tokens of the
- * pages page_table[s * table_stride ..], its new tokens (already appended) the
- * last of them.  The cache's type is `type` or I8.  max_q and max_kv (0: not
+ * pages page_table[s * table_stride ..] (table_stride below 2^31), its new
+ * tokens (already appended) the last of them.  The cache's type is `type` or I8.  max_q and max_kv (0: not
  * known): the longest of the sequences' query rows and cache lengths, which
  * choose the launch shape alone: longer sequences are still right. */
 int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, int64_t heads_q,

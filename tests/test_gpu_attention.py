@@ -876,3 +876,35 @@ def test_refusals(ctx):
     with pytest.raises(ValueError):
         _lib.check(_lib.lib().tkv_hip_dev_attention_paged(ctx.handle, A.BF16, 1, 1, 0, 1, None, None,
                                                           A.BF16, None, 0, None, None, 0, 0, 1.0, 1, 0))
+
+
+def test_paged_refuses_tables_without_bound(ctx):
+    """A row of 2^31 page ids: its keys would pass the kernels' 32-bit key numbers."""
+    z, cu = _dev(ctx, np.zeros(256, np.float32)), _i32(ctx, [0, 1])
+    rows = A.Rows(z, 64, 64)
+    pool = A.KVCache(ctx, A.F32, 1, 16, 1, 64)
+    for stride in (-1, 1 << 31, 1 << 62):
+        with pytest.raises(ValueError):
+            A.AttentionPaged(ctx, A.F32, 1, 1, pool, 1, rows, rows, cu, stride, cu)()
+
+
+@pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F32, A.I8)])
+def test_paged_bounds_beyond_every_size(ctx, typ, cache):
+    """max_q and max_kv of 2^62 are bounds as well."""
+    p = Paged(ctx, typ, cache, 4, 1, 128, [1, 30, 2], [300, 100, 3])
+    call = A.AttentionPaged(ctx, typ, 33, 4, p.pool, 3, A.Rows(p.qd, 512, 128), A.Rows(p.od, 512, 128),
+                            p.tab, p.tab.shape[1], p.lens, p.cu, 1 << 62, 1 << 62, p.scale)
+    call()
+    p.check("bounds beyond every size")
+
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F32], ids=lambda t: NAME[t])
+def test_prompt_largest_scale(ctx, typ):
+    """Keys of zero have logits of zero at any finite scale: equal weights."""
+    p = Prompt(ctx, typ, 2, 2, 64, [70], scale=float(np.finfo(np.float32).max))
+    x = p.x.reshape(-1, 6, 64)
+    x[:, 2:4] = 0
+    p.xd.upload(_bytes(p.x.reshape(-1), typ))
+    p.call()
+    got = p.result()[:70]
+    _check(got, x[:70, :2], x[:70, 2:4], x[:70, 4:], _seen(70, 70, True, 0), 0.0, typ, typ, "largest scale")

@@ -47,8 +47,8 @@ static void common_args(AttnArgs* a, int32_t type, int32_t type_out, int64_t tok
     a->causal = causal != 0;
     a->window = window;
     // a scale of zero (equal weights) as one that no finite logit notices, so
-    // that hidden logits of -inf stay -inf
-    a->scale_log2 = std::max((float)((double)scale * 1.4426950408889634), 1e-30f);
+    // that hidden logits of -inf stay -inf; and finite, so that those of zero stay zero
+    a->scale_log2 = (float)std::min(std::max((double)scale * 1.4426950408889634, 1e-30), 3.4028234e38);
     a->out_f32 = type_out == TKV_HIP_F32;
 }
 
@@ -177,7 +177,7 @@ int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, i
                                sequences, q, out, scale, window));
     if (kv->type != type && kv->type != TKV_HIP_I8)
         return set_error(TKV_HIP_BAD_ARG, "attention_paged: the cache's type is neither type nor I8");
-    if (table_stride < 0 || max_q < 0 || max_kv < 0 ||
+    if (table_stride < 0 || table_stride >= (1ll << 31) || max_q < 0 || max_kv < 0 ||
         (sequences > 0 && (!kv_lens || (table_stride > 0 && !page_table))))
         return set_error(TKV_HIP_BAD_ARG, "attention_paged: bad page table, lengths or bounds");
     if (!cu_q && tokens != sequences)
@@ -203,7 +203,7 @@ int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, i
     a.cu_q = cu_q;
     a.kv_lens = kv_lens;
     const int64_t held = table_stride * kv->page;
-    return launch_attention(c, a, type, kv->type, max_q, max_kv ? std::min(max_kv, held) : held);
+    return launch_attention(c, a, type, kv->type, std::min(max_q, tokens), max_kv ? std::min(max_kv, held) : held);
 }
 
 }  // extern "C"
