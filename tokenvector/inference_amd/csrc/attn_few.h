@@ -250,10 +250,10 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     }
 
     f32x4 o[NB][NDB];
-    float m[NB], l[NB], vexp[NB];  // SCALED: O is in units of vexp, 0 or a power of two
+    float m[NB], l[NB], vexp[NB], wtop[NB];  // SCALED: O is in units of vexp (product_unit)
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        m[b] = -kInf, l[b] = 0.0f, vexp[b] = SCALED ? 0.0f : 1.0f;
+        m[b] = -kInf, l[b] = 0.0f, vexp[b] = SCALED ? 0.0f : 1.0f, wtop[b] = 0.0f;
 #pragma unroll
         for (int n = 0; n < NDB; n++) o[b][n] = f32x4{};
     }
@@ -351,6 +351,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                 const float fix = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
                 m[n] = mn;
                 l[n] *= fix;
+                if constexpr (SCALED) wtop[n] *= fix;
 #pragma unroll
                 for (int d = 0; d < NDB; d++) o[n][d] *= fix;
             }
@@ -363,29 +364,30 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                     l[n] += x[n][b][j];
                 }
             if constexpr (I8) {
-                if constexpr (SCALED) {
-                    // f16 weights times scales of any size: O is kept in units of
-                    // the largest scale's power of two so far
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < BN / 4; i++) top = fmaxf(top, vs[i]);
-                    top = join_max(top);
-                    const float unit2 = top > 0.0f && top < kInf
-                                            ? __builtin_ldexpf(1.0f, max(ilogbf(top), -100)) : 0.0f;
-                    if (__any(unit2 > vexp[n])) {
-                        const float nu = fmaxf(unit2, vexp[n]), fix = nu > 0.0f ? vexp[n] / nu : 1.0f;
-                        vexp[n] = nu;
-#pragma unroll
-                        for (int d = 0; d < NDB; d++) o[n][d] *= fix;
-                    }
-                    const float inv = vexp[n] > 0.0f ? 1.0f / vexp[n] : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < BN / 4; i++) vs[i] *= inv;
-                }
 #pragma unroll
                 for (int b = 0; b < NKB; b++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[n][b][j] *= vs[b * 4 + j];
+                if constexpr (SCALED) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < NKB; b++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(x[n][b][j]));
+                    wtop[n] = fmaxf(wtop[n], join_max(top));
+                    const float unit = product_unit(vexp[n], wtop[n]);
+                    if (__any(unit != vexp[n])) {
+                        const float fix = vexp[n] * inverse_unit(unit);
+                        vexp[n] = unit;
+#pragma unroll
+                        for (int d = 0; d < NDB; d++) o[n][d] *= fix;
+                    }
+                    const float inv = inverse_unit(vexp[n]);
+#pragma unroll
+                    for (int b = 0; b < NKB; b++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[n][b][j] *= inv;
+                }
             }
         }
         // values: steps of 32 keys (blocks 2 st and 2 st + 1) or of 16
@@ -475,7 +477,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
 #pragma unroll
         for (int d = 0; d < NDB; d++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) bad |= !(fabsf(o[n][d][j]) < kInf);
+            for (int j = 0; j < 4; j++) bad |= !(fabsf(o[n][d][j] * vexp[n]) < kInf);
             *reinterpret_cast<f32x4*>(sums + (n * 16 + l15) * DP + d * 16 + 4 * g) = o[n][d] * vexp[n];
         }
         if (bad) row_bad[n * 16 + l15] = 1;

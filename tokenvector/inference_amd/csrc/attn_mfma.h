@@ -151,6 +151,24 @@ __device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first)
     return uniform(found);
 }
 
+// f16 weights over an int8 cache: each weight is multiplied by its value's scale,
+// and the products reach over more octaves than f16 has, so they are taken, and O
+// is kept, in units of a power of two.  The unit follows the row's largest product
+// so far, `top`, in the weights' present base (never the scales alone: a key of no
+// weight may have any).  It is raised at once, to 2^14 below the product, and
+// lowered once that is over 2^8 too high: a product is off by 2^-11 of itself or
+// 2^-31 of the largest.  0 while every product is.
+__device__ __forceinline__ float product_unit(float unit, float top) {
+    const int e = (int)(__float_as_uint(top) >> 23);  // top >= 0; 255: not finite
+    if (top == 0.0f || e == 255) return unit;
+    const float u = __uint_as_float((unsigned)max(e - 14, 27) << 23);  // 2^-100 at least
+    return u > unit || u < unit * 0x1p-8f ? fmaxf(u, unit * 0x1p-100f) : unit;
+}
+// 1 / unit (2^127 for 0).
+__device__ __forceinline__ float inverse_unit(float unit) {
+    return __uint_as_float((254u << 23) - __float_as_uint(unit));
+}
+
 // Partial sums of a split, written where the unit's last workgroup, on whatever
 // XCD, reads them (agent scope: past this XCD's L2; see arrive_last).  8 bytes is
 // the widest such access, so sums are laid out for lanes to be 8 bytes apart: a

@@ -292,7 +292,7 @@ void k_attn_tile(AttnArgs a) {
     for (int b = 0; b < NDB; b++) o[b] = f32x16{};
     float m = -kInf, l = 0.0f;
     constexpr bool SCALED = I8 && std::is_same<T, _Float16>::value;
-    float vexp = SCALED ? 0.0f : 1.0f;  // SCALED: O is in units of vexp, 0 or a power of two
+    float vexp = SCALED ? 0.0f : 1.0f, wtop = 0.0f;  // SCALED: O is in units of vexp (product_unit)
 
     // LDS offsets of this lane's reads
     const int k_row = l31 * (CPR * 16), k_swz = swz_k<CPR>(l31);
@@ -379,6 +379,7 @@ void k_attn_tile(AttnArgs a) {
                 const float fix = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= fix;
+                if constexpr (SCALED) wtop *= fix;
 #pragma unroll
                 for (int b = 0; b < NDB; b++)
 #pragma unroll
@@ -395,31 +396,32 @@ void k_attn_tile(AttnArgs a) {
                 }
             l += sum;
             if constexpr (I8) {
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[b][e] *= vs[b * 16 + e];
                 if constexpr (SCALED) {
-                    // f16 weights times scales of any size: O is kept in units of
-                    // the largest scale's power of two so far
                     float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < NKB * 16; i++) top = fmaxf(top, vs[i]);
-                    top = fmaxf(top, other_half(top));
-                    const float unit2 = top > 0.0f && top < kInf
-                                            ? __builtin_ldexpf(1.0f, max(ilogbf(top), -100)) : 0.0f;
-                    if (__any(unit2 > vexp)) {
-                        const float nu = fmaxf(unit2, vexp), fix = nu > 0.0f ? vexp / nu : 1.0f;
-                        vexp = nu;
+                    for (int b = 0; b < NKB; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[b][e]));
+                    wtop = fmaxf(wtop, fmaxf(top, other_half(top)));
+                    const float unit = product_unit(vexp, wtop);
+                    if (__any(unit != vexp)) {
+                        const float fix = vexp * inverse_unit(unit);
+                        vexp = unit;
 #pragma unroll
                         for (int b = 0; b < NDB; b++)
 #pragma unroll
                             for (int e = 0; e < 16; e++) o[b][e] *= fix;
                     }
-                    const float inv = vexp > 0.0f ? 1.0f / vexp : 0.0f;
+                    const float inv = inverse_unit(vexp);
 #pragma unroll
-                    for (int i = 0; i < NKB * 16; i++) vs[i] *= inv;
+                    for (int b = 0; b < NKB; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[b][e] *= inv;
                 }
-#pragma unroll
-                for (int b = 0; b < NKB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[b][e] *= vs[b * 16 + e];
             }
             if constexpr (F32) {
 #pragma unroll
@@ -466,7 +468,7 @@ void k_attn_tile(AttnArgs a) {
 #pragma unroll
     for (int b = 0; b < NDB; b++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) bad |= !(fabsf(o[b][e]) < kInf);
+        for (int e = 0; e < 16; e++) bad |= !(fabsf(o[b][e] * vexp) < kInf);
     const unsigned long long ball = __ballot(bad && mine);
     unsigned again = uniform((unsigned)ball | (unsigned)(ball >> 32));
 
