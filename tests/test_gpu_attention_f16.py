@@ -120,3 +120,60 @@ def test_int8_scales_far_apart_in_weight_and_size(ctx, new):
     p = Scales(ctx, new, 400, far, A.F32)
     p.call()
     p.check("products of every size")
+
+
+def _tail(r, tokens, heads, d, sink, at):
+    """Queries of 0.5 to 1 and keys that they see as a sink `sink` octaves (at scale
+    1 / 8) above a long tail; values of the tail about 1, the sink's about 2^-10."""
+    q = _round(r.uniform(0.5, 1.0, (tokens, heads, d)), A.F16)
+    k = _round(r.uniform(-0.02, 0.02, (tokens, heads, d)), A.F16)
+    v = _round(r.uniform(0.5, 1.5, (tokens, heads, d)), A.F16)
+    k[at] = _round(np.full((heads, d), sink * np.log(2.0) / 6.0 * 64 / d), A.F16)
+    v[at] = _round(v[at] * 2.0 ** -10, A.F16)
+    return q, k, v
+
+
+@pytest.mark.parametrize("typ_out", [A.F16, A.F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 700])
+@pytest.mark.parametrize("sink", [26.0, 30.0])
+def test_prompt_tail_below_a_sink(ctx, typ_out, d, at, sink):
+    """Keys of 2^-26 and 2^-30 of the largest weight, and the larger values, have their part."""
+    n = 1500
+    say(f"f16 prompt of {n}, sink {sink} octaves up at {at}, heads of {d}")
+    p = Prompt(ctx, A.F16, 2, 2, d, [n], typ_out=typ_out, scale=0.125)
+    q, k, v = _tail(np.random.default_rng(11), n, 2, d, sink, at)
+    x = p.x.reshape(-1, 6, d)
+    x[:n] = np.concatenate([q, k, v], 1)
+    p.xd.upload(_bytes(p.x.reshape(-1), A.F16))
+    p.call()
+    _check_f16(p.result()[:n], q, k, v, _seen(n, n, True, 0), 0.125, typ_out, 2.0 ** -32,
+               np.abs(v).max(2).astype(np.float64), "a prompt's tail below a sink")
+
+
+@pytest.mark.parametrize("typ_out", [A.F16, A.F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("new", [1, 60], ids=["token", "chunk"])
+@pytest.mark.parametrize("at", [0, 15000])
+@pytest.mark.parametrize("sink", [26.0, 30.0])
+def test_cache_tail_below_a_sink(ctx, typ_out, new, at, sink):
+    """The same over a long cache, in splits of which one has the sink."""
+    t, d, page = 20000, 64, 256
+    say(f"f16 {new} new over {t}, sink {sink} octaves up at {at}")
+    q, k, v = _tail(np.random.default_rng(12), t, 2, d, sink, at)
+    q, pages = q[:new], -(-t // page)
+    pools = []
+    for x in (k, v):
+        pool = np.zeros((pages * page, 2, d), np.float32)
+        pool[:t] = x
+        pools.append(D.DeviceBuffer.from_host(ctx, _bytes(
+            pool.reshape(pages, page, 2, d).transpose(0, 2, 1, 3), A.F16)))
+    cache = A.KVCache(ctx, A.F16, pages, page, 2, d, *pools)
+    put = lambda a: D.DeviceBuffer.from_host(ctx, np.asarray(a, np.int32))  # noqa: E731
+    qd = D.DeviceBuffer.from_host(ctx, _bytes(q, A.F16))
+    od = D.DeviceBuffer.empty(ctx, q.shape, np.uint16 if typ_out == A.F16 else np.float32)
+    A.AttentionPaged(ctx, A.F16, new, 2, cache, 1, A.Rows(qd, 2 * d, d), A.Rows(od, 2 * d, d),
+                     put(np.arange(pages)), pages, put([t]), put([0, new]), new, t, 0.125, type_out=typ_out)()
+    got = od.download()
+    got = got.view(np.float16).astype(np.float32) if typ_out == A.F16 else got
+    _check_f16(got, q, k, v, _seen(new, t, True, 0), 0.125, typ_out, 2.0 ** -32,
+               np.abs(v).max(2).astype(np.float64), "a cache's tail below a sink")

@@ -80,6 +80,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
     using V8 = typename Vec<T>::type;
     using C = typename std::conditional<I8, int8_t, T>::type;
     constexpr bool F32 = sizeof(T) == 4, SCALED = I8 && std::is_same<T, _Float16>::value;
+    constexpr float LIFT = kLift<T, SCALED>;
     constexpr int BN = S::BN, CPR = S::CPR, NW = S::NW, ROWS = 16 * NB;
     constexpr int CE = Vec<T>::N, QC = DP / (4 * CE);  // 16-byte chunks of a lane's query
     constexpr int NKB = BN / 16, NDB = DP / 16;
@@ -355,7 +356,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
 #pragma unroll
                 for (int d = 0; d < NDB; d++) o[n][d] *= fix;
             }
-            const float base = m[n] == -kInf ? 0.0f : m[n];
+            const float base = m[n] == -kInf ? 0.0f : m[n] - LIFT;
 #pragma unroll
             for (int b = 0; b < NKB; b++)
 #pragma unroll
@@ -481,7 +482,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
             *reinterpret_cast<f32x4*>(sums + (n * 16 + l15) * DP + d * 16 + 4 * g) = o[n][d] * vexp[n];
         }
         if (bad) row_bad[n * 16 + l15] = 1;
-        if (g == 0) row_ml[wave][n * 16 + l15] = make_float2(m[n], l[n]);
+        if (g == 0) row_ml[wave][n * 16 + l15] = make_float2(m[n] - LIFT, l[n]);
     }
     barrier();
     const bool split = splits > 1;

@@ -151,6 +151,14 @@ __device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first)
     return uniform(found);
 }
 
+// f16 weights are exp2(a - m + 7): with the 2^8 that the maximum may lag, up to
+// 2^15, below f16's largest.  The top one of a row is at least 2^7, so f16's
+// smallest step rounds weights down to 2^-21 of it to 11 bits and drops none
+// above 2^-32 of it (at exp2(a - m), 2^-25: 131071 keys just below that are 2^-8 of
+// the sum).  (m - kLift, l, O) is what the joins of waves and splits get.
+template <typename T, bool SCALED>
+constexpr float kLift = std::is_same<T, _Float16>::value && !SCALED ? 7.0f : 0.0f;
+
 // f16 weights over an int8 cache: each weight is multiplied by its value's scale,
 // and the products reach over more octaves than f16 has, so they are taken, and O
 // is kept, in units of a power of two.  The unit follows the row's largest product

@@ -292,6 +292,7 @@ void k_attn_tile(AttnArgs a) {
     for (int b = 0; b < NDB; b++) o[b] = f32x16{};
     float m = -kInf, l = 0.0f;
     constexpr bool SCALED = I8 && std::is_same<T, _Float16>::value;
+    constexpr float LIFT = kLift<T, SCALED>;
     float vexp = SCALED ? 0.0f : 1.0f, wtop = 0.0f;  // SCALED: O is in units of vexp (product_unit)
 
     // LDS offsets of this lane's reads
@@ -372,7 +373,7 @@ void k_attn_tile(AttnArgs a) {
                 for (int e = 0; e < 16; e++) mx = fmaxf(mx, x[b][e]);
             mx = fmaxf(mx, other_half(mx)) * a.scale_log2;
             // O and l are rescaled only once the maximum has grown by 2^8: the
-            // weights stay below that, far inside every type's range, and most
+            // weights stay below that (f16: times 2^kLift), inside every type's range, and most
             // tiles skip 4 * DP multiplications per row
             if (__any(mx > m + 8.0f || (m == -kInf && mx > -kInf))) {
                 const float mn = fmaxf(m, mx);
@@ -385,7 +386,7 @@ void k_attn_tile(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) o[b][e] *= fix;
             }
-            const float base = m == -kInf ? 0.0f : m;
+            const float base = m == -kInf ? 0.0f : m - LIFT;
             float sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < NKB; b++)
@@ -460,6 +461,7 @@ void k_attn_tile(AttnArgs a) {
         if (t + 1 < t1) put_codes(buf ^ 1);
     }
     l += other_half(l);
+    m -= LIFT;
 
     // A value that no row of a wave's tile may see still meets a weight of zero
     // in the product; where that left something that is not finite, those rows
