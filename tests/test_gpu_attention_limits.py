@@ -1,0 +1,73 @@
+"""Attention where a call stands at an edge of what the entry points take: rows
+that no sequence covers before the first one, outputs over the queries, the
+largest sizes, scales and lengths, values that are not finite.
+"""
+import numpy as np
+import pytest
+
+from tokenvector.inference_amd import attention as A
+from tokenvector.inference_amd import device as D
+
+from test_gpu_attention import NAME, Paged, _bytes, _check, _dev, _i32, _round, _seen, _values, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx(hip):
+    c = D.Context(0)
+    yield c
+    c.close()
+
+
+# ---- rows before the first sequence ----------------------------------------------
+
+# query rows, and key rows (the same, or over 256 each, which are split), of the
+# sequences behind 200 rows that are nobody's: over 128 rows of two heads
+LEADING = [([120, 90], [120, 90]), ([40], [3000]), ([70, 130], [2000, 600])]
+
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F16, A.F32], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lens_q,lens_k", LEADING)
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in place"])
+def test_prompt_behind_uncovered_rows(ctx, typ, lens_q, lens_k, in_place):
+    lead, hq, hkv, d = 200, 4, 2, 64
+    say(f"prompt {NAME[typ]} {lens_q} over {lens_k} behind {lead} rows, in place {in_place}")
+    r = np.random.default_rng(sum(lens_q))
+    cu_q, cu_k = lead + np.r_[0, np.cumsum(lens_q)], np.r_[0, np.cumsum(lens_k)]
+    tq, tk = int(cu_q[-1]) + 9, int(cu_k[-1])
+    q = _round(r.standard_normal((tq, hq, d)), typ)
+    kv = _round(r.standard_normal((tk, 2 * hkv, d)), typ)
+    qd, kvd = _dev(ctx, _bytes(q, typ)), _dev(ctx, _bytes(kv, typ))
+    out0 = q if in_place else np.full_like(q, 7.25)
+    od = qd if in_place else _dev(ctx, _bytes(out0, typ))
+    w = 4 if typ == A.F32 else 2
+    A.AttentionPrompt(ctx, typ, tq, hq, hkv, d, len(lens_q), A.Rows(qd, hq * d, d),
+                      A.Rows(kvd, 2 * hkv * d, d), A.Rows(kvd.ptr + hkv * d * w, 2 * hkv * d, d),
+                      A.Rows(od, hq * d, d), _i32(ctx, cu_q), _i32(ctx, cu_k), tk)()
+    got = _values(od.download(), typ).reshape(q.shape)
+    for s, (n, t) in enumerate(zip(lens_q, lens_k)):
+        rows, keys = slice(cu_q[s], cu_q[s + 1]), slice(cu_k[s], cu_k[s + 1])
+        _check(got[rows], q[rows], kv[keys, :hkv], kv[keys, hkv:], _seen(n, t, True, 0), d ** -0.5, typ, typ,
+               f"sequence {s} behind uncovered rows")
+    assert np.array_equal(got[:lead], out0[:lead]) and np.array_equal(got[cu_q[-1]:], out0[cu_q[-1]:])
+
+
+@pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F32, A.F32), (A.F16, A.I8)],
+                         ids=lambda t: NAME[t])
+@pytest.mark.parametrize("total", [100, 5000])
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in place"])
+def test_chunk_behind_uncovered_rows(ctx, typ, cache, total, in_place):
+    """200 of the call's rows come before the only sequence, which has 40."""
+    lead, n = 200, 40
+    say(f"chunk {NAME[typ]} over {NAME[cache]}, {total} keys, behind {lead} rows, in place {in_place}")
+    p = Paged(ctx, typ, cache, 4, 2, 64, [lead, n], [0, total])
+    out = p.qd if in_place else p.od
+    call = A.AttentionPaged(ctx, typ, lead + n, 4, p.pool, 1, A.Rows(p.qd, 256, 64), A.Rows(out, 256, 64),
+                            _i32(ctx, p.tab.download()[1:]), p.tab.shape[1], _i32(ctx, [total]),
+                            _i32(ctx, [lead, lead + n]), n, total, p.scale)
+    call()
+    got = _values(out.download(), typ).reshape(p.q.shape)
+    k, v = p.kv[1]
+    _check(got[lead:], p.q[lead:], k, v, _seen(n, total, True, 0), p.scale, typ, typ, "the covered chunk")
+    assert np.array_equal(got[:lead], (p.q if in_place else p.out0)[:lead])

@@ -128,11 +128,14 @@ enum { KV_PACKED = 0, KV_PAGED = 1, KV_I8 = 2 };
 // Sequence of a unit of ROWS query rows, and the sequence's first unit: sequence
 // i's units begin at floor(cu[i] g / ROWS) + i, which leaves each sequence room
 // for all of its rows (and up to one unit without any).  Lanes look at 64
-// sequences at a time: the last one that begins at or before the unit.
+// sequences at a time: the last one that begins at or before the unit.  -1 for a
+// unit before the first sequence's: its rows are nobody's, and taking the first
+// sequence's again would write them from two workgroups, the second of which
+// could read queries that the first had stored its outputs over.
 template <bool PAGED, int ROWS>
 __device__ __forceinline__ int tile_seq(const AttnArgs& a, int unit, int* first) {
     const int lane = threadIdx.x & 63;
-    int found = 0, begin = 0;
+    int found = -1, begin = 0;
     for (int b = 0; b < a.seqs; b += 64) {
         const int i = b + lane;
         int at = 0x7fffffff;

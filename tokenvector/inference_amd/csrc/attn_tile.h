@@ -81,6 +81,7 @@ void k_attn_tile(AttnArgs a) {
     const int unit = a.units - 1 - (int)(blockIdx.x / a.hkv);
     int first;
     const int seq = tile_seq<PAGED, kTileRows>(a, unit, &first);
+    if (seq < 0) return;
     Seq s = seq_of<PAGED>(a, seq);
     s.q0 = uniform(s.q0), s.n = uniform(s.n), s.len = uniform(s.len);
     const int rows = s.n * a.g;
