@@ -630,12 +630,12 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
  * (the unrounded sums of the same computation).  head_dim <= 256; sizes that
  * are multiples of 16 bytes with 16-byte aligned rows take the fast kernels.
  * Length arrays are read on the device and clamped to the tokens and pages
- * that there are, page ids outside the pool read page 0; query rows that no
- * sequence covers are not written.
+ * that there are (and to 2^31 - 256 keys), page ids outside the pool read page 0;
+ * query rows that no sequence covers are not written.
  *
  * Whole prompts, packed: sequence s has the query rows cu_q[s] .. cu_q[s + 1]
  * and the key rows cu_k[s] .. cu_k[s + 1] (cu_k NULL: cu_q's), device arrays of
- * `sequences` + 1 rising entries. */
+ * `sequences` + 1 rising entries.  tokens < 2^31, tokens_k <= 2^31 - 256. */
 int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, int64_t tokens_k,
                                      int64_t heads_q, int64_t heads_kv, int64_t head_dim,
                                      int64_t sequences, const tkv_hip_rows* q,

@@ -5,6 +5,7 @@ largest sizes, scales and lengths, values that are not finite.
 import numpy as np
 import pytest
 
+from tokenvector.inference_amd import _lib
 from tokenvector.inference_amd import attention as A
 from tokenvector.inference_amd import device as D
 
@@ -71,3 +72,47 @@ def test_chunk_behind_uncovered_rows(ctx, typ, cache, total, in_place):
     k, v = p.kv[1]
     _check(got[lead:], p.q[lead:], k, v, _seen(n, total, True, 0), p.scale, typ, typ, "the covered chunk")
     assert np.array_equal(got[:lead], (p.q if in_place else p.out0)[:lead])
+
+
+# ---- the longest caches ------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def long_table(ctx):
+    """Page ids of 2^31 keys, all of them page 0."""
+    t = _dev(ctx, np.zeros(1 << 27, np.int32))
+    yield t
+    t.close()
+
+
+@pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F16, A.I8), (A.F32, A.F32)], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("d", [64, 20])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("held", [(1 << 31) - 1, (1 << 31) - 256, (1 << 31) - 300])
+def test_cache_of_the_most_keys(ctx, long_table, typ, cache, d, new, held):
+    """Lengths up to 2^31 - 1 count as 2^31 - 256 at most; a window keeps it short."""
+    window, hkv, page = 100, 2, 16
+    say(f"{new} new of {held} keys, {NAME[typ]} over {NAME[cache]}, heads of {d}")
+    p = Paged(ctx, typ, cache, 2, hkv, d, [new], [page], page=page)
+    total = min(held, (1 << 31) - 256)
+    first = total - new - window
+    slot = np.arange(first, total) % page
+    # page 0 of the pool as the only one: the sequence's page by a pool of its own
+    pg = int(p.tab.download()[0, 0])
+    at = [b.download()[pg:pg + 1] for b in p.bufs]
+    pools = [_dev(ctx, x) for x in at]
+    scales = [_dev(ctx, s[pg:pg + 1]) for s in (p.ks, p.vs)] if cache == A.I8 else [None, None]
+    pool = A.KVCache(ctx, cache, 1, page, hkv, d, *pools, *scales)
+    call = A.AttentionPaged(ctx, typ, new, 2, pool, 1, A.Rows(p.qd, 2 * d, d), A.Rows(p.od, 2 * d, d), long_table,
+                            1 << 27, _i32(ctx, [held]), _i32(ctx, [0, new]), new, 0, p.scale, True, window)
+    call()
+    k, v = p.kv[0]
+    mask = _seen(new, new + window, True, window)
+    _check(p.result(), p.q, k[slot], v[slot], mask, p.scale, typ, typ, "the most keys")
+
+
+def test_refuses_rows_beyond_the_kernels_numbers(ctx):
+    """Refused on the host: nothing of this size is read."""
+    z = _dev(ctx, np.zeros(256, np.float32))
+    rows, cu = A.Rows(z, 64, 64), _i32(ctx, [0, 1])
+    with pytest.raises(_lib.TkvHipError):
+        A.AttentionPrompt(ctx, A.F32, (1 << 30) - 4096, 2, 1, 64, 1, rows, rows, rows, rows, cu)()

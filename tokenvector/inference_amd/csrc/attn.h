@@ -83,6 +83,10 @@ struct AttnArgs {
     unsigned* arrivals;
 };
 
+// Keys of a sequence, at most.  The kernels number keys, and round their ends up to
+// tiles, in 32 bits.
+constexpr int kMaxKeys = 0x7fffff00;
+
 // The rows of sequence i, clamped to what there is.
 struct Seq {
     int q0, n;       // query rows q0 .. q0 + n
@@ -107,7 +111,8 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int i) {
     }
     if (PAGED) {
         s.k0 = 0;
-        s.len = clamp_to(a.kv_lens[i], a.pages_st * (int64_t)a.page.d);
+        const int64_t held = a.pages_st * (int64_t)a.page.d;
+        s.len = clamp_to(a.kv_lens[i], held < kMaxKeys ? held : kMaxKeys);
     } else {
         const int32_t* cu = a.cu_k ? a.cu_k : a.cu_q;
         const int k0 = clamp_to(cu[i], a.tokens_k);

@@ -66,7 +66,9 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
         std::min(a.k_st, a.v_st) < 0 || std::max(a.k_st, a.v_st) >= (1ll << 22))
         return launch_attn_any(c, a, type, kv_type);
     a.gdiv = fast_div((uint32_t)a.g);
-    if (a.tokens * a.g >= (1ll << 31))
+    // row numbers, rounded up to units of 128 and to the 64 sequences that are looked at
+    // together, in 32 bits
+    if (a.tokens * a.g > (1ll << 31) - (1 << 14))
         return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     // up to 32 rows per sequence take the streaming kernel, blocks of 16 rows, a
     // unit per sequence; else units of 128 rows (see tile_seq)
@@ -143,7 +145,7 @@ int32_t tkv_hip_dev_attention_prompt(int64_t ctx, int32_t type, int64_t tokens, 
                                      int32_t causal, int64_t window) {
     TKV_RC_TRY(check_attention("attention_prompt", type, type_out, tokens, heads_q, heads_kv,
                                head_dim, sequences, q, out, scale, window));
-    if (tokens_k < 0 || tokens_k >= (1ll << 31) || !k || !v || (tokens_k > 0 && (!k->data || !v->data)) ||
+    if (tokens_k < 0 || tokens_k > kMaxKeys || !k || !v || (tokens_k > 0 && (!k->data || !v->data)) ||
         (sequences > 0 && !cu_q))
         return set_error(TKV_HIP_BAD_ARG, "attention_prompt: bad keys, values or cu_q");
     Ctx* c;
