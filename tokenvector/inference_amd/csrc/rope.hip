@@ -423,7 +423,7 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
     const KvCache* kv = reinterpret_cast<const KvCache*>(cache);
     if (!float_type(type_in) || !float_type(type_out))
         return set_error(TKV_HIP_BAD_ARG, "rope_append: types are F32, F16 or BF16");
-    if (tokens < 0 || heads_q < 0 || heads_kv < 0 || heads_q > 65535 || heads_kv > 65535 ||
+    if (tokens < 0 || tokens >= (1ll << 31) || heads_q < 0 || heads_kv < 0 || heads_q > 65535 || heads_kv > 65535 ||
         head_dim <= 0 || head_dim > 256)
         return set_error(TKV_HIP_BAD_ARG, "rope_append: sizes out of range (head_dim 1 .. 256)");
     if (table && (rot_dim < 2 || rot_dim > head_dim || rot_dim % 2 || table_len < 0 || !positions ||
