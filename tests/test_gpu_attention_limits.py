@@ -116,3 +116,41 @@ def test_refuses_rows_beyond_the_kernels_numbers(ctx):
     rows, cu = A.Rows(z, 64, 64), _i32(ctx, [0, 1])
     with pytest.raises(_lib.TkvHipError):
         A.AttentionPrompt(ctx, A.F32, (1 << 30) - 4096, 2, 1, 64, 1, rows, rows, rows, rows, cu)()
+
+
+# ---- calls of more than 2^24 workgroups -----------------------------------------------
+
+def _single_keys(ctx, tokens, hq, hkv, d):
+    """As many sequences of one token: every output row is its value, to the bit."""
+    r = np.random.default_rng(d)
+    q = r.integers(0x3e00, 0x4000, (tokens, hq, d), dtype=np.uint16)       # bf16 of 1 / 8 to 2
+    kv = r.integers(0x3e00, 0x4000, (tokens, 2 * hkv, d), dtype=np.uint16)
+    qd, kvd = _dev(ctx, q), _dev(ctx, kv)
+    A.AttentionPrompt(ctx, A.BF16, tokens, hq, hkv, d, tokens, A.Rows(qd, hq * d, d),
+                      A.Rows(kvd, 2 * hkv * d, d), A.Rows(kvd.ptr + 2 * hkv * d, 2 * hkv * d, d),
+                      A.Rows(qd, hq * d, d), _i32(ctx, np.arange(tokens + 1)))()
+    got = qd.download()
+    assert np.array_equal(got, np.repeat(kv[:, hkv:], hq // hkv, axis=1))
+
+
+def test_any_layout_of_2_26_rows(ctx):
+    """A row per wave, four waves a workgroup."""
+    _single_keys(ctx, (1 << 20) + 5, 64, 1, 2)
+
+
+def test_tiles_of_2_24_units(ctx):
+    """A unit per sequence and key / value head, and more."""
+    _single_keys(ctx, (1 << 20) + 3, 16, 16, 8)
+
+
+def test_table_of_2_32_entries(ctx):
+    positions, inv = (1 << 30) + 7, A.rope_inv_freq(8)
+    table = A.rope_table(ctx, positions, inv)
+    p = np.arange(positions - 5, positions)
+    got = np.empty((5, 4, 2), np.float32)
+    _lib.check(_lib.lib().tkv_hip_memcpy_d2h(ctx.handle, got.ctypes.data, table.ptr + (positions - 5) * 32,
+                                             got.nbytes))
+    table.close()
+    a = p[:, None].astype(np.float64) * inv
+    # the product's rounding in f64 (2^-24 at 2^30), and f32's
+    assert np.all(np.abs(got - np.stack([np.cos(a), np.sin(a)], -1)) <= 2.0 ** -24 + 2.0 ** -23)

@@ -28,6 +28,17 @@ inline bool float_type(int type) {
     return type == TKV_HIP_F32 || type == TKV_HIP_F16 || type == TKV_HIP_BF16;
 }
 
+// HIP takes fewer than 2^32 work items in a dimension of a grid: 2^24 workgroups of
+// 256.  Kernels that may need more number them over two.
+constexpr int64_t kGridItems = (1ll << 32) - 1;
+constexpr int64_t kWideX = 1 << 22;
+constexpr int64_t kWideBlocks = kWideX * 65535;
+inline dim3 wide_grid(int64_t blocks) {
+    const int64_t x = blocks < kWideX ? blocks : kWideX;
+    return dim3((unsigned)x, (unsigned)ceil_div(blocks, x));
+}
+__device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // n / d for n < 2^31 by a multiplication: (mulhi(m, n) + n) >> l.
 struct FastDiv {
     uint32_t d, m, l;

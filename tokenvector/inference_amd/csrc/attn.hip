@@ -77,7 +77,7 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     const int blocks16 = longest <= 16 ? 1 : 2;
     const int64_t block = few ? 16 * blocks16 : kTileRows;
     const int64_t units = few ? a.seqs : a.tokens * a.g / block + a.seqs;
-    if (units >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
+    if (units * a.hkv * 256 > kGridItems) return launch_attn_any(c, a, type, kv_type);
     a.units = (int32_t)units;
     const int64_t tiles = (few ? a.seqs : std::max<int64_t>(ceil_div(a.tokens * a.g, block), a.seqs)) * a.hkv;
     // Splits over the keys: as many as fill the chip once, 128 keys (streaming) or

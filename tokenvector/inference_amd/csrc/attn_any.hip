@@ -5,7 +5,7 @@
 // the running maximum and sum of the softmax in f32.  Every key row is read by
 // one lane at a time, so this form is bound by its scattered loads: 1000 tokens of
 // 4 heads of 33, bf16, 267 us, 1.0 TFLOP/s.  Layouts that the matrix kernels take
-// (16-byte rows) never come here.
+// (16-byte rows) come here only where a call has more units than a grid takes.
 #include "attn.h"
 
 namespace tkv {
@@ -13,7 +13,7 @@ namespace tkv {
 template <typename T, typename C, bool PAGED>
 __global__ __launch_bounds__(256) void k_attn_any(AttnArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t unit = wide_block() * 4 + wave;
     const int64_t row = unit / a.hq;
     const int h = (int)(unit - row * a.hq), kvh = h / a.g;
     if (row >= a.tokens) return;
@@ -39,13 +39,13 @@ __global__ __launch_bounds__(256) void k_attn_any(AttnArgs a) {
 
 template <typename T, typename C>
 static void launch_any(Ctx* c, const AttnArgs& a) {
-    const dim3 grid((unsigned)ceil_div(a.tokens * a.hq, 4));
+    const dim3 grid = wide_grid(ceil_div(a.tokens * a.hq, 4));
     if (a.pages) k_attn_any<T, C, true><<<grid, 256, 0, c->stream>>>(a);
     else k_attn_any<T, C, false><<<grid, 256, 0, c->stream>>>(a);
 }
 
 int launch_attn_any(Ctx* c, const AttnArgs& a, int type, int kv_type) {
-    if (ceil_div(a.tokens * a.hq, 4) >= (1ll << 31))
+    if (ceil_div(a.tokens * a.hq, 4) > kWideBlocks)
         return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     const bool i8 = kv_type == TKV_HIP_I8;
     if (type == TKV_HIP_F32) i8 ? launch_any<float, int8_t>(c, a) : launch_any<float, float>(c, a);

@@ -606,7 +606,6 @@ int launch_few_dp(Ctx* c, const AttnArgs& a, int blocks_of_16) {
     static_assert(LDS <= 163840 - 4096 && S::NW * 32 * DP * 4 <= LDS, "LDS of a workgroup");
     if ((size_t)LDS + 4096 > c->max_lds) return set_error(TKV_HIP_UNSUPPORTED, "attention: not enough LDS");
     const int64_t blocks = (int64_t)a.units * a.hkv;
-    if (blocks >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
     const dim3 grid((unsigned)blocks, (unsigned)a.splits);
     if (blocks_of_16 == 1) k_attn_few<T, DP, I8, 1><<<grid, 64 * S::NW, LDS, c->stream>>>(a);
     else k_attn_few<T, DP, I8, 2><<<grid, 64 * S::NW, LDS, c->stream>>>(a);

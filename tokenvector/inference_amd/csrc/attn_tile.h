@@ -592,7 +592,6 @@ int launch_tile_dp(Ctx* c, const AttnArgs& a) {
     static_assert(S::LDS <= 163840, "LDS of a workgroup");
     if ((size_t)S::LDS > c->max_lds) return set_error(TKV_HIP_UNSUPPORTED, "attention: not enough LDS");
     const int64_t blocks = (int64_t)a.units * a.hkv;
-    if (blocks >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "attention: too many tiles");
     k_attn_tile<T, DP, KV, NARROW>
         <<<dim3((unsigned)blocks, (unsigned)a.splits), 256, S::LDS, c->stream>>>(a);
     TKV_LAUNCH_CHECK();

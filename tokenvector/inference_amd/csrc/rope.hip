@@ -20,7 +20,7 @@ struct Freqs {
 
 __global__ __launch_bounds__(256) void k_rope_table(Freqs fr, int half, int64_t n, double amplitude,
                                                     float2* __restrict__ table) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = wide_block() * 256 + threadIdx.x;
     if (t >= n) return;
     const int64_t p = t / half;
     double s, c;
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
 // again, so that it is bound by its load instructions.
 template <typename TI, typename TO, typename C>
 __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = wide_block() * 256 + threadIdx.x;
     const int64_t r64 = t >> a.lanes_log2;
     if (r64 >= a.tokens * a.heads.d) return;  // whole groups: the rows' lanes stay together
     const uint32_t r = (uint32_t)r64;
@@ -273,12 +273,15 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
 template <typename TI, typename TO, typename C>
 static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
     const int64_t heads = a.heads.d;
-    if (!vec) {
+    int rows_log2 = 0;
+    while (16 << rows_log2 < a.d) rows_log2++;
+    // (a dimension of the grid holds 2^28 tokens of heads of 256)
+    if (!vec || (a.tokens << rows_log2) + 255 > kGridItems) {
         while (8 << a.lanes_log2 < a.d) a.lanes_log2++;
-        k_rope_any<TI, TO, C><<<(unsigned)ceil_div(a.tokens * heads << a.lanes_log2, 256), 256, 0, c->stream>>>(a);
+        k_rope_any<TI, TO, C><<<wide_grid(ceil_div(a.tokens * heads << a.lanes_log2, 256)), 256, 0, c->stream>>>(a);
         return;
     }
-    while (16 << a.lanes_log2 < a.d) a.lanes_log2++;
+    a.lanes_log2 = rows_log2;
     const int64_t blocks = ceil_div(a.tokens << a.lanes_log2, 256);
     // four heads per lane where that still leaves eight workgroups per CU
     if (blocks * ceil_div(heads, 4) >= 8 * c->num_cus)
@@ -405,10 +408,8 @@ int32_t tkv_hip_dev_rope_table(int64_t ctx, int64_t positions, int64_t rot_dim,
     const int64_t n = positions * half;
     Freqs fr;
     for (int i = 0; i < 128; i++) fr.f[i] = i < half ? inv_freq[i] : 0.0;
-    if (ceil_div(n, 256) >= (1ll << 31))
-        return set_error(TKV_HIP_UNSUPPORTED, "rope_table: too many entries");
-    k_rope_table<<<(unsigned)ceil_div(n, 256), 256, 0, c->stream>>>(fr, half, n, amplitude,
-                                                                    reinterpret_cast<float2*>(table));
+    k_rope_table<<<wide_grid(ceil_div(n, 256)), 256, 0, c->stream>>>(fr, half, n, amplitude,
+                                                                     reinterpret_cast<float2*>(table));
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
