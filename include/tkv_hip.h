@@ -569,7 +569,7 @@ typedef struct {
 /* A paged cache: K and V [num_pages, heads, page_size, head_dim] of `type`,
  * and for I8 f32 scales [num_pages, heads, page_size] each.  Slot s of the
  * pool is (s / page_size, s % page_size).  k == NULL: the handle allocates
- * (zeroed) and frees the memory; otherwise the four device pointers are the
+ * (zeroed on return, for every stream) and frees the memory; otherwise the four device pointers are the
  * caller's (scales NULL unless I8) and have to outlive the handle.
  * num_pages * page_size < 2^31, times heads < 2^32; head_dim <= 256. */
 int32_t tkv_hip_kv_create(int64_t ctx, int32_t type, int64_t num_pages, int64_t page_size,

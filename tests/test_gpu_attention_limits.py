@@ -154,3 +154,35 @@ def test_table_of_2_32_entries(ctx):
     a = p[:, None].astype(np.float64) * inv
     # the product's rounding in f64 (2^-24 at 2^30), and f32's
     assert np.all(np.abs(got - np.stack([np.cos(a), np.sin(a)], -1)) <= 2.0 ** -24 + 2.0 ** -23)
+
+
+# ---- a cache between contexts ----------------------------------------------------------
+
+def test_new_cache_belongs_to_every_context(ctx):
+    """Tokens appended from a second context right after the cache was made stay: the
+    zeros are there before the handle is."""
+    heads, page, d = 8, 256, 128
+    pages = 8192                                     # 4 GiB each of keys and values
+    slots = np.linspace(0, pages * page - 1, 4096).astype(np.int64)
+    x = _round(np.random.default_rng(6).uniform(1.0, 2.0, (slots.size, heads, d)), A.BF16)
+    other = D.Context(0)
+    try:
+        xd, sd = _dev(other, _bytes(x, A.BF16)), _dev(other, slots)
+        rows = A.Rows(xd, heads * d, d)
+        other.synchronize()
+        cache = A.KVCache(ctx, A.BF16, pages, page, heads, d)
+        A.RopeAppend(other, A.BF16, slots.size, 0, heads, d, None, rows, rows, cache=cache, slots=sd)()
+        other.synchronize()
+        ctx.synchronize()
+        got = np.empty((heads, d), np.int16)
+        row = np.empty(d, np.int16)
+        for i in (0, 1, 2047, 4094, 4095):
+            for pool in (cache.k, cache.v):
+                for h in range(heads):
+                    at = ((slots[i] // page * heads + h) * page + slots[i] % page) * d * 2
+                    _lib.check(_lib.lib().tkv_hip_memcpy_d2h(other.handle, row.ctypes.data, int(pool + at), row.nbytes))
+                    got[h] = row
+                assert np.array_equal(got, _bytes(x[i], A.BF16))
+        cache.close()
+    finally:
+        other.close()

@@ -376,6 +376,14 @@ int32_t tkv_hip_kv_create(int64_t ctx, int32_t type, int64_t num_pages, int64_t 
                 return rc;
             }
         }
+        // the handle is any context's of this device, and its pointers the caller's:
+        // what they write must not meet the fill on this context's stream
+        const hipError_t e = hipStreamSynchronize(c->stream);
+        if (e != hipSuccess) {
+            const int rc = fail_hip(e, "hipStreamSynchronize(cache)", __FILE__, __LINE__);
+            kv_release(kv);
+            return rc;
+        }
     }
     *handle_out = reinterpret_cast<int64_t>(kv);
     return TKV_HIP_OK;
