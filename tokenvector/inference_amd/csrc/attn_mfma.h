@@ -45,28 +45,32 @@ __device__ __forceinline__ f32x16 mfma32(Vec<_Float16>::type a, Vec<_Float16>::t
 // In asm, since the compiler would put a wait for every copy in flight before
 // each LDS read it cannot tell apart from the copy's destination; the waits
 // here are the callers' own (wait_vm below, before a barrier).  No register is
-// written; the s_nop is the wait state between a scalar write of m0 and the
-// copy that uses it.
+// written but m0, which is named as clobbered, so that the compiler carries no value
+// of its own in it across the copy (it warns of any reserved register there); the
+// s_nop is the wait state between a scalar write of m0 and the copy that uses it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16_to_lds(const void* src, unsigned dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :
                  : "v"(src), "s"(dst)
-                 : "memory");
+                 : "memory", "m0");
 }
 // The same from a wave-uniform base and a byte offset per lane.
 __device__ __forceinline__ void copy16_to_lds(const char* base, uint32_t offset, unsigned dst) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
                  : "v"(offset), "s"(base), "s"(dst)
-                 : "memory");
+                 : "memory", "m0");
 }
 // 4 bytes per lane, to `dst` + 4 lane.
 __device__ __forceinline__ void copy4_to_lds(const void* src, unsigned dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                  :
                  : "v"(src), "s"(dst)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Waits until at most N of the wave's memory operations are in flight.
 template <int N>
 __device__ __forceinline__ void wait_vm_but() {
