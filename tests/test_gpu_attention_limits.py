@@ -186,3 +186,32 @@ def test_new_cache_belongs_to_every_context(ctx):
         cache.close()
     finally:
         other.close()
+
+
+# ---- the least scales --------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F32], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("scale,size", [(1e-35, 1e17), (3e-38, 3e18), (0.0, 1e17), (0.0, 1e18)])
+@pytest.mark.parametrize("d", [64, 33])
+@pytest.mark.parametrize("new", [1, 60])
+def test_least_scales(ctx, typ, scale, size, d, new):
+    """Products as large as the scale is small have ordinary logits; at scale 0 all
+    weights are equal whatever the products.  Products are f32: rows with one past
+    its range are not compared."""
+    say(f"{NAME[typ]} scale {scale} of products of {size * size}, {new} new, heads of {d}")
+    p = Paged(ctx, typ, typ, 4, 2, d, [new], [300], scale=scale)
+    k, v = p.kv[0]
+    tab, raw = p.tab.download(), p.bufs[0].download()
+    p.q = _round(p.q * np.float32(size), typ)
+    k[:] = _round(k * np.float32(size), typ)
+    for j in range(300):
+        raw[tab[0, j // 16], :, j % 16] = _bytes(k[j], typ)
+    p.qd.upload(_bytes(p.q, typ))
+    p.bufs[0].upload(raw)
+    p.call()
+    got, mask = p.result(), _seen(new, 300, True, 0)
+    for h in range(4):
+        products = p.q[:, h].astype(np.float64) @ k[:, h // 2].T.astype(np.float64)
+        rows = np.abs(products).max(1) <= np.finfo(np.float32).max
+        _check(got[rows, h:h + 1], p.q[rows, h:h + 1], k[:, h // 2:h // 2 + 1], v[:, h // 2:h // 2 + 1], mask[rows],
+               p.scale, typ, typ, f"least scale, head {h}")

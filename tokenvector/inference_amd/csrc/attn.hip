@@ -46,9 +46,10 @@ static void common_args(AttnArgs* a, int32_t type, int32_t type_out, int64_t tok
     a->d = (int32_t)head_dim;
     a->causal = causal != 0;
     a->window = window;
-    // a scale of zero (equal weights) as one that no finite logit notices, so
-    // that hidden logits of -inf stay -inf; and finite, so that those of zero stay zero
-    a->scale_log2 = (float)std::min(std::max((double)scale * 1.4426950408889634, 1e-30), 3.4028234e38);
+    // a scale of zero (equal weights) as f32's least, 2^-149, so that hidden logits of
+    // -inf stay -inf: it makes less than 2^-21 of the largest f32 product.  And
+    // finite, so that logits of zero stay zero
+    a->scale_log2 = (float)std::min(std::max((double)scale * 1.4426950408889634, 0x1p-149), 3.4028234e38);
     a->out_f32 = type_out == TKV_HIP_F32;
 }
 
