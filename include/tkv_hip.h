@@ -598,7 +598,8 @@ int32_t tkv_hip_dev_rope_table(int64_t ctx, int64_t positions, int64_t rot_dim,
  *   cache (0: none): token t's k and v go to pool slot slots[t]; a slot outside
  *     the pool appends nothing.  Cache types: type_out, or I8, whose rows are
  *     coded from the f32 values as scale = fl32(max(max|x|, 1e-8) * fl32(1 / 127)),
- *     code = clamp(rne(fl32(x * fl32(1 / scale))), -127, 127), NaN 0.
+ *     code = clamp(rne(fl32(x * fl32(1 / scale))), -127, 127), NaN 0.  A row with a
+ *     NaN has a NaN for max|x| and so for its scale and every value.
  * A position outside [0, table_len) marks a padding token: its q_out and k_out
  * rows are zeros and it is not appended.  q, k, v may be NULL with their head
  * count 0 (k and v go together where there is a cache).  positions and slots

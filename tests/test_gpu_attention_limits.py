@@ -215,3 +215,49 @@ def test_least_scales(ctx, typ, scale, size, d, new):
         rows = np.abs(products).max(1) <= np.finfo(np.float32).max
         _check(got[rows, h:h + 1], p.q[rows, h:h + 1], k[:, h // 2:h // 2 + 1], v[:, h // 2:h // 2 + 1], mask[rows],
                p.scale, typ, typ, f"least scale, head {h}")
+
+
+# ---- values that are not finite in an int8 cache -----------------------------------------
+
+@pytest.mark.parametrize("typ", [A.BF16, A.F32], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("d", [64, 96, 33])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_int8_rows_that_are_not_finite(ctx, typ, d, bad):
+    """One element that is not a number, or infinite, makes its row's values NaN, as
+    code times scale; the rows beside it are coded as ever, and tokens that attend
+    to it are not finite."""
+    tokens, heads, page = 40, 3, 16
+    r = np.random.default_rng(d)
+    x = _round(r.standard_normal((tokens, 2 * heads, d)), typ)
+    rows = [(3, 0, 0), (17, 2, d - 1), (17, 4, 5), (30, 5, d // 2)]     # keys of heads 0, 2; values of 1, 2
+    for t, h, e in rows:
+        x[t, h, e] = bad
+    xd = _dev(ctx, _bytes(x, typ))
+    w, pages = (4 if typ == A.F32 else 2), 3
+    bufs = [_dev(ctx, np.zeros((pages, heads, page, d), np.int8)) for _ in range(2)]
+    scales = [_dev(ctx, np.zeros((pages, heads, page), np.float32)) for _ in range(2)]
+    pool = A.KVCache(ctx, A.I8, pages, page, heads, d, *bufs, *scales)
+    A.RopeAppend(ctx, typ, tokens, 0, heads, d, None, A.Rows(xd, 2 * heads * d, d),
+                 A.Rows(xd.ptr + heads * d * w, 2 * heads * d, d), cache=pool,
+                 slots=_dev(ctx, np.arange(tokens, dtype=np.int64)))()
+    hit = np.zeros((tokens, 2 * heads), bool)
+    for t, h, _ in rows:
+        hit[t, h] = True
+    for i in range(2):
+        codes, sc = bufs[i].download(), scales[i].download()
+        at, slot = np.arange(tokens) // page, np.arange(tokens) % page
+        with np.errstate(invalid="ignore"):
+            value = codes[at, :, slot] * sc[at, :, slot][..., None]
+        part, sick = x[:, i * heads:(i + 1) * heads], hit[:, i * heads:(i + 1) * heads]
+        assert np.isnan(value[sick]).all()
+        y = part[~sick]
+        scale = np.maximum(np.abs(y).max(-1), np.float32(1e-8)) * (np.float32(1) / np.float32(127))
+        want = np.clip(np.rint(y * (np.float32(1) / scale)[:, None]), -127, 127)
+        assert np.array_equal(sc[at, :, slot][~sick], scale) and np.array_equal(codes[at, :, slot][~sick], want)
+    q = _round(r.standard_normal((tokens, heads, d)), typ)
+    qd = _dev(ctx, _bytes(q, typ))
+    A.AttentionPaged(ctx, typ, tokens, heads, pool, 1, A.Rows(qd, heads * d, d), A.Rows(qd, heads * d, d),
+                     _i32(ctx, np.arange(pages)), pages, _i32(ctx, [tokens]), _i32(ctx, [0, tokens]), tokens, tokens)()
+    got = _values(qd.download(), typ).reshape(q.shape)
+    for h, first in ((0, 3), (1, 17), (2, 17)):
+        assert np.isfinite(got[:first, h]).all() and not np.isfinite(got[first:, h]).any()

@@ -74,14 +74,17 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
         *reinterpret_cast<Vec8<T>*>(p) = v;
     }
 }
-// codes of a row from its max |x| (over 1 << lanes lanes)
-__device__ __forceinline__ float row_max(float m, int lanes) {
-    for (int o = 1 << lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    return m;
+// codes of a row from its max |x| (over 1 << lanes lanes), as bits: a NaN's are
+// above every number's, so a row that has one gets a NaN for its scale, and values
+// of NaN, where f32's maximum would leave it out and code it as 0
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float row_max(unsigned m, int lanes) {
+    for (int o = 1 << lanes >> 1; o; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
+    return __uint_as_float(m);
 }
 // By the rounded reciprocal, as elementwise tensor libraries divide by a constant:
 // within an ulp of max / 127, and the same codes as their operations give.
-__device__ __forceinline__ float scale_of(float m) { return fmaxf(m, 1e-8f) * (1.0f / 127.0f); }
+__device__ __forceinline__ float scale_of(float m) { return (m < 1e-8f ? 1e-8f : m) * (1.0f / 127.0f); }
 __device__ __forceinline__ int8_t code_of(float x, float inv) {
     const float y = __builtin_rintf(x * inv);
     return y != y ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(y, -127.0f), 127.0f);
@@ -178,10 +181,10 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
         if (isq || !a.kc) continue;
         const int64_t at = ((int64_t)pg * a.hkv + h) * a.page.d + (s32 - pg * a.page.d);
         if constexpr (sizeof(C) == 1) {
-            float m = 0.0f;
+            unsigned most = 0;
 #pragma unroll
-            for (int k = 0; k < 8; k++) m = fmaxf(m, fmaxf(fabsf(x0[u][k]), fabsf(x1[u][k])));
-            m = row_max(m, a.lanes_log2);
+            for (int k = 0; k < 8; k++) most = max(most, max(abs_bits(x0[u][k]), abs_bits(x1[u][k])));
+            const float m = row_max(most, a.lanes_log2);
             if (!put) continue;
             const float scale = scale_of(m), inv = 1.0f / scale;
             if (i == 0) (isv ? a.vs : a.ks)[at] = scale;
@@ -253,10 +256,10 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
     const uint32_t s32 = put ? (uint32_t)slot : 0, pg = div_by(a.page, s32);
     const int64_t at = ((int64_t)pg * a.hkv + h) * a.page.d + (s32 - pg * a.page.d);
     if constexpr (sizeof(C) == 1) {
-        float m = 0.0f;
+        unsigned most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-        m = row_max(m, a.lanes_log2);
+        for (int i = 0; i < 8; i++) most = max(most, abs_bits(x[i]));
+        const float m = row_max(most, a.lanes_log2);
         if (!put) return;
         const float scale = scale_of(m), inv = 1.0f / scale;
         if (e0 == 0) (isv ? a.vs : a.ks)[at] = scale;
