@@ -82,3 +82,11 @@ def test_call_made_of_a_closed_cache():
         call._fn = lambda *args: pytest.fail("launched")
         with pytest.raises(ValueError, match="closed"):
             call()
+
+
+def test_prompt_keys_of_their_own_come_with_their_number():
+    """Taken for the number of query tokens, it cut longer keys off unsaid."""
+    rows, cu = A.Rows(16, 64, 64), _Memory()
+    with pytest.raises(ValueError, match="tokens_k"):
+        A.AttentionPrompt(_Ctx, A.BF16, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, cu)
+    A.AttentionPrompt(_Ctx, A.BF16, 1, 1, 1, 64, 1, rows, rows, rows, rows, cu, cu, 5)

@@ -165,12 +165,15 @@ class RopeAppend(_Call):
 class AttentionPrompt(_Call):
     """Attention of packed prompts: sequence s has the query rows cu_q[s] ..
     cu_q[s + 1] and the key rows cu_k[s] .. cu_k[s + 1] (cu_k None: cu_q's;
-    int32 device arrays).  scale None: 1 / sqrt(head_dim)."""
+    int32 device arrays) of the tokens_k that k and v have, which goes with cu_k.
+    scale None: 1 / sqrt(head_dim)."""
 
     def __init__(self, ctx: Context, type: int, tokens: int, heads_q: int, heads_kv: int,
                  head_dim: int, sequences: int, q: Rows, k: Rows, v: Rows, out: Rows, cu_q,
                  cu_k=None, tokens_k: Optional[int] = None, scale: Optional[float] = None,
                  causal: bool = True, window: int = 0, type_out: Optional[int] = None):
+        if cu_k is not None and tokens_k is None:
+            raise ValueError("cu_k without tokens_k: keys past it are cut off")
         self._also = (q, k, v, out, cu_q, cu_k)
         super().__init__(
             "tkv_hip_dev_attention_prompt", ctx, int(type), int(tokens),
