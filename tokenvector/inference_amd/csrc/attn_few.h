@@ -379,11 +379,11 @@ __global__ __launch_bounds__((64 * FewShape<T, DP, I8>::NW)) void k_attn_few(Att
                     const float unit = product_unit(vexp[n], wtop[n]);
                     if (__any(unit != vexp[n])) {
                         const float fix = vexp[n] * inverse_unit(unit);
-                        vexp[n] = unit;
 #pragma unroll
                         for (int d = 0; d < NDB; d++) o[n][d] *= fix;
                     }
-                    const float inv = inverse_unit(vexp[n]);
+                    vexp[n] = unit;
+                    const float inv = inverse_unit(unit);
 #pragma unroll
                     for (int b = 0; b < NKB; b++)
 #pragma unroll

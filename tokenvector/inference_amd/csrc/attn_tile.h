@@ -412,13 +412,15 @@ void k_attn_tile(AttnArgs a) {
                     const float unit = product_unit(vexp, wtop);
                     if (__any(unit != vexp)) {
                         const float fix = vexp * inverse_unit(unit);
-                        vexp = unit;
 #pragma unroll
                         for (int b = 0; b < NDB; b++)
 #pragma unroll
                             for (int e = 0; e < 16; e++) o[b][e] *= fix;
                     }
-                    const float inv = inverse_unit(vexp);
+                    // (of unit: taken from vexp, the compiler multiplied in both branches,
+                    // and tiles of heads of 128 spilled 45 registers)
+                    vexp = unit;
+                    const float inv = inverse_unit(unit);
 #pragma unroll
                     for (int b = 0; b < NKB; b++)
 #pragma unroll
