@@ -261,3 +261,18 @@ def test_int8_rows_that_are_not_finite(ctx, typ, d, bad):
     got = _values(qd.download(), typ).reshape(q.shape)
     for h, first in ((0, 3), (1, 17), (2, 17)):
         assert np.isfinite(got[:first, h]).all() and not np.isfinite(got[first:, h]).any()
+
+
+# ---- more units than there are arrival counters ---------------------------------------------
+
+@pytest.mark.parametrize("typ,cache", [(A.BF16, A.BF16), (A.F16, A.I8)], ids=lambda t: NAME[t])
+@pytest.mark.parametrize("new", [1, 9], ids=["token", "chunk"])
+def test_more_than_1024_units(ctx, typ, cache, new):
+    """130 sequences of 8 key / value heads, one of them long: no splits."""
+    say(f"1040 units, {new} new, {NAME[typ]} over {NAME[cache]}")
+    r = np.random.default_rng(3)
+    total = (new + r.integers(0, 40, 130)).tolist()
+    total[77] = 3000
+    p = Paged(ctx, typ, cache, 32, 8, 64, [new] * 130, total)
+    p.call()
+    p.check("more than 1024 units")
