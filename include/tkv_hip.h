@@ -624,9 +624,11 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
  * not see (NaN and infinities included) does not touch it.  Query head h reads key / value head h / (heads_q / heads_kv).
  * Statistics and sums are f32.  For f16 and bf16 the products run on the
  * matrix units from values of that type, the weights exp(a - m) rounded to it
- * for the second product; f32 stays f32 throughout.  An int8 cache's codes are
+ * for the second product (2^-8 of a weight in bf16; in f16 2^-11, or 2^-32 of the
+ * row's largest); f32 stays f32 throughout.  An int8 cache's codes are
  * exact in every type; its keys' scales multiply the logits, its values' scales
- * the weights before that rounding.  out may be q itself where the types agree.
+ * the weights before that rounding (f16: 2^-11 of a product, or 2^-31 of the
+ * largest).  out may be q itself where the types agree.
  * Results do not depend on timing: splits are joined in their order.  type_out: `type`, or F32
  * (the unrounded sums of the same computation).  head_dim <= 256; sizes that
  * are multiples of 16 bytes with 16-byte aligned rows take the fast kernels.

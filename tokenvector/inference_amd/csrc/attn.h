@@ -39,7 +39,8 @@ inline dim3 wide_grid(int64_t blocks) {
 }
 __device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
-// n / d for n < 2^31 by a multiplication: (mulhi(m, n) + n) >> l.
+// n / d for n < 2^31 by a multiplication, (mulhi(m, n) + n) >> l: the method of
+// Granlund and Montgomery, "Division by invariant integers using multiplication" (1994).
 struct FastDiv {
     uint32_t d, m, l;
 };

@@ -71,8 +71,16 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     // together, in 32 bits
     if (a.tokens * a.g > (1ll << 31) - (1 << 14))
         return set_error(TKV_HIP_UNSUPPORTED, "attention: too many rows");
-    // up to 32 rows per sequence take the streaming kernel, blocks of 16 rows, a
-    // unit per sequence; else units of 128 rows (see tile_seq)
+    // Up to 32 rows per sequence take the streaming kernel, blocks of 16 rows, a
+    // unit per sequence; else units of 128 rows (see tile_seq).  Both at 4, 16 and 32
+    // rows of each of 8 heads of 128, streaming / tiles, us:
+    //                 32 x 4096 keys               1 x 8192
+    //   bf16          99/111  102/113  113/113     13/45  21/45  34/45
+    //   f32           237/369 249/441  379/480     25/75  35/76  59/75
+    //   bf16 on int8  52/92   54/93    63/94       15/45  22/45  35/45
+    //   f32 on int8   73/331  76/424   121/456     17/74  23/74  40/74
+    // (8 x 1024, and 12 heads of 64, between them.)  The choice is the call's: one
+    // sequence of more rows takes all of them to the tiles.
     const int64_t longest = a.pages ? (a.cu_q ? max_q : 1) * a.g : 0;
     const bool few = longest > 0 && longest <= 32 && !(i8 && a.d % 16);
     const int blocks16 = longest <= 16 ? 1 : 2;
@@ -100,8 +108,8 @@ static int launch_attention(Ctx* c, AttnArgs a, int type, int kv_type, int64_t m
     if (few)
         want = std::max(want, std::min<int64_t>(8 * slots / tiles, keys * 2 * a.d * kb / (512 << 10)));
     a.splits = (int32_t)std::min<int64_t>(std::max<int64_t>(want, 1), kMaxSplits);
-    // many short rows (see TileShape): clearly over two workgroups per CU, up to 4096
-    // keys each as far as the host knows
+    // many short rows (measured at TileShape): clearly over two workgroups per CU, up
+    // to 4096 keys each as far as the host knows
     int64_t per_row = a.pages ? keys : a.tokens_k / a.seqs;
     if (a.window > 0) per_row = std::min(per_row, a.window + kTileRows);
     a.narrow = 10 * tiles > 23 * c->num_cus && per_row <= 4096;

@@ -68,7 +68,9 @@ struct FewShape {
     static constexpr int CPR = DP * E / 16;
     static constexpr int IDS = 4 * 256;
     static constexpr int WAVE = 4 * TILE + IDS + (I8 ? 2 * 512 : 0);
-    // as many waves, up to four, as let two workgroups share a CU's LDS
+    // as many waves, up to four, as let two workgroups share a CU's LDS.  (Three and
+    // four waves also need 256 registers at most: with 32 rows over int8, heads of 96
+    // and 192, and f32 queries of heads of 64, are 10 to 92 above, one workgroup per CU.)
     static constexpr int FIT = 80 * 1024 / WAVE;
     static constexpr int NW = FIT < 1 ? 1 : FIT > 4 ? 4 : FIT;
     static constexpr int COPIES = 2 * TILE / 1024 + (I8 ? 2 : 0);  // memory operations of a tile

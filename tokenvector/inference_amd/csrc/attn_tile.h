@@ -20,15 +20,15 @@
 // its registers.  f32 uses the 32x32x2 product, whose two-key steps take the
 // same registers as they are.
 //
-// Measured: 16384 f16 tokens of 16 / 4 heads of 128 in 1.18 ms, 933 TFLOP/s (a
+// Measured: 16384 f16 tokens of 16 / 4 heads of 128 in 1.20 ms, 919 TFLOP/s (a
 // library product of 8192^3: 1160); 4 x 512 new tokens over 16384 cached ones, 32 /
-// 8 heads, 0.61 ms, 911; f32, 4096 tokens of 12 heads of 64, 283 us, 91 (library:
+// 8 heads, 0.63 ms, 885; f32, 4096 tokens of 12 heads of 64, 283 us, 91 (library:
 // 154).  There the matrix units are busy in 50 % of the cycles and the vector units
 // in 47 %, LDS in 25 % (no bank conflicts): the two waves of a SIMD rarely have one
 // multiply while the other takes exponentials.  Short rows are bound by latency: a
 // wave alone takes 0.9 us (heads of 64) to 1.6 us (128) for a tile of 64 keys, LDS
 // reads, products and exponentials after each other, and 5 us to start and end: 8 x
-// 1024 tokens of 12 heads of 64 30 us, 434 TFLOP/s.  What did not help: 64 rows
+// 1024 tokens of 12 heads of 64 31 us, 421 TFLOP/s.  What did not help: 64 rows
 // per wave (half the LDS reads, half the waves: 16384 tokens of heads of 64 467 ->
 // 515 us, 8 x 1024 30 -> 42), two teams of four waves with every other tile each (30
 // -> 36), three buffers (no change: the copies are there in time), products of the
@@ -44,9 +44,15 @@ namespace attn {
 // tile: as many as two workgroups per CU have registers and LDS for, 64 where the
 // maximum, the rescaling test and the barrier of a tile spread over more of them.
 // NARROW: 32 keys, and three workgroups per CU (heads of 128), which pays where
-// many short rows make starts and ends weigh: 17 prompts of 12001 tokens 149 ->
-// 136 us, 13 chunks under a window of 1024 88 -> 71; one prompt of 16384 tokens
-// 1139 -> 1175, 4 of 1024 in exactly two workgroups per CU 38 -> 45.
+// many short rows make starts and ends weigh (the rule is launch_attention's).  64
+// keys -> 32, us, 32 / 8 heads:
+//   prompts   64 of 64 25 -> 21, 64 of 256 116 -> 98, 300 of up to 200 102 -> 87, 12
+//             of 1024 147 -> 142, 8 of 4096 1288 -> 1231; 6 of 1024 80 -> 83, one of
+//             16384 1090 -> 1110
+//   chunks    13 x 350 under a window of 256 57 -> 47, of 1024 121 -> 110, of 2048 213
+//             -> 196; 64 x 64 over 512 68 -> 60; 64 x 100 over 1000 177 -> 179
+// It loses where two workgroups per CU come out even and three do not: chunks of 16 x
+// 256 over 1024 82 -> 95, over 4096 323 -> 410; 32 x 128 over 2048 179 -> 218.
 template <typename T, int DP, bool NARROW>
 struct TileShape {
     static constexpr int E = sizeof(T);

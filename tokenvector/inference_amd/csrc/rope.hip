@@ -9,11 +9,10 @@
 
 namespace tkv {
 
-// table[p][i] = amplitude * (cos, sin)(p * inv_freq[i]).  The product of a
-// position below 2^29 and a frequency of 24 significant bits is exact in f64,
-// and sincos reduces it there: the table is right to f32 rounding at any
-// position, where an f32 angle would be off by 2^-24 of itself (0.006 rad at
-// position 100000).
+// table[p][i] = amplitude * (cos, sin)(p * inv_freq[i]).  The product is rounded
+// once in f64, 2^-53 of itself (10^-7 rad at position 2^29), and sincos reduces it
+// there: the entries are right to f32 rounding, where an f32 angle would be off by
+// 2^-24 of itself (0.006 rad at position 100000).
 struct Freqs {
     double f[128];
 };
