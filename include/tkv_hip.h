@@ -659,6 +659,56 @@ int32_t tkv_hip_dev_attention_paged(int64_t ctx, int32_t type, int64_t tokens, i
                                     const int32_t* cu_q, const int32_t* kv_lens, int64_t max_q,
                                     int64_t max_kv, float scale, int32_t causal, int64_t window);
 
+/* ======================================================================== */
+/* Microscaled 4-bit floating point (extension): rows coded and decoded, and */
+/* their products on the scaled matrix units.  No counterpart in the         */
+/* reference.                                                                */
+/* ======================================================================== */
+
+/* A row of `cols` elements is ceil(cols / 32) blocks of 32 neighbours (the
+ * last filled up with zeros): codes [rows][blocks][16] bytes, element 2i in the
+ * low half of byte i, 16-byte aligned, and scales [rows][blocks] bytes.  Code
+ * c of a block with scale byte s stands for +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}[c % 8]
+ * 2^(s - 127), negative from 8 on; s = 255: NaN, whatever the code.
+ *
+ * quantize: s = clamp(floor(log2(max|x|)) - 2, -127, 127) + 127 and code =
+ * x / 2^(s - 127) rounded to the nearest value, ties to even, magnitudes above 6
+ * to 6.  A block of zeros has s = 0; one with a NaN or an infinity s = 255 and
+ * codes 0.  x: rows of F32, F16 or BF16, `stride` (>= cols) elements apart; of
+ * one row the stride is not used.
+ * dequantize: the values, rounded once to `type` (F32: exact; what passes the
+ * type's range is infinite). */
+int32_t tkv_hip_dev_quantize_mxfp4(int64_t ctx, int32_t type, const void* x, int64_t stride,
+                                   int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales);
+int32_t tkv_hip_dev_dequantize_mxfp4(int64_t ctx, const uint8_t* codes, const uint8_t* scales,
+                                     int64_t rows, int64_t cols, int32_t type, void* y,
+                                     int64_t stride);
+/* y[m, n] = sum_k a[m, k] w[n, k] + bias[n] (bias NULL: 0), a [M, K] and w
+ * [N, K] in codes and scales.  Products are exact, sums f32, y rounded once to
+ * type_out (F32, F16, BF16), its rows `stride` (>= N) elements apart.  A NaN
+ * block makes its row's (or column's) outputs NaN and touches no other.  Where K
+ * is no multiple of 32, the codes past K have to be zeros in a or in w (quantize
+ * writes them so).  A sum's terms below 2^-126 may be taken as zero.
+ * K >= 2^17, M >= 2^31 or N >= 2^28: UNSUPPORTED. */
+int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a_scales,
+                                 const uint8_t* w, const uint8_t* w_scales, int64_t m, int64_t n,
+                                 int64_t k, const float* bias, int32_t type_out, void* y,
+                                 int64_t stride);
+/* A resident weight in this format: from floats by tkv_hip_weight_create with
+ * this format, or from codes and scales (copied).  tkv_hip_linear_forward codes
+ * the activation's rows by `quantize` and multiplies; act_mode (either) makes
+ * no difference, every block has its own scale.  tkv_hip_weight_info returns
+ * the codes, the scale bytes [N, ceil(K / 32)] as `scales`, and as k the codes'
+ * row stride in elements, 32 ceil(K / 32). */
+#define TKV_HIP_WEIGHT_MXFP4 4
+int32_t tkv_hip_weight_create_mxfp4(int64_t ctx, const uint8_t* codes, const uint8_t* scales,
+                                    int64_t n, int64_t k, const float* bias, int64_t* handle_out);
+/* The linear on rows of F32, F16 or BF16, stride_x (>= K) elements apart, y of
+ * type_out with rows stride_y (>= N) apart.  MXFP4 weights; others: UNSUPPORTED. */
+int32_t tkv_hip_linear_forward_typed(int64_t ctx, int64_t weight, int32_t type_in, const void* x,
+                                     int64_t stride_x, int64_t m, int32_t type_out, void* y,
+                                     int64_t stride_y);
+
 #ifdef __cplusplus
 }
 #endif

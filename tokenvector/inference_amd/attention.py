@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 import numpy as np
 
 from . import _lib
-from .device import Context, DeviceBuffer, _vp
+from .device import Context, DeviceBuffer, QuantizedLinear, _vp
 
 F32, F16, BF16, I8 = 0, 1, 2, 3
 ROPE_HALF, ROPE_PAIRS = 0, 1
@@ -76,8 +76,8 @@ class KVCache:
 
 class _Call:
     """An entry point and its arguments, converted once; calling it launches.
-    The addresses are those of its construction, so a cache or buffer that was
-    closed since is refused."""
+    The addresses are those of its construction, so a cache, weight or buffer that
+    was closed since is refused."""
 
     def __init__(self, name, ctx, *args):
         lib = _lib.lib()
@@ -89,6 +89,7 @@ class _Call:
         given = [x.data if isinstance(x, Rows) else x for x in self._also]
         self._caches = [x for x in given if isinstance(x, KVCache)]
         given += [x for cache in self._caches for x in cache._kept]
+        self._weights = [x for x in given if isinstance(x, QuantizedLinear)]
         self._buffers = [x for x in given if isinstance(x, DeviceBuffer)]
         self._args = tuple(C.cast(C.byref(a), C.c_void_p) if isinstance(a, C.Structure)
                            else C.c_void_p() if a is None else a if isinstance(a, t) else t(a)
@@ -98,6 +99,9 @@ class _Call:
         for cache in self._caches:
             if not cache.handle:
                 raise ValueError("the cache of this call is closed")
+        for weight in self._weights:
+            if not weight.handle:
+                raise ValueError("the weight of this call is closed")
         for buffer in self._buffers:
             if not buffer.ptr and buffer.nbytes:
                 raise ValueError("a buffer of this call is closed")

@@ -12,6 +12,7 @@
 #include <new>
 #include <string>
 
+#include "mxfp4.h"
 #include "tkv_device.h"
 #include "tkv_internal.h"
 
@@ -25,6 +26,8 @@ struct Weight {
     void* codes16 = nullptr; // WEIGHT_FP8: [n, ldk] halves, the codes' reference decode
     float* scales = nullptr; // [n] per-channel scales
     float* gscales = nullptr;// WEIGHT_Q8_0: [n, ldk / 32] group scales (the blocks' d)
+    uint8_t* mscales = nullptr; // WEIGHT_MXFP4: [n, ldk / 32] scale bytes,
+    uint8_t* slabs = nullptr;   // and as the products take them
     float* bias = nullptr;   // [n] or null
 };
 
@@ -83,9 +86,46 @@ static void weight_release(Weight* wt) {
     if (wt->codes) (void)hipFree(wt->codes);
     if (wt->codes16) (void)hipFree(wt->codes16);
     if (wt->gscales) (void)hipFree(wt->gscales);
+    if (wt->mscales) (void)hipFree(wt->mscales);
+    if (wt->slabs) (void)hipFree(wt->slabs);
     if (wt->scales) (void)hipFree(wt->scales);
     if (wt->bias) (void)hipFree(wt->bias);
     delete wt;
+}
+
+// WEIGHT_MXFP4: whole blocks, their scale bytes and slabs.
+static int weight_alloc_mx(Ctx* c, Weight* wt, int64_t n, int64_t k, const float* bias) {
+    wt->device = c->device;
+    wt->format = TKV_HIP_WEIGHT_MXFP4;
+    wt->n = n;
+    wt->k = k;
+    const int64_t blocks = mx::blocks_of(k);
+    wt->ldk = blocks * 32;
+    TKV_HIP_TRY(hipMalloc(&wt->codes, (size_t)(n * blocks * 16)));
+    TKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&wt->mscales), (size_t)(n * blocks)));
+    TKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&wt->slabs), mx::slab_bytes(n, k)));
+    if (bias) {
+        TKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&wt->bias), (size_t)n * 4));
+        TKV_HIP_TRY(hipMemcpyAsync(wt->bias, bias, (size_t)n * 4, hipMemcpyDeviceToDevice, c->stream));
+    }
+    return TKV_HIP_OK;
+}
+
+// The linear of an MXFP4 weight on rows of `type`.
+static int linear_mx(Ctx* c, const Weight* wt, int type, const void* x, int64_t stride_x, int64_t m, int type_out,
+                     void* y, int64_t stride_y) {
+    mx::Product p = {};
+    p.w = static_cast<const uint8_t*>(wt->codes);
+    p.ws = wt->slabs;
+    p.m = m;
+    p.n = wt->n;
+    p.w_rows = mx::slab_rows(wt->n);
+    p.blocks = (int32_t)(wt->ldk / 32);
+    p.bias = wt->bias;
+    p.y = y;
+    p.ldy = stride_y;
+    p.y_type = type_out;
+    return launch_mx_linear(c, type, x, stride_x, wt->k, p);
 }
 
 // The per-call part of CS1 on context c: activation calibrate + quantize
@@ -95,6 +135,13 @@ static int linear_forward(Ctx* c, Weight* wt, const float* x, int64_t m, int32_t
     if (!wt || !x || !y || m < 0) return set_error(TKV_HIP_BAD_ARG, "linear_forward: bad arguments");
     if (m == 0) return TKV_HIP_OK;
     const int64_t k = wt->k;
+    if (wt->format == TKV_HIP_WEIGHT_MXFP4) {
+        if (act_mode != TKV_HIP_ACT_PER_TENSOR && act_mode != TKV_HIP_ACT_PER_TOKEN)
+            return set_error(TKV_HIP_BAD_ARG, "linear_forward: unknown act_mode");
+        if (m >= (1ll << 31) || wt->device != c->device)
+            return set_error(TKV_HIP_BAD_ARG, "linear_forward: M >= 2^31, or the weight is on another device");
+        return linear_mx(c, wt, TKV_HIP_F32, x, k, m, TKV_HIP_F32, y, wt->n);
+    }
     if (wt->format == TKV_HIP_WEIGHT_INT8 && act_mode == TKV_HIP_ACT_PER_TOKEN) {
         // decode batches: quantize + GEMM + epilogue in one kernel, reading
         // the weight through its padded row stride
@@ -233,6 +280,37 @@ static int static_scratch(int dev, uint8_t** out, int* cus, size_t* lds) {
 static int linear_forward_static_on(Weight* wt, const float* x, int64_t m, int32_t act_mode,
                                     float* y, void* stream);
 
+// An MXFP4 weight from floats w [n, k], or from codes and scales.
+static int weight_create_mx(Ctx* c, const float* w, const uint8_t* codes, const uint8_t* scales, int64_t n, int64_t k,
+                            const float* bias, int64_t* handle_out) {
+    if (n >= (1ll << 28) || k >= (1ll << 17))
+        return set_error(TKV_HIP_UNSUPPORTED, "MXFP4 weight: K must be below 2^17 and N below 2^28");
+    Weight* wt = new (std::nothrow) Weight();
+    if (!wt) return set_error(TKV_HIP_OOM, "MXFP4 weight: host allocation failed");
+    int rc = weight_alloc_mx(c, wt, n, k, bias);
+    if (rc == TKV_HIP_OK && w) {
+        rc = launch_mx_quantize(c, TKV_HIP_F32, w, k, n, k, static_cast<uint8_t*>(wt->codes), wt->mscales, false);
+    } else if (rc == TKV_HIP_OK) {
+        const int64_t blocks = mx::blocks_of(k);
+        hipError_t e = hipMemcpyAsync(wt->codes, codes, (size_t)(n * blocks * 16), hipMemcpyDeviceToDevice, c->stream);
+        if (e == hipSuccess)
+            e = hipMemcpyAsync(wt->mscales, scales, (size_t)(n * blocks), hipMemcpyDeviceToDevice, c->stream);
+        if (e != hipSuccess) rc = fail_hip(e, "MXFP4 weight copy", __FILE__, __LINE__);
+    }
+    if (rc == TKV_HIP_OK) rc = launch_mx_slabs(c, wt->mscales, n, k, wt->slabs);
+    if (rc == TKV_HIP_OK) {
+        hipError_t e = hipStreamSynchronize(c->stream);
+        if (e != hipSuccess) rc = fail_hip(e, "hipStreamSynchronize", __FILE__, __LINE__);
+    }
+    if (rc != TKV_HIP_OK) {
+        if (rc == TKV_HIP_OOM) (void)hipGetLastError();
+        weight_release(wt);
+        return rc;
+    }
+    *handle_out = reinterpret_cast<int64_t>(wt);
+    return TKV_HIP_OK;
+}
+
 }  // namespace tkv
 
 using namespace tkv;
@@ -248,8 +326,9 @@ int32_t tkv_hip_weight_create(int64_t ctx, const float* w, int64_t n, int64_t k,
     if (c->capturing)
         return set_error(TKV_HIP_BAD_ARG, "weight_create: allocates and synchronizes, not inside a stream capture");
     if (format != TKV_HIP_WEIGHT_INT8 && format != TKV_HIP_WEIGHT_FP8 &&
-        format != TKV_HIP_WEIGHT_FP8_FAST)
+        format != TKV_HIP_WEIGHT_FP8_FAST && format != TKV_HIP_WEIGHT_MXFP4)
         return set_error(TKV_HIP_BAD_ARG, "weight_create: unknown format");
+    if (format == TKV_HIP_WEIGHT_MXFP4) return weight_create_mx(c, w, nullptr, nullptr, n, k, bias, handle_out);
     Weight* wt = new (std::nothrow) Weight();
     if (!wt) return set_error(TKV_HIP_OOM, "weight_create: host allocation failed");
     int rc = weight_alloc(c, wt, n, k, format, bias);
@@ -362,6 +441,17 @@ int32_t tkv_hip_weight_create_gguf_q8_0(int64_t ctx, const uint8_t* raw, int64_t
     return TKV_HIP_OK;
 }
 
+int32_t tkv_hip_weight_create_mxfp4(int64_t ctx, const uint8_t* codes, const uint8_t* scales, int64_t n, int64_t k,
+                                    const float* bias, int64_t* handle_out) {
+    if (!codes || !scales || !handle_out || n <= 0 || k <= 0)
+        return set_error(TKV_HIP_BAD_ARG, "weight_create_mxfp4: bad arguments");
+    Ctx* c;
+    TKV_RC_TRY(ctx_get(ctx, &c));
+    if (c->capturing)
+        return set_error(TKV_HIP_BAD_ARG, "weight_create_mxfp4: allocates and synchronizes, not inside a stream capture");
+    return weight_create_mx(c, nullptr, codes, scales, n, k, bias, handle_out);
+}
+
 int32_t tkv_hip_weight_free(int64_t handle) {
     weight_release(reinterpret_cast<Weight*>(handle));
     return TKV_HIP_OK;
@@ -372,7 +462,10 @@ int32_t tkv_hip_weight_info(int64_t handle, void** codes, float** scales, float*
     Weight* wt = reinterpret_cast<Weight*>(handle);
     if (!wt) return set_error(TKV_HIP_BAD_ARG, "NULL weight handle");
     if (codes) *codes = wt->codes;
-    if (scales) *scales = wt->format == TKV_HIP_WEIGHT_Q8_0 ? wt->gscales : wt->scales;
+    if (scales)
+        *scales = wt->format == TKV_HIP_WEIGHT_Q8_0    ? wt->gscales
+                  : wt->format == TKV_HIP_WEIGHT_MXFP4 ? reinterpret_cast<float*>(wt->mscales)
+                                                       : wt->scales;
     if (bias) *bias = wt->bias;
     if (n) *n = wt->n;
     if (k) *k = wt->ldk;
@@ -385,6 +478,25 @@ int32_t tkv_hip_linear_forward(int64_t ctx, int64_t weight, const float* x, int6
     Ctx* c;
     TKV_RC_TRY(ctx_get(ctx, &c));
     return linear_forward(c, reinterpret_cast<Weight*>(weight), x, m, act_mode, y);
+}
+
+int32_t tkv_hip_linear_forward_typed(int64_t ctx, int64_t weight, int32_t type_in, const void* x, int64_t stride_x,
+                                     int64_t m, int32_t type_out, void* y, int64_t stride_y) {
+    const Weight* wt = reinterpret_cast<const Weight*>(weight);
+    if (!wt || m < 0 || m >= (1ll << 31) || !float_type(type_in) || !float_type(type_out))
+        return set_error(TKV_HIP_BAD_ARG, "linear_forward_typed: NULL weight, M out of range or unknown types");
+    if (wt->format != TKV_HIP_WEIGHT_MXFP4)
+        return set_error(TKV_HIP_UNSUPPORTED, "linear_forward_typed: MXFP4 weights only");
+    if (m > 1 && (stride_x < wt->k || stride_y < wt->n))
+        return set_error(TKV_HIP_BAD_ARG, "linear_forward_typed: a stride below K or N");
+    if (m == 0) return TKV_HIP_OK;
+    if (!x || !y || !aligned(x, type_bytes(type_in)) || !aligned(y, type_bytes(type_out)))
+        return set_error(TKV_HIP_BAD_ARG, "linear_forward_typed: NULL or unaligned buffers");
+    Ctx* c;
+    TKV_RC_TRY(ctx_get(ctx, &c));
+    if (wt->device != c->device)
+        return set_error(TKV_HIP_BAD_ARG, "linear_forward_typed: the weight is on another device");
+    return linear_mx(c, wt, type_in, x, m > 1 ? stride_x : wt->k, m, type_out, y, m > 1 ? stride_y : wt->n);
 }
 
 int32_t tkv_hip_linear_forward_static(int64_t weight, const float* x, int64_t m,

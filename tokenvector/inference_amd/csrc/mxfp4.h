@@ -1,0 +1,83 @@
+// mxfp4.h -- microscaled 4-bit floating point: its layouts, and what the
+// kernels that code, decode and multiply it share.
+//
+// A row of k elements is ceil(k / 32) blocks of 16 code bytes (element 2i in
+// the low half of byte i; the last block's missing elements are zeros) and as
+// many scale bytes, 2^(byte - 127), 255 for a block that stands for NaN.
+// The matrix kernels take the scales in slabs: [ceil(blocks / 8)][rows rounded
+// up to 256][8], so that the scales of a tile's rows and of the 256 elements of
+// a K slice are one run, which the copies to LDS and a wave's loads take whole.
+// Blocks past the row's last have scale 0: 2^-127 on either side, products
+// below 2^-240, which add nothing to an f32 sum.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "attn.h"
+
+namespace tkv {
+namespace mx {
+
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int kSlabRows = 256;
+inline int64_t blocks_of(int64_t k) { return ceil_div(k, 32); }
+inline int64_t slabs_of(int64_t k) { return ceil_div(blocks_of(k), 8); }
+inline int64_t slab_rows(int64_t rows) { return ceil_div(rows, kSlabRows) * kSlabRows; }
+inline size_t slab_bytes(int64_t rows, int64_t k) { return (size_t)(slabs_of(k) * slab_rows(rows) * 8); }
+
+// A product's operands and output.  y rows ldy elements apart, of y_type.
+struct Product {
+    const uint8_t *a, *as;  // codes [m][blocks][16], slabs
+    const uint8_t *w, *ws;  // codes [n][blocks][16], slabs
+    int64_t m, n;
+    int64_t a_rows, w_rows;  // of the slabs
+    int32_t blocks;
+    const float* bias;
+    void* y;
+    int64_t ldy;
+    int32_t y_type;
+};
+
+// The block's scale byte from its largest |x| as bits: floor(log2) - 2 (the
+// largest code is 1.5 * 2^2), at least 2^-127, which blocks of zeros and
+// subnormals get.
+__device__ __forceinline__ unsigned scale_byte(unsigned most) {
+    const unsigned e = most >> 23;
+    return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
+}
+// 2^(byte - 127), byte < 255
+__device__ __forceinline__ float scale_value(unsigned byte) {
+    return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+// Eight codes of x / scale: rounded to nearest even and saturated at 6 by
+// v_cvt_scalef32_pk_fp4_f32 (the same as comparing with the midpoints for every
+// finite float, subnormal scale included).
+__device__ __forceinline__ unsigned code8(const float (&x)[8], float scale) {
+    unsigned c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
+}
+
+}  // namespace mx
+
+// mxfp4.hip.  x: rows of `cols` elements of `type`, `stride` elements apart.
+// Scales to [rows][blocks], or to slabs.
+int launch_mx_quantize(Ctx* c, int type, const void* x, int64_t stride, int64_t rows, int64_t cols,
+                       uint8_t* codes, uint8_t* scales, bool slabs);
+int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                         int64_t cols, int type, void* y, int64_t stride);
+int launch_mx_slabs(Ctx* c, const uint8_t* scales, int64_t rows, int64_t k, uint8_t* slabs);
+// mxfp4_tile.hip
+int launch_mx_product(Ctx* c, const mx::Product& p);
+// The linear of a resident weight on float rows (mxfp4.hip).
+int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, mx::Product p);
+
+}  // namespace tkv

@@ -21,6 +21,7 @@ WEIGHT_INT8 = 0
 WEIGHT_FP8 = 1
 WEIGHT_FP8_FAST = 2
 WEIGHT_Q8_0 = 3      # GGUF Q8_0 blocks on the INT8 GEMM with group scales (extension)
+WEIGHT_MXFP4 = 4     # microscaled 4-bit floating point, weight and activations (extension)
 
 
 def _vp(x) -> C.c_void_p:
@@ -389,6 +390,16 @@ class QuantizedLinear:
         h = C.c_int64()
         _lib.check(_lib.lib().tkv_hip_weight_create_gguf_q8_0(ctx.handle, _vp(raw), int(n), int(k),
                                                               _vp(bias), C.byref(h)))
+        return cls(ctx, h.value)
+
+    @classmethod
+    def from_mxfp4(cls, ctx: Context, codes, scales, n: int, k: int, bias=None) -> "QuantizedLinear":
+        """A weight [n, k] from codes [n, ceil(k / 32), 16] and scale bytes
+        [n, ceil(k / 32)] on the device (copied), as mxfp4.Quantize writes them;
+        `scales` is then those bytes and k the padded row stride."""
+        h = C.c_int64()
+        _lib.check(_lib.lib().tkv_hip_weight_create_mxfp4(ctx.handle, _vp(codes), _vp(scales), int(n),
+                                                          int(k), _vp(bias), C.byref(h)))
         return cls(ctx, h.value)
 
     def forward(self, x, m: int, y, act_mode: int = ACT_PER_TENSOR) -> None:
