@@ -614,6 +614,41 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
                                 const tkv_hip_rows* k_out, int32_t type_out, int64_t cache,
                                 const int64_t* slots);
 
+/* rope_append with norms per head and with positions on several axes.
+ *   norm (NULL: none): each head of q and of k becomes
+ *     x / sqrt(mean(x^2) + eps) * gain, in f32, before its rotation; gains f32
+ *     [head_dim] on the device, one for the queries' heads and one for the
+ *     keys', NULL for ones.  eps > 0.  Values are not normed.
+ *   rope (NULL: no rotation): as there, but pair i takes entry i of the table's
+ *     row of its own axis' position, positions[pair_axis[i] * stride_axis +
+ *     token] (time, height and width of images and video).  pair_axis: rot_dim / 2
+ *     bytes in host memory, each below `axes` (1 .. 4); NULL with one axis.  The
+ *     table's columns are the pairs', so axes with frequencies of their own are a
+ *     choice of the table.
+ * A token with a position outside [0, table_len) on any axis is a padding token.
+ * Without norm and with one axis it is rope_append, bit for bit. */
+typedef struct {
+    float eps;
+    const float* q_gain;
+    const float* k_gain;
+} tkv_hip_head_norm;
+typedef struct {
+    const float* table;
+    int64_t table_len;
+    int64_t rot_dim;
+    int32_t layout;
+    int32_t axes;
+    const int32_t* positions;
+    int64_t stride_axis;
+    const uint8_t* pair_axis;
+} tkv_hip_rope;
+int32_t tkv_hip_dev_norm_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, int64_t heads_q,
+                                     int64_t heads_kv, int64_t head_dim, const tkv_hip_rows* q,
+                                     const tkv_hip_rows* k, const tkv_hip_rows* v,
+                                     const tkv_hip_head_norm* norm, const tkv_hip_rope* rope,
+                                     const tkv_hip_rows* q_out, const tkv_hip_rows* k_out,
+                                     int32_t type_out, int64_t cache, const int64_t* slots);
+
 /* Attention.  For every query row i of a sequence of n query and t key rows,
  * at position pos = t - n + i,
  *   out_i = sum_j exp(a_ij - m_i) v_j / sum_j exp(a_ij - m_i),

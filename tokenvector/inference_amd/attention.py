@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -161,6 +161,84 @@ class RopeAppend(_Call):
             "tkv_hip_dev_rope_append", ctx, int(type_in), int(tokens), int(heads_q),
             int(heads_kv), int(head_dim), _rows(q), _rows(k), _rows(v), _vp(positions), _vp(table),
             int(table_len), int(rot_dim), int(layout), _rows(q_out), _rows(k_out),
+            int(type_in if type_out is None else type_out), cache.handle if cache else 0, _vp(slots))
+
+
+class HeadNorm(NamedTuple):
+    """Norms per head: x / sqrt(mean(x^2) + eps) * gain, gains f32 [head_dim] on
+    the device (None: ones) for the queries' heads and for the keys'."""
+    eps: float
+    q_gain: object = None
+    k_gain: object = None
+
+
+class Rope(NamedTuple):
+    """A rotation: the table (rope_table), int32 device positions, `axes` rows of
+    them stride_axis apart, and the axis of each pair (rope_pair_axes)."""
+    table: object
+    table_len: int
+    rot_dim: int
+    layout: int
+    positions: object
+    axes: int = 1
+    stride_axis: int = 0
+    pair_axis: Optional[Sequence[int]] = None
+
+
+class _HeadNorm(C.Structure):
+    _fields_ = [("eps", C.c_float), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_len", C.c_int64), ("rot_dim", C.c_int64), ("layout", C.c_int32),
+                ("axes", C.c_int32), ("positions", C.c_void_p), ("stride_axis", C.c_int64),
+                ("pair_axis", C.c_void_p)]
+
+
+def rope_pair_axes(sections: Sequence[int], interleaved: bool = False) -> list:
+    """The axis of each of sum(sections) pairs: the axes' sections behind each
+    other, or interleaved (one pair of each axis in turn, as long as it has any)."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= 4 or min(left) < 0 or sum(left) == 0:
+        raise ValueError("sections: the pairs of 1 to 4 axes")
+    if not interleaved:
+        return [axis for axis, n in enumerate(left) for _ in range(n)]
+    out = []
+    while any(left):
+        for axis, n in enumerate(left):
+            if n:
+                out.append(axis)
+                left[axis] -= 1
+    return out
+
+
+class NormRopeAppend(_Call):
+    """RopeAppend with norms of each head of q and k before the rotation, and
+    with positions on several axes.  norm or rope None: without it."""
+
+    def __init__(self, ctx: Context, type_in: int, tokens: int, heads_q: int, heads_kv: int,
+                 head_dim: int, q: Optional[Rows], k: Optional[Rows] = None,
+                 v: Optional[Rows] = None, norm: Optional[HeadNorm] = None, rope: Optional[Rope] = None,
+                 q_out: Optional[Rows] = None, k_out: Optional[Rows] = None,
+                 type_out: Optional[int] = None, cache: Optional[KVCache] = None, slots=None):
+        self._also = (q, k, v, q_out, k_out, cache, slots) + tuple(norm or ())[1:]
+        n = r = None
+        if norm is not None:
+            n = _HeadNorm(float(norm.eps), _vp(norm.q_gain).value, _vp(norm.k_gain).value)
+        if rope is not None:
+            self._also += (rope.table, rope.positions)
+            self._axes = None
+            if rope.pair_axis is not None:
+                pairs = [int(x) for x in rope.pair_axis]
+                if len(pairs) != int(rope.rot_dim) // 2 or not all(0 <= x <= 255 for x in pairs):
+                    raise ValueError("pair_axis: the axis of each of rot_dim / 2 pairs")
+                self._axes = (C.c_uint8 * len(pairs))(*pairs)  # kept: read at every call
+            r = _Rope(_vp(rope.table).value, int(rope.table_len), int(rope.rot_dim), int(rope.layout),
+                      int(rope.axes), _vp(rope.positions).value, int(rope.stride_axis),
+                      C.cast(self._axes, C.c_void_p).value if self._axes is not None else None)
+        super().__init__(
+            "tkv_hip_dev_norm_rope_append", ctx, int(type_in), int(tokens), int(heads_q),
+            int(heads_kv), int(head_dim), _rows(q), _rows(k), _rows(v), n, r, _rows(q_out), _rows(k_out),
             int(type_in if type_out is None else type_out), cache.handle if cache else 0, _vp(slots))
 
 

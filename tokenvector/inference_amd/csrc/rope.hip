@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include <new>
+#include <string>
 
 #include "attn.h"
 
@@ -43,7 +44,15 @@ struct RopeArgs {
     int64_t tokens;
     int32_t hq, hkv, d, rot, pairs;
     int32_t lanes_log2;  // lanes of a head row
+    // the kernels with NORM or AXES (below) alone
+    int32_t normed;
+    float eps;
+    const float *qg, *kg;     // gains, or null
+    int32_t axes;
+    int64_t axis_stride;      // of the positions
+    uint32_t pair_axis[8];    // two bits a pair
 };
+constexpr int kMaxAxes = 4;
 
 template <typename T>
 struct alignas(16) Vec8 {
@@ -81,6 +90,14 @@ __device__ __forceinline__ float row_max(unsigned m, int lanes) {
     for (int o = 1 << lanes >> 1; o; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
     return __uint_as_float(m);
 }
+// 1 / sqrt(mean of the squares + eps), from their sum over a row's lanes
+__device__ __forceinline__ float row_sum(float s, int lanes) {
+    for (int o = 1 << lanes >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+    return s;
+}
+__device__ __forceinline__ float inv_norm(float sum, int d, float eps) {
+    return 1.0f / __builtin_sqrtf(sum / (float)d + eps);
+}
 // By the rounded reciprocal, as elementwise tensor libraries divide by a constant:
 // within an ulp of max / 127, and the same codes as their operations give.
 __device__ __forceinline__ float scale_of(float m) { return (m < 1e-8f ? 1e-8f : m) * (1.0f / 127.0f); }
@@ -97,7 +114,11 @@ __device__ __forceinline__ int8_t code_of(float x, float inv) {
 // workgroup's.  HBM bound: 8192 tokens of 32 + 8 heads of 128, bf16, 45.7 us, 4.5
 // TB/s, where a large copy reaches 5.1; 32 tokens of 12 + 12 heads of 64 take 3.4 us,
 // one launch.
-template <typename TI, typename TO, typename C, int HEADS>
+//
+// MORE: with norms per head, positions on several axes, or both.  The squares' sum
+// of a head goes over its lanes; the gains are loaded once for heads of one role in
+// turn; a pair's entry is in the row of its own axis' position.
+template <typename TI, typename TO, typename C, int HEADS, bool MORE>
 __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const int64_t t64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
     if (t64 >= a.tokens) return;  // whole groups: the rows' lanes stay together
@@ -109,7 +130,16 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const int c1 = i < turns ? i + turns : c0 < chunks ? c0 + (rest + 1) / 2 : chunks;
     const bool in0 = c0 < chunks, in1 = c1 < chunks;
     const int pos = a.table ? a.positions[tok] : 0;
-    const bool pad = a.table && (pos < 0 || pos >= a.table_len);
+    bool pad = a.table && (pos < 0 || pos >= a.table_len);
+    int at_axis[kMaxAxes] = {pos, pos, pos, pos};
+    if (MORE && a.table) {
+#pragma unroll
+        for (int x = 1; x < kMaxAxes; x++)
+            if (x < a.axes) {
+                at_axis[x] = a.positions[x * a.axis_stride + tok];
+                pad = pad || at_axis[x] < 0 || at_axis[x] >= a.table_len;
+            }
+    }
     int64_t slot = -1;
     if (a.kc && !pad) slot = a.slots[tok];
     const bool put = slot >= 0 && slot < a.n_slots;
@@ -118,6 +148,16 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const bool turn0 = a.pairs ? c0 < a.rot >> 3 : i < turns, turn1 = a.pairs ? c1 < a.rot >> 3 : i < turns;
     float2 w[8];
     const auto entries = [&](int at, float2* to) {
+        if (MORE && a.axes > 1) {
+            const uint32_t which = a.pair_axis[at >> 4] >> (2 * (at & 15));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int x = (which >> (2 * k)) & 3;
+                const int p = x == 0 ? at_axis[0] : x == 1 ? at_axis[1] : x == 2 ? at_axis[2] : at_axis[3];
+                to[k] = a.table[(int64_t)p * (a.rot >> 1) + at + k];
+            }
+            return;
+        }
         const float4* cs = reinterpret_cast<const float4*>(a.table + (int64_t)pos * (a.rot >> 1) + at);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
@@ -143,12 +183,32 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
         if (in0 && !pad) load8(src + 8 * c0, x0[u]);
         if (in1 && !pad) load8(src + 8 * c1, x1[u]);
     }
+    float g0[8], g1[8];
+    const float* have = nullptr;
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
         const int row = first + u;
         if (row >= (int)a.heads.d) break;
         const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
         const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
+        if (MORE && a.normed && !isv) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum += x0[u][k] * x0[u][k] + x1[u][k] * x1[u][k];
+            const float r = inv_norm(row_sum(sum, a.lanes_log2), a.d, a.eps);
+            const float* gain = isq ? a.qg : a.kg;
+            if (gain && gain != have) {
+                if (in0) load8(gain + 8 * c0, g0);
+                if (in1) load8(gain + 8 * c1, g1);
+                have = gain;
+            }
+            // (a padding token's zeros stay zeros whatever the gains)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (in0 && !pad) x0[u][k] = x0[u][k] * r * (gain ? g0[k] : 1.0f);
+                if (in1 && !pad) x1[u][k] = x1[u][k] * r * (gain ? g1[k] : 1.0f);
+            }
+        }
         if (!isv && !pad) {
             // each product and sum is rounded by itself (no contraction in this
             // library): the same bits as separate elementwise operations
@@ -208,7 +268,7 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
 // Any head size, rotation and alignment: one head row per 2^lanes lanes, 8
 // elements a lane, one by one; the element that one is rotated with is loaded
 // again, so that it is bound by its load instructions.
-template <typename TI, typename TO, typename C>
+template <typename TI, typename TO, typename C, bool MORE>
 __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
     const int64_t t = wide_block() * 256 + threadIdx.x;
     const int64_t r64 = t >> a.lanes_log2;
@@ -223,21 +283,47 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
                     (int64_t)tok * (isq ? a.q_st : isv ? a.v_st : a.k_st) +
                     (int64_t)h * (isq ? a.q_sh : isv ? a.v_sh : a.k_sh);
     const int pos = a.table ? a.positions[tok] : 0;
-    const bool pad = a.table && (pos < 0 || pos >= a.table_len);
+    bool pad = a.table && (pos < 0 || pos >= a.table_len);
+    if (MORE && a.table)
+        for (int x = 1; x < a.axes; x++) {
+            const int p = a.positions[x * a.axis_stride + tok];
+            pad = pad || p < 0 || p >= a.table_len;
+        }
     int64_t slot = -1;
     if (!isq && a.kc && !pad) slot = a.slots[tok];
     const int half = a.rot >> 1;
     const float2* cs = a.table + (int64_t)pos * half;
+    const bool normed = MORE && a.normed && !isv;
+    const float* gain = isq ? a.qg : a.kg;
+    float inv = 1.0f;
+    if (MORE && a.normed) {  // every lane of the wave takes part in the sum
+        float sum = 0.0f;
+        for (int i = 0; i < 8; i++) {
+            const float e = e0 + i < a.d && !pad ? to_f32(src[e0 + i]) : 0.0f;
+            sum += e * e;
+        }
+        inv = inv_norm(row_sum(sum, a.lanes_log2), a.d, a.eps);
+    }
+    const auto element = [&](int e) {
+        const float v = to_f32(src[e]);
+        return normed ? v * inv * (gain ? gain[e] : 1.0f) : v;
+    };
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int e = e0 + i;
-        x[i] = e < a.d && !pad ? to_f32(src[e]) : 0.0f;
+        x[i] = e < a.d && !pad ? element(e) : 0.0f;
         if (e < a.rot && !isv && !pad) {
             const bool low = a.pairs ? !(e & 1) : e < half;
             const int mate = a.pairs ? e ^ 1 : low ? e + half : e - half;
-            const float2 w = cs[a.pairs ? e >> 1 : low ? e : e - half];
-            const float o = to_f32(src[mate]);
+            const int pair = a.pairs ? e >> 1 : low ? e : e - half;
+            const float2* from = cs;
+            if (MORE && a.axes > 1) {
+                const int axis = (a.pair_axis[pair >> 4] >> (2 * (pair & 15))) & 3;
+                from = a.table + (int64_t)a.positions[axis * a.axis_stride + tok] * half;
+            }
+            const float2 w = from[pair];
+            const float o = element(mate);
             x[i] = low ? x[i] * w.x - o * w.y : x[i] * w.x + o * w.y;
         }
     }
@@ -272,7 +358,7 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
     }
 }
 
-template <typename TI, typename TO, typename C>
+template <typename TI, typename TO, typename C, bool MORE>
 static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
     const int64_t heads = a.heads.d;
     int rows_log2 = 0;
@@ -280,22 +366,29 @@ static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
     // (a dimension of the grid holds 2^28 tokens of heads of 256)
     if (!vec || (a.tokens << rows_log2) + 255 > kGridItems) {
         while (8 << a.lanes_log2 < a.d) a.lanes_log2++;
-        k_rope_any<TI, TO, C><<<wide_grid(ceil_div(a.tokens * heads << a.lanes_log2, 256)), 256, 0, c->stream>>>(a);
+        k_rope_any<TI, TO, C, MORE>
+            <<<wide_grid(ceil_div(a.tokens * heads << a.lanes_log2, 256)), 256, 0, c->stream>>>(a);
         return;
     }
     a.lanes_log2 = rows_log2;
     const int64_t blocks = ceil_div(a.tokens << a.lanes_log2, 256);
     // four heads per lane where that still leaves eight workgroups per CU
     if (blocks * ceil_div(heads, 4) >= 8 * c->num_cus)
-        k_rope_rows<TI, TO, C, 4><<<dim3((unsigned)blocks, (unsigned)ceil_div(heads, 4)), 256, 0, c->stream>>>(a);
+        k_rope_rows<TI, TO, C, 4, MORE>
+            <<<dim3((unsigned)blocks, (unsigned)ceil_div(heads, 4)), 256, 0, c->stream>>>(a);
     else
-        k_rope_rows<TI, TO, C, 1><<<dim3((unsigned)blocks, (unsigned)heads), 256, 0, c->stream>>>(a);
+        k_rope_rows<TI, TO, C, 1, MORE><<<dim3((unsigned)blocks, (unsigned)heads), 256, 0, c->stream>>>(a);
 }
 
 template <typename TI, typename TO>
 static void launch_rope_to(Ctx* c, const RopeArgs& a, bool i8, bool vec) {
-    if (i8) launch_rope<TI, TO, int8_t>(c, a, vec);
-    else launch_rope<TI, TO, TO>(c, a, vec);
+    if (a.normed || a.axes > 1) {
+        if (i8) launch_rope<TI, TO, int8_t, true>(c, a, vec);
+        else launch_rope<TI, TO, TO, true>(c, a, vec);
+    } else {
+        if (i8) launch_rope<TI, TO, int8_t, false>(c, a, vec);
+        else launch_rope<TI, TO, TO, false>(c, a, vec);
+    }
 }
 
 template <typename TI>
@@ -308,6 +401,103 @@ static void launch_rope_from(Ctx* c, const RopeArgs& a, int type_out, bool i8, b
 static bool rows_aligned(const tkv_hip_rows* r, int64_t bytes) {
     return !r || (aligned(r->data, 16) && r->stride_token * bytes % 16 == 0 &&
                   r->stride_head * bytes % 16 == 0);
+}
+
+// Both entry points: checks, arguments, launch.  norm and rope may be null.
+static int rope_append(const char* who, int64_t ctx, int32_t type_in, int64_t tokens, int64_t heads_q,
+                       int64_t heads_kv, int64_t head_dim, const tkv_hip_rows* q, const tkv_hip_rows* k,
+                       const tkv_hip_rows* v, const tkv_hip_head_norm* norm, const tkv_hip_rope* rope,
+                       const tkv_hip_rows* q_out, const tkv_hip_rows* k_out, int32_t type_out, int64_t cache,
+                       const int64_t* slots) {
+    const auto bad = [&](const char* what) { return set_error(TKV_HIP_BAD_ARG, std::string(who) + ": " + what); };
+    const KvCache* kv = reinterpret_cast<const KvCache*>(cache);
+    if (!float_type(type_in) || !float_type(type_out)) return bad("types are F32, F16 or BF16");
+    if (tokens < 0 || tokens >= (1ll << 31) || heads_q < 0 || heads_kv < 0 || heads_q > 65535 || heads_kv > 65535 ||
+        head_dim <= 0 || head_dim > 256)
+        return bad("sizes out of range (head_dim 1 .. 256)");
+    if (rope && (rope->rot_dim < 2 || rope->rot_dim > head_dim || rope->rot_dim % 2 || rope->table_len < 0 ||
+                 !rope->positions || !aligned(rope->table, 8) ||
+                 (rope->layout != TKV_HIP_ROPE_HALF && rope->layout != TKV_HIP_ROPE_PAIRS)))
+        return bad("a table takes positions, an even rot_dim in 2 .. head_dim and a known layout");
+    if (rope && (rope->axes < 1 || rope->axes > kMaxAxes || (rope->axes > 1 && !rope->pair_axis)))
+        return bad("1 to 4 axes, several with the axis of each pair");
+    if (rope && rope->axes > 1)
+        for (int64_t i = 0; i < rope->rot_dim / 2; i++)
+            if (rope->pair_axis[i] >= rope->axes) return bad("a pair's axis is not among the axes");
+    if (norm && !(norm->eps > 0.0f && norm->eps <= 3.402823466e38f)) return bad("eps: positive and finite");
+    if (norm && (!aligned(norm->q_gain, 4) || !aligned(norm->k_gain, 4))) return bad("unaligned gains");
+    const bool has_q = q && heads_q > 0, has_k = k && heads_kv > 0, has_v = v && heads_kv > 0;
+    if ((heads_q > 0 && !has_q) || (heads_kv > 0 && !has_k) || (has_q && !q->data) ||
+        (has_k && !k->data) || (has_v && !v->data))
+        return bad("NULL rows with a positive head count");
+    if ((q_out && (!has_q || !q_out->data)) || (k_out && (!has_k || !k_out->data)))
+        return bad("an output without its rows");
+    if (kv) {
+        if (!has_k || !has_v || !slots) return bad("a cache takes k, v and slots");
+        if (kv->heads != heads_kv || kv->d != head_dim) return bad("the cache has other heads");
+        if (kv->type != type_out && kv->type != TKV_HIP_I8)
+            return bad("the cache's type is neither type_out nor I8");
+    }
+    Ctx* c;
+    TKV_RC_TRY(ctx_get(ctx, &c));
+    if (kv && kv->device != c->device) return bad("the cache is on another device");
+    RopeArgs a = {};
+    // without a cache the values have nowhere to go: no rows for them
+    const int64_t heads = heads_q + heads_kv + (kv ? heads_kv : 0);
+    if (tokens == 0 || heads == 0) return TKV_HIP_OK;
+    if (tokens * heads >= (1ll << 31))
+        return set_error(TKV_HIP_UNSUPPORTED, std::string(who) + ": tokens * heads >= 2^31");
+    if (has_q) a.q = q->data, a.q_st = q->stride_token, a.q_sh = q->stride_head;
+    if (has_k) a.k = k->data, a.k_st = k->stride_token, a.k_sh = k->stride_head;
+    if (has_v) a.v = v->data, a.v_st = v->stride_token, a.v_sh = v->stride_head;
+    if (q_out) a.qo = q_out->data, a.qo_st = q_out->stride_token, a.qo_sh = q_out->stride_head;
+    if (k_out) a.ko = k_out->data, a.ko_st = k_out->stride_token, a.ko_sh = k_out->stride_head;
+    if (kv) {
+        a.kc = kv->k;
+        a.vc = kv->v;
+        a.ks = kv->ks;
+        a.vs = kv->vs;
+        a.slots = slots;
+        a.n_slots = kv->pages * kv->page;
+        a.page = fast_div((uint32_t)kv->page);
+    } else {
+        a.page = fast_div(1);
+    }
+    a.heads = fast_div((uint32_t)heads);
+    a.tokens = tokens;
+    a.hq = (int32_t)heads_q;
+    a.hkv = (int32_t)heads_kv;
+    a.d = (int32_t)head_dim;
+    a.axes = 1;
+    if (rope) {
+        a.positions = rope->positions;
+        a.table = reinterpret_cast<const float2*>(rope->table);
+        a.table_len = rope->table_len;
+        a.rot = (int32_t)rope->rot_dim;
+        a.pairs = rope->layout == TKV_HIP_ROPE_PAIRS;
+        a.axes = rope->axes;
+        a.axis_stride = rope->stride_axis;
+        for (int i = 0; a.axes > 1 && i < a.rot / 2; i++)
+            a.pair_axis[i >> 4] |= (uint32_t)rope->pair_axis[i] << (2 * (i & 15));
+    }
+    if (norm) {
+        a.normed = 1;
+        a.eps = norm->eps;
+        a.qg = norm->q_gain;
+        a.kg = norm->k_gain;
+    }
+    const int64_t bi = type_bytes(type_in), bo = type_bytes(type_out);
+    const bool vec = head_dim % 8 == 0 && a.rot % (a.pairs ? 8 : 16) == 0 && aligned(a.table, 16) &&
+                     aligned(a.qg, 16) && aligned(a.kg, 16) && heads < 65536 &&
+                     rows_aligned(has_q ? q : nullptr, bi) && rows_aligned(has_k ? k : nullptr, bi) &&
+                     rows_aligned(has_v ? v : nullptr, bi) && rows_aligned(q_out, bo) && rows_aligned(k_out, bo) &&
+                     (!kv || (aligned(kv->k, 16) && aligned(kv->v, 16)));
+    const bool i8 = kv && kv->type == TKV_HIP_I8;
+    if (type_in == TKV_HIP_F32) launch_rope_from<float>(c, a, type_out, i8, vec);
+    else if (type_in == TKV_HIP_F16) launch_rope_from<_Float16>(c, a, type_out, i8, vec);
+    else launch_rope_from<__bf16>(c, a, type_out, i8, vec);
+    TKV_LAUNCH_CHECK();
+    return TKV_HIP_OK;
 }
 
 static void kv_release(KvCache* kv) {
@@ -431,78 +621,20 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
                                 int64_t rot_dim, int32_t layout, const tkv_hip_rows* q_out,
                                 const tkv_hip_rows* k_out, int32_t type_out, int64_t cache,
                                 const int64_t* slots) {
-    const KvCache* kv = reinterpret_cast<const KvCache*>(cache);
-    if (!float_type(type_in) || !float_type(type_out))
-        return set_error(TKV_HIP_BAD_ARG, "rope_append: types are F32, F16 or BF16");
-    if (tokens < 0 || tokens >= (1ll << 31) || heads_q < 0 || heads_kv < 0 || heads_q > 65535 || heads_kv > 65535 ||
-        head_dim <= 0 || head_dim > 256)
-        return set_error(TKV_HIP_BAD_ARG, "rope_append: sizes out of range (head_dim 1 .. 256)");
-    if (table && (rot_dim < 2 || rot_dim > head_dim || rot_dim % 2 || table_len < 0 || !positions ||
-                  !aligned(table, 8) || (layout != TKV_HIP_ROPE_HALF && layout != TKV_HIP_ROPE_PAIRS)))
-        return set_error(TKV_HIP_BAD_ARG,
-                         "rope_append: a table takes positions, an even rot_dim in 2 .. head_dim and a known layout");
-    const bool has_q = q && heads_q > 0, has_k = k && heads_kv > 0, has_v = v && heads_kv > 0;
-    if ((heads_q > 0 && !has_q) || (heads_kv > 0 && !has_k) || (has_q && !q->data) ||
-        (has_k && !k->data) || (has_v && !v->data))
-        return set_error(TKV_HIP_BAD_ARG, "rope_append: NULL rows with a positive head count");
-    if ((q_out && (!has_q || !q_out->data)) || (k_out && (!has_k || !k_out->data)))
-        return set_error(TKV_HIP_BAD_ARG, "rope_append: an output without its rows");
-    if (kv) {
-        if (!has_k || !has_v || !slots)
-            return set_error(TKV_HIP_BAD_ARG, "rope_append: a cache takes k, v and slots");
-        if (kv->heads != heads_kv || kv->d != head_dim)
-            return set_error(TKV_HIP_BAD_ARG, "rope_append: the cache has other heads");
-        if (kv->type != type_out && kv->type != TKV_HIP_I8)
-            return set_error(TKV_HIP_BAD_ARG, "rope_append: the cache's type is neither type_out nor I8");
-    }
-    Ctx* c;
-    TKV_RC_TRY(ctx_get(ctx, &c));
-    if (kv && kv->device != c->device)
-        return set_error(TKV_HIP_BAD_ARG, "rope_append: the cache is on another device");
-    RopeArgs a = {};
-    // without a cache the values have nowhere to go: no rows for them
-    const int64_t heads = heads_q + heads_kv + (kv ? heads_kv : 0);
-    if (tokens == 0 || heads == 0) return TKV_HIP_OK;
-    if (tokens * heads >= (1ll << 31))
-        return set_error(TKV_HIP_UNSUPPORTED, "rope_append: tokens * heads >= 2^31");
-    if (has_q) a.q = q->data, a.q_st = q->stride_token, a.q_sh = q->stride_head;
-    if (has_k) a.k = k->data, a.k_st = k->stride_token, a.k_sh = k->stride_head;
-    if (has_v) a.v = v->data, a.v_st = v->stride_token, a.v_sh = v->stride_head;
-    if (q_out) a.qo = q_out->data, a.qo_st = q_out->stride_token, a.qo_sh = q_out->stride_head;
-    if (k_out) a.ko = k_out->data, a.ko_st = k_out->stride_token, a.ko_sh = k_out->stride_head;
-    if (kv) {
-        a.kc = kv->k;
-        a.vc = kv->v;
-        a.ks = kv->ks;
-        a.vs = kv->vs;
-        a.slots = slots;
-        a.n_slots = kv->pages * kv->page;
-        a.page = fast_div((uint32_t)kv->page);
-    } else {
-        a.page = fast_div(1);
-    }
-    a.heads = fast_div((uint32_t)heads);
-    a.positions = positions;
-    a.table = reinterpret_cast<const float2*>(table);
-    a.table_len = table_len;
-    a.tokens = tokens;
-    a.hq = (int32_t)heads_q;
-    a.hkv = (int32_t)heads_kv;
-    a.d = (int32_t)head_dim;
-    a.rot = table ? (int32_t)rot_dim : 0;
-    a.pairs = layout == TKV_HIP_ROPE_PAIRS;
-    const int64_t bi = type_bytes(type_in), bo = type_bytes(type_out);
-    const bool vec = head_dim % 8 == 0 && a.rot % (a.pairs ? 8 : 16) == 0 && aligned(table, 16) &&
-                     heads < 65536 && rows_aligned(has_q ? q : nullptr, bi) &&
-                     rows_aligned(has_k ? k : nullptr, bi) && rows_aligned(has_v ? v : nullptr, bi) &&
-                     rows_aligned(q_out, bo) && rows_aligned(k_out, bo) &&
-                     (!kv || (aligned(kv->k, 16) && aligned(kv->v, 16)));
-    const bool i8 = kv && kv->type == TKV_HIP_I8;
-    if (type_in == TKV_HIP_F32) launch_rope_from<float>(c, a, type_out, i8, vec);
-    else if (type_in == TKV_HIP_F16) launch_rope_from<_Float16>(c, a, type_out, i8, vec);
-    else launch_rope_from<__bf16>(c, a, type_out, i8, vec);
-    TKV_LAUNCH_CHECK();
-    return TKV_HIP_OK;
+    const tkv_hip_rope r = {table, table_len, rot_dim, layout, 1, positions, 0, nullptr};
+    return rope_append("rope_append", ctx, type_in, tokens, heads_q, heads_kv, head_dim, q, k, v, nullptr,
+                       table ? &r : nullptr, q_out, k_out, type_out, cache, slots);
+}
+
+int32_t tkv_hip_dev_norm_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, int64_t heads_q,
+                                     int64_t heads_kv, int64_t head_dim, const tkv_hip_rows* q,
+                                     const tkv_hip_rows* k, const tkv_hip_rows* v,
+                                     const tkv_hip_head_norm* norm, const tkv_hip_rope* rope,
+                                     const tkv_hip_rows* q_out, const tkv_hip_rows* k_out,
+                                     int32_t type_out, int64_t cache, const int64_t* slots) {
+    if (rope && !rope->table) return set_error(TKV_HIP_BAD_ARG, "norm_rope_append: a rotation without its table");
+    return rope_append("norm_rope_append", ctx, type_in, tokens, heads_q, heads_kv, head_dim, q, k, v, norm, rope,
+                       q_out, k_out, type_out, cache, slots);
 }
 
 }  // extern "C"
