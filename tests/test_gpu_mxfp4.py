@@ -54,6 +54,11 @@ def _round(x, typ):
     return _values(_bits(x, typ), typ)
 
 
+def same(got, want):
+    bad = np.argwhere(~((got == want) | ((got != got) & (want != want))))
+    assert len(bad) == 0, f"{len(bad)} of {got.size} differ, first at {bad[0]}: {got[tuple(bad[0])]}, not {want[tuple(bad[0])]}"
+
+
 def code_of(x):
     """Codes [rows, blocks, 16] and scales [rows, blocks] of x, from the definition."""
     rows, cols = x.shape
@@ -140,8 +145,8 @@ def test_codes_and_values(ctx, typ, rows, cols, pad, shift):
     want_c, want_s = code_of(x)
     got_s = scales.read(np.uint8, (rows, b), "scales")
     got_c = codes.read(np.uint8, (rows, b, 16), "codes")
-    assert np.array_equal(got_s, want_s)
-    assert np.array_equal(got_c, want_c)
+    same(got_s, want_s)
+    same(got_c, want_c)
     for out in TYPES:
         size = np.dtype(RAW[out]).itemsize
         y = _rows_buffer(ctx, np.zeros((rows, cols), np.float32), out, cols + pad, shift)
@@ -216,7 +221,8 @@ def _unpad(y, m, n, out, pad):
 SIZES = [(1, 1, 1), (1, 7, 31), (2, 3, 32), (1, 64, 96), (3, 17, 64), (16, 16, 128), (16, 130, 4100), (17, 33, 256),
          (32, 100, 1000), (33, 65, 257), (64, 64, 256), (65, 130, 511), (63, 1000, 512), (100, 5, 2048), (128, 300, 1024),
          (129, 127, 288), (256, 256, 544), (1000, 768, 768), (333, 1000, 2000), (2049, 2100, 640),
-         (4111, 4120, 1056)]
+         (4111, 4120, 1056), (4096, 4096, 1024), (3999, 4071, 1100), (3, 16390, 64), (20, 8200, 96), (9, 8211, 2080), (60, 16390, 288), (1, 16400, 544),
+         (48, 8200, 4000), (30, 16400, 320)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -233,7 +239,7 @@ def test_product_exact(ctx, m, n, k, out):
     pad = (m * n) % 3 * 8
     got = _product(ctx, a, w, m, n, k, out, bias, pad)
     want = exact if bias is None else exact + bias.astype(np.float64)
-    assert np.array_equal(got, _round(want.astype(np.float32), out))
+    same(got, _round(want.astype(np.float32), out))
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 33, 2000), (20, 64, 512), (96, 200, 1056), (260, 300, 768), (5, 7, 131071)])
@@ -279,7 +285,8 @@ def test_nan_blocks_stay_in_their_row_and_column(ctx, m):
 @pytest.mark.parametrize("typ", TYPES, ids=NAME.get)
 @pytest.mark.parametrize("m,n,k,pad,shift", [(1, 130, 800, 0, 0), (4, 64, 4096, 8, 0), (13, 768, 768, 5, 0),
                                              (32, 2304, 768, 0, 0), (33, 96, 1000, 0, 4), (200, 768, 768, 0, 0),
-                                             (1500, 1024, 320, 8, 0)])
+                                             (1500, 1024, 320, 8, 0), (2, 16400, 800, 0, 0), (16, 8210, 2100, 4, 0),
+                                             (7, 40, 4000, 0, 0), (16, 33, 8200, 0, 0)])
 def test_linear(ctx, typ, m, n, k, pad, shift):
     """The activation's codes are the definition's, so the outputs are those of
     the codes' values: exact sums where the scales are near each other."""
@@ -297,12 +304,54 @@ def test_linear(ctx, typ, m, n, k, pad, shift):
     for out in TYPES:
         y = _rows_buffer(ctx, np.zeros((m, n), np.float32), out, n + pad)
         X.Linear(ctx, lin, typ, src.ptr, k + pad, m, out, y.ptr, n + pad)()
-        assert np.array_equal(_unpad(y, m, n, out, pad), _round(exact.astype(np.float32), out))
+        same(_unpad(y, m, n, out, pad), _round(exact.astype(np.float32), out))
     if typ == A.F32 and not pad and not shift:
         y = Guarded(ctx, m * n * 4)
         for mode in (D.ACT_PER_TENSOR, D.ACT_PER_TOKEN):
             lin.forward(src.ptr, m, y.ptr, mode)
             assert np.array_equal(y.read(np.float32, (m, n), "forward"), exact.astype(np.float32))
+    lin.close()
+
+
+@pytest.mark.parametrize("typ", TYPES, ids=NAME.get)
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 70])
+def test_values_that_the_linear_multiplies(ctx, typ, m):
+    """A weight with a one in each row gives the activation's values back: those of
+    the definition, over the type's range (f32 sums have no subnormal terms)."""
+    k = 200
+    rng = np.random.default_rng(m)
+    x = _round(_special(rng, m, k), typ)
+    x = np.where(np.isfinite(x), x, 0.0).astype(np.float32)
+    w = np.eye(k, dtype=np.float32)
+    lin = D.QuantizedLinear.from_float(ctx, D.DeviceBuffer.from_host(ctx, w), k, k, None, D.WEIGHT_MXFP4)
+    src = _rows_buffer(ctx, x, typ, k)
+    y = D.DeviceBuffer.empty(ctx, (m, k), np.float32)
+    X.Linear(ctx, lin, typ, src.ptr, k, m, A.F32, y)()
+    with np.errstate(over="ignore"):
+        want = value_of(*code_of(x), k).astype(np.float32)
+    got = y.download()
+    seen = (np.abs(want) >= 2.0 ** -126) & np.isfinite(want)
+    same(got[seen], want[seen])
+    assert np.all(np.abs(got[np.abs(want) < 2.0 ** -126]) < 2.0 ** -126)
+    lin.close()
+
+
+@pytest.mark.parametrize("typ", TYPES, ids=NAME.get)
+@pytest.mark.parametrize("m", [3, 20])
+def test_activations_that_are_not_finite(ctx, typ, m):
+    rng = np.random.default_rng(m)
+    n, k = 40, 300
+    x = _round(rng.uniform(0.6, 1.9, (m, k)).astype(np.float32), typ)
+    x[0, 299], x[m - 1, 5] = np.inf, np.nan
+    w = _operand(rng, n, k, 1)
+    lin = D.QuantizedLinear.from_mxfp4(ctx, *(D.DeviceBuffer.from_host(ctx, v) for v in w), n, k)
+    src = _rows_buffer(ctx, x, typ, k)
+    y = D.DeviceBuffer.empty(ctx, (m, n), np.float32)
+    X.Linear(ctx, lin, typ, src.ptr, k, m, A.F32, y)()
+    got = y.download()
+    assert np.isnan(got[[0, m - 1]]).all()
+    exact = value_of(*code_of(x[1:m - 1]), k) @ value_of(*w, k).T
+    same(got[1:m - 1], exact.astype(np.float32))
     lin.close()
 
 

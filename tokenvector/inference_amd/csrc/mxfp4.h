@@ -77,6 +77,10 @@ int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, in
 int launch_mx_slabs(Ctx* c, const uint8_t* scales, int64_t rows, int64_t k, uint8_t* slabs);
 // mxfp4_tile.hip
 int launch_mx_product(Ctx* c, const mx::Product& p);
+// mxfp4_few.hip: m <= kFewRows; and the linear that codes m <= kFewCoded rows itself.
+constexpr int kFewRows = 64, kFewCoded = 16;
+int launch_mx_few(Ctx* c, const mx::Product& p);
+int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const mx::Product& p);
 // The linear of a resident weight on float rows (mxfp4.hip).
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, mx::Product p);
 

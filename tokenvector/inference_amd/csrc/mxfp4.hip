@@ -209,6 +209,7 @@ int launch_mx_slabs(Ctx* c, const uint8_t* scales, int64_t rows, int64_t k, uint
 }
 
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
+    if (p.m <= kFewCoded) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
     TKV_RC_TRY(ctx_workspace(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
     TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(p.m, k), &slabs));

@@ -6,18 +6,27 @@
 // instruction).
 //
 // Tiles: 4 waves, each a quarter of the workgroup's BM x BN outputs.  K goes in
-// slices of 256 elements, 128 bytes a row: copied HBM / L2 -> LDS by
-// global_load_lds into one of two stages while the other is multiplied.  Rows
-// lie in LDS in 16-byte chunks whose place is XORed with the row, so that the
-// 32 rows that a fragment's read takes spread over the banks; the copies are
-// linear in LDS, so each lane fetches the chunk that belongs there.
+// slices of 256 elements, 128 bytes a row: copied HBM / L2 -> LDS by buffer loads
+// into one of two stages while the other is multiplied.  Rows lie in LDS in
+// 16-byte chunks whose place is XORed with the row, so that the 32 rows that a
+// fragment's read takes spread over the banks; the copies are linear in LDS, so
+// each lane fetches the chunk that belongs there.
 //
 // Order within a slice, of four steps of 64 elements: the next step's fragments
-// are read while this one's are multiplied.  Before the last step's products
-// the wave waits for its part of the next slice (copied during the whole slice)
-// and for its own reads; behind the barrier the stage just read is free for the
-// copies of the slice after next, and the next slice's first fragments are
-// read while the last step is multiplied.
+// are read between this one's products.  Before the last step the wave waits for
+// its part of the next slice and for its own reads; behind the barrier the stage
+// just read is free for the slice after next: half of its copies go between the
+// last step's products, half between the next slice's first ones.  The wave is
+// alone on its SIMD (its sums take half the registers), so what does not stand
+// between two products stops them: copies and reads in one run, or a branch, past
+// which the compiler moves the products, cost 2.13 us a slice instead of 1.77.
+//
+// What bounds it: 8192 x 8192 x 8192 in bf16 263 us, 4.2 PFLOP/s.  A slice of a tile
+// alone on the card takes 1.14 us (2048 of its 2700 cycles the matrix units'), with
+// all CUs at work 1.77: power.  Of random codes the matrix units alone, all operands
+// in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros).  (The
+// 16x16x128 form reaches 6.9, its sums moved half as often, but took the same time
+// here, with twice the scales to read.)
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -42,7 +51,7 @@ __device__ __forceinline__ void tile_of(int64_t block, int tiles_m, int tiles_n,
     tn = in / high;
 }
 
-template <int TM, int TN>  // 32 x 32 blocks of a wave
+template <int TM, int TN>  // a wave's blocks of 32 tokens and of 32 weight rows
 struct Tile {
     static constexpr int BM = 64 * TM, BN = 64 * TN;
     static constexpr int CODES = (BM + BN) * 128, SCALES = (BM + BN) * 8;
@@ -51,7 +60,8 @@ struct Tile {
 };
 
 template <int TM, int TN, typename TO>
-__global__ __launch_bounds__(256, (Tile<TM, TN>::PER_CU)) void k_mx_tile(Product p, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(256, (Tile<TM, TN>::PER_CU)) void k_mx_tile(Product p, int tiles_m, int tiles_n,
+                                                                         int vec) {
     using T = Tile<TM, TN>;
     constexpr int BM = T::BM, BN = T::BN;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * T::STAGE];
@@ -70,30 +80,36 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::PER_CU)) void k_mx_tile(Product
     // row, which the scales 2^-127 there leave out.
     constexpr int COPIES = (BM + BN) / 32;
     const int rows_a = p.m - m0 < BM ? (int)(p.m - m0) : BM, rows_w = p.n - n0 < BN ? (int)(p.n - n0) : BN;
-    const auto buffer_of = [&](const uint8_t* base, int rows) {
-        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * (int)row_bytes, 0x00020000);
-    };
-    const __amdgpu_buffer_rsrc_t from_a = buffer_of(p.a + m0 * row_bytes, rows_a);
-    const __amdgpu_buffer_rsrc_t from_w = buffer_of(p.w + n0 * row_bytes, rows_w);
+    const uint32_t bytes_a = (uint32_t)rows_a * row_bytes, bytes_w = (uint32_t)rows_w * row_bytes;
+    const uint8_t *base_a = p.a + m0 * row_bytes, *base_w = p.w + n0 * row_bytes;
     // (a copy's first row is a multiple of 8: its part of chunk_xor is the wave's)
     const uint32_t lane_at =
         (uint32_t)(lane >> 3) * row_bytes + (uint32_t)(((lane & 7) ^ chunk_xor(wave * 8 + (lane >> 3))) * 16);
     constexpr int SBYTES = T::SCALES / 4;  // of a wave
     constexpr int SWIDTH = SBYTES % 1024 == 0 ? 16 : 4, SCOPIES = SBYTES / (64 * SWIDTH);
-    const auto copy = [&](int slice, uint8_t* stage) {
+    constexpr int ITEMS = COPIES + SCOPIES;
+    const int slices = (p.blocks + 7) >> 3;
+    const uint8_t* scale_at[SCOPIES];
+    int64_t scale_step[SCOPIES];
 #pragma unroll
-        for (int d = 0; d < COPIES; d++) {
-            const int first = (d * 4 + wave) * 8, in = d * 32 < BM ? first : first - BM;
-            const uint32_t at = (in < (d * 32 < BM ? rows_a : rows_w) ? (uint32_t)in * row_bytes : 0u) + (uint32_t)slice * 128u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(d * 32 < BM ? from_a : from_w, (lds_ptr)(stage + first * 128), 16,
-                                                     (int)lane_at, (int)at, 0, 0);
-        }
-#pragma unroll
-        for (int d = 0; d < SCOPIES; d++) {
-            const int at = (d * 4 + wave) * 64 * SWIDTH;
-            const uint8_t* src = at < BM * 8 ? p.as + ((int64_t)slice * p.a_rows + m0) * 8 + at
-                                             : p.ws + ((int64_t)slice * p.w_rows + n0) * 8 + (at - BM * 8);
-            const void* from = src + lane * SWIDTH;
+    for (int d = 0; d < SCOPIES; d++) {
+        const int at = (d * 4 + wave) * 64 * SWIDTH;
+        scale_at[d] = at < BM * 8 ? p.as + m0 * 8 + at : p.ws + n0 * 8 + (at - BM * 8);
+        scale_step[d] = (at < BM * 8 ? p.a_rows : p.w_rows) * 8;
+    }
+    // one of a wave's copies of a slice.  Of a slice that is not there only the
+    // scales of the last are copied: no branch keeps the products from the copies.
+    const auto copy = [&](int slice, uint8_t* stage, int d) {
+        if (d < COPIES) {
+            const bool is_a = d * 32 < BM;
+            const int first = (d * 4 + wave) * 8, in = is_a ? first : first - BM;
+            const uint32_t at = (in < (is_a ? rows_a : rows_w) ? (uint32_t)in * row_bytes : 0u) + (uint32_t)slice * 128u;
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(is_a ? base_a : base_w), 0, slice < slices ? (int)(is_a ? bytes_a : bytes_w) : 0, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(stage + first * 128), 16, (int)lane_at, (int)at, 0, 0);
+        } else {
+            const int k = d - COPIES, have = slice < slices ? slice : slices - 1, at = (k * 4 + wave) * 64 * SWIDTH;
+            const void* from = scale_at[k] + (int64_t)have * scale_step[k] + lane * SWIDTH;
             if constexpr (SWIDTH == 16)
                 __builtin_amdgcn_global_load_lds(from, (lds_ptr)(stage + T::CODES + at), 16, 0, 0);
             else
@@ -101,35 +117,30 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::PER_CU)) void k_mx_tile(Product
         }
     };
 
-    v16f acc[TM][TN];
+    v16f acc[TN][TM];
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+    for (int j = 0; j < TN; j++)
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+        for (int i = 0; i < TM; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+            for (int r = 0; r < 16; r++) acc[j][i][r] = 0.0f;
 
     v4i fa[2][TM], fw[2][TN];
     v2i sa[TM], sw[TN];                      // a slice's scales as read,
     int la[TM], ha[TM], lw[TN], hw[TN];      // and shifted
     const int ra = wm * TM * 32 + l32, rw = BM + wn * TN * 32 + l32;
     const int x = chunk_xor(l32);
-    const auto read = [&](const uint8_t* stage, int step, int set) {
-        const int c = ((2 * step + half) ^ x) * 16;
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-            fa[set][i] = *reinterpret_cast<const v4i*>(stage + (ra + i * 32) * 128 + c);
-#pragma unroll
-        for (int j = 0; j < TN; j++)
-            fw[set][j] = *reinterpret_cast<const v4i*>(stage + (rw + j * 32) * 128 + c);
+    constexpr int F = TM + TN;  // fragments of a step
+    const auto read = [&](const uint8_t* stage, int step, int k) {
+        const int c = ((2 * step + half) ^ x) * 16, set = step & 1;
+        if (k < TN) fw[set][k] = *reinterpret_cast<const v4i*>(stage + (rw + k * 32) * 128 + c);
+        else fa[set][k - TN] = *reinterpret_cast<const v4i*>(stage + (ra + (k - TN) * 32) * 128 + c);
+    };
+    const auto read_scales = [&](const uint8_t* stage, int k) {
+        if (k < TN) sw[k] = *reinterpret_cast<const v2i*>(stage + T::CODES + (rw + k * 32) * 8);
+        else sa[k - TN] = *reinterpret_cast<const v2i*>(stage + T::CODES + (ra + (k - TN) * 32) * 8);
     };
     // a lane's blocks are 2 step + half: shifted so, step's byte is 2 (step % 2)
-    const auto read_scales = [&](const uint8_t* stage) {
-#pragma unroll
-        for (int i = 0; i < TM; i++) sa[i] = *reinterpret_cast<const v2i*>(stage + T::CODES + (ra + i * 32) * 8);
-#pragma unroll
-        for (int j = 0; j < TN; j++) sw[j] = *reinterpret_cast<const v2i*>(stage + T::CODES + (rw + j * 32) * 8);
-    };
     const auto shift_scales = [&]() {
 #pragma unroll
         for (int i = 0; i < TM; i++) {
@@ -142,86 +153,124 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::PER_CU)) void k_mx_tile(Product
             hw[j] = (int)((unsigned)sw[j].y >> (8 * half));
         }
     };
-    // the products of one step, between them nothing else
-    const auto multiply = [&](auto step) {
-        constexpr int S = decltype(step)::value;
+    // the products of one step, and `n` copies and reads spread between them
+    const auto multiply = [&](auto step, auto n, auto&& other) {
+        constexpr int S = decltype(step)::value, N = decltype(n)::value, P = TM * TN;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < TM; i++)
+        for (int t = 0; t < P; t++) {
+            const int i = t / TN, j = t % TN;
+            const v4i a4 = fa[S & 1][i], w4 = fw[S & 1][j];
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                v8i{w4.x, w4.y, w4.z, w4.w, 0, 0, 0, 0}, v8i{a4.x, a4.y, a4.z, a4.w, 0, 0, 0, 0}, acc[j][i], 4, 4,
+                2 * (S & 1), S < 2 ? lw[j] : hw[j], 2 * (S & 1), S < 2 ? la[i] : ha[i]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const v4i a4 = fa[S & 1][i], w4 = fw[S & 1][j];
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                    v8i{a4.x, a4.y, a4.z, a4.w, 0, 0, 0, 0}, v8i{w4.x, w4.y, w4.z, w4.w, 0, 0, 0, 0}, acc[i][j], 4, 4,
-                    2 * (S & 1), S < 2 ? la[i] : ha[i], 2 * (S & 1), S < 2 ? lw[j] : hw[j]);
-            }
-        __builtin_amdgcn_sched_barrier(0);
+            for (int k = t * N / P; k < (t + 1) * N / P; k++) other(k);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     const auto sync = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    const int slices = (p.blocks + 7) >> 3;
-    constexpr int VM = COPIES + SCOPIES;
-    static_assert(VM < 64, "vmcnt range");
-    copy(0, lds);
-    if (slices > 1) {
-        copy(1, lds + T::STAGE);
-        __builtin_amdgcn_s_waitcnt(0x0F70 | (VM & 15) | ((VM >> 4) << 14));
-    } else {
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-    }
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    // (a third to two thirds early: the same; all of them 5% slower)
+    constexpr int EARLY = (ITEMS + 1) / 2, LATE = ITEMS - EARLY;
+    static_assert(ITEMS < 64, "vmcnt range");
+#pragma unroll
+    for (int d = 0; d < ITEMS; d++) copy(0, lds, d);
+#pragma unroll
+    for (int d = 0; d < EARLY; d++) copy(1, lds + T::STAGE, d);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (EARLY & 15) | ((EARLY >> 4) << 14));
     sync();
-    read_scales(lds);
-    read(lds, 0, 0);
-    for (int s = 0; s < slices - 1; s++) {
+#pragma unroll
+    for (int k = 0; k < F; k++) read_scales(lds, k);
+#pragma unroll
+    for (int k = 0; k < F; k++) read(lds, 0, k);
+#pragma unroll 1
+    for (int s = 0; s < slices; s++) {
         uint8_t* stage = lds + (s & 1) * T::STAGE;
-        const uint8_t* next = lds + ((s + 1) & 1) * T::STAGE;
+        uint8_t* next = lds + ((s + 1) & 1) * T::STAGE;
         shift_scales();
-        read(stage, 1, 1);
-        multiply(std::integral_constant<int, 0>{});
-        read(stage, 2, 0);
-        multiply(std::integral_constant<int, 1>{});
-        read(stage, 3, 1);
-        multiply(std::integral_constant<int, 2>{});
+        multiply(I0{}, std::integral_constant<int, F + LATE>{}, [&](int k) {
+            if (k < F) read(stage, 1, k);
+            else copy(s + 1, next, EARLY + k - F);
+        });
+        multiply(I1{}, std::integral_constant<int, F>{}, [&](int k) { read(stage, 2, k); });
+        multiply(I2{}, std::integral_constant<int, F>{}, [&](int k) { read(stage, 3, k); });
         __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's copies of slice s + 1
         sync();
-        if (s + 2 < slices) copy(s + 2, stage);
-        read_scales(next);
-        read(next, 0, 0);
-        multiply(std::integral_constant<int, 3>{});
+        multiply(I3{}, std::integral_constant<int, 2 * F + EARLY>{}, [&](int k) {
+            if (k < F) read(next, 0, k);
+            else if (k < F + EARLY) copy(s + 2, stage, k - F);
+            else read_scales(next, k - F - EARLY);
+        });
     }
-    const uint8_t* stage = lds + ((slices - 1) & 1) * T::STAGE;
-    shift_scales();
-    read(stage, 1, 1);
-    multiply(std::integral_constant<int, 0>{});
-    read(stage, 2, 0);
-    multiply(std::integral_constant<int, 1>{});
-    read(stage, 3, 1);
-    multiply(std::integral_constant<int, 2>{});
-    multiply(std::integral_constant<int, 3>{});
+    __builtin_amdgcn_s_waitcnt(0x0F70);
 
-    // a lane holds column l32 of each block, register r its row 8 (r / 4) + 4 half + r % 4
-    const int64_t mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
-    float b[TN];
+    // A lane holds token l32 of each block, registers 4 q .. 4 q + 3 its outputs
+    // 8 q + 4 half .. of 32.  They go out through LDS, 32 tokens at a time, so that a
+    // store takes whole lines, and the code is a short loop: unrolled over the
+    // registers it was longer to fetch than to run (a tile of 256 x 256 with edges
+    // 45 us, 1024 deep).
+    constexpr int ROW = TN * 32 * (int)sizeof(TO) + 16;  // bytes of a token in LDS
+    static_assert(4 * 32 * ROW <= 2 * T::STAGE, "the waves' parts");
+    sync();  // the others may still read the last slice
+    uint8_t* own = lds + wave * (32 * ROW);
+    const int64_t nw = n0 + wn * TN * 32, mw = m0 + wm * TM * 32;
+    float b[TN][16];
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-        const int64_t col = nw + j * 32 + l32;
-        b[j] = p.bias ? p.bias[col < p.n ? col : p.n - 1] : 0.0f;
-    }
-    const int64_t lane_y = 4 * half * p.ldy + l32;
-    const auto store = [&](auto whole) {
+    for (int j = 0; j < TN; j++)
 #pragma unroll
-        for (int i = 0; i < TM; i++)
+        for (int r = 0; r < 16; r++) {
+            const int64_t c = nw + j * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            b[j][r] = p.bias ? p.bias[c < p.n ? c : p.n - 1] : 0.0f;
+        }
+    constexpr int LANES = TN * 32 * (int)sizeof(TO) / 16, ROWS = 64 / LANES, E = 16 / (int)sizeof(TO);
+    const int64_t n = nw + (lane % LANES) * E;
+    const int64_t left = p.n - n;  // outputs from n on
+    const bool whole = vec && m0 + BM <= p.m && n0 + BN <= p.n;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int64_t row = mw + i * 32 + 8 * (r >> 2) + (r & 3);
-                TO* at = static_cast<TO*>(p.y) + row * p.ldy + nw;
+    for (int i = 0; i < TM; i++) {
 #pragma unroll
-                for (int j = 0; j < TN; j++)
-                    if (decltype(whole)::value || (row + 4 * half < p.m && nw + j * 32 + l32 < p.n))
-                        at[lane_y + j * 32] = from_f32<TO>(acc[i][j][r] + b[j]);
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                struct alignas(4 * sizeof(TO)) { TO e[4]; } v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v.e[e] = from_f32<TO>(acc[j][i][4 * q + e] + b[j][4 * q + e]);
+                __builtin_memcpy(own + l32 * ROW + (j * 32 + 8 * q + 4 * half) * sizeof(TO), &v, sizeof(v));
             }
-    };
-    if (m0 + BM <= p.m && n0 + BN <= p.n) store(std::true_type{});
-    else store(std::false_type{});
+        __builtin_amdgcn_wave_barrier();
+        if (whole) {
+            v4i v[32 / ROWS];
+#pragma unroll
+            for (int t = 0; t < 32 / ROWS; t++)
+                v[t] = *reinterpret_cast<const v4i*>(own + (t * ROWS + lane / LANES) * ROW + (lane % LANES) * 16);
+            TO* at = static_cast<TO*>(p.y) + (mw + i * 32 + lane / LANES) * p.ldy + n;
+#pragma unroll
+            for (int t = 0; t < 32 / ROWS; t++) *reinterpret_cast<v4i*>(at + t * ROWS * p.ldy) = v[t];
+        } else {
+#pragma unroll 1
+            for (int t = lane / LANES; t < 32; t += ROWS) {
+                const int64_t m = mw + i * 32 + t;
+                const v4i v = *reinterpret_cast<const v4i*>(own + t * ROW + (lane % LANES) * 16);
+                TO* at = static_cast<TO*>(p.y) + m * p.ldy + n;
+                if (m >= p.m || left <= 0) continue;
+                if (vec && left >= E) {
+                    *reinterpret_cast<v4i*>(at) = v;
+                } else {
+                    TO e[E];
+                    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+                    for (int k = 0; k < E; k++)
+                        if (k < left) at[k] = e[k];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <int TM, int TN>
@@ -229,19 +278,44 @@ static int launch_tile(Ctx* c, const Product& p) {
     const int64_t tm = ceil_div(p.m, 64 * TM), tn = ceil_div(p.n, 64 * TN);
     if (tm * tn >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "matmul_mxfp4: 2^31 tiles and more");
     const dim3 grid = wide_grid(tm * tn);
-    if (p.y_type == TKV_HIP_F32) k_mx_tile<TM, TN, float><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn);
-    else if (p.y_type == TKV_HIP_F16) k_mx_tile<TM, TN, _Float16><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn);
-    else k_mx_tile<TM, TN, __bf16><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn);
+    const int vec = aligned(p.y, 16) && p.ldy * type_bytes(p.y_type) % 16 == 0;
+    if (p.y_type == TKV_HIP_F32) k_mx_tile<TM, TN, float><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn, vec);
+    else if (p.y_type == TKV_HIP_F16) k_mx_tile<TM, TN, _Float16><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn, vec);
+    else k_mx_tile<TM, TN, __bf16><<<grid, 256, 0, c->stream>>>(p, (int)tm, (int)tn, vec);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
 
 }  // namespace mx
 
+// The tile that the times measured for each say is fastest, in us: a slice with the
+// CUs' last workgroup but one, two, ... (of those that a CU holds) there, and what a
+// workgroup takes besides.  256 x 256 to 64 x 64, f32 sums of 768: 8192 x 2304 31,
+// 25, 26 us; of 4096: 512 x 4096 26, 15, 12; 1024 x 14336 37, 41, 58; 4096 x 4096
+// 39, 45, 63.
 int launch_mx_product(Ctx* c, const mx::Product& p) {
-    const auto tiles = [&](int64_t bm, int64_t bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn); };
-    if (tiles(256, 256) >= c->num_cus) return mx::launch_tile<4, 4>(c, p);
-    if (tiles(128, 128) >= c->num_cus) return mx::launch_tile<2, 2>(c, p);
+    if (p.m <= kFewRows) return launch_mx_few(c, p);
+    struct Kind {
+        int64_t side;
+        int held;         // workgroups of a CU
+        float slice[4];   // us a slice with so many of them at work
+        float rest;
+    };
+    static constexpr Kind kinds[3] = {{256, 1, {1.7f}, 8.0f}, {128, 2, {0.68f, 1.2f}, 3.0f},
+                                      {64, 4, {0.49f, 0.58f, 0.75f, 0.93f}, 1.5f}};
+    const float slices = (float)((p.blocks + 7) >> 3);
+    int best = 0;
+    float least = 0.0f;
+    for (int i = 0; i < 3; i++) {
+        const Kind& k = kinds[i];
+        const int64_t tiles = ceil_div(p.m, k.side) * ceil_div(p.n, k.side), round = (int64_t)k.held * c->num_cus;
+        const int64_t full = tiles / round, left = ceil_div(tiles % round, c->num_cus);
+        float t = (float)full * (slices * k.slice[k.held - 1] + k.rest);
+        if (left) t += slices * k.slice[left - 1] + k.rest;
+        if (i == 0 || t < least) best = i, least = t;
+    }
+    if (best == 0) return mx::launch_tile<4, 4>(c, p);
+    if (best == 1) return mx::launch_tile<2, 2>(c, p);
     return mx::launch_tile<1, 1>(c, p);
 }
 
