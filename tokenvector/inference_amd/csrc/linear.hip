@@ -297,7 +297,7 @@ static int weight_create_mx(Ctx* c, const float* w, const uint8_t* codes, const 
             e = hipMemcpyAsync(wt->mscales, scales, (size_t)(n * blocks), hipMemcpyDeviceToDevice, c->stream);
         if (e != hipSuccess) rc = fail_hip(e, "MXFP4 weight copy", __FILE__, __LINE__);
     }
-    if (rc == TKV_HIP_OK) rc = launch_mx_slabs(c, wt->mscales, n, k, wt->slabs);
+    if (rc == TKV_HIP_OK) rc = launch_mx_slabs(c, k, wt->mscales, n, wt->slabs);
     if (rc == TKV_HIP_OK) {
         hipError_t e = hipStreamSynchronize(c->stream);
         if (e != hipSuccess) rc = fail_hip(e, "hipStreamSynchronize", __FILE__, __LINE__);

@@ -33,10 +33,10 @@ inline size_t slab_bytes(int64_t rows, int64_t k) { return (size_t)(slabs_of(k) 
 
 // A product's operands and output.  y rows ldy elements apart, of y_type.
 struct Product {
-    const uint8_t *a, *as;  // codes [m][blocks][16], slabs
-    const uint8_t *w, *ws;  // codes [n][blocks][16], slabs
+    const uint8_t *a, *as;  // codes [m][blocks][16], scales
+    const uint8_t *w, *ws;  // codes [n][blocks][16], scales
     int64_t m, n;
-    int64_t a_rows, w_rows;  // of the slabs
+    int64_t a_rows, w_rows;  // of the scales' slabs; 0: they are [rows][blocks]
     int32_t blocks;
     const float* bias;
     void* y;
@@ -66,6 +66,23 @@ __device__ __forceinline__ unsigned code8(const float (&x)[8], float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
 }
 
+// The scales of a row's blocks 8 s .. 8 s + 7 from its [blocks] bytes, those past its
+// last 0.  Nothing behind the row is read, and there is no branch on s, so that the
+// loads of several s are in flight together.
+__device__ __forceinline__ v2i row_scales(const uint8_t* row, int s, int blocks) {
+    uint64_t v = 0;
+    if (blocks >= 8) {
+        const int at = 8 * s < blocks - 8 ? 8 * s : blocks - 8, past = 8 * s - at;
+        __builtin_memcpy(&v, row + at, 8);
+        v = past < 8 ? v >> (8 * past) : 0;
+    } else if (s == 0) {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            if (i < blocks) v |= (uint64_t)row[i] << (8 * i);
+    }
+    return v2i{(int)(uint32_t)v, (int)(uint32_t)(v >> 32)};
+}
+
 }  // namespace mx
 
 // mxfp4.hip.  x: rows of `cols` elements of `type`, `stride` elements apart.
@@ -74,8 +91,11 @@ int launch_mx_quantize(Ctx* c, int type, const void* x, int64_t stride, int64_t 
                        uint8_t* codes, uint8_t* scales, bool slabs);
 int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, int64_t rows,
                          int64_t cols, int type, void* y, int64_t stride);
-int launch_mx_slabs(Ctx* c, const uint8_t* scales, int64_t rows, int64_t k, uint8_t* slabs);
-// mxfp4_tile.hip
+// Two operands' scales to slabs (rows_b 0: one's).
+int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* a, int64_t rows_a, uint8_t* slabs_a, const uint8_t* b = nullptr,
+                    int64_t rows_b = 0, uint8_t* slabs_b = nullptr);
+// mxfp4_tile.hip.  Scales as slabs, or as rows where mx_takes_rows(p).
+bool mx_takes_rows(const Ctx* c, const mx::Product& p);
 int launch_mx_product(Ctx* c, const mx::Product& p);
 // mxfp4_few.hip: m <= kFewRows; and the linear that codes m <= kFewCoded rows itself.
 constexpr int kFewRows = 64, kFewCoded = 16;

@@ -109,19 +109,23 @@ __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
     }
 }
 
-// Row-major scales to slabs, eight blocks of a row per lane.
-__global__ __launch_bounds__(256) void k_mx_slabs(const uint8_t* __restrict__ scales, int64_t rows, int32_t blocks,
-                                                  int64_t slab_rows, uint8_t* __restrict__ out) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// Row-major scales of one or two operands to slabs, eight blocks of a row per lane.
+struct SlabArgs {
+    const uint8_t* scales[2];
+    uint8_t* out[2];
+    int64_t rows[2];
+    int32_t blocks;
+    unsigned first;  // workgroups of the first operand
+};
+__global__ __launch_bounds__(256) void k_mx_slabs(SlabArgs a) {
+    const int which = blockIdx.x >= a.first;
+    const int64_t row = (int64_t)(blockIdx.x - (which ? a.first : 0)) * 256 + threadIdx.x;
+    const int64_t rows = which ? a.rows[1] : a.rows[0], padded = (rows + kSlabRows - 1) / kSlabRows * kSlabRows;
     if (row >= rows) return;
-    for (int64_t g = blockIdx.y; g * 8 < blocks; g += gridDim.y) {
-        uint8_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = g * 8 + i < blocks ? scales[row * blocks + g * 8 + i] : (uint8_t)0;
-        uint2 w;
-        __builtin_memcpy(&w, v, 8);
-        *reinterpret_cast<uint2*>(out + (g * slab_rows + row) * 8) = w;
-    }
+    const uint8_t* from = (which ? a.scales[1] : a.scales[0]) + row * a.blocks;
+    uint8_t* out = which ? a.out[1] : a.out[0];
+    for (int g = blockIdx.y; g * 8 < a.blocks; g += gridDim.y)
+        *reinterpret_cast<v2i*>(out + (g * padded + row) * 8) = row_scales(from, g, a.blocks);
 }
 
 // Blocks of one launch, at most: their number is divided in 32 bits, and 4 lanes
@@ -200,10 +204,12 @@ int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, in
     return decode_rows<__bf16>(c, codes, scales, rows, cols, y, stride);
 }
 
-int launch_mx_slabs(Ctx* c, const uint8_t* scales, int64_t rows, int64_t k, uint8_t* slabs) {
-    const int64_t groups = slabs_of(k);
-    k_mx_slabs<<<dim3((unsigned)ceil_div(rows, 256), (unsigned)(groups < 65535 ? groups : 65535)), 256, 0, c->stream>>>(
-        scales, rows, (int32_t)blocks_of(k), slab_rows(rows), slabs);
+int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_t* slabs_a, const uint8_t* sb,
+                    int64_t rows_b, uint8_t* slabs_b) {
+    const int64_t groups = slabs_of(k), first = ceil_div(rows_a, 256);
+    const SlabArgs a = {{sa, sb}, {slabs_a, slabs_b}, {rows_a, rows_b}, (int32_t)blocks_of(k), (unsigned)first};
+    k_mx_slabs<<<dim3((unsigned)(first + ceil_div(rows_b, 256)), (unsigned)(groups < 65535 ? groups : 65535)), 256, 0,
+                 c->stream>>>(a);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
@@ -273,25 +279,28 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
         return set_error(TKV_HIP_BAD_ARG, "matmul_mxfp4: NULL or unaligned buffers (codes: 16 bytes)");
     Ctx* c;
     TKV_RC_TRY(ctx_get(ctx, &c));
-    void *as, *ws;
-    TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(m, k), &as));
-    TKV_RC_TRY(ctx_workspace(c, 2, slab_bytes(n, k), &ws));
-    TKV_RC_TRY(launch_mx_slabs(c, a_scales, m, k, static_cast<uint8_t*>(as)));
-    TKV_RC_TRY(launch_mx_slabs(c, w_scales, n, k, static_cast<uint8_t*>(ws)));
     mx::Product p = {};
     p.a = a;
-    p.as = static_cast<uint8_t*>(as);
+    p.as = a_scales;
     p.w = w;
-    p.ws = static_cast<uint8_t*>(ws);
+    p.ws = w_scales;
     p.m = m;
     p.n = n;
-    p.a_rows = slab_rows(m);
-    p.w_rows = slab_rows(n);
     p.blocks = (int32_t)blocks_of(k);
     p.bias = bias;
     p.y = y;
     p.ldy = m > 1 ? stride : n;
     p.y_type = type_out;
+    if (!mx_takes_rows(c, p)) {
+        void *as, *ws;
+        TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(m, k), &as));
+        TKV_RC_TRY(ctx_workspace(c, 2, slab_bytes(n, k), &ws));
+        TKV_RC_TRY(launch_mx_slabs(c, k, a_scales, m, static_cast<uint8_t*>(as), w_scales, n, static_cast<uint8_t*>(ws)));
+        p.as = static_cast<uint8_t*>(as);
+        p.ws = static_cast<uint8_t*>(ws);
+        p.a_rows = slab_rows(m);
+        p.w_rows = slab_rows(n);
+    }
     return launch_mx_product(c, p);
 }
 

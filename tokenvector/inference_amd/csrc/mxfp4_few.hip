@@ -109,11 +109,12 @@ __device__ __forceinline__ v4i code_block(const Block<T>& b, unsigned& byte) {
     return c;
 }
 
-struct Coded {};  // the tokens come as codes and slabs
+struct Coded {};      // the tokens come as codes and slabs,
+struct CodedRows {};  // or the scales of both as [rows][blocks]
 
 template <typename TI, int NR, int MT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
-    constexpr bool CODED = std::is_same<TI, Coded>::value;
+    constexpr bool ROWS = std::is_same<TI, CodedRows>::value, CODED = ROWS || std::is_same<TI, Coded>::value;
     typedef typename std::conditional<CODED, float, TI>::type TX;
     const Product& p = a.p;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -152,7 +153,12 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         for (int r = 0; r < NR; r++) {
 #pragma unroll
             for (int h = 0; h < 2; h++) b.w[r][h] = *reinterpret_cast<const v4i*>(w_row[r] + at[h]);
-            b.ws[r] = *reinterpret_cast<const v2i*>(p.ws + ((int64_t)s * p.w_rows + n0 + r * 16 + l16) * 8);
+            if constexpr (ROWS) {
+                const int64_t row = n0 + r * 16 + l16;
+                b.ws[r] = row_scales(p.ws + (row < p.n ? row : p.n - 1) * p.blocks, s, p.blocks);
+            } else {
+                b.ws[r] = *reinterpret_cast<const v2i*>(p.ws + ((int64_t)s * p.w_rows + n0 + r * 16 + l16) * 8);
+            }
         }
 #pragma unroll
         for (int t = 0; t < MT; t++) {
@@ -160,7 +166,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
 #pragma unroll
                 for (int h = 0; h < 2; h++)
                     b.t[t][h] = *reinterpret_cast<const v4i*>(p.a + token[t] * row_bytes + at[h]);
-                b.ts[t] = *reinterpret_cast<const v2i*>(p.as + ((int64_t)s * p.a_rows + t * 16 + l16) * 8);
+                if constexpr (ROWS) b.ts[t] = row_scales(p.as + token[t] * p.blocks, s, p.blocks);
+                else b.ts[t] = *reinterpret_cast<const v2i*>(p.as + ((int64_t)s * p.a_rows + t * 16 + l16) * 8);
             } else {
                 // (one lane of a token that is not there does what the last token's does)
                 const TX* row = static_cast<const TX*>(a.x) + token[t] * a.stride;
@@ -256,6 +263,11 @@ using namespace mx;
 int launch_mx_few(Ctx* c, const Product& p) {
     FewArgs a = {};
     a.p = p;
+    if (p.a_rows == 0) {
+        if (p.m <= 16) return launch_few<CodedRows, 1>(c, a);
+        if (p.m <= 32) return launch_few<CodedRows, 2>(c, a);
+        return launch_few<CodedRows, 4>(c, a);
+    }
     if (p.m <= 16) return launch_few<Coded, 1>(c, a);
     if (p.m <= 32) return launch_few<Coded, 2>(c, a);
     return launch_few<Coded, 4>(c, a);
