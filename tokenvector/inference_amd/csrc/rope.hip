@@ -46,7 +46,7 @@ struct RopeArgs {
     int32_t lanes_log2;  // lanes of a head row
     // the kernels with NORM or AXES (below) alone
     int32_t normed;
-    float eps;
+    float eps, inv_d;
     const float *qg, *kg;     // gains, or null
     int32_t axes;
     int64_t axis_stride;      // of the positions
@@ -90,13 +90,29 @@ __device__ __forceinline__ float row_max(unsigned m, int lanes) {
     for (int o = 1 << lanes >> 1; o; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
     return __uint_as_float(m);
 }
-// 1 / sqrt(mean of the squares + eps), from their sum over a row's lanes
+// 1 / sqrt(mean of the squares + eps), from their sum over a row's lanes.  Lanes are
+// exchanged within rows of 16 without LDS: neighbours, pairs, then halves of 8 and
+// of 16 mirrored, whose lanes hold the same sums by then.  (A row of 32 lanes, which
+// only the kernel for any size has, takes one exchange more.)
+template <int CTRL>
+__device__ __forceinline__ float swapped(float x) {
+    return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float row_sum(float s, int lanes) {
-    for (int o = 1 << lanes >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+    if (lanes > 0) s += swapped<0xb1>(s);   // quad_perm 1 0 3 2
+    if (lanes > 1) s += swapped<0x4e>(s);   // quad_perm 2 3 0 1
+    if (lanes > 2) s += swapped<0x141>(s);  // row_half_mirror
+    if (lanes > 3) s += swapped<0x140>(s);  // row_mirror
+    if (lanes > 4) s += __shfl_xor(s, 16);
     return s;
 }
-__device__ __forceinline__ float inv_norm(float sum, int d, float eps) {
-    return 1.0f / __builtin_sqrtf(sum / (float)d + eps);
+// v_rsq_f32, an ulp off at most, which takes no subnormals: those are scaled.
+__device__ __forceinline__ float inv_norm(float sum, float inv_d, float eps) {
+    float v = sum * inv_d + eps;
+    const bool tiny = v < 0x1p-100f;
+    v = tiny ? v * 0x1p64f : v;
+    const float r = __builtin_amdgcn_rsqf(v);
+    return tiny ? r * 0x1p32f : r;
 }
 // By the rounded reciprocal, as elementwise tensor libraries divide by a constant:
 // within an ulp of max / 127, and the same codes as their operations give.
@@ -114,11 +130,7 @@ __device__ __forceinline__ int8_t code_of(float x, float inv) {
 // workgroup's.  HBM bound: 8192 tokens of 32 + 8 heads of 128, bf16, 45.7 us, 4.5
 // TB/s, where a large copy reaches 5.1; 32 tokens of 12 + 12 heads of 64 take 3.4 us,
 // one launch.
-//
-// MORE: with norms per head, positions on several axes, or both.  The squares' sum
-// of a head goes over its lanes; the gains are loaded once for heads of one role in
-// turn; a pair's entry is in the row of its own axis' position.
-template <typename TI, typename TO, typename C, int HEADS, bool MORE>
+template <typename TI, typename TO, typename C, int HEADS>
 __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const int64_t t64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
     if (t64 >= a.tokens) return;  // whole groups: the rows' lanes stay together
@@ -130,16 +142,7 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const int c1 = i < turns ? i + turns : c0 < chunks ? c0 + (rest + 1) / 2 : chunks;
     const bool in0 = c0 < chunks, in1 = c1 < chunks;
     const int pos = a.table ? a.positions[tok] : 0;
-    bool pad = a.table && (pos < 0 || pos >= a.table_len);
-    int at_axis[kMaxAxes] = {pos, pos, pos, pos};
-    if (MORE && a.table) {
-#pragma unroll
-        for (int x = 1; x < kMaxAxes; x++)
-            if (x < a.axes) {
-                at_axis[x] = a.positions[x * a.axis_stride + tok];
-                pad = pad || at_axis[x] < 0 || at_axis[x] >= a.table_len;
-            }
-    }
+    const bool pad = a.table && (pos < 0 || pos >= a.table_len);
     int64_t slot = -1;
     if (a.kc && !pad) slot = a.slots[tok];
     const bool put = slot >= 0 && slot < a.n_slots;
@@ -148,16 +151,6 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     const bool turn0 = a.pairs ? c0 < a.rot >> 3 : i < turns, turn1 = a.pairs ? c1 < a.rot >> 3 : i < turns;
     float2 w[8];
     const auto entries = [&](int at, float2* to) {
-        if (MORE && a.axes > 1) {
-            const uint32_t which = a.pair_axis[at >> 4] >> (2 * (at & 15));
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int x = (which >> (2 * k)) & 3;
-                const int p = x == 0 ? at_axis[0] : x == 1 ? at_axis[1] : x == 2 ? at_axis[2] : at_axis[3];
-                to[k] = a.table[(int64_t)p * (a.rot >> 1) + at + k];
-            }
-            return;
-        }
         const float4* cs = reinterpret_cast<const float4*>(a.table + (int64_t)pos * (a.rot >> 1) + at);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
@@ -183,32 +176,12 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
         if (in0 && !pad) load8(src + 8 * c0, x0[u]);
         if (in1 && !pad) load8(src + 8 * c1, x1[u]);
     }
-    float g0[8], g1[8];
-    const float* have = nullptr;
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
         const int row = first + u;
         if (row >= (int)a.heads.d) break;
         const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
         const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
-        if (MORE && a.normed && !isv) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; k++) sum += x0[u][k] * x0[u][k] + x1[u][k] * x1[u][k];
-            const float r = inv_norm(row_sum(sum, a.lanes_log2), a.d, a.eps);
-            const float* gain = isq ? a.qg : a.kg;
-            if (gain && gain != have) {
-                if (in0) load8(gain + 8 * c0, g0);
-                if (in1) load8(gain + 8 * c1, g1);
-                have = gain;
-            }
-            // (a padding token's zeros stay zeros whatever the gains)
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                if (in0 && !pad) x0[u][k] = x0[u][k] * r * (gain ? g0[k] : 1.0f);
-                if (in1 && !pad) x1[u][k] = x1[u][k] * r * (gain ? g1[k] : 1.0f);
-            }
-        }
         if (!isv && !pad) {
             // each product and sum is rounded by itself (no contraction in this
             // library): the same bits as separate elementwise operations
@@ -265,6 +238,214 @@ __global__ __launch_bounds__(256) void k_rope_rows(RopeArgs a) {
     }
 }
 
+// A chunk as it is in memory.
+template <typename T>
+struct alignas(16) Raw8 {
+    unsigned v[2 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ void from_raw(const Raw8<T>& r, float (&x)[8]) {
+    unsigned v[2 * sizeof(T)];
+#pragma unroll
+    for (int k = 0; k < (int)(2 * sizeof(T)); k++) {
+        v[k] = r.v[k];
+        asm volatile("" : "+v"(v[k]));
+    }
+    Vec8<T> e;
+    __builtin_memcpy(&e, v, sizeof(e));
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = to_f32(e.e[k]);
+}
+__device__ __forceinline__ void norm_turn(float& p, float& q, float2 w, float r, bool turn) {
+    const float c = turn ? w.x * r : r, s = turn ? w.y * r : 0.0f, a = p, b = q;
+    p = __builtin_fmaf(a, c, -(b * s));
+    q = __builtin_fmaf(b, c, a * s);
+}
+
+// The same with norms per head, positions on several axes, or both: a lane's two
+// chunks of `HEADS` heads in flight as they are in memory, and converted one head at
+// a time.  A pair's entry is in the table's row of its own axis' position.
+//   Normed rows: the squares' sum goes over the row's lanes; with r the inverse norm
+// and g the gains, y_a = (a g_a)(r c) - (b g_b)(r s), the second product added by an
+// fma.  Others are rotated as above, each product and sum rounded by itself.
+//   HBM bound, and by what it computes beside: 8192 tokens of 32 + 8 heads of 128 in
+// bf16 take @@PROMPT@@ us (45.9 without norms, by the kernel above); with three axes,
+// whose entries are 8 bytes from rows of their own, @@AXES@@.
+template <typename TI, typename TO, typename C, int HEADS>
+__global__ __launch_bounds__(256) void k_norm_rope_rows(RopeArgs a) {
+    const int64_t t64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
+    if (t64 >= a.tokens) return;  // whole groups: the rows' lanes stay together
+    const int tok = (int)t64, i = (int)threadIdx.x & ((1 << a.lanes_log2) - 1);
+    const int chunks = a.d >> 3;
+    const int turns = a.pairs ? 0 : a.rot >> 4;  // chunk pairs rotated with each other
+    const int rest = chunks - 2 * turns, j = i - turns;
+    const int c0 = i < turns ? i : j < (rest + 1) / 2 ? 2 * turns + j : chunks;
+    const int c1 = i < turns ? i + turns : c0 < chunks ? c0 + (rest + 1) / 2 : chunks;
+    const bool in0 = c0 < chunks, in1 = c1 < chunks;
+    const int first = blockIdx.y * HEADS;
+
+    // positions; the rows themselves do not wait for them
+    int at_axis[kMaxAxes] = {0, 0, 0, 0};
+    bool pad = false;
+    if (a.table) {
+#pragma unroll
+        for (int x = 0; x < kMaxAxes; x++)
+            if (x < a.axes) at_axis[x] = a.positions[x * a.axis_stride + tok];
+    }
+    int64_t slot = a.kc ? a.slots[tok] : -1;
+    Raw8<TI> raw[HEADS][2];
+#pragma unroll
+    for (int u = 0; u < HEADS; u++) {
+        const int row = min(first + u, (int)a.heads.d - 1);
+        const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
+        const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
+        const TI* src = static_cast<const TI*>(isq ? a.q : isv ? a.v : a.k) +
+                        (int64_t)h * (isq ? a.q_sh : isv ? a.v_sh : a.k_sh) +
+                        (int64_t)tok * (isq ? a.q_st : isv ? a.v_st : a.k_st);
+        raw[u][0] = raw[u][1] = Raw8<TI>{};
+        if (in0) raw[u][0] = *reinterpret_cast<const Raw8<TI>*>(src + 8 * c0);
+        if (in1) raw[u][1] = *reinterpret_cast<const Raw8<TI>*>(src + 8 * c1);
+    }
+    float g0[8], g1[8];
+    const float* have = first < a.hq ? a.qg : a.kg;
+    const auto load_gains = [&]() {
+#pragma unroll
+        for (int k = 0; k < 8; k++) g0[k] = g1[k] = 1.0f;
+        if (have && in0) load8(have + 8 * c0, g0);
+        if (have && in1) load8(have + 8 * c1, g1);
+    };
+    load_gains();
+    if (a.table) {
+#pragma unroll
+        for (int x = 0; x < kMaxAxes; x++)
+            if (x < a.axes) pad = pad || at_axis[x] < 0 || at_axis[x] >= a.table_len;
+    }
+    if (pad) slot = -1;
+    const bool put = slot >= 0 && slot < a.n_slots;
+    const uint32_t s32 = put ? (uint32_t)slot : 0, pg = div_by(a.page, s32);
+    // (cos, sin): of the 8 pairs of a chunk pair, or the 4 of either chunk
+    const bool turn0 = a.pairs ? c0 < a.rot >> 3 : i < turns, turn1 = a.pairs ? c1 < a.rot >> 3 : i < turns;
+    float2 w[8];
+    const auto entries = [&](int at, float2* to) {
+        const int half = a.rot >> 1;
+        if (a.axes > 1) {
+            const uint32_t which = a.pair_axis[at >> 4] >> (2 * (at & 15));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int x = (which >> (2 * k)) & 3;
+                const int p = x == 0 ? at_axis[0] : x == 1 ? at_axis[1] : x == 2 ? at_axis[2] : at_axis[3];
+                to[k] = a.table[(int64_t)p * half + at + k];
+            }
+        } else {
+            const float4* cs = reinterpret_cast<const float4*>(a.table + (int64_t)at_axis[0] * half + at);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float4 v = cs[k];
+                to[2 * k] = make_float2(v.x, v.y);
+                to[2 * k + 1] = make_float2(v.z, v.w);
+            }
+        }
+    };
+    if (turn0 && !pad) entries(a.pairs ? 4 * c0 : 8 * i, w);
+    if (turn1 && !pad) entries(a.pairs ? 4 * c1 : 8 * i + 4, w + 4);
+
+#pragma unroll
+    for (int u = 0; u < HEADS; u++) {
+        const int row = first + u;
+        if (row >= (int)a.heads.d) break;
+        const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
+        const int h = row - (isq ? 0 : isv ? a.hq + a.hkv : a.hq);
+        // (a head's conversions stay behind the heads before it: done at once they
+        // hold twice the registers)
+        float x0[8], x1[8];
+        from_raw(raw[u][0], x0);
+        from_raw(raw[u][1], x1);
+        if (pad) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x0[k] = x1[k] = 0.0f;
+        }
+        if (!isv && a.normed) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum = __builtin_fmaf(x1[k], x1[k], __builtin_fmaf(x0[k], x0[k], sum));
+            const float r = inv_norm(row_sum(sum, a.lanes_log2), a.inv_d, a.eps);
+            const float* gain = isq ? a.qg : a.kg;
+            if (u > 0 && gain != have) {
+                have = gain;
+                load_gains();
+            }
+            if (gain) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x0[k] *= g0[k], x1[k] *= g1[k];
+            }
+            if (a.pairs) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    norm_turn(x0[2 * k], x0[2 * k + 1], w[k], r, turn0);
+                    norm_turn(x1[2 * k], x1[2 * k + 1], w[4 + k], r, turn1);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) norm_turn(x0[k], x1[k], w[k], r, turn0);
+            }
+            if (pad) {  // zeros whatever the gains
+#pragma unroll
+                for (int k = 0; k < 8; k++) x0[k] = x1[k] = 0.0f;
+            }
+        } else if (!isv && !pad) {
+            if (a.pairs) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (!(k < 4 ? turn0 : turn1)) continue;
+                    float* x = k < 4 ? x0 : x1;
+                    const int e = 2 * (k & 3);
+                    const float p = x[e], q = x[e + 1];
+                    x[e] = p * w[k].x - q * w[k].y;
+                    x[e + 1] = q * w[k].x + p * w[k].y;
+                }
+            } else if (turn0) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float p = x0[k], q = x1[k];
+                    x0[k] = p * w[k].x - q * w[k].y;
+                    x1[k] = q * w[k].x + p * w[k].y;
+                }
+            }
+        }
+        if (!isv && (isq ? a.qo : a.ko)) {
+            TO* dst = static_cast<TO*>(isq ? a.qo : a.ko) + (int64_t)tok * (isq ? a.qo_st : a.ko_st) +
+                      (int64_t)h * (isq ? a.qo_sh : a.ko_sh);
+            if (in0) store8(dst + 8 * c0, x0);
+            if (in1) store8(dst + 8 * c1, x1);
+        }
+        if (isq || !a.kc) continue;
+        const int64_t at = ((int64_t)pg * a.hkv + h) * a.page.d + (s32 - pg * a.page.d);
+        if constexpr (sizeof(C) == 1) {
+            unsigned most = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) most = max(most, max(abs_bits(x0[k]), abs_bits(x1[k])));
+            const float m = row_max(most, a.lanes_log2);
+            if (!put) continue;
+            const float scale = scale_of(m), inv = 1.0f / scale;
+            if (i == 0) (isv ? a.vs : a.ks)[at] = scale;
+            int8_t* dst = static_cast<int8_t*>(isv ? a.vc : a.kc) + at * a.d;
+            int8_t z[8];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) z[k] = code_of(half ? x1[k] : x0[k], inv);
+                uint2 v;
+                __builtin_memcpy(&v, z, 8);
+                if (half ? in1 : in0) *reinterpret_cast<uint2*>(dst + 8 * (half ? c1 : c0)) = v;
+            }
+        } else if (put) {
+            C* dst = static_cast<C*>(isv ? a.vc : a.kc) + at * a.d;
+            if (in0) store8(dst + 8 * c0, x0);
+            if (in1) store8(dst + 8 * c1, x1);
+        }
+    }
+}
+
 // Any head size, rotation and alignment: one head row per 2^lanes lanes, 8
 // elements a lane, one by one; the element that one is rotated with is loaded
 // again, so that it is bound by its load instructions.
@@ -302,7 +483,7 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeArgs a) {
             const float e = e0 + i < a.d && !pad ? to_f32(src[e0 + i]) : 0.0f;
             sum += e * e;
         }
-        inv = inv_norm(row_sum(sum, a.lanes_log2), a.d, a.eps);
+        inv = inv_norm(row_sum(sum, a.lanes_log2), a.inv_d, a.eps);
     }
     const auto element = [&](int e) {
         const float v = to_f32(src[e]);
@@ -373,11 +554,15 @@ static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
     a.lanes_log2 = rows_log2;
     const int64_t blocks = ceil_div(a.tokens << a.lanes_log2, 256);
     // four heads per lane where that still leaves eight workgroups per CU
-    if (blocks * ceil_div(heads, 4) >= 8 * c->num_cus)
-        k_rope_rows<TI, TO, C, 4, MORE>
-            <<<dim3((unsigned)blocks, (unsigned)ceil_div(heads, 4)), 256, 0, c->stream>>>(a);
-    else
-        k_rope_rows<TI, TO, C, 1, MORE><<<dim3((unsigned)blocks, (unsigned)heads), 256, 0, c->stream>>>(a);
+    const bool four = blocks * ceil_div(heads, 4) >= 8 * c->num_cus;
+    const dim3 grid((unsigned)blocks, (unsigned)(four ? ceil_div(heads, 4) : heads));
+    if constexpr (MORE) {
+        if (four) k_norm_rope_rows<TI, TO, C, 4><<<grid, 256, 0, c->stream>>>(a);
+        else k_norm_rope_rows<TI, TO, C, 1><<<grid, 256, 0, c->stream>>>(a);
+    } else {
+        if (four) k_rope_rows<TI, TO, C, 4><<<grid, 256, 0, c->stream>>>(a);
+        else k_rope_rows<TI, TO, C, 1><<<grid, 256, 0, c->stream>>>(a);
+    }
 }
 
 template <typename TI, typename TO>
@@ -483,6 +668,7 @@ static int rope_append(const char* who, int64_t ctx, int32_t type_in, int64_t to
     if (norm) {
         a.normed = 1;
         a.eps = norm->eps;
+        a.inv_d = 1.0f / (float)head_dim;
         a.qg = norm->q_gain;
         a.kg = norm->k_gain;
     }
