@@ -269,8 +269,8 @@ __device__ __forceinline__ void norm_turn(float& p, float& q, float2 w, float r,
 // and g the gains, y_a = (a g_a)(r c) - (b g_b)(r s), the second product added by an
 // fma.  Others are rotated as above, each product and sum rounded by itself.
 //   HBM bound, and by what it computes beside: 8192 tokens of 32 + 8 heads of 128 in
-// bf16 take @@PROMPT@@ us (45.9 without norms, by the kernel above); with three axes,
-// whose entries are 8 bytes from rows of their own, @@AXES@@.
+// bf16 take 46.4 us (46.2 without norms, by the kernel above), 4.4 TB/s; with three
+// axes, whose entries are 8 bytes from rows of their own, 46.9.
 template <typename TI, typename TO, typename C, int HEADS>
 __global__ __launch_bounds__(256) void k_norm_rope_rows(RopeArgs a) {
     const int64_t t64 = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
@@ -553,8 +553,10 @@ static void launch_rope(Ctx* c, RopeArgs a, bool vec) {
     }
     a.lanes_log2 = rows_log2;
     const int64_t blocks = ceil_div(a.tokens << a.lanes_log2, 256);
-    // four heads per lane where that still leaves eight workgroups per CU
-    const bool four = blocks * ceil_div(heads, 4) >= 8 * c->num_cus;
+    // four heads per lane where that still leaves eight workgroups per CU, with norms
+    // two (5001 tokens of 12 + 12 heads of 64 12.1 us, of one head 14.5; 2000 of 32 + 8
+    // of 128 11.9 and 14.2; with one per CU 700 of those 7.3 and 6.4)
+    const bool four = blocks * ceil_div(heads, 4) >= (MORE ? 2 : 8) * c->num_cus;
     const dim3 grid((unsigned)blocks, (unsigned)(four ? ceil_div(heads, 4) : heads));
     if constexpr (MORE) {
         if (four) k_norm_rope_rows<TI, TO, C, 4><<<grid, 256, 0, c->stream>>>(a);
