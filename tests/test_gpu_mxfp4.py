@@ -286,7 +286,9 @@ def test_nan_blocks_stay_in_their_row_and_column(ctx, m):
 @pytest.mark.parametrize("m,n,k,pad,shift", [(1, 130, 800, 0, 0), (4, 64, 4096, 8, 0), (13, 768, 768, 5, 0),
                                              (32, 2304, 768, 0, 0), (33, 96, 1000, 0, 4), (200, 768, 768, 0, 0),
                                              (1500, 1024, 320, 8, 0), (2, 16400, 800, 0, 0), (16, 8210, 2100, 4, 0),
-                                             (7, 40, 4000, 0, 0), (16, 33, 8200, 0, 0)])
+                                             (7, 40, 4000, 0, 0), (16, 33, 8200, 0, 0),
+                                             (2, 50, 16000, 0, 0), (5, 8200, 2000, 8, 0), (3, 16400, 4096, 0, 0),
+                                             (1, 8200, 8192, 0, 0), (1, 16384, 16352, 0, 0), (30, 16400, 96, 0, 0)])
 def test_linear(ctx, typ, m, n, k, pad, shift):
     """The activation's codes are the definition's, so the outputs are those of
     the codes' values: exact sums where the scales are near each other."""

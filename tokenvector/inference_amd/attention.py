@@ -87,24 +87,19 @@ class _Call:
         self._fn = lib._FuncPtr((name, lib))
         self._ctx, self._kept = ctx, args
         given = [x.data if isinstance(x, Rows) else x for x in self._also]
-        self._caches = [x for x in given if isinstance(x, KVCache)]
-        given += [x for cache in self._caches for x in cache._kept]
-        self._weights = [x for x in given if isinstance(x, QuantizedLinear)]
-        self._buffers = [x for x in given if isinstance(x, DeviceBuffer)]
+        given += [x for cache in given if isinstance(cache, KVCache) for x in cache._kept]
+        self._held = [x for x in given if isinstance(x, (KVCache, QuantizedLinear, DeviceBuffer))]
         self._args = tuple(C.cast(C.byref(a), C.c_void_p) if isinstance(a, C.Structure)
                            else C.c_void_p() if a is None else a if isinstance(a, t) else t(a)
                            for t, a in zip(types, args))
 
     def __call__(self) -> None:
-        for cache in self._caches:
-            if not cache.handle:
-                raise ValueError("the cache of this call is closed")
-        for weight in self._weights:
-            if not weight.handle:
-                raise ValueError("the weight of this call is closed")
-        for buffer in self._buffers:
-            if not buffer.ptr and buffer.nbytes:
-                raise ValueError("a buffer of this call is closed")
+        for held in self._held:
+            if isinstance(held, DeviceBuffer):
+                if not held.ptr and held.nbytes:
+                    raise ValueError("a buffer of this call is closed")
+            elif not held.handle:
+                raise ValueError("the cache or weight of this call is closed")
         rc = self._fn(C.c_int64(self._ctx.handle), *self._args)
         if rc:
             _lib.check(rc)

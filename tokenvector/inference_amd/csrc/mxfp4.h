@@ -66,6 +66,40 @@ __device__ __forceinline__ unsigned code8(const float (&x)[8], float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
 }
 
+// The code dword and scale byte of 8 elements, whose block's others are in the
+// lane's three neighbours of four.
+__device__ __forceinline__ unsigned neighbour_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
+    return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+}
+__device__ __forceinline__ unsigned code_quarter(const float (&x)[8], unsigned& byte) {
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+    byte = scale_byte(neighbour_max(most));
+    return byte == 255 ? 0u : code8(x, scale_value(byte));
+}
+
+// 8 elements from `at` of a row of `cols`, zeros past its end.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_quarter(const T* row, int64_t at, int64_t cols, float (&x)[8]) {
+    if (VEC) {
+        struct alignas(16) Chunk {
+            T e[8];
+        };
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = 0.0f;
+        if (at < cols) {
+            const Chunk v = *reinterpret_cast<const Chunk*>(row + at);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = to_f32(v.e[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = at + i < cols ? to_f32(row[at + i]) : 0.0f;
+    }
+}
+
 // The scales of a row's blocks 8 s .. 8 s + 7 from its [blocks] bytes, those past its
 // last 0.  Nothing behind the row is read, and there is no branch on s, so that the
 // loads of several s are in flight together.
@@ -97,9 +131,11 @@ int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* a, int64_t rows_a, uint8_t
 // mxfp4_tile.hip.  Scales as slabs, or as rows where mx_takes_rows(p).
 bool mx_takes_rows(const Ctx* c, const mx::Product& p);
 int launch_mx_product(Ctx* c, const mx::Product& p);
-// mxfp4_few.hip: m <= kFewRows; and the linear that codes m <= kFewCoded rows itself.
-constexpr int kFewRows = 64, kFewCoded = 16;
+// mxfp4_few.hip: m <= kFewRows; and the linear that codes its rows itself, where
+// mx_codes_few.
+constexpr int kFewRows = 64;
 int launch_mx_few(Ctx* c, const mx::Product& p);
+bool mx_codes_few(const Ctx* c, const mx::Product& p);
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const mx::Product& p);
 // The linear of a resident weight on float rows (mxfp4.hip).
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, mx::Product p);

@@ -30,27 +30,10 @@ __global__ __launch_bounds__(256) void k_mx_code(CodeArgs a) {
     const uint32_t row = div_by(a.div, b);
     const int block = (int)(b - row * a.per_row), part = (int)threadIdx.x & 3;
     const int64_t at = (int64_t)block * 32 + part * 8;
-    const T* src = static_cast<const T*>(a.x) + (int64_t)row * a.stride + at;
     float x[8];
-    if (VEC) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = 0.0f;
-        if (at < a.cols) {
-            const Chunk<T> v = *reinterpret_cast<const Chunk<T>*>(src);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = to_f32(v.e[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = at + i < a.cols ? to_f32(src[i]) : 0.0f;
-    }
-    unsigned most = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-    most = max(most, (unsigned)__shfl_xor((int)most, 1));
-    most = max(most, (unsigned)__shfl_xor((int)most, 2));
-    const unsigned byte = scale_byte(most);
-    const unsigned code = byte == 255 ? 0u : code8(x, scale_value(byte));
+    load_quarter<T, VEC>(static_cast<const T*>(a.x) + (int64_t)row * a.stride, at, a.cols, x);
+    unsigned byte;
+    const unsigned code = code_quarter(x, byte);
     if (block < a.blocks)
         reinterpret_cast<unsigned*>(a.codes)[((int64_t)row * a.blocks + block) * 4 + part] = code;
     if (part == 0) {
@@ -215,7 +198,7 @@ int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_
 }
 
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
-    if (p.m <= kFewCoded) return launch_mx_few_linear(c, type, x, stride, k, p);
+    if (mx_codes_few(c, p)) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
     TKV_RC_TRY(ctx_workspace(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
     TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(p.m, k), &slabs));

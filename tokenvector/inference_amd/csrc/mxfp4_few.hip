@@ -8,10 +8,8 @@
 // 256-element slabs of K in turn, each for all of the workgroup's 16 NR rows, and
 // their sums are added in LDS in the waves' order.
 //
-// The linear's form codes the tokens on the way: a lane that multiplies block b of
-// token t loads its 32 elements, has their maximum without any other lane, and
-// holds the codes as the instruction takes them.  That is done again by every
-// workgroup.
+// The linear's form codes the tokens on the way, every workgroup all of them, into
+// LDS, while the first of its weights are on their way.
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -19,95 +17,17 @@
 namespace tkv {
 namespace mx {
 
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
 struct FewArgs {
     Product p;
     const void* x;  // the linear's rows
     int64_t stride, k;
     int32_t vec;    // rows of 16 bytes
+    FastDiv quarters;  // of a row, as slabs have them
 };
 
-template <typename T>
-struct Block {
-    u32x4 raw[sizeof(T) * 2];
-};
-
-// 32 elements from `at` of a row of k, zeros past its end.
-template <typename T>
-__device__ __forceinline__ Block<T> load_block(const T* row, int64_t at, int64_t k, bool vec) {
-    Block<T> b;
-    if (vec && at + 32 <= k) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) * 2; i++) b.raw[i] = reinterpret_cast<const u32x4*>(row + at)[i];
-    } else {
-        T e[32];
-#pragma unroll
-        for (int i = 0; i < 32; i++) e[i] = at + i < k ? row[at + i] : (T)0.0f;
-        __builtin_memcpy(&b, e, sizeof(b));
-    }
-    return b;
-}
-
-// Codes and scale byte of a block held by one lane.  16-bit types: the largest
-// magnitude of two at a time as integers (infinities and NaN above all numbers),
-// and the conversions that take them.
-template <typename T>
-__device__ __forceinline__ v4i code_block(const Block<T>& b, unsigned& byte) {
-    unsigned most = 0;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) most = max(most, b.raw[i][j] & 0x7fffffffu);
-    } else {
-        u16x2 m = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, b.raw[i][j] & 0x7fff7fffu));
-        const unsigned short one = m.x > m.y ? m.x : m.y;
-        if constexpr (std::is_same<T, __bf16>::value)
-            most = (unsigned)one << 16;
-        else
-            most = __float_as_uint((float)__builtin_bit_cast(_Float16, one));
-    }
-    byte = scale_byte(most);
-    if (byte == 255) return v4i{0, 0, 0, 0};
-    const float scale = scale_value(byte);
-    v4i c;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        unsigned w = 0;
-        if constexpr (sizeof(T) == 4) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = __uint_as_float(b.raw[2 * i + j / 4][j & 3]);
-            w = code8(x, scale);
-        } else {
-            // (values of their own: the compiler takes a vector's first element for
-            // each where a bit cast names an element)
-            const unsigned e0 = b.raw[i][0], e1 = b.raw[i][1], e2 = b.raw[i][2], e3 = b.raw[i][3];
-            if constexpr (std::is_same<T, __bf16>::value) {
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(b16x2, e0), scale, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(b16x2, e1), scale, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(b16x2, e2), scale, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(b16x2, e3), scale, 3);
-            } else {
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h16x2, e0), scale, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h16x2, e1), scale, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h16x2, e2), scale, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h16x2, e3), scale, 3);
-            }
-        }
-        c[i] = (int)w;
-    }
-    return c;
-}
+// Bytes of a coded token in LDS, and of its scales.
+__host__ __device__ __forceinline__ uint32_t coded_bytes(uint32_t blocks) { return blocks * 16u + 16u; }
+__host__ __device__ __forceinline__ uint32_t scale_bytes(uint32_t blocks) { return ((blocks + 7) >> 3) * 8u; }
 
 struct Coded {};      // the tokens come as codes and slabs,
 struct CodedRows {};  // or the scales of both as [rows][blocks]
@@ -116,6 +36,7 @@ template <typename TI, int NR, int MT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     constexpr bool ROWS = std::is_same<TI, CodedRows>::value, CODED = ROWS || std::is_same<TI, Coded>::value;
     typedef typename std::conditional<CODED, float, TI>::type TX;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Product& p = a.p;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -131,50 +52,49 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         const int64_t row = n0 + r * 16 + l16;
         w_row[r] = p.w + (row < p.n ? row : p.n - 1) * row_bytes;
     }
-    int64_t token[MT];
+    int token[MT];
 #pragma unroll
-    for (int t = 0; t < MT; t++) token[t] = t * 16 + l16 < p.m ? t * 16 + l16 : p.m - 1;
+    for (int t = 0; t < MT; t++) token[t] = t * 16 + l16 < (int)p.m ? t * 16 + l16 : (int)p.m - 1;
 
-    struct Slab {
+    struct Weights {
         v4i w[NR][2];
-        v2i ws[NR];
-        v4i t[CODED ? MT : 1][2];
-        v2i ts[CODED ? MT : 1];
-        Block<TX> x[CODED ? 1 : MT][2];
+        v2i s[NR];
     };
-    const auto load = [&](int s, Slab& b) {
-        uint32_t at[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            at[h] = (uint32_t)s * 128u + (uint32_t)(h * 64 + g * 16);
-            at[h] = at[h] < row_bytes ? at[h] : row_bytes - 16;  // past the row: its scales are 2^-127
-        }
+    struct Tokens {
+        v4i t[MT][2];
+        v2i s[MT];
+    };
+    // chunks past the row: its last, whose scales are 2^-127
+    const auto place = [&](int s, int h) {
+        const uint32_t at = (uint32_t)s * 128u + (uint32_t)(h * 64 + g * 16);
+        return at < row_bytes ? at : row_bytes - 16;
+    };
+    const auto load_weight = [&](int s, Weights& b) {
 #pragma unroll
         for (int r = 0; r < NR; r++) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) b.w[r][h] = *reinterpret_cast<const v4i*>(w_row[r] + at[h]);
+            for (int h = 0; h < 2; h++) b.w[r][h] = *reinterpret_cast<const v4i*>(w_row[r] + place(s, h));
             if constexpr (ROWS) {
                 const int64_t row = n0 + r * 16 + l16;
-                b.ws[r] = row_scales(p.ws + (row < p.n ? row : p.n - 1) * p.blocks, s, p.blocks);
+                b.s[r] = row_scales(p.ws + (row < p.n ? row : p.n - 1) * p.blocks, s, p.blocks);
             } else {
-                b.ws[r] = *reinterpret_cast<const v2i*>(p.ws + ((int64_t)s * p.w_rows + n0 + r * 16 + l16) * 8);
+                b.s[r] = *reinterpret_cast<const v2i*>(p.ws + ((int64_t)s * p.w_rows + n0 + r * 16 + l16) * 8);
             }
         }
+    };
+    uint8_t* const scales = lds + (uint32_t)p.m * coded_bytes(p.blocks);  // of the tokens coded here
+    const auto load_tokens = [&](int s, Tokens& b) {
 #pragma unroll
         for (int t = 0; t < MT; t++) {
-            if constexpr (CODED) {
+            const uint8_t* row = CODED ? p.a + (uint64_t)token[t] * row_bytes : lds + (uint32_t)token[t] * coded_bytes(p.blocks);
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    b.t[t][h] = *reinterpret_cast<const v4i*>(p.a + token[t] * row_bytes + at[h]);
-                if constexpr (ROWS) b.ts[t] = row_scales(p.as + token[t] * p.blocks, s, p.blocks);
-                else b.ts[t] = *reinterpret_cast<const v2i*>(p.as + ((int64_t)s * p.a_rows + t * 16 + l16) * 8);
-            } else {
-                // (one lane of a token that is not there does what the last token's does)
-                const TX* row = static_cast<const TX*>(a.x) + token[t] * a.stride;
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    b.x[t][h] = load_block<TX>(row, ((int64_t)s * 8 + h * 4 + g) * 32, a.k, a.vec);
-            }
+            for (int h = 0; h < 2; h++) b.t[t][h] = *reinterpret_cast<const v4i*>(row + place(s, h));
+            if constexpr (!CODED)
+                b.s[t] = *reinterpret_cast<const v2i*>(scales + (uint32_t)token[t] * scale_bytes(p.blocks) + s * 8);
+            else if constexpr (ROWS)
+                b.s[t] = row_scales(p.as + (int64_t)token[t] * p.blocks, s, p.blocks);
+            else
+                b.s[t] = *reinterpret_cast<const v2i*>(p.as + ((int64_t)s * p.a_rows + t * 16 + l16) * 8);
         }
     };
 
@@ -183,50 +103,88 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int t = 0; t < MT; t++) acc[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    Slab cur;
-    if (wave < slabs) load(wave, cur);
-    for (int s = wave; s < slabs; s += WAVES) {
-        Slab next;
-        if (s + WAVES < slabs) load(s + WAVES, next);
+    // a wave's next slabs on their way (four instead of two were no faster)
+    constexpr int DEPTH = 2;
+    Weights weights[DEPTH];
+    Tokens tokens[DEPTH];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            v4i tc[MT];
-            unsigned tb[MT];
+    for (int u = 0; u < DEPTH; u++)
+        if (wave + u * WAVES < slabs) {
+            load_weight(wave + u * WAVES, weights[u]);
+            if constexpr (CODED) load_tokens(wave + u * WAVES, tokens[u]);
+        }
+    if constexpr (!CODED) {
+        const uint32_t per = a.quarters.d, all = per * (uint32_t)p.m;
+        const auto code = [&](uint32_t q, const float (&x)[8]) {
+            const uint32_t t = div_by(a.quarters, q), c = q - t * per;
+            unsigned byte;
+            const unsigned w = code_quarter(x, byte);
+            if (c < (uint32_t)p.blocks * 4)
+                *reinterpret_cast<unsigned*>(lds + t * coded_bytes(p.blocks) + c * 4) = w;
+            if ((c & 3) == 0) scales[t * scale_bytes(p.blocks) + (c >> 2)] = (uint8_t)byte;
+        };
+        const auto fetch = [&](uint32_t q, float (&x)[8]) {
+            const uint32_t t = div_by(a.quarters, q), c = q - t * per;
+            const TX* row = static_cast<const TX*>(a.x) + (int64_t)t * a.stride;
+            if (a.vec) load_quarter<TX, true>(row, (int64_t)c * 8, a.k, x);
+            else load_quarter<TX, false>(row, (int64_t)c * 8, a.k, x);
+        };
+        constexpr uint32_t STEP = WAVES * 64;
+        uint32_t q = threadIdx.x;
+        for (; q + 3 * STEP < all; q += 4 * STEP) {  // (whole blocks: four lanes stay together)
+            float x[4][8];
 #pragma unroll
-            for (int t = 0; t < MT; t++) {
-                if constexpr (CODED) {
-                    tc[t] = cur.t[t][h];
-                    tb[t] = (unsigned)cur.ts[t][h] >> (8 * g);
-                } else {
-                    tc[t] = code_block<TX>(cur.x[t][h], tb[t]);
-                    // (blocks past the row are zeros, and their scale 2^-127)
+            for (int u = 0; u < 4; u++) fetch(q + u * STEP, x[u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++) code(q + u * STEP, x[u]);
+        }
+        for (; q < all; q += STEP) {
+            float x[8];
+            fetch(q, x);
+            code(q, x);
+        }
+        __syncthreads();
+    }
+    for (int s0 = wave; s0 < slabs; s0 += DEPTH * WAVES) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; u++) {
+            const int s = s0 + u * WAVES, then = s + DEPTH * WAVES;
+            if (s >= slabs) break;
+            if constexpr (!CODED) load_tokens(s, tokens[u]);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    const v4i w = weights[u].w[r][h];
+                    const unsigned wb = (unsigned)weights[u].s[r][h] >> (8 * g);
+#pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        const v4i x = tokens[u].t[t][h];
+                        const unsigned tb = (unsigned)tokens[u].s[t][h] >> (8 * g);
+                        acc[r][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            v8i{w.x, w.y, w.z, w.w, 0, 0, 0, 0}, v8i{x.x, x.y, x.z, x.w, 0, 0, 0, 0}, acc[r][t], 4, 4,
+                            0, (int)wb, 0, (int)tb);
+                    }
                 }
-            }
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const v4i w = cur.w[r][h];
-                const unsigned wb = (unsigned)cur.ws[r][h] >> (8 * g);
-#pragma unroll
-                for (int t = 0; t < MT; t++)
-                    acc[r][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                        v8i{w.x, w.y, w.z, w.w, 0, 0, 0, 0}, v8i{tc[t].x, tc[t].y, tc[t].z, tc[t].w, 0, 0, 0, 0},
-                        acc[r][t], 4, 4, 0, (int)wb, 0, (int)tb[t]);
+            if (then < slabs) {
+                load_weight(then, weights[u]);
+                if constexpr (CODED) load_tokens(then, tokens[u]);
             }
         }
-        cur = next;
     }
+    if constexpr (!CODED) __syncthreads();  // the codes' place is the sums'
 
     // a lane holds rows 4 g .. 4 g + 3 of 16 for token l16
-    __shared__ v4f part[WAVES][NR * MT][64];
+    v4f* part = reinterpret_cast<v4f*>(lds);  // [WAVES][NR * MT][64]
 #pragma unroll
     for (int r = 0; r < NR; r++)
 #pragma unroll
-        for (int t = 0; t < MT; t++) part[wave][r * MT + t][lane] = acc[r][t];
+        for (int t = 0; t < MT; t++) part[(wave * NR * MT + r * MT + t) * 64 + lane] = acc[r][t];
     __syncthreads();
     for (int i = wave; i < NR * MT; i += WAVES) {
-        v4f sum = part[0][i][lane];
+        v4f sum = part[i * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) sum += part[w][i][lane];
+        for (int w = 1; w < WAVES; w++) sum += part[(w * NR * MT + i) * 64 + lane];
         const int64_t tok = (i % MT) * 16 + l16, n = n0 + (i / MT) * 16 + g * 4;
         if (tok >= p.m) continue;
 #pragma unroll
@@ -241,17 +199,26 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     }
 }
 
+template <typename TI, int NR, int MT, int WAVES = 8>
+static void start_few(Ctx* c, const FewArgs& a, int64_t rows) {
+    constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
+    const uint32_t sums = WAVES * NR * MT * 1024;
+    const uint32_t codes = CODED ? 0 : (uint32_t)a.p.m * (coded_bytes(a.p.blocks) + scale_bytes(a.p.blocks));
+    k_mx_few<TI, NR, MT, WAVES><<<wide_grid(ceil_div(rows, NR)), WAVES * 64, sums > codes ? sums : codes, c->stream>>>(a);
+}
+
+// 16-row blocks a workgroup: as many as leave a workgroup per CU, four for long rows
+// or many tokens alone (16 x 16384 rows of 16384: 29.8 us, with two 34.7; of 4096 9.0
+// and 8.3; 32 x 16384 of 4096 10.1 and 11.4).  Coding for a block, 16 waves from three
+// tokens on (8 x 4096 of 4096: 6.4 us, with 8 waves 7.2; 1 x 4096 4.6 and 4.4).
 template <typename TI, int MT>
 static int launch_few(Ctx* c, const FewArgs& a) {
-    constexpr int WAVES = 8;
+    constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
     const int64_t rows = ceil_div(a.p.n, 16);
-    // rows a workgroup: as many as leave a workgroup per CU
-    if (rows >= 4 * c->num_cus)
-        k_mx_few<TI, 4, MT, WAVES><<<wide_grid(ceil_div(rows, 4)), WAVES * 64, 0, c->stream>>>(a);
-    else if (rows >= 2 * c->num_cus)
-        k_mx_few<TI, 2, MT, WAVES><<<wide_grid(ceil_div(rows, 2)), WAVES * 64, 0, c->stream>>>(a);
-    else
-        k_mx_few<TI, 1, MT, WAVES><<<wide_grid(rows), WAVES * 64, 0, c->stream>>>(a);
+    if (MT < 4 && rows >= 4 * c->num_cus && (MT == 2 || a.p.blocks >= 256)) start_few<TI, MT < 4 ? 4 : 2, MT>(c, a, rows);
+    else if (rows >= 2 * c->num_cus) start_few<TI, 2, MT>(c, a, rows);
+    else if (!CODED && a.p.m > 2) start_few<TI, 1, MT, CODED ? 8 : 16>(c, a, rows);
+    else start_few<TI, 1, MT>(c, a, rows);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
@@ -273,13 +240,21 @@ int launch_mx_few(Ctx* c, const Product& p) {
     return launch_few<Coded, 4>(c, a);
 }
 
+// Every workgroup codes all rows, 0.25 us for each 4096 elements (with one block of
+// rows a workgroup; 0.4 with several), where a launch of its own costs 2.2: 8 x 4096
+// of 4096 6.4 us against 6.7, 16 x 4096 8.6 and 7.1, 8 x 16384 12.7 and 11.0.
+bool mx_codes_few(const Ctx* c, const Product& p) {
+    return p.m <= 16 && p.m * p.blocks <= (ceil_div(p.n, 16) >= 2 * c->num_cus ? 512 : 1024);
+}
+
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const Product& p) {
     FewArgs a = {};
     a.p = p;
     a.x = x;
     a.stride = stride;
     a.k = k;
-    a.vec = aligned(x, 16) && stride * type_bytes(type) % 16 == 0;
+    a.vec = k % 8 == 0 && aligned(x, 16) && stride * type_bytes(type) % 16 == 0;
+    a.quarters = fast_div((uint32_t)slabs_of(k) * 32);
     if (type == TKV_HIP_F32) return launch_few<float, 1>(c, a);
     if (type == TKV_HIP_F16) return launch_few<_Float16, 1>(c, a);
     return launch_few<__bf16, 1>(c, a);
