@@ -84,7 +84,11 @@ __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
         Chunk<T> v;
 #pragma unroll
         for (int i = 0; i < 8; i++) v.e[i] = from_f32<T>(x[i]);
-        *reinterpret_cast<Chunk<T>*>(dst) = v;
+        // past the L2's reuse: 16384 x 8192 coded and read back 130 -> 110 us
+        v4i w[sizeof(T) / 2];
+        __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_nontemporal_store(w[i], reinterpret_cast<v4i*>(dst) + i);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
