@@ -626,6 +626,7 @@ int32_t tkv_hip_dev_rope_append(int64_t ctx, int32_t type_in, int64_t tokens, in
  *     table's columns are the pairs', so axes with frequencies of their own are a
  *     choice of the table.
  * A token with a position outside [0, table_len) on any axis is a padding token.
+ * Where two tokens of a call have one slot, it holds either's values or a mixture.
  * Without norm and with one axis it is rope_append, bit for bit. */
 typedef struct {
     float eps;
@@ -723,7 +724,8 @@ int32_t tkv_hip_dev_dequantize_mxfp4(int64_t ctx, const uint8_t* codes, const ui
  * type_out (F32, F16, BF16), its rows `stride` (>= N) elements apart.  A NaN
  * block makes its row's (or column's) outputs NaN and touches no other.  Where K
  * is no multiple of 32, the codes past K have to be zeros in a or in w (quantize
- * writes them so).  A sum's terms below 2^-126 may be taken as zero.
+ * writes them so).  A sum's terms below 2^-126 may be taken as zero.  y shares
+ * no memory with the operands.
  * K >= 2^17, M >= 2^31 or N >= 2^28: UNSUPPORTED. */
 int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a_scales,
                                  const uint8_t* w, const uint8_t* w_scales, int64_t m, int64_t n,
@@ -739,7 +741,8 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
 int32_t tkv_hip_weight_create_mxfp4(int64_t ctx, const uint8_t* codes, const uint8_t* scales,
                                     int64_t n, int64_t k, const float* bias, int64_t* handle_out);
 /* The linear on rows of F32, F16 or BF16, stride_x (>= K) elements apart, y of
- * type_out with rows stride_y (>= N) apart.  MXFP4 weights; others: UNSUPPORTED. */
+ * type_out with rows stride_y (>= N) apart, sharing no memory with x.  MXFP4
+ * weights; others: UNSUPPORTED. */
 int32_t tkv_hip_linear_forward_typed(int64_t ctx, int64_t weight, int32_t type_in, const void* x,
                                      int64_t stride_x, int64_t m, int32_t type_out, void* y,
                                      int64_t stride_y);

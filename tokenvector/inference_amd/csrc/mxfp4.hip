@@ -201,11 +201,19 @@ int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_
     return TKV_HIP_OK;
 }
 
+// A workspace; hipMalloc's error is taken off, or the next launch's check would
+// report it.
+static int room(Ctx* c, int slot, size_t bytes, void** out) {
+    const int rc = ctx_workspace(c, slot, bytes, out);
+    if (rc == TKV_HIP_OOM) (void)hipGetLastError();
+    return rc;
+}
+
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
     if (mx_codes_few(c, p)) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
-    TKV_RC_TRY(ctx_workspace(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
-    TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(p.m, k), &slabs));
+    TKV_RC_TRY(room(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
+    TKV_RC_TRY(room(c, 1, slab_bytes(p.m, k), &slabs));
     TKV_RC_TRY(launch_mx_quantize(c, type, x, stride, p.m, k, static_cast<uint8_t*>(codes),
                                   static_cast<uint8_t*>(slabs), true));
     p.a = static_cast<uint8_t*>(codes);
@@ -214,8 +222,8 @@ int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k,
     return launch_mx_product(c, p);
 }
 
-// Sizes that the entry points take: rows whose blocks pass 2^26 would not be
-// numbered, nor (checked as a quotient) their bytes in 63 bits.
+// Sizes that coding and decoding take: a launch's blocks are numbered in 32 bits, and
+// a row's (2^26 at most) are one launch's.
 static bool sizes_ok(int64_t rows, int64_t cols) {
     return rows >= 0 && rows < (1ll << 31) && cols > 0 && cols < (1ll << 31);
 }
@@ -262,7 +270,7 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
         return set_error(TKV_HIP_UNSUPPORTED, "matmul_mxfp4: K must be below 2^17, M below 2^31 and N below 2^28");
     if (m == 0 || n == 0) return TKV_HIP_OK;
     if (!a || !a_scales || !w || !w_scales || !y || !aligned(a, 16) || !aligned(w, 16) ||
-        !aligned(y, type_bytes(type_out)))
+        !aligned(y, type_bytes(type_out)) || !aligned(bias, 4))
         return set_error(TKV_HIP_BAD_ARG, "matmul_mxfp4: NULL or unaligned buffers (codes: 16 bytes)");
     Ctx* c;
     TKV_RC_TRY(ctx_get(ctx, &c));
@@ -280,8 +288,8 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
     p.y_type = type_out;
     if (!mx_takes_rows(c, p)) {
         void *as, *ws;
-        TKV_RC_TRY(ctx_workspace(c, 1, slab_bytes(m, k), &as));
-        TKV_RC_TRY(ctx_workspace(c, 2, slab_bytes(n, k), &ws));
+        TKV_RC_TRY(room(c, 1, slab_bytes(m, k), &as));
+        TKV_RC_TRY(room(c, 2, slab_bytes(n, k), &ws));
         TKV_RC_TRY(launch_mx_slabs(c, k, a_scales, m, static_cast<uint8_t*>(as), w_scales, n, static_cast<uint8_t*>(ws)));
         p.as = static_cast<uint8_t*>(as);
         p.ws = static_cast<uint8_t*>(ws);
