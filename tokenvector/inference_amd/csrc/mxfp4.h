@@ -66,38 +66,76 @@ __device__ __forceinline__ unsigned code8(const float (&x)[8], float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
 }
 
-// The code dword and scale byte of 8 elements, whose block's others are in the
-// lane's three neighbours of four.
+// 8 elements as they are in memory.
+template <typename T>
+struct alignas(16) Quarter {
+    unsigned v[2 * sizeof(T)];
+};
+
+// 8 elements from `at` of a row of `cols`, zeros past its end.
+template <typename T, bool VEC>
+__device__ __forceinline__ Quarter<T> load_quarter(const T* row, int64_t at, int64_t cols) {
+    Quarter<T> q = {};
+    if (VEC) {
+        if (at < cols) q = *reinterpret_cast<const Quarter<T>*>(row + at);
+    } else {
+        T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = at + i < cols ? row[at + i] : (T)0.0f;
+        __builtin_memcpy(&q, e, sizeof(q));
+    }
+    return q;
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+
+// The largest of a lane's and its three neighbours' of four.
 __device__ __forceinline__ unsigned neighbour_max(unsigned v) {
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
     return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
 }
-__device__ __forceinline__ unsigned code_quarter(const float (&x)[8], unsigned& byte) {
-    unsigned most = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-    byte = scale_byte(neighbour_max(most));
-    return byte == 255 ? 0u : code8(x, scale_value(byte));
-}
 
-// 8 elements from `at` of a row of `cols`, zeros past its end.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_quarter(const T* row, int64_t at, int64_t cols, float (&x)[8]) {
-    if (VEC) {
-        struct alignas(16) Chunk {
-            T e[8];
-        };
+// The code dword and scale byte of 8 elements, whose block's others are in the
+// lane's three neighbours of four.  Of 16-bit types two magnitudes at a time are
+// compared, as integers (infinities and NaN above all numbers), and converted as
+// they are: the same codes as from f32, which every value of theirs was compared
+// with at every scale.
+template <typename T>
+__device__ __forceinline__ unsigned code_quarter(const Quarter<T>& q, unsigned& byte) {
+    unsigned code = 0;
+    if constexpr (sizeof(T) == 4) {
+        unsigned most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = 0.0f;
-        if (at < cols) {
-            const Chunk v = *reinterpret_cast<const Chunk*>(row + at);
+        for (int i = 0; i < 8; i++) most = max(most, q.v[i] & 0x7fffffffu);
+        byte = scale_byte(neighbour_max(most));
+        float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = to_f32(v.e[i]);
-        }
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(q.v[i]);
+        code = code8(x, scale_value(byte));
     } else {
+        u16x2 m = __builtin_bit_cast(u16x2, q.v[0] & 0x7fff7fffu);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = at + i < cols ? to_f32(row[at + i]) : 0.0f;
+        for (int i = 1; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, q.v[i] & 0x7fff7fffu));
+        unsigned most = neighbour_max(m.x > m.y ? m.x : m.y);
+        if constexpr (__is_same(T, __bf16)) {
+            byte = scale_byte(most << 16);
+            const float scale = scale_value(byte);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(b16x2, q.v[0]), scale, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(b16x2, q.v[1]), scale, 1);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(b16x2, q.v[2]), scale, 2);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(b16x2, q.v[3]), scale, 3);
+        } else {
+            byte = scale_byte(__float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)most)));
+            const float scale = scale_value(byte);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, __builtin_bit_cast(h16x2, q.v[0]), scale, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, __builtin_bit_cast(h16x2, q.v[1]), scale, 1);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, __builtin_bit_cast(h16x2, q.v[2]), scale, 2);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, __builtin_bit_cast(h16x2, q.v[3]), scale, 3);
+        }
     }
+    return byte == 255 ? 0u : code;
 }
 
 // The scales of a row's blocks 8 s .. 8 s + 7 from its [blocks] bytes, those past its

@@ -30,10 +30,9 @@ __global__ __launch_bounds__(256) void k_mx_code(CodeArgs a) {
     const uint32_t row = div_by(a.div, b);
     const int block = (int)(b - row * a.per_row), part = (int)threadIdx.x & 3;
     const int64_t at = (int64_t)block * 32 + part * 8;
-    float x[8];
-    load_quarter<T, VEC>(static_cast<const T*>(a.x) + (int64_t)row * a.stride, at, a.cols, x);
     unsigned byte;
-    const unsigned code = code_quarter(x, byte);
+    const unsigned code =
+        code_quarter<T>(load_quarter<T, VEC>(static_cast<const T*>(a.x) + (int64_t)row * a.stride, at, a.cols), byte);
     if (block < a.blocks)
         reinterpret_cast<unsigned*>(a.codes)[((int64_t)row * a.blocks + block) * 4 + part] = code;
     if (part == 0) {

@@ -3,8 +3,8 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 with the weight's rows as its rows and the
 // tokens as its columns.  A lane's operand is a block of a row, 16 bytes and a
-// scale byte, straight from memory: lanes of a row take the chunks of a 128-byte
-// line (two instructions, 256 elements).  The waves of a workgroup take
+// scale byte, straight from memory: a row's four lanes take the chunks of a
+// 128-byte line with two instructions, 256 elements.  The waves of a workgroup take
 // 256-element slabs of K in turn, each for all of the workgroup's 16 NR rows, and
 // their sums are added in LDS in the waves' order.
 //
@@ -114,34 +114,40 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
             if constexpr (CODED) load_tokens(wave + u * WAVES, tokens[u]);
         }
     if constexpr (!CODED) {
-        const uint32_t per = a.quarters.d, all = per * (uint32_t)p.m;
-        const auto code = [&](uint32_t q, const float (&x)[8]) {
-            const uint32_t t = div_by(a.quarters, q), c = q - t * per;
-            unsigned byte;
-            const unsigned w = code_quarter(x, byte);
-            if (c < (uint32_t)p.blocks * 4)
-                *reinterpret_cast<unsigned*>(lds + t * coded_bytes(p.blocks) + c * 4) = w;
-            if ((c & 3) == 0) scales[t * scale_bytes(p.blocks) + (c >> 2)] = (uint8_t)byte;
-        };
-        const auto fetch = [&](uint32_t q, float (&x)[8]) {
-            const uint32_t t = div_by(a.quarters, q), c = q - t * per;
-            const TX* row = static_cast<const TX*>(a.x) + (int64_t)t * a.stride;
-            if (a.vec) load_quarter<TX, true>(row, (int64_t)c * 8, a.k, x);
-            else load_quarter<TX, false>(row, (int64_t)c * 8, a.k, x);
-        };
-        constexpr uint32_t STEP = WAVES * 64;
-        uint32_t q = threadIdx.x;
-        for (; q + 3 * STEP < all; q += 4 * STEP) {  // (whole blocks: four lanes stay together)
-            float x[4][8];
+        // a thread takes one quarter of a block of every token, or of every `apart`-th
+        // where the rows are short
+        constexpr int THREADS = WAVES * 64;
+        const int per = (int)a.quarters.d, apart = per < THREADS ? THREADS / per : 1;
+        const int first = per < THREADS ? (int)div_by(a.quarters, threadIdx.x) : 0;
+        const int many = first < apart ? (int)p.m : 0;
+        for (int c = (int)threadIdx.x - first * per; c < per; c += THREADS) {  // (whole blocks: four lanes stay together)
+            const TX* from = static_cast<const TX*>(a.x) + (int64_t)first * a.stride;
+            uint8_t* to = lds + (uint32_t)first * coded_bytes(p.blocks) + c * 4;
+            uint8_t* scale = scales + (uint32_t)first * scale_bytes(p.blocks) + (c >> 2);
+            const int64_t step = (int64_t)apart * a.stride;
+            const uint32_t to_step = (uint32_t)apart * coded_bytes(p.blocks), scale_step = (uint32_t)apart * scale_bytes(p.blocks);
+            const bool there = c < p.blocks * 4;
+            const auto fetch = [&](const TX* row) {
+                return a.vec ? load_quarter<TX, true>(row, (int64_t)c * 8, a.k) : load_quarter<TX, false>(row, (int64_t)c * 8, a.k);
+            };
+            const auto code = [&](const Quarter<TX>& x) {
+                unsigned byte;
+                const unsigned w = code_quarter<TX>(x, byte);
+                if (there) *reinterpret_cast<unsigned*>(to) = w;
+                if ((c & 3) == 0) *scale = (uint8_t)byte;
+                to += to_step;
+                scale += scale_step;
+            };
+            for (int t = first; t < many; t += 4 * apart) {
+                Quarter<TX> x[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) fetch(q + u * STEP, x[u]);
+                for (int u = 0; u < 4; u++)
+                    if (t + u * apart < many) x[u] = fetch(from + u * step);
+                from += 4 * step;
 #pragma unroll
-            for (int u = 0; u < 4; u++) code(q + u * STEP, x[u]);
-        }
-        for (; q < all; q += STEP) {
-            float x[8];
-            fetch(q, x);
-            code(q, x);
+                for (int u = 0; u < 4; u++)
+                    if (t + u * apart < many) code(x[u]);
+            }
         }
         __syncthreads();
     }
@@ -209,15 +215,15 @@ static void start_few(Ctx* c, const FewArgs& a, int64_t rows) {
 
 // 16-row blocks a workgroup: as many as leave a workgroup per CU, four for long rows
 // or many tokens alone (16 x 16384 rows of 16384: 29.8 us, with two 34.7; of 4096 9.0
-// and 8.3; 32 x 16384 of 4096 10.1 and 11.4).  Coding for a block, 16 waves from three
-// tokens on (8 x 4096 of 4096: 6.4 us, with 8 waves 7.2; 1 x 4096 4.6 and 4.4).
+// and 8.3; 32 x 16384 of 4096 10.1 and 11.4).  Coding long rows for a block, 16 waves
+// (1 x 1024 of 16384: 8.3 us, with 8 waves 8.9; 4 x 4096 of 4096 5.1 and 4.9).
 template <typename TI, int MT>
 static int launch_few(Ctx* c, const FewArgs& a) {
     constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
     const int64_t rows = ceil_div(a.p.n, 16);
     if (MT < 4 && rows >= 4 * c->num_cus && (MT == 2 || a.p.blocks >= 256)) start_few<TI, MT < 4 ? 4 : 2, MT>(c, a, rows);
     else if (rows >= 2 * c->num_cus) start_few<TI, 2, MT>(c, a, rows);
-    else if (!CODED && a.p.m > 2) start_few<TI, 1, MT, CODED ? 8 : 16>(c, a, rows);
+    else if (!CODED && a.p.blocks >= 256) start_few<TI, 1, MT, CODED ? 8 : 16>(c, a, rows);
     else start_few<TI, 1, MT>(c, a, rows);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
@@ -240,9 +246,9 @@ int launch_mx_few(Ctx* c, const Product& p) {
     return launch_few<Coded, 4>(c, a);
 }
 
-// Every workgroup codes all rows, 0.25 us for each 4096 elements (with one block of
-// rows a workgroup; 0.4 with several), where a launch of its own costs 2.2: 8 x 4096
-// of 4096 6.4 us against 6.7, 16 x 4096 8.6 and 7.1, 8 x 16384 12.7 and 11.0.
+// Every workgroup codes all rows, 0.15 us for each 4096 elements (with several blocks
+// of rows a workgroup 0.25), where a launch of its own costs 2.2: 8 x 4096 of 4096
+// 5.9 us against 6.7, 16 x 4096 7.9 and 7.1; 4 x 16384 9.2 and 10.6, 8 x 16384 11.0 and 11.0.
 bool mx_codes_few(const Ctx* c, const Product& p) {
     return p.m <= 16 && p.m * p.blocks <= (ceil_div(p.n, 16) >= 2 * c->num_cus ? 512 : 1024);
 }
