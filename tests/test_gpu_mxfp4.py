@@ -316,6 +316,41 @@ def test_linear(ctx, typ, m, n, k, pad, shift):
 
 
 @pytest.mark.parametrize("typ", TYPES, ids=NAME.get)
+@pytest.mark.parametrize("cols", [2, 5, 7, 8, 9, 12, 15, 39, 63, 71, 1001, 4095])
+def test_rows_that_start_anywhere(ctx, typ, cols):
+    """Rows of every remainder of 8, at every place of a 16-byte line, NaN before,
+    between and behind them: coded, read back and multiplied."""
+    say(f"rows of {cols} {NAME[typ]}")
+    rng = np.random.default_rng(cols)
+    size, b = np.dtype(RAW[typ]).itemsize, X.blocks(cols)
+    for rows, pad in ((11, 1), (3, 0), (1, 0), (70, 3)):
+        x = _round(_special(rng, rows, cols), typ)
+        x = np.where(np.isfinite(x), x, 0.0).astype(np.float32)
+        src = _rows_buffer(ctx, x, typ, cols + pad, size)
+        codes, scales = Guarded(ctx, rows * b * 16), Guarded(ctx, rows * b)
+        X.Quantize(ctx, typ, src.ptr, cols + pad, rows, cols, codes.ptr, scales.ptr)()
+        want_c, want_s = code_of(x)
+        same(scales.read(np.uint8, (rows, b), "scales"), want_s)
+        same(codes.read(np.uint8, (rows, b, 16), "codes"), want_c)
+        y = _rows_buffer(ctx, np.zeros((rows, cols), np.float32), typ, cols + pad, size)
+        X.Dequantize(ctx, codes.ptr, scales.ptr, rows, cols, typ, y.ptr, cols + pad)()
+        with np.errstate(over="ignore"):
+            want = value_of(want_c, want_s, cols).astype(np.float32)
+        assert np.array_equal(_unpad(y, rows, cols, typ, pad), _round(want, typ))
+        # the weight's rows as many, so that the outputs' have odd strides too
+        n = cols + 60
+        z = _round(rng.uniform(0.6, 1.9, (rows, cols)).astype(np.float32), typ)
+        src = _rows_buffer(ctx, z, typ, cols + pad, size)
+        w = _operand(rng, n, cols, 1)
+        lin = D.QuantizedLinear.from_mxfp4(ctx, *(D.DeviceBuffer.from_host(ctx, v) for v in w), n, cols)
+        y = _rows_buffer(ctx, np.zeros((rows, n), np.float32), typ, n + pad, size)
+        X.Linear(ctx, lin, typ, src.ptr, cols + pad, rows, typ, y.ptr, n + pad)()
+        exact = value_of(*code_of(z), cols) @ value_of(*w, cols).T
+        same(_unpad(y, rows, n, typ, pad), _round(exact.astype(np.float32), typ))
+        lin.close()
+
+
+@pytest.mark.parametrize("typ", TYPES, ids=NAME.get)
 @pytest.mark.parametrize("m", [1, 5, 16, 17, 70])
 def test_values_that_the_linear_multiplies(ctx, typ, m):
     """A weight with a one in each row gives the activation's values back: those of

@@ -20,6 +20,7 @@ namespace mx {
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef v4i v4i_any __attribute__((aligned(2)));  // in memory, of any alignment
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -72,19 +73,45 @@ struct alignas(16) Quarter {
     unsigned v[2 * sizeof(T)];
 };
 
-// 8 elements from `at` of a row of `cols`, zeros past its end.
-template <typename T, bool VEC>
-__device__ __forceinline__ Quarter<T> load_quarter(const T* row, int64_t at, int64_t cols) {
-    Quarter<T> q = {};
-    if (VEC) {
-        if (at < cols) q = *reinterpret_cast<const Quarter<T>*>(row + at);
-    } else {
-        T e[8];
+// Without its first n elements, zeros behind the others.
+template <typename T>
+__device__ __forceinline__ void drop(Quarter<T>& q, int n) {
+    constexpr int D = 2 * (int)sizeof(T);  // dwords
+    const auto move = [&](bool is, int by) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = at + i < cols ? row[at + i] : (T)0.0f;
-        __builtin_memcpy(&q, e, sizeof(q));
+        for (int i = 0; i < D; i++) q.v[i] = !is ? q.v[i] : i + by < D ? q.v[i + by] : 0u;
+    };
+    move(n & 8, D);
+    move(n & 4, D / 2);
+    move(n & 2, D / 4);
+    if constexpr (sizeof(T) == 4) {
+        move(n & 1, 1);
+    } else if (n & 1) {
+#pragma unroll
+        for (int i = 0; i < D; i++) q.v[i] = q.v[i] >> 16 | (i + 1 < D ? q.v[i + 1] << 16 : 0u);
     }
+}
+// 8 elements from `at` of a row of `cols` >= 8, zeros past its end, in two halves: at
+// the row's end its last 8 are loaded, and end_quarter, when they are there, drops those
+// before `at`.  So no lane's loads differ from the others', and several rows' are in
+// flight together (8 x 4095 coded for 4096 outputs 6.5 us, with a branch for the last
+// elements 9.3).  Global memory takes wide accesses of any alignment: 10482 x 2861 of
+// f32 coded and read back 50 us, element by element 128.  RAGGED: cols is no multiple
+// of 8.
+template <typename T>
+__device__ __forceinline__ Quarter<T> load_quarter(const T* row, int64_t at, int64_t cols) {
+    Quarter<T> q;
+    __builtin_memcpy(&q, row + (at < cols - 8 ? at : cols - 8), sizeof(q));
     return q;
+}
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void end_quarter(Quarter<T>& q, int64_t at, int64_t cols) {
+    const int64_t past = at - (cols - 8);
+    if (RAGGED) {
+        if (past > 0) drop(q, past < 8 ? (int)past : 8);
+    } else if (past >= 8) {
+        q = Quarter<T>{};
+    }
 }
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -170,10 +197,10 @@ int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* a, int64_t rows_a, uint8_t
 bool mx_takes_rows(const Ctx* c, const mx::Product& p);
 int launch_mx_product(Ctx* c, const mx::Product& p);
 // mxfp4_few.hip: m <= kFewRows; and the linear that codes its rows itself, where
-// mx_codes_few.
+// mx_codes_few(p, k).
 constexpr int kFewRows = 64;
 int launch_mx_few(Ctx* c, const mx::Product& p);
-bool mx_codes_few(const Ctx* c, const mx::Product& p);
+bool mx_codes_few(const Ctx* c, const mx::Product& p, int64_t k);
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const mx::Product& p);
 // The linear of a resident weight on float rows (mxfp4.hip).
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, mx::Product p);

@@ -22,7 +22,7 @@ struct CodeArgs {
 
 // A lane takes 8 elements of a block, so that loads, and the stores of codes,
 // are runs of a wave; the block's maximum goes over its 4 lanes.
-template <typename T, bool SLABS, bool VEC>
+template <typename T, bool SLABS, bool RAGGED>
 __global__ __launch_bounds__(256) void k_mx_code(CodeArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t b = (uint32_t)(t >> 2);
@@ -31,8 +31,18 @@ __global__ __launch_bounds__(256) void k_mx_code(CodeArgs a) {
     const int block = (int)(b - row * a.per_row), part = (int)threadIdx.x & 3;
     const int64_t at = (int64_t)block * 32 + part * 8;
     unsigned byte;
-    const unsigned code =
-        code_quarter<T>(load_quarter<T, VEC>(static_cast<const T*>(a.x) + (int64_t)row * a.stride, at, a.cols), byte);
+    const T* from = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
+    Quarter<T> x = {};
+    if (!RAGGED || a.cols >= 8) {
+        x = load_quarter<T>(from, at, a.cols);
+        end_quarter<T, RAGGED>(x, at, a.cols);
+    } else {
+        T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = at + i < a.cols ? from[at + i] : (T)0.0f;
+        __builtin_memcpy(&x, e, sizeof(x));
+    }
+    const unsigned code = code_quarter<T>(x, byte);
     if (block < a.blocks)
         reinterpret_cast<unsigned*>(a.codes)[((int64_t)row * a.blocks + block) * 4 + part] = code;
     if (part == 0) {
@@ -54,8 +64,11 @@ struct DecodeArgs {
 };
 
 // Each value is its code's times a power of two: exact in f32 but for what
-// passes its range, and rounded once to the output's type.
-template <typename T, bool VEC>
+// passes its range, and rounded once to the output's type.  STREAM: the stores go past
+// the L2's reuse (16384 x 8192 of bf16 coded and read back 130 -> 110 us, 8001 x 4001
+// 34 -> 28); not f32 rows that start anywhere, whose two stores a lane leave parts of
+// lines to each other (10482 x 2861 50 -> 70).
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t b = (uint32_t)(t >> 2);
@@ -79,15 +92,17 @@ __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; i++) asm("" : "+v"(x[i]));
     T* dst = static_cast<T*>(a.y) + (int64_t)row * a.stride + at;
-    if (VEC) {
+    if (at + 8 <= a.cols) {
         Chunk<T> v;
 #pragma unroll
         for (int i = 0; i < 8; i++) v.e[i] = from_f32<T>(x[i]);
-        // past the L2's reuse: 16384 x 8192 coded and read back 130 -> 110 us
         v4i w[sizeof(T) / 2];
         __builtin_memcpy(w, &v, sizeof(v));
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_nontemporal_store(w[i], reinterpret_cast<v4i*>(dst) + i);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            if (STREAM) __builtin_nontemporal_store(w[i], reinterpret_cast<v4i_any*>(dst) + i);
+            else reinterpret_cast<v4i_any*>(dst)[i] = w[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -122,7 +137,6 @@ template <typename T>
 static int code_rows(Ctx* c, const void* x, int64_t stride, int64_t rows, int64_t cols, uint8_t* codes,
                      uint8_t* scales, bool slabs) {
     const int64_t blocks = blocks_of(cols), per_row = slabs ? slabs_of(cols) * 8 : blocks;
-    const bool vec = cols % 8 == 0 && aligned(x, 16) && stride * (int64_t)sizeof(T) % 16 == 0;
     const int64_t step = kLaunchBlocks / per_row;
     for (int64_t r = 0; r < rows; r += step) {
         CodeArgs a;
@@ -138,10 +152,10 @@ static int code_rows(Ctx* c, const void* x, int64_t stride, int64_t rows, int64_
         a.div = fast_div((uint32_t)per_row);
         const unsigned grid = (unsigned)ceil_div(a.rows * per_row * 4, 256);
         if (slabs) {
-            if (vec) k_mx_code<T, true, true><<<grid, 256, 0, c->stream>>>(a);
+            if (cols % 8) k_mx_code<T, true, true><<<grid, 256, 0, c->stream>>>(a);
             else k_mx_code<T, true, false><<<grid, 256, 0, c->stream>>>(a);
         } else {
-            if (vec) k_mx_code<T, false, true><<<grid, 256, 0, c->stream>>>(a);
+            if (cols % 8) k_mx_code<T, false, true><<<grid, 256, 0, c->stream>>>(a);
             else k_mx_code<T, false, false><<<grid, 256, 0, c->stream>>>(a);
         }
         TKV_LAUNCH_CHECK();
@@ -153,7 +167,7 @@ template <typename T>
 static int decode_rows(Ctx* c, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y,
                        int64_t stride) {
     const int64_t blocks = blocks_of(cols), step = kLaunchBlocks / blocks;
-    const bool vec = cols % 8 == 0 && aligned(y, 16) && stride * (int64_t)sizeof(T) % 16 == 0;
+    const bool past = sizeof(T) == 2 || (aligned(y, 16) && stride * (int64_t)sizeof(T) % 16 == 0);
     for (int64_t r = 0; r < rows; r += step) {
         DecodeArgs a;
         a.codes = codes + r * blocks * 16;
@@ -165,7 +179,7 @@ static int decode_rows(Ctx* c, const uint8_t* codes, const uint8_t* scales, int6
         a.blocks = (int32_t)blocks;
         a.div = fast_div((uint32_t)blocks);
         const unsigned grid = (unsigned)ceil_div(a.rows * blocks * 4, 256);
-        if (vec) k_mx_decode<T, true><<<grid, 256, 0, c->stream>>>(a);
+        if (past) k_mx_decode<T, true><<<grid, 256, 0, c->stream>>>(a);
         else k_mx_decode<T, false><<<grid, 256, 0, c->stream>>>(a);
         TKV_LAUNCH_CHECK();
     }
@@ -209,7 +223,7 @@ static int room(Ctx* c, int slot, size_t bytes, void** out) {
 }
 
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
-    if (mx_codes_few(c, p)) return launch_mx_few_linear(c, type, x, stride, k, p);
+    if (mx_codes_few(c, p, k)) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
     TKV_RC_TRY(room(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
     TKV_RC_TRY(room(c, 1, slab_bytes(p.m, k), &slabs));

@@ -21,7 +21,6 @@ struct FewArgs {
     Product p;
     const void* x;  // the linear's rows
     int64_t stride, k;
-    int32_t vec;    // rows of 16 bytes
     FastDiv quarters;  // of a row, as slabs have them
 };
 
@@ -120,35 +119,43 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         const int per = (int)a.quarters.d, apart = per < THREADS ? THREADS / per : 1;
         const int first = per < THREADS ? (int)div_by(a.quarters, threadIdx.x) : 0;
         const int many = first < apart ? (int)p.m : 0;
-        for (int c = (int)threadIdx.x - first * per; c < per; c += THREADS) {  // (whole blocks: four lanes stay together)
-            const TX* from = static_cast<const TX*>(a.x) + (int64_t)first * a.stride;
-            uint8_t* to = lds + (uint32_t)first * coded_bytes(p.blocks) + c * 4;
-            uint8_t* scale = scales + (uint32_t)first * scale_bytes(p.blocks) + (c >> 2);
-            const int64_t step = (int64_t)apart * a.stride;
-            const uint32_t to_step = (uint32_t)apart * coded_bytes(p.blocks), scale_step = (uint32_t)apart * scale_bytes(p.blocks);
-            const bool there = c < p.blocks * 4;
-            const auto fetch = [&](const TX* row) {
-                return a.vec ? load_quarter<TX, true>(row, (int64_t)c * 8, a.k) : load_quarter<TX, false>(row, (int64_t)c * 8, a.k);
-            };
-            const auto code = [&](const Quarter<TX>& x) {
-                unsigned byte;
-                const unsigned w = code_quarter<TX>(x, byte);
-                if (there) *reinterpret_cast<unsigned*>(to) = w;
-                if ((c & 3) == 0) *scale = (uint8_t)byte;
-                to += to_step;
-                scale += scale_step;
-            };
-            for (int t = first; t < many; t += 4 * apart) {
-                Quarter<TX> x[4];
+        const auto code_tokens = [&](auto ragged, auto batch) {
+            constexpr bool RAGGED = decltype(ragged)::value;
+            constexpr int B = decltype(batch)::value;  // tokens in flight
+            for (int c = (int)threadIdx.x - first * per; c < per; c += THREADS) {  // (whole blocks: four lanes stay together)
+                const TX* from = static_cast<const TX*>(a.x) + (int64_t)first * a.stride;
+                uint8_t* to = lds + (uint32_t)first * coded_bytes(p.blocks) + c * 4;
+                uint8_t* scale = scales + (uint32_t)first * scale_bytes(p.blocks) + (c >> 2);
+                const int64_t step = (int64_t)apart * a.stride, at = (int64_t)c * 8;
+                const uint32_t to_step = (uint32_t)apart * coded_bytes(p.blocks);
+                const uint32_t scale_step = (uint32_t)apart * scale_bytes(p.blocks);
+                for (int t = first; t < many; t += B * apart) {
+                    Quarter<TX> x[B];  // (of tokens past the last: the first again)
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (t + u * apart < many) x[u] = fetch(from + u * step);
-                from += 4 * step;
+                    for (int u = 0; u < B; u++) {
+                        const int v = t + u * apart < many ? u : 0;
+                        x[u] = load_quarter<TX>(from + v * step, at, a.k);
+                    }
+                    from += B * step;
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (t + u * apart < many) code(x[u]);
+                    for (int u = 0; u < B; u++) {
+                        if (t + u * apart >= many) break;
+                        end_quarter<TX, RAGGED>(x[u], at, a.k);
+                        unsigned byte;
+                        const unsigned code = code_quarter<TX>(x[u], byte);
+                        if (c < p.blocks * 4) *reinterpret_cast<unsigned*>(to) = code;
+                        if ((c & 3) == 0) *scale = (uint8_t)byte;
+                        to += to_step;
+                        scale += scale_step;
+                    }
+                }
             }
-        }
+        };
+        using One = std::integral_constant<int, 1>;
+        using Four = std::integral_constant<int, 4>;
+        if (a.k & 7) code_tokens(std::true_type{}, Four{});
+        else if (p.m == 1) code_tokens(std::false_type{}, One{});
+        else code_tokens(std::false_type{}, Four{});
         __syncthreads();
     }
     for (int s0 = wave; s0 < slabs; s0 += DEPTH * WAVES) {
@@ -249,8 +256,8 @@ int launch_mx_few(Ctx* c, const Product& p) {
 // Every workgroup codes all rows, 0.15 us for each 4096 elements (with several blocks
 // of rows a workgroup 0.25), where a launch of its own costs 2.2: 8 x 4096 of 4096
 // 5.9 us against 6.7, 16 x 4096 7.9 and 7.1; 4 x 16384 9.2 and 10.6, 8 x 16384 11.0 and 11.0.
-bool mx_codes_few(const Ctx* c, const Product& p) {
-    return p.m <= 16 && p.m * p.blocks <= (ceil_div(p.n, 16) >= 2 * c->num_cus ? 512 : 1024);
+bool mx_codes_few(const Ctx* c, const Product& p, int64_t k) {
+    return k >= 8 && p.m <= 16 && p.m * p.blocks <= (ceil_div(p.n, 16) >= 2 * c->num_cus ? 512 : 1024);
 }
 
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const Product& p) {
@@ -259,7 +266,6 @@ int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_
     a.x = x;
     a.stride = stride;
     a.k = k;
-    a.vec = k % 8 == 0 && aligned(x, 16) && stride * type_bytes(type) % 16 == 0;
     a.quarters = fast_div((uint32_t)slabs_of(k) * 32);
     if (type == TKV_HIP_F32) return launch_few<float, 1>(c, a);
     if (type == TKV_HIP_F16) return launch_few<_Float16, 1>(c, a);

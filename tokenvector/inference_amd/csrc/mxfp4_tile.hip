@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     constexpr int LANES = TN * 32 * (int)sizeof(TO) / 16, STEP = 64 / LANES, E = 16 / (int)sizeof(TO);
     const int64_t n = nw + (lane % LANES) * E;
     const int64_t left = p.n - n;  // outputs from n on
-    const bool whole = vec && m0 + BM <= p.m && n0 + BN <= p.n;
+    const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
 #pragma unroll
@@ -283,11 +283,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
             TO* at = static_cast<TO*>(p.y) + (mw + i * 32 + lane / LANES) * p.ldy + n;
 #pragma unroll
             for (int t = 0; t < 32 / STEP; t++) {
-                v4i* to = reinterpret_cast<v4i*>(at + t * STEP * p.ldy);
+                v4i_any* to = reinterpret_cast<v4i_any*>(at + t * STEP * p.ldy);
                 // past the L2's reuse, which the operands need more (8192 x 2304 of 768
-                // 31.9 -> 28.9 us, 8192 x 8192 of 8192 255 -> 247); small outputs lose
-                // by it
-                if constexpr (TM * TN > 1) __builtin_nontemporal_store(v[t], to);
+                // 31.9 -> 28.9 us, 8192 x 8192 of 8192 255 -> 247); small outputs and
+                // parts of lines lose by it (1000 x 12001 of 1001 21.5 -> 27.8)
+                if (TM * TN > 1 && vec) __builtin_nontemporal_store(v[t], to);
                 else *to = v[t];
             }
         } else {
@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
                 const v4i v = *reinterpret_cast<const v4i*>(own + t * ROW + (lane % LANES) * 16);
                 TO* at = static_cast<TO*>(p.y) + m * p.ldy + n;
                 if (m >= p.m || left <= 0) continue;
-                if (vec && left >= E) {
-                    *reinterpret_cast<v4i*>(at) = v;
+                if (left >= E) {
+                    __builtin_memcpy(at, &v, 16);  // (of any alignment)
                 } else {
                     TO e[E];
                     __builtin_memcpy(e, &v, 16);
