@@ -454,6 +454,60 @@ def test_captured_and_replayed(ctx, m):
     own.close()
 
 
+LONG = [(1, 16, 16384), (1, 384, 15808), (6, 721, 15969), (7, 384, 12736), (12, 960, 9600), (16, 40, 8193),
+        (17, 130, 16352), (33, 200, 9000), (64, 640, 16000), (64, 16, 131040)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+def test_long_rows_of_few_outputs(ctx, m, n, k):
+    """Sums over parts of K, joined: exact, the same in every call, beside attention
+    that counts its own arrivals, and in graphs that take turns."""
+    say(f"long rows {m}x{n}x{k}")
+    rng = np.random.default_rng(m + n + k)
+    a, w = _operand(rng, m, k, 1), _operand(rng, n, k, 1)
+    exact = (value_of(*a, k) @ value_of(*w, k).T).astype(np.float32)
+    for out in (A.F32, A.BF16):
+        same(_product(ctx, a, w, m, n, k, out, pad=3), _round(exact, out))
+    own = D.Context(0)
+    dw, ds = (D.DeviceBuffer.from_host(own, v) for v in w)
+    lin = D.QuantizedLinear.from_mxfp4(own, dw, ds, n, k)
+    rows = [m, max(1, m // 2)]
+    x = D.DeviceBuffer.empty(own, (m, k), np.float32)
+    ys = [D.DeviceBuffer.empty(own, (r, n), np.float32) for r in rows]
+    calls = [X.Linear(own, lin, A.F32, x, k, r, A.F32, y) for r, y in zip(rows, ys)]
+    # one query of four heads over 3000 keys, whose splits are joined the same way
+    q, kv, o = (D.DeviceBuffer.from_host(own, rng.standard_normal(s).astype(np.float32))
+                for s in ((1, 4, 64), (3000, 2, 64), (1, 4, 64)))
+    ends = [D.DeviceBuffer.from_host(own, np.array([0, t], np.int32)) for t in (1, 3000)]
+    heads = [A.Rows(t, t.shape[1] * 64, 64) for t in (q, kv, kv, o)]
+    attend = A.AttentionPrompt(own, A.F32, 1, 4, 2, 64, 1, *heads, ends[0], ends[1], 3000)
+    for call in (*calls, attend):
+        call()
+    first = o.download()
+    graphs = []
+    for call in calls:
+        with D.Graph(own) as g:
+            call()
+        graphs.append(g)
+    for turn in range(3):
+        xs = (rng.uniform(0.6, 1.9, (m, k)) * rng.choice([-1.0, 1.0], (m, k))).astype(np.float32)
+        x.upload(xs)
+        exact = (value_of(*code_of(xs), k) @ value_of(*w, k).T).astype(np.float32)
+        for y, call, g in zip(ys, calls, graphs):
+            for go in (g.launch, call, g.launch):
+                D.memset(own, y, 0, y.nbytes)
+                go()
+                attend()
+                assert np.array_equal(y.download(), exact[:y.shape[0]]), turn
+        assert np.array_equal(o.download(), first)
+    for g in graphs:
+        g.close()
+    lin.close()
+    for b in (dw, ds, x, *ys, q, kv, o, *ends):
+        b.close()
+    own.close()
+
+
 def test_two_contexts_at_once(ctx):
     """Each has its own stream and workspaces; one weight."""
     rng = np.random.default_rng(11)

@@ -184,6 +184,9 @@ __device__ __forceinline__ v2i row_scales(const uint8_t* row, int s, int blocks)
 
 }  // namespace mx
 
+// A workspace; hipMalloc's error is taken off, or the next launch's check would
+// report it.
+int mx_room(Ctx* c, int slot, size_t bytes, void** out);
 // mxfp4.hip.  x: rows of `cols` elements of `type`, `stride` elements apart.
 // Scales to [rows][blocks], or to slabs.
 int launch_mx_quantize(Ctx* c, int type, const void* x, int64_t stride, int64_t rows, int64_t cols,

@@ -214,9 +214,7 @@ int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_
     return TKV_HIP_OK;
 }
 
-// A workspace; hipMalloc's error is taken off, or the next launch's check would
-// report it.
-static int room(Ctx* c, int slot, size_t bytes, void** out) {
+int mx_room(Ctx* c, int slot, size_t bytes, void** out) {
     const int rc = ctx_workspace(c, slot, bytes, out);
     if (rc == TKV_HIP_OOM) (void)hipGetLastError();
     return rc;
@@ -225,8 +223,8 @@ static int room(Ctx* c, int slot, size_t bytes, void** out) {
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
     if (mx_codes_few(c, p, k)) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
-    TKV_RC_TRY(room(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
-    TKV_RC_TRY(room(c, 1, slab_bytes(p.m, k), &slabs));
+    TKV_RC_TRY(mx_room(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
+    TKV_RC_TRY(mx_room(c, 1, slab_bytes(p.m, k), &slabs));
     TKV_RC_TRY(launch_mx_quantize(c, type, x, stride, p.m, k, static_cast<uint8_t*>(codes),
                                   static_cast<uint8_t*>(slabs), true));
     p.a = static_cast<uint8_t*>(codes);
@@ -301,8 +299,8 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
     p.y_type = type_out;
     if (!mx_takes_rows(c, p)) {
         void *as, *ws;
-        TKV_RC_TRY(room(c, 1, slab_bytes(m, k), &as));
-        TKV_RC_TRY(room(c, 2, slab_bytes(n, k), &ws));
+        TKV_RC_TRY(mx_room(c, 1, slab_bytes(m, k), &as));
+        TKV_RC_TRY(mx_room(c, 2, slab_bytes(n, k), &ws));
         TKV_RC_TRY(launch_mx_slabs(c, k, a_scales, m, static_cast<uint8_t*>(as), w_scales, n, static_cast<uint8_t*>(ws)));
         p.as = static_cast<uint8_t*>(as);
         p.ws = static_cast<uint8_t*>(ws);

@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "mxfp4.h"
+#include "tkv_reduce.h"
 
 namespace tkv {
 namespace mx {
@@ -21,17 +22,25 @@ struct FewArgs {
     Product p;
     const void* x;  // the linear's rows
     int64_t stride, k;
-    FastDiv quarters;  // of a row, as slabs have them
+    int32_t slabs;     // of a workgroup, at most
+    FastDiv quarters;  // of those
+    // split over K: the sums [row blocks][splits][tokens / 16][64 lanes] of v4f, and
+    // an arrival count a row block
+    int32_t splits;
+    unsigned long long* sums;
+    unsigned* arrivals;
 };
 
 // Bytes of a coded token in LDS, and of its scales.
 __host__ __device__ __forceinline__ uint32_t coded_bytes(uint32_t blocks) { return blocks * 16u + 16u; }
 __host__ __device__ __forceinline__ uint32_t scale_bytes(uint32_t blocks) { return ((blocks + 7) >> 3) * 8u; }
 
+constexpr int kFewSplits = 8;
+
 struct Coded {};      // the tokens come as codes and slabs,
 struct CodedRows {};  // or the scales of both as [rows][blocks]
 
-template <typename TI, int NR, int MT, int WAVES>
+template <typename TI, int NR, int MT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     constexpr bool ROWS = std::is_same<TI, CodedRows>::value, CODED = ROWS || std::is_same<TI, Coded>::value;
     typedef typename std::conditional<CODED, float, TI>::type TX;
@@ -42,7 +51,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     const int64_t n0 = wide_block() * (16 * NR);
     if (n0 >= p.n) return;
     const uint32_t row_bytes = (uint32_t)p.blocks * 16u;
-    const int slabs = (p.blocks + 7) >> 3;
+    const int all = (p.blocks + 7) >> 3;
+    const int begin = SPLIT ? (int)blockIdx.z * a.slabs : 0, slabs = SPLIT ? min(all, begin + a.slabs) : all;
+    const uint32_t blocks = (uint32_t)(SPLIT ? min(p.blocks, slabs * 8) - begin * 8 : p.blocks);  // of this workgroup
 
     // rows past the weight's, and tokens past m, read the last one
     const uint8_t* w_row[NR];
@@ -64,15 +75,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         v2i s[MT];
     };
     // chunks past the row: its last, whose scales are 2^-127
-    const auto place = [&](int s, int h) {
+    const auto place = [&](int s, int h, uint32_t bytes) {
         const uint32_t at = (uint32_t)s * 128u + (uint32_t)(h * 64 + g * 16);
-        return at < row_bytes ? at : row_bytes - 16;
+        return at < bytes ? at : bytes - 16;
     };
     const auto load_weight = [&](int s, Weights& b) {
 #pragma unroll
         for (int r = 0; r < NR; r++) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) b.w[r][h] = *reinterpret_cast<const v4i*>(w_row[r] + place(s, h));
+            for (int h = 0; h < 2; h++) b.w[r][h] = *reinterpret_cast<const v4i*>(w_row[r] + place(s, h, row_bytes));
             if constexpr (ROWS) {
                 const int64_t row = n0 + r * 16 + l16;
                 b.s[r] = row_scales(p.ws + (row < p.n ? row : p.n - 1) * p.blocks, s, p.blocks);
@@ -81,15 +92,16 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
             }
         }
     };
-    uint8_t* const scales = lds + (uint32_t)p.m * coded_bytes(p.blocks);  // of the tokens coded here
+    uint8_t* const scales = lds + (uint32_t)p.m * coded_bytes(blocks);  // of the tokens coded here
     const auto load_tokens = [&](int s, Tokens& b) {
 #pragma unroll
         for (int t = 0; t < MT; t++) {
-            const uint8_t* row = CODED ? p.a + (uint64_t)token[t] * row_bytes : lds + (uint32_t)token[t] * coded_bytes(p.blocks);
+            const uint8_t* row = CODED ? p.a + (uint64_t)token[t] * row_bytes : lds + (uint32_t)token[t] * coded_bytes(blocks);
 #pragma unroll
-            for (int h = 0; h < 2; h++) b.t[t][h] = *reinterpret_cast<const v4i*>(row + place(s, h));
+            for (int h = 0; h < 2; h++)
+                b.t[t][h] = *reinterpret_cast<const v4i*>(row + (CODED ? place(s, h, row_bytes) : place(s - begin, h, blocks * 16)));
             if constexpr (!CODED)
-                b.s[t] = *reinterpret_cast<const v2i*>(scales + (uint32_t)token[t] * scale_bytes(p.blocks) + s * 8);
+                b.s[t] = *reinterpret_cast<const v2i*>(scales + (uint32_t)token[t] * scale_bytes(blocks) + (s - begin) * 8);
             else if constexpr (ROWS)
                 b.s[t] = row_scales(p.as + (int64_t)token[t] * p.blocks, s, p.blocks);
             else
@@ -108,9 +120,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     Tokens tokens[DEPTH];
 #pragma unroll
     for (int u = 0; u < DEPTH; u++)
-        if (wave + u * WAVES < slabs) {
-            load_weight(wave + u * WAVES, weights[u]);
-            if constexpr (CODED) load_tokens(wave + u * WAVES, tokens[u]);
+        if (begin + wave + u * WAVES < slabs) {
+            load_weight(begin + wave + u * WAVES, weights[u]);
+            if constexpr (CODED) load_tokens(begin + wave + u * WAVES, tokens[u]);
         }
     if constexpr (!CODED) {
         // a thread takes one quarter of a block of every token, or of every `apart`-th
@@ -118,17 +130,17 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         constexpr int THREADS = WAVES * 64;
         const int per = (int)a.quarters.d, apart = per < THREADS ? THREADS / per : 1;
         const int first = per < THREADS ? (int)div_by(a.quarters, threadIdx.x) : 0;
-        const int many = first < apart ? (int)p.m : 0;
+        const int many = first < apart ? (int)p.m : 0, quarters = (slabs - begin) * 32;
         const auto code_tokens = [&](auto ragged, auto batch) {
             constexpr bool RAGGED = decltype(ragged)::value;
             constexpr int B = decltype(batch)::value;  // tokens in flight
-            for (int c = (int)threadIdx.x - first * per; c < per; c += THREADS) {  // (whole blocks: four lanes stay together)
+            for (int c = (int)threadIdx.x - first * per; c < quarters; c += THREADS) {  // (whole blocks: four lanes stay together)
                 const TX* from = static_cast<const TX*>(a.x) + (int64_t)first * a.stride;
-                uint8_t* to = lds + (uint32_t)first * coded_bytes(p.blocks) + c * 4;
-                uint8_t* scale = scales + (uint32_t)first * scale_bytes(p.blocks) + (c >> 2);
-                const int64_t step = (int64_t)apart * a.stride, at = (int64_t)c * 8;
-                const uint32_t to_step = (uint32_t)apart * coded_bytes(p.blocks);
-                const uint32_t scale_step = (uint32_t)apart * scale_bytes(p.blocks);
+                uint8_t* to = lds + (uint32_t)first * coded_bytes(blocks) + c * 4;
+                uint8_t* scale = scales + (uint32_t)first * scale_bytes(blocks) + (c >> 2);
+                const int64_t step = (int64_t)apart * a.stride, at = ((int64_t)begin * 32 + c) * 8;
+                const uint32_t to_step = (uint32_t)apart * coded_bytes(blocks);
+                const uint32_t scale_step = (uint32_t)apart * scale_bytes(blocks);
                 for (int t = first; t < many; t += B * apart) {
                     Quarter<TX> x[B];  // (of tokens past the last: the first again)
 #pragma unroll
@@ -143,7 +155,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
                         end_quarter<TX, RAGGED>(x[u], at, a.k);
                         unsigned byte;
                         const unsigned code = code_quarter<TX>(x[u], byte);
-                        if (c < p.blocks * 4) *reinterpret_cast<unsigned*>(to) = code;
+                        if (c < (int)blocks * 4) *reinterpret_cast<unsigned*>(to) = code;
                         if ((c & 3) == 0) *scale = (uint8_t)byte;
                         to += to_step;
                         scale += scale_step;
@@ -158,7 +170,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
         else code_tokens(std::false_type{}, Four{});
         __syncthreads();
     }
-    for (int s0 = wave; s0 < slabs; s0 += DEPTH * WAVES) {
+    for (int s0 = begin + wave; s0 < slabs; s0 += DEPTH * WAVES) {
 #pragma unroll
         for (int u = 0; u < DEPTH; u++) {
             const int s = s0 + u * WAVES, then = s + DEPTH * WAVES;
@@ -194,10 +206,45 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
 #pragma unroll
         for (int t = 0; t < MT; t++) part[(wave * NR * MT + r * MT + t) * 64 + lane] = acc[r][t];
     __syncthreads();
-    for (int i = wave; i < NR * MT; i += WAVES) {
+    const auto join = [&](int i) {
         v4f sum = part[i * 64 + lane];
 #pragma unroll
         for (int w = 1; w < WAVES; w++) sum += part[(w * NR * MT + i) * 64 + lane];
+        return sum;
+    };
+    // the row block's last workgroup adds the splits' sums in their order
+    unsigned long long* const sums = SPLIT ? a.sums + (n0 / 16 * a.splits * MT * 64 + lane) * 2 : nullptr;
+    if constexpr (SPLIT) {
+        for (int i = wave; i < MT; i += WAVES) {
+            const v4f sum = join(i);
+            unsigned long long two[2];
+            __builtin_memcpy(two, &sum, 16);
+            for (int e = 0; e < 2; e++)
+                __hip_atomic_store(sums + ((int)blockIdx.z * MT + i) * 128 + e, two[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        unsigned* const count = a.arrivals + n0 / 16;
+        if (!arrive_last(count, (unsigned)a.splits)) return;
+        arrive_clear(count, (unsigned)a.splits);
+    }
+    for (int i = wave; i < NR * MT; i += WAVES) {
+        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (SPLIT) {
+            v4f v[kFewSplits];  // (all on their way at once)
+#pragma unroll
+            for (int z = 0; z < kFewSplits; z++) {
+                const int have = z < a.splits ? z : 0;
+                unsigned long long two[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    two[e] = __hip_atomic_load(sums + (have * MT + i) * 128 + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __builtin_memcpy(&v[z], two, 16);
+            }
+#pragma unroll
+            for (int z = 0; z < kFewSplits; z++)
+                if (z < a.splits) sum += v[z];
+        } else {
+            sum = join(i);
+        }
         const int64_t tok = (i % MT) * 16 + l16, n = n0 + (i / MT) * 16 + g * 4;
         if (tok >= p.m) continue;
 #pragma unroll
@@ -212,26 +259,60 @@ __global__ __launch_bounds__(WAVES * 64) void k_mx_few(FewArgs a) {
     }
 }
 
-template <typename TI, int NR, int MT, int WAVES = 8>
-static void start_few(Ctx* c, const FewArgs& a, int64_t rows) {
+template <typename TI, int NR, int MT, int WAVES = 8, bool SPLIT = false>
+static void start_few(Ctx* c, FewArgs& a, int64_t rows) {
     constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
+    const int64_t slabs = ceil_div(a.p.blocks, 8);
+    a.slabs = (int32_t)ceil_div(slabs, a.splits);
+    a.splits = (int32_t)ceil_div(slabs, a.slabs);
+    a.quarters = fast_div((uint32_t)a.slabs * 32);
     const uint32_t sums = WAVES * NR * MT * 1024;
-    const uint32_t codes = CODED ? 0 : (uint32_t)a.p.m * (coded_bytes(a.p.blocks) + scale_bytes(a.p.blocks));
-    k_mx_few<TI, NR, MT, WAVES><<<wide_grid(ceil_div(rows, NR)), WAVES * 64, sums > codes ? sums : codes, c->stream>>>(a);
+    const uint32_t blocks = (uint32_t)(a.p.blocks < a.slabs * 8 ? a.p.blocks : a.slabs * 8);
+    const uint32_t codes = CODED ? 0 : (uint32_t)a.p.m * (coded_bytes(blocks) + scale_bytes(blocks));
+    dim3 grid = wide_grid(ceil_div(rows, NR));
+    grid.z = (unsigned)a.splits;
+    k_mx_few<TI, NR, MT, WAVES, SPLIT><<<grid, WAVES * 64, sums > codes ? sums : codes, c->stream>>>(a);
+}
+
+// Workgroups of a row block.  A CU's loads in flight bound what it reads (0.08 us for
+// 256 elements of 16 rows, as long again for each 16 tokens more, and a row coded on the
+// way as long for 70 blocks), so long rows of few outputs are split over the idle CUs,
+// eight slabs each at least; the join costs 1.9 us.  1 x 1024 of 16384: 6.9 us, by one
+// workgroup 8.9; 64 x 1024 of 8192 8.5 and 13.5; 12 x 960 of 9600, coded before, 6.0 and
+// 6.3; in two 4 x 2048 of 8192 7.3 and 7.1.
+static int few_splits(const Ctx* c, const Product& p, bool coded) {
+    const int64_t rows = ceil_div(p.n, 16), slabs = ceil_div(p.blocks, 8);
+    int64_t s = slabs / 8 < c->num_cus / rows ? slabs / 8 : c->num_cus / rows;
+    if (s > kFewSplits) s = kFewSplits;
+    const int64_t work = slabs * ceil_div(p.m, 16) + (coded ? 0 : p.m * p.blocks / 70);
+    return s > 1 && c->attn_arrivals && work * (s - 1) >= 27 * s ? (int)s : 1;
 }
 
 // 16-row blocks a workgroup: as many as leave a workgroup per CU, four for long rows
 // or many tokens alone (16 x 16384 rows of 16384: 29.8 us, with two 34.7; of 4096 9.0
 // and 8.3; 32 x 16384 of 4096 10.1 and 11.4).  Coding long rows for a block, 16 waves
-// (1 x 1024 of 16384: 8.3 us, with 8 waves 8.9; 4 x 4096 of 4096 5.1 and 4.9).
+// (4 x 2048 of 8192: 7.1 us, with 8 waves 8.0; 4 x 4096 of 4096 5.1 and 4.9).
 template <typename TI, int MT>
-static int launch_few(Ctx* c, const FewArgs& a) {
+static int launch_few(Ctx* c, FewArgs& a) {
     constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
+    constexpr bool WIDE = CODED || MT == 1;  // mx_codes_few has one block and 8 waves else
     const int64_t rows = ceil_div(a.p.n, 16);
-    if (MT < 4 && rows >= 4 * c->num_cus && (MT == 2 || a.p.blocks >= 256)) start_few<TI, MT < 4 ? 4 : 2, MT>(c, a, rows);
-    else if (rows >= 2 * c->num_cus) start_few<TI, 2, MT>(c, a, rows);
-    else if (!CODED && a.p.blocks >= 256) start_few<TI, 1, MT, CODED ? 8 : 16>(c, a, rows);
-    else start_few<TI, 1, MT>(c, a, rows);
+    a.splits = few_splits(c, a.p, CODED);
+    if (a.splits > 1) {
+        void* ws;
+        TKV_RC_TRY(mx_room(c, 16, (size_t)(rows * a.splits * MT * 1024), &ws));
+        a.sums = static_cast<unsigned long long*>(ws);
+        a.arrivals = c->attn_arrivals;
+        start_few<TI, 1, MT, 8, true>(c, a, rows);
+    } else if (WIDE && MT < 4 && rows >= 4 * c->num_cus && (MT == 2 || a.p.blocks >= 256)) {
+        start_few<TI, WIDE && MT < 4 ? 4 : 1, MT>(c, a, rows);
+    } else if (WIDE && rows >= 2 * c->num_cus) {
+        start_few<TI, WIDE ? 2 : 1, MT>(c, a, rows);
+    } else if (WIDE && !CODED && a.p.blocks >= 256) {
+        start_few<TI, 1, MT, WIDE && !CODED ? 16 : 8>(c, a, rows);
+    } else {
+        start_few<TI, 1, MT>(c, a, rows);
+    }
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
@@ -253,11 +334,25 @@ int launch_mx_few(Ctx* c, const Product& p) {
     return launch_few<Coded, 4>(c, a);
 }
 
-// Every workgroup codes all rows, 0.15 us for each 4096 elements (with several blocks
-// of rows a workgroup 0.25), where a launch of its own costs 2.2: 8 x 4096 of 4096
-// 5.9 us against 6.7, 16 x 4096 7.9 and 7.1; 4 x 16384 9.2 and 10.6, 8 x 16384 11.0 and 11.0.
+// Every workgroup codes all rows (its part of them), 0.15 us for each 4096 elements
+// (with several blocks of rows a workgroup 0.25), where a launch of its own costs 2.2 and
+// more: 8 x 4096 of 4096 5.9 us against 6.7, 16 x 4096 7.9 and 7.1; 4 x 16384 9.2 and
+// 10.6, 8 x 16384 11.0 and 11.0; one call after another, where two launches are 7.4 at least, 32 x 512 of 768 5.3 and 7.4, 12 x 4096
+// of 4096 7.0 and 7.7, 24 x 7000 of 1300 8.5 and 7.5.
 bool mx_codes_few(const Ctx* c, const Product& p, int64_t k) {
-    return k >= 8 && p.m <= 16 && p.m * p.blocks <= (ceil_div(p.n, 16) >= 2 * c->num_cus ? 512 : 1024);
+    const int64_t rows = ceil_div(p.n, 16);
+    if (k < 8 || p.m > (rows >= 2 * c->num_cus ? 16 : kFewRows)) return false;
+    // (CUs with two workgroups code twice)
+    const bool twice = rows >= 2 * c->num_cus || (p.m > 16 && rows > c->num_cus);
+    const int64_t most = twice ? 512 : rows > c->num_cus || k % 8 ? 1024 : 1536;
+    return p.m * p.blocks <= most * few_splits(c, p, false);
+}
+
+template <typename T>
+static int launch_few_linear(Ctx* c, FewArgs& a) {
+    if (a.p.m <= 16) return launch_few<T, 1>(c, a);
+    if (a.p.m <= 32) return launch_few<T, 2>(c, a);
+    return launch_few<T, 4>(c, a);
 }
 
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const Product& p) {
@@ -266,10 +361,9 @@ int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_
     a.x = x;
     a.stride = stride;
     a.k = k;
-    a.quarters = fast_div((uint32_t)slabs_of(k) * 32);
-    if (type == TKV_HIP_F32) return launch_few<float, 1>(c, a);
-    if (type == TKV_HIP_F16) return launch_few<_Float16, 1>(c, a);
-    return launch_few<__bf16, 1>(c, a);
+    if (type == TKV_HIP_F32) return launch_few_linear<float>(c, a);
+    if (type == TKV_HIP_F16) return launch_few_linear<_Float16>(c, a);
+    return launch_few_linear<__bf16>(c, a);
 }
 
 }  // namespace tkv

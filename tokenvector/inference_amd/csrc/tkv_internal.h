@@ -104,7 +104,8 @@ struct Ctx {
     // grow-only workspaces
     // 10, 11: f16-decoded FP8 operands; 12: INT4 split-K partials (any kernel);
     // 13, 14, 15: INT4 digit planes, retiled weight codes, permuted activations
-    // 16: partial sums of the attention's splits over the keys
+    // 16: partial sums of the attention's splits over the keys, and of the 4-bit
+    // products' over K, which count their arrivals on attn_arrivals too
     static constexpr int kSlots = 17;
     void* ws[kSlots] = {};
     size_t ws_bytes[kSlots] = {};
