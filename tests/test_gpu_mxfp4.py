@@ -455,7 +455,8 @@ def test_captured_and_replayed(ctx, m):
 
 
 LONG = [(1, 16, 16384), (1, 384, 15808), (6, 721, 15969), (7, 384, 12736), (12, 960, 9600), (16, 40, 8193),
-        (17, 130, 16352), (33, 200, 9000), (64, 640, 16000), (64, 16, 131040)]
+        (17, 130, 16352), (33, 200, 9000), (64, 640, 16000), (64, 16, 131040),
+        (70, 64, 16384), (65, 33, 20001), (100, 640, 16000), (129, 300, 12001), (200, 1000, 9000), (256, 1030, 8192)]
 
 
 @pytest.mark.parametrize("m,n,k", LONG)

@@ -27,9 +27,12 @@
 // in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros).  (The
 // 16x16x128 form reaches 6.9, its sums moved half as often, but took the same time
 // here, with twice the scales to read.)
+#include <math.h>
+
 #include <type_traits>
 
 #include "mxfp4.h"
+#include "tkv_reduce.h"
 
 namespace tkv {
 namespace mx {
@@ -64,9 +67,18 @@ struct Tile {
     static constexpr int PER_CU = LDS * 4 <= 163840 ? 4 : LDS * 2 <= 163840 ? 2 : 1;
 };
 
-template <int TM, int TN, int STAGES, bool ROWS, typename TO>
+// K split over workgroups (blockIdx.z): their slices, sums [tiles][splits][256 lanes] of
+// 16 f32, and an arrival count a tile.
+struct Split {
+    int32_t slices, splits;
+    unsigned long long* sums;
+    unsigned* arrivals;
+};
+
+template <int TM, int TN, int STAGES, bool ROWS, bool SPLIT, typename TO>
 __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_mx_tile(Product p, int tiles_m,
-                                                                                      int tiles_n, int vec) {
+                                                                                      int tiles_n, int vec,
+                                                                                      Split split) {
     using T = Tile<TM, TN, STAGES, ROWS>;
     constexpr int BM = T::BM, BN = T::BN;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
@@ -93,7 +105,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     constexpr int SBYTES = T::SCALES / 4;  // of a wave
     constexpr int SWIDTH = SBYTES % 1024 == 0 ? 16 : 4, SCOPIES = ROWS ? 0 : (SBYTES + 64 * SWIDTH - 1) / (64 * SWIDTH);
     constexpr int ITEMS = COPIES + SCOPIES;
-    const int slices = (p.blocks + 7) >> 3;
+    const int all = (p.blocks + 7) >> 3, begin = SPLIT ? (int)blockIdx.z * split.slices : 0;
+    const int slices = SPLIT ? min(all, begin + split.slices) : all;  // from begin to here
     // (copies more than there are scales for copy the last again)
     const auto scale_place = [&](int d) {
         const int at = (d * 4 + wave) * 64 * SWIDTH;
@@ -146,9 +159,9 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
         if (k < TN) fw[set][k] = *reinterpret_cast<const v4i*>(stage + (rw + k * 32) * 128 + c);
         else fa[set][k - TN] = *reinterpret_cast<const v4i*>(stage + (ra + (k - TN) * 32) * 128 + c);
     };
-    const auto stage_of = [&](int slice) { return lds + (slice % STAGES) * T::STAGE; };
+    const auto stage_of = [&](int slice) { return lds + ((unsigned)slice % STAGES) * T::STAGE; };
     const auto read_scales = [&](int slice, int k) {
-        const uint8_t* at = ROWS ? lds + STAGES * T::STAGE + (slice < slices ? slice : 0) * T::SCALES
+        const uint8_t* at = ROWS ? lds + STAGES * T::STAGE + (slice < slices ? slice - begin : 0) * T::SCALES
                                  : stage_of(slice) + T::CODES;
         if (k < TN) sw[k] = *reinterpret_cast<const v2i*>(at + (rw + k * 32) * 8);
         else sa[k - TN] = *reinterpret_cast<const v2i*>(at + (ra + (k - TN) * 32) * 8);
@@ -196,9 +209,9 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
 #pragma unroll
     for (int t = 0; t < STAGES - 1; t++)
 #pragma unroll
-        for (int d = 0; d < ITEMS; d++) copy(t, stage_of(t), d);
+        for (int d = 0; d < ITEMS; d++) copy(begin + t, stage_of(begin + t), d);
 #pragma unroll
-    for (int d = 0; d < EARLY; d++) copy(STAGES - 1, stage_of(STAGES - 1), d);
+    for (int d = 0; d < EARLY; d++) copy(begin + STAGES - 1, stage_of(begin + STAGES - 1), d);
     if constexpr (ROWS) {
         // a thread loads a part of a row's, all of its loads in flight together
         constexpr int PARTS = 256 / (BM + BN) > 0 ? 256 / (BM + BN) : 1, OWN = kRowSlices / PARTS;
@@ -209,7 +222,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
         v2i part[OWN];
 #pragma unroll
         for (int h = 0; h < OWN; h++)
-            part[h] = row_scales(from, first + h, p.blocks);
+            part[h] = row_scales(from, begin + first + h, p.blocks);
 #pragma unroll
         for (int h = 0; h < OWN; h++)
             *reinterpret_cast<v2i*>(lds + STAGES * T::STAGE + (first + h) * T::SCALES + r * 8) = part[h];
@@ -217,11 +230,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     TKV_MX_COPIES_LEFT(ROWS ? 0 : (STAGES - 2) * ITEMS + EARLY);
     sync();
 #pragma unroll
-    for (int k = 0; k < F; k++) read_scales(0, k);
+    for (int k = 0; k < F; k++) read_scales(begin, k);
 #pragma unroll
-    for (int k = 0; k < F; k++) read(lds, 0, k);
+    for (int k = 0; k < F; k++) read(stage_of(begin), 0, k);
 #pragma unroll 1
-    for (int s = 0; s < slices; s++) {
+    for (int s = begin; s < slices; s++) {
         uint8_t *stage = stage_of(s), *next = stage_of(s + 1), *last = stage_of(s + STAGES - 1);
         shift_scales();
         multiply(I0{}, std::integral_constant<int, F + LATE>{}, [&](int k) {
@@ -240,6 +253,42 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     }
 #undef TKV_MX_COPIES_LEFT
     __builtin_amdgcn_s_waitcnt(0x0F70);
+
+    if constexpr (SPLIT) {  // the tile's last workgroup adds the splits' sums in their order
+        static_assert(TM * TN == 1, "a lane's 16 sums");
+        unsigned long long* const sums = split.sums + block * split.splits * 2048 + threadIdx.x;
+        const auto put = [&](int e) { return sums + ((int)blockIdx.z * 8 + e) * 256; };
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            __hip_atomic_store(put(e),
+                               (unsigned long long)__float_as_uint(acc[0][0][2 * e]) |
+                                   (unsigned long long)__float_as_uint(acc[0][0][2 * e + 1]) << 32,
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        unsigned* const count = split.arrivals + block;
+        if (!arrive_last(count, (unsigned)split.splits, *reinterpret_cast<int*>(lds))) return;
+        arrive_clear(count, (unsigned)split.splits);
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[0][0][r] = 0.0f;
+        for (int z0 = 0; z0 < split.splits; z0 += 4) {  // (four splits' on their way at once)
+            unsigned long long two[4][8];
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int from = z0 + z < split.splits ? z0 + z : z0;
+                    two[z][e] = __hip_atomic_load(sums + (from * 8 + e) * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                if (z0 + z >= split.splits) break;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    acc[0][0][2 * e] += __uint_as_float((unsigned)two[z][e]);
+                    acc[0][0][2 * e + 1] += __uint_as_float((unsigned)(two[z][e] >> 32));
+                }
+            }
+        }
+    }
 
     // A lane holds token l32 of each block, registers 4 q .. 4 q + 3 its outputs
     // 8 q + 4 half .. of 32.  They go out through LDS, 32 tokens at a time, so that a
@@ -312,15 +361,27 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     }
 }
 
-template <int TM, int TN, int STAGES, bool ROWS>
-static int launch_tile(Ctx* c, const Product& p) {
+template <int TM, int TN, int STAGES, bool ROWS, bool SPLIT = false>
+static int launch_tile(Ctx* c, const Product& p, int splits = 1) {
     const int64_t tm = ceil_div(p.m, 64 * TM), tn = ceil_div(p.n, 64 * TN);
     if (tm * tn >= (1ll << 31)) return set_error(TKV_HIP_UNSUPPORTED, "matmul_mxfp4: 2^31 tiles and more");
-    const dim3 grid = wide_grid(tm * tn);
+    dim3 grid = wide_grid(tm * tn);
+    Split split = {};
+    if (SPLIT) {
+        const int64_t slices = ceil_div(p.blocks, 8);
+        split.slices = (int32_t)ceil_div(slices, splits);
+        split.splits = (int32_t)ceil_div(slices, split.slices);
+        grid.z = (unsigned)split.splits;
+        void* ws;
+        TKV_RC_TRY(mx_room(c, 16, (size_t)(tm * tn * split.splits) << 14, &ws));
+        split.sums = static_cast<unsigned long long*>(ws);
+        split.arrivals = c->attn_arrivals;
+    }
     const int m = (int)tm, n = (int)tn, vec = aligned(p.y, 16) && p.ldy * type_bytes(p.y_type) % 16 == 0;
-    if (p.y_type == TKV_HIP_F32) k_mx_tile<TM, TN, STAGES, ROWS, float><<<grid, 256, 0, c->stream>>>(p, m, n, vec);
-    else if (p.y_type == TKV_HIP_F16) k_mx_tile<TM, TN, STAGES, ROWS, _Float16><<<grid, 256, 0, c->stream>>>(p, m, n, vec);
-    else k_mx_tile<TM, TN, STAGES, ROWS, __bf16><<<grid, 256, 0, c->stream>>>(p, m, n, vec);
+    const auto start = [&](auto k) { k<<<grid, 256, 0, c->stream>>>(p, m, n, vec, split); };
+    if (p.y_type == TKV_HIP_F32) start(k_mx_tile<TM, TN, STAGES, ROWS, SPLIT, float>);
+    else if (p.y_type == TKV_HIP_F16) start(k_mx_tile<TM, TN, STAGES, ROWS, SPLIT, _Float16>);
+    else start(k_mx_tile<TM, TN, STAGES, ROWS, SPLIT, __bf16>);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
@@ -334,8 +395,15 @@ static int launch_tile(Ctx* c, const Product& p) {
 // 768 (f32) 30, 24, 22, 25, 34; 1024 x 14336 of 4096 35, 40, 45, 55, 66; 512 x 4096
 // of 4096 26, 15, 12, 12, 11; 128 x 8192 of 8192 46, 25, 21, 19, 13; 333 x 1000 of
 // 2000 21, 9, 7, 5, 6.
+// K is split over up to four workgroups of the last kind where its tiles leave CUs
+// idle, 3.5 us for the join: 100 x 640 of 16000 20.6 -> 10.4 us (by eight 10.4), 200 x
+// 1000 of 9000 13.6 -> 9.4, 128 x 4096 of 16384 (128 tiles in three) 21.1 -> 14.8 (in
+// four 16.1); 300 x 300 of 3000 stays whole, 6.6 (7.2).
 enum { TILE_256, TILE_128, TILE_128_64, TILE_64, TILE_64_RING, TILE_KINDS };
-static int tile_kind(const Ctx* c, const mx::Product& p) {
+struct TilePlan {
+    int kind, splits;
+};
+static TilePlan tile_plan(const Ctx* c, const mx::Product& p) {
     struct Kind {
         int64_t m, n;
         int held;
@@ -357,19 +425,32 @@ static int tile_kind(const Ctx* c, const mx::Product& p) {
         if (left) t += slices * k.slice[left - 1] + k.rest;
         if (i == 0 || t < least) best = i, least = t;
     }
-    return best;
+    const Kind& ring = kinds[TILE_64_RING];
+    const int64_t tiles = ceil_div(p.m, ring.m) * ceil_div(p.n, ring.n);
+    const int64_t splits = 3 * c->num_cus / 2 / tiles < 4 ? 3 * c->num_cus / 2 / tiles : 4;
+    if (splits > 1 && c->attn_arrivals) {
+        const float t = ceilf(slices / (float)splits) * ring.slice[tiles * splits > c->num_cus] + ring.rest + 3.5f;
+        if (t < least) return {TILE_64_RING, (int)splits};
+    }
+    return {best, 1};
 }
 
 // The few-row kernel and the smallest tiles take the scales as they come, a launch
-// less where a launch counts (333 x 1000 of 2000: 11.5 -> 8 us).
+// less where a launch counts (333 x 1000 of 2000: 8 -> 6.4 us).
 bool mx_takes_rows(const Ctx* c, const mx::Product& p) {
-    return p.m <= kFewRows || (tile_kind(c, p) >= TILE_64 && (p.blocks + 7) / 8 <= mx::kRowSlices);
+    const TilePlan plan = tile_plan(c, p);
+    const int64_t slices = ceil_div(ceil_div(p.blocks, 8), plan.splits);
+    return p.m <= kFewRows || (plan.kind >= TILE_64 && slices <= mx::kRowSlices);
 }
 
 int launch_mx_product(Ctx* c, const mx::Product& p) {
     if (p.m <= kFewRows) return launch_mx_few(c, p);
+    const TilePlan plan = tile_plan(c, p);
+    if (plan.splits > 1)
+        return p.a_rows == 0 ? mx::launch_tile<1, 1, 4, true, true>(c, p, plan.splits)
+                             : mx::launch_tile<1, 1, 4, false, true>(c, p, plan.splits);
     if (p.a_rows == 0) return mx::launch_tile<1, 1, 4, true>(c, p);
-    switch (tile_kind(c, p)) {
+    switch (plan.kind) {
         case TILE_256: return mx::launch_tile<4, 4, 2, false>(c, p);
         case TILE_128: return mx::launch_tile<2, 2, 2, false>(c, p);
         case TILE_128_64: return mx::launch_tile<2, 1, 2, false>(c, p);

@@ -113,8 +113,10 @@ __device__ __forceinline__ void nan_first(const float* x, double& dmn, double& d
 // below total.  Min / max of 25 MB (512 workgroups), one tensor call after call,
 // 10.2 -> 5.4 us (8.4 in a trace where other kernels run in between), of 4 MB (256)
 // 6.6 -> 4.5; with 32 the second round trip costs 0.3 us more than it saves.
-__device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned total) {
-    __shared__ int s_last;
+//   `s_last` is a word of LDS that nothing is read from behind the barrier.  (Kernels
+// that copy to LDS past the registers give a word of their own array: beside a second
+// LDS variable the compiler waits for such copies before reads of the first.)
+__device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned total, int& s_last) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -132,6 +134,10 @@ __device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned total) {
     }
     __syncthreads();
     return s_last != 0;
+}
+__device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned total) {
+    __shared__ int s_last;
+    return arrive_last(counter, total, s_last);
 }
 
 // Clears the words that arrive_last(counter, total) counted on: all 17 lines where
