@@ -6,10 +6,11 @@
 // scale byte, straight from memory: a row's four lanes take the chunks of a
 // 128-byte line with two instructions, 256 elements.  The waves of a workgroup take
 // 256-element slabs of K in turn, each for all of the workgroup's 16 NR rows, and
-// their sums are added in LDS in the waves' order.
+// their sums are added in LDS in the waves' order.  Where the row blocks leave CUs idle
+// K is split over workgroups too, whose sums the last of them adds in their order.
 //
-// The linear's form codes the tokens on the way, every workgroup all of them, into
-// LDS, while the first of its weights are on their way.
+// The linear's form codes the tokens on the way, every workgroup all of them (of its
+// part of K), into LDS, while the first of its weights are on their way.
 #include <type_traits>
 
 #include "mxfp4.h"

@@ -21,7 +21,7 @@
 // between two products stops them: copies and reads in one run, or a branch, past
 // which the compiler moves the products, cost 2.13 us a slice instead of 1.77.
 //
-// What bounds it: 8192 x 8192 x 8192 in bf16 263 us, 4.2 PFLOP/s.  A slice of a tile
+// What bounds it: 8192 x 8192 x 8192 in bf16 247 us, 4.4 PFLOP/s.  A slice of a tile
 // alone on the card takes 1.14 us (2048 of its 2700 cycles the matrix units'), with
 // all CUs at work 1.77: power.  Of random codes the matrix units alone, all operands
 // in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros).  (The
