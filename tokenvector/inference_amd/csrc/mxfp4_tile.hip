@@ -311,7 +311,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
     constexpr int LANES = TN * 32 * (int)sizeof(TO) / 16, STEP = 64 / LANES, E = 16 / (int)sizeof(TO);
     const int64_t n = nw + (lane % LANES) * E;
     const int64_t left = p.n - n;  // outputs from n on
-    const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;
+    const bool whole = vec && m0 + BM <= p.m && n0 + BN <= p.n;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
 #pragma unroll
@@ -332,11 +332,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
             TO* at = static_cast<TO*>(p.y) + (mw + i * 32 + lane / LANES) * p.ldy + n;
 #pragma unroll
             for (int t = 0; t < 32 / STEP; t++) {
-                v4i_any* to = reinterpret_cast<v4i_any*>(at + t * STEP * p.ldy);
+                v4i* to = reinterpret_cast<v4i*>(at + t * STEP * p.ldy);
                 // past the L2's reuse, which the operands need more (8192 x 2304 of 768
-                // 31.9 -> 28.9 us, 8192 x 8192 of 8192 255 -> 247); small outputs and
+                // 33.6 -> 28.8 us, 8192 x 8192 of 8192 264 -> 247); small outputs and
                 // parts of lines lose by it (1000 x 12001 of 1001 21.5 -> 27.8)
-                if (TM * TN > 1 && vec) __builtin_nontemporal_store(v[t], to);
+                if constexpr (TM * TN > 1) __builtin_nontemporal_store(v[t], to);
                 else *to = v[t];
             }
         } else {
