@@ -110,7 +110,9 @@ __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
     }
 }
 
-// Row-major scales of one or two operands to slabs, eight blocks of a row per lane.
+// Row-major scales of one or two operands to slabs: a workgroup takes 32 rows of eight
+// slabs, so that loads and stores are both runs of 64 bytes (products of 4096 x 256 of
+// 16384 26.2 -> 24.4 us, 1024 x 14336 of 4096 39.1 -> 38.0; before, a row a lane).
 struct SlabArgs {
     const uint8_t* scales[2];
     uint8_t* out[2];
@@ -120,13 +122,13 @@ struct SlabArgs {
 };
 __global__ __launch_bounds__(256) void k_mx_slabs(SlabArgs a) {
     const int which = blockIdx.x >= a.first;
-    const int64_t row = (int64_t)(blockIdx.x - (which ? a.first : 0)) * 256 + threadIdx.x;
+    const int64_t row = (int64_t)(blockIdx.x - (which ? a.first : 0)) * 32 + (threadIdx.x >> 3);
     const int64_t rows = which ? a.rows[1] : a.rows[0], padded = (rows + kSlabRows - 1) / kSlabRows * kSlabRows;
-    if (row >= rows) return;
+    const int g = (int)blockIdx.y * 8 + (threadIdx.x & 7);
+    if (row >= rows || g * 8 >= a.blocks) return;
     const uint8_t* from = (which ? a.scales[1] : a.scales[0]) + row * a.blocks;
     uint8_t* out = which ? a.out[1] : a.out[0];
-    for (int g = blockIdx.y; g * 8 < a.blocks; g += gridDim.y)
-        *reinterpret_cast<v2i*>(out + (g * padded + row) * 8) = row_scales(from, g, a.blocks);
+    *reinterpret_cast<v2i*>(out + (g * padded + row) * 8) = row_scales(from, g, a.blocks);
 }
 
 // Blocks of one launch, at most: their number is divided in 32 bits, and 4 lanes
@@ -206,10 +208,9 @@ int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, in
 
 int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_t* slabs_a, const uint8_t* sb,
                     int64_t rows_b, uint8_t* slabs_b) {
-    const int64_t groups = slabs_of(k), first = ceil_div(rows_a, 256);
+    const int64_t first = ceil_div(rows_a, 32);
     const SlabArgs a = {{sa, sb}, {slabs_a, slabs_b}, {rows_a, rows_b}, (int32_t)blocks_of(k), (unsigned)first};
-    k_mx_slabs<<<dim3((unsigned)(first + ceil_div(rows_b, 256)), (unsigned)(groups < 65535 ? groups : 65535)), 256, 0,
-                 c->stream>>>(a);
+    k_mx_slabs<<<dim3((unsigned)(first + ceil_div(rows_b, 32)), (unsigned)ceil_div(slabs_of(k), 8)), 256, 0, c->stream>>>(a);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
