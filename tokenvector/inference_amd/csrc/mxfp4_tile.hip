@@ -93,8 +93,9 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
 
     // copies: 1 KB, 8 rows, each; (BM + BN) / 32 of them a wave.  Groups of rows
     // that the operand does not have read its first instead; what passes its last
-    // row's end the buffer's bounds turn into zeros.  Past a row's end is the next
-    // row, which the scales 2^-127 there leave out.
+    // row's end the buffer's bounds turn into zeros: they are checked against the
+    // vector offset alone, so the whole offset is in it and the scalar one is 0.
+    // Past a row's end is the next row, which the scales 2^-127 there leave out.
     constexpr int COPIES = (BM + BN) / 32;
     const int rows_a = p.m - m0 < BM ? (int)(p.m - m0) : BM, rows_w = p.n - n0 < BN ? (int)(p.n - n0) : BN;
     const uint32_t bytes_a = (uint32_t)rows_a * row_bytes, bytes_w = (uint32_t)rows_w * row_bytes;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN, STAGES, ROWS>::PER_CU)) void k_m
             const uint32_t at = (in < (is_a ? rows_a : rows_w) ? (uint32_t)in * row_bytes : 0u) + (uint32_t)slice * 128u;
             const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
                 (void*)(is_a ? base_a : base_w), 0, slice < slices ? (int)(is_a ? bytes_a : bytes_w) : 0, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(stage + first * 128), 16, (int)lane_at, (int)at, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(stage + first * 128), 16, (int)(lane_at + at), 0, 0, 0);
         } else if constexpr (!ROWS) {
             const int k = d - COPIES, have = slice < slices ? slice : slices - 1, at = scale_place(k);
             const void* from = scale_at[k] + (int64_t)have * scale_step[k] + lane * SWIDTH;
