@@ -154,3 +154,27 @@ def test_workspace_that_cannot_be_had(ctx):
     for b in (dx, y):
         b.close()
     own.close()
+
+
+def test_scales_of_many_rows_laid_out(ctx):
+    """Rows whose scales' slabs take more workgroups than a dimension of the grid,
+    161 GB in all: 2^29 and more of two K slices each, the second one block."""
+    m, n, k = (1 << 29) + 77, 65, 288
+    import torch
+    if torch.cuda.mem_get_info(0)[0] < 180 << 30:
+        pytest.skip("161 GB of operands and outputs")
+    say(f"product {m}x{n}x{k}")
+    rng = np.random.default_rng(6)
+    a, w = _small(rng, 100, k), _small(rng, n, k)
+    a[1][:, 8] = rng.integers(126, 129, 100)
+    ac, as_ = _coded(ctx, m, k, a)
+    wc, ws = (D.DeviceBuffer.from_host(ctx, v) for v in w)
+    y = D.DeviceBuffer(ctx, 2 * m * n)
+    X.Matmul(ctx, ac, as_, wc, ws, m, n, k, A.BF16, y)()
+    exact = (value_of(*a, k) @ value_of(*w, k).T).astype(np.float32).view(np.uint32)
+    want = (exact + 0x7FFF + ((exact >> 16) & 1)) >> 16  # to nearest even
+    got = _At(y, 2 * (m - 100) * n, (100, n), np.uint16).download()
+    assert np.array_equal(got, want)
+    assert not _At(y, 2 * (m - 5100) * n, (5000, n), np.uint16).download().any()
+    for b in (wc, ws, ac, as_, y):
+        b.close()

@@ -110,21 +110,22 @@ __global__ __launch_bounds__(256) void k_mx_decode(DecodeArgs a) {
     }
 }
 
-// Row-major scales of one or two operands to slabs: a workgroup takes 32 rows of eight
-// slabs, so that loads and stores are both runs of 64 bytes (products of 4096 x 256 of
+// Row-major scales of one or two operands to slabs: a workgroup takes 32 rows (numbered
+// over two dimensions of the grid) of eight slabs, so that loads and stores are both runs of 64 bytes (products of 4096 x 256 of
 // 16384 26.2 -> 24.4 us, 1024 x 14336 of 4096 39.1 -> 38.0; before, a row a lane).
 struct SlabArgs {
     const uint8_t* scales[2];
     uint8_t* out[2];
     int64_t rows[2];
     int32_t blocks;
-    unsigned first;  // workgroups of the first operand
+    int64_t first;  // groups of 32 rows of the first operand
 };
 __global__ __launch_bounds__(256) void k_mx_slabs(SlabArgs a) {
-    const int which = blockIdx.x >= a.first;
-    const int64_t row = (int64_t)(blockIdx.x - (which ? a.first : 0)) * 32 + (threadIdx.x >> 3);
+    const int64_t group = wide_block();
+    const int which = group >= a.first;
+    const int64_t row = (group - (which ? a.first : 0)) * 32 + (threadIdx.x >> 3);
     const int64_t rows = which ? a.rows[1] : a.rows[0], padded = (rows + kSlabRows - 1) / kSlabRows * kSlabRows;
-    const int g = (int)blockIdx.y * 8 + (threadIdx.x & 7);
+    const int g = (int)blockIdx.z * 8 + (threadIdx.x & 7);
     if (row >= rows || g * 8 >= a.blocks) return;
     const uint8_t* from = (which ? a.scales[1] : a.scales[0]) + row * a.blocks;
     uint8_t* out = which ? a.out[1] : a.out[0];
@@ -209,8 +210,10 @@ int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, in
 int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* sa, int64_t rows_a, uint8_t* slabs_a, const uint8_t* sb,
                     int64_t rows_b, uint8_t* slabs_b) {
     const int64_t first = ceil_div(rows_a, 32);
-    const SlabArgs a = {{sa, sb}, {slabs_a, slabs_b}, {rows_a, rows_b}, (int32_t)blocks_of(k), (unsigned)first};
-    k_mx_slabs<<<dim3((unsigned)(first + ceil_div(rows_b, 32)), (unsigned)ceil_div(slabs_of(k), 8)), 256, 0, c->stream>>>(a);
+    const SlabArgs a = {{sa, sb}, {slabs_a, slabs_b}, {rows_a, rows_b}, (int32_t)blocks_of(k), first};
+    dim3 grid = wide_grid(first + ceil_div(rows_b, 32));
+    grid.z = (unsigned)ceil_div(slabs_of(k), 8);
+    k_mx_slabs<<<grid, 256, 0, c->stream>>>(a);
     TKV_LAUNCH_CHECK();
     return TKV_HIP_OK;
 }
