@@ -178,3 +178,36 @@ def test_scales_of_many_rows_laid_out(ctx):
     assert not _At(y, 2 * (m - 5100) * n, (5000, n), np.uint16).download().any()
     for b in (wc, ws, ac, as_, y):
         b.close()
+
+
+def test_rows_of_more_than_one_launch(ctx):
+    """More blocks than a launch of the coding takes, marked at the ends of both."""
+    cols = 32768
+    b = X.blocks(cols)
+    per = (1 << 29) // b  # rows of a launch
+    m = per + 5
+    say(f"code {m}x{cols}")
+    rng = np.random.default_rng(8)
+    x = rng.choice([-1.5, 1.0, 2.0, -3.0, 0.75], (15, cols)).astype(np.float32)
+    codes, scales = code_of(x)
+    marked = ((0, slice(0, 5)), (per - 5, slice(5, 15)))
+    src = D.DeviceBuffer(ctx, 2 * m * cols)
+    dc, ds = D.DeviceBuffer(ctx, m * b * 16), D.DeviceBuffer(ctx, m * b)
+    D.memset(ctx, src, 0, src.nbytes)
+    for at, r in marked:
+        raw = (x[r].view(np.uint32) >> 16).astype(np.uint16)
+        _At(src, 2 * at * cols, raw.shape, np.uint16).upload(raw)
+    X.Quantize(ctx, A.BF16, src, cols, m, cols, dc, ds)()
+    for at, r in marked:
+        assert np.array_equal(_At(dc, at * b * 16, codes[r].shape, np.uint8).download(), codes[r])
+        assert np.array_equal(_At(ds, at * b, scales[r].shape, np.uint8).download(), scales[r])
+    assert not _At(dc, 5 * b * 16, (100, b, 16), np.uint8).download().any()
+    assert not _At(dc, (per - 105) * b * 16, (100, b, 16), np.uint8).download().any()
+    D.memset(ctx, src, 0xFF, src.nbytes)
+    X.Dequantize(ctx, dc, ds, m, cols, A.BF16, src, cols)()
+    for at, r in marked:
+        got = _At(src, 2 * at * cols, x[r].shape, np.uint16).download().astype(np.uint32) << 16
+        assert np.array_equal(got, value_of(codes[r], scales[r], cols).astype(np.float32).view(np.uint32))
+    assert not _At(src, 2 * (per - 105) * cols, (100, cols), np.uint16).download().any()
+    for buf in (src, dc, ds):
+        buf.close()
