@@ -285,6 +285,35 @@ def test_nan_and_infinity_stay_in_their_head(ctx):
     _near(got_k[clean], want[:, 4:][clean], size[:, 4:][clean], 64, A.F32, "other keys")
 
 
+@pytest.mark.parametrize("layout", [A.ROPE_HALF, A.ROPE_PAIRS], ids=["half", "pairs"])
+@pytest.mark.parametrize("d,rot,pad", [(64, 0, 0), (64, 32, 0), (128, 64, 0), (64, 32, 3), (36, 0, 0), (36, 16, 0)])
+def test_infinity_in_elements_that_are_not_rotated(ctx, layout, d, rot, pad):
+    """One in a head makes the head's finite elements zeros and is NaN itself, with
+    its partner in the rotation if it has one; one in a gain is its own element's."""
+    say(f"infinity d {d} rot {rot} pad {pad}")
+    s = Setting(ctx, A.F32, A.F32, A.F32, layout, 4, 2, d, rot, 40, pad=pad)
+    width = 8 * d + pad
+    raw = s.xd.download().view(np.float32).reshape(40, width)
+    rows = {(7, 1): rot, (9, 4): d - 1, (11, 5): rot + (d - rot) // 2, (20, 0): 0, (21, 2): max(rot - 1, 0)}
+    for (t, h), e in rows.items():
+        raw[t, h * d + e] = s.x[t, h, e] = np.inf
+    s.xd.upload(raw.view(np.int32))
+    for g, gd in zip(s.g, s.gd):
+        g[d - 2] = np.inf
+        gd.upload(g)
+    s.call()
+    with np.errstate(invalid="ignore"):
+        want, size, real = s.expected(np.float64)
+    got = np.concatenate([s.qo.download().view(np.float32).reshape(40, 4, d),
+                          s.ko.download().view(np.float32).reshape(40, 2, d)], 1)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.isnan(want[7, 1]).sum() == 2 and all(real[t] for t, _ in rows)  # its own, and 0 times the gain's
+    far = np.isinf(want)
+    assert far.any() and np.array_equal(got[far], want[far])
+    seen = np.isfinite(want)
+    _near(got[seen], want[seen], size[seen], d, A.F32, "finite elements")
+
+
 def test_captured_and_replayed(ctx):
     s = Setting(ctx, A.BF16, A.BF16, A.BF16, A.ROPE_HALF, 8, 2, 64, 64, 64, (12, 10, 10), True)
     s.call()

@@ -257,9 +257,12 @@ __device__ __forceinline__ void from_raw(const Raw8<T>& r, float (&x)[8]) {
     for (int k = 0; k < 8; k++) x[k] = to_f32(e.e[k]);
 }
 __device__ __forceinline__ void norm_turn(float& p, float& q, float2 w, float r, bool turn) {
-    const float c = turn ? w.x * r : r, s = turn ? w.y * r : 0.0f, a = p, b = q;
-    p = __builtin_fmaf(a, c, -(b * s));
-    q = __builtin_fmaf(b, c, a * s);
+    // (the products are chosen, not their factor: 0 times an infinity beside an element
+    // that is not rotated would make that a NaN)
+    const float c = turn ? w.x * r : r, s = w.y * r, a = p, b = q;
+    const float bs = turn ? b * s : 0.0f, as = turn ? a * s : 0.0f;
+    p = __builtin_fmaf(a, c, -bs);
+    q = __builtin_fmaf(b, c, as);
 }
 
 // The same with norms per head, positions on several axes, or both: a lane's two
