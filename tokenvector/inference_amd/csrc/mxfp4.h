@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include "attn.h"
+#include "mxfp4_plan.h"
 
 namespace tkv {
 namespace mx {
@@ -44,6 +45,9 @@ struct Product {
     int64_t ldy;
     int32_t y_type;
 };
+inline Shape shape_of(const Ctx* c, const Product& p) {
+    return {p.m, p.n, p.blocks, c->num_cus, c->attn_arrivals != nullptr};
+}
 
 // The block's scale byte from its largest |x| as bits: floor(log2) - 2 (the
 // largest code is 1.5 * 2^2), at least 2^-127, which blocks of zeros and
@@ -196,14 +200,11 @@ int launch_mx_dequantize(Ctx* c, const uint8_t* codes, const uint8_t* scales, in
 // Two operands' scales to slabs (rows_b 0: one's).
 int launch_mx_slabs(Ctx* c, int64_t k, const uint8_t* a, int64_t rows_a, uint8_t* slabs_a, const uint8_t* b = nullptr,
                     int64_t rows_b = 0, uint8_t* slabs_b = nullptr);
-// mxfp4_tile.hip.  Scales as slabs, or as rows where mx_takes_rows(p).
-bool mx_takes_rows(const Ctx* c, const mx::Product& p);
+// mxfp4_tile.hip.  Scales as slabs, or as rows where mx::takes_rows.
 int launch_mx_product(Ctx* c, const mx::Product& p);
 // mxfp4_few.hip: m <= kFewRows; and the linear that codes its rows itself, where
-// mx_codes_few(p, k).
-constexpr int kFewRows = 64;
+// mx::codes_few.
 int launch_mx_few(Ctx* c, const mx::Product& p);
-bool mx_codes_few(const Ctx* c, const mx::Product& p, int64_t k);
 int launch_mx_few_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, const mx::Product& p);
 // The linear of a resident weight on float rows (mxfp4.hip).
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, mx::Product p);

@@ -225,7 +225,7 @@ int mx_room(Ctx* c, int slot, size_t bytes, void** out) {
 }
 
 int launch_mx_linear(Ctx* c, int type, const void* x, int64_t stride, int64_t k, Product p) {
-    if (mx_codes_few(c, p, k)) return launch_mx_few_linear(c, type, x, stride, k, p);
+    if (codes_few(shape_of(c, p), k)) return launch_mx_few_linear(c, type, x, stride, k, p);
     void *codes, *slabs;
     TKV_RC_TRY(mx_room(c, 0, (size_t)(p.m * p.blocks) * 16, &codes));
     TKV_RC_TRY(mx_room(c, 1, slab_bytes(p.m, k), &slabs));
@@ -301,7 +301,7 @@ int32_t tkv_hip_dev_matmul_mxfp4(int64_t ctx, const uint8_t* a, const uint8_t* a
     p.y = y;
     p.ldy = m > 1 ? stride : n;
     p.y_type = type_out;
-    if (!mx_takes_rows(c, p)) {
+    if (!mx::takes_rows(mx::shape_of(c, p))) {
         void *as, *ws;
         TKV_RC_TRY(mx_room(c, 1, slab_bytes(m, k), &as));
         TKV_RC_TRY(mx_room(c, 2, slab_bytes(n, k), &ws));

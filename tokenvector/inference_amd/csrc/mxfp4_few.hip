@@ -36,8 +36,6 @@ struct FewArgs {
 __host__ __device__ __forceinline__ uint32_t coded_bytes(uint32_t blocks) { return blocks * 16u + 16u; }
 __host__ __device__ __forceinline__ uint32_t scale_bytes(uint32_t blocks) { return ((blocks + 7) >> 3) * 8u; }
 
-constexpr int kFewSplits = 8;
-
 struct Coded {};      // the tokens come as codes and slabs,
 struct CodedRows {};  // or the scales of both as [rows][blocks]
 
@@ -275,41 +273,24 @@ static void start_few(Ctx* c, FewArgs& a, int64_t rows) {
     k_mx_few<TI, NR, MT, WAVES, SPLIT><<<grid, WAVES * 64, sums > codes ? sums : codes, c->stream>>>(a);
 }
 
-// Workgroups of a row block.  A CU's loads in flight bound what it reads (0.08 us for
-// 256 elements of 16 rows, as long again for each 16 tokens more, and a row coded on the
-// way as long for 70 blocks), so long rows of few outputs are split over the idle CUs,
-// eight slabs each at least; the join costs 1.9 us.  1 x 1024 of 16384: 6.9 us, by one
-// workgroup 8.9; 64 x 1024 of 8192 8.5 and 13.5; 12 x 960 of 9600, coded before, 6.0 and
-// 6.3; in two 4 x 2048 of 8192 7.3 and 7.1.
-static int few_splits(const Ctx* c, const Product& p, bool coded) {
-    const int64_t rows = ceil_div(p.n, 16), slabs = ceil_div(p.blocks, 8);
-    int64_t s = slabs / 8 < c->num_cus / rows ? slabs / 8 : c->num_cus / rows;
-    if (s > kFewSplits) s = kFewSplits;
-    const int64_t work = slabs * ceil_div(p.m, 16) + (coded ? 0 : p.m * p.blocks / 70);
-    return s > 1 && c->attn_arrivals && work * (s - 1) >= 27 * s ? (int)s : 1;
-}
-
-// 16-row blocks a workgroup: as many as leave a workgroup per CU, four for long rows
-// or many tokens alone (16 x 16384 rows of 16384: 29.8 us, with two 34.7; of 4096 9.0
-// and 8.3; 32 x 16384 of 4096 10.1 and 11.4).  Coding long rows for a block, 16 waves
-// (4 x 2048 of 8192: 7.1 us, with 8 waves 8.0; 4 x 4096 of 4096 5.1 and 4.9).
 template <typename TI, int MT>
 static int launch_few(Ctx* c, FewArgs& a) {
     constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
-    constexpr bool WIDE = CODED || MT == 1;  // mx_codes_few has one block and 8 waves else
+    constexpr bool WIDE = CODED || MT == 1;
+    const FewPlan plan = few_plan(shape_of(c, a.p), CODED);
     const int64_t rows = ceil_div(a.p.n, 16);
-    a.splits = few_splits(c, a.p, CODED);
+    a.splits = plan.splits;
     if (a.splits > 1) {
         void* ws;
         TKV_RC_TRY(mx_room(c, 16, (size_t)(rows * a.splits * MT * 1024), &ws));
         a.sums = static_cast<unsigned long long*>(ws);
         a.arrivals = c->attn_arrivals;
         start_few<TI, 1, MT, 8, true>(c, a, rows);
-    } else if (WIDE && MT < 4 && rows >= 4 * c->num_cus && (MT == 2 || a.p.blocks >= 256)) {
+    } else if (plan.row_blocks == 4) {
         start_few<TI, WIDE && MT < 4 ? 4 : 1, MT>(c, a, rows);
-    } else if (WIDE && rows >= 2 * c->num_cus) {
+    } else if (plan.row_blocks == 2) {
         start_few<TI, WIDE ? 2 : 1, MT>(c, a, rows);
-    } else if (WIDE && !CODED && a.p.blocks >= 256) {
+    } else if (plan.waves == 16) {
         start_few<TI, 1, MT, WIDE && !CODED ? 16 : 8>(c, a, rows);
     } else {
         start_few<TI, 1, MT>(c, a, rows);
@@ -333,20 +314,6 @@ int launch_mx_few(Ctx* c, const Product& p) {
     if (p.m <= 16) return launch_few<Coded, 1>(c, a);
     if (p.m <= 32) return launch_few<Coded, 2>(c, a);
     return launch_few<Coded, 4>(c, a);
-}
-
-// Every workgroup codes all rows (its part of them), 0.15 us for each 4096 elements
-// (with several blocks of rows a workgroup 0.25), where a launch of its own costs 2.2 and
-// more: 8 x 4096 of 4096 5.9 us against 6.7, 16 x 4096 7.9 and 7.1; 4 x 16384 9.2 and
-// 10.6, 8 x 16384 11.0 and 11.0; one call after another, where two launches are 7.4 at least, 32 x 512 of 768 5.3 and 7.4, 12 x 4096
-// of 4096 7.0 and 7.7, 24 x 7000 of 1300 8.5 and 7.5.
-bool mx_codes_few(const Ctx* c, const Product& p, int64_t k) {
-    const int64_t rows = ceil_div(p.n, 16);
-    if (k < 8 || p.m > (rows >= 2 * c->num_cus ? 16 : kFewRows)) return false;
-    // (CUs with two workgroups code twice)
-    const bool twice = rows >= 2 * c->num_cus || (p.m > 16 && rows > c->num_cus);
-    const int64_t most = twice ? 512 : rows > c->num_cus || k % 8 ? 1024 : 1536;
-    return p.m * p.blocks <= most * few_splits(c, p, false);
 }
 
 template <typename T>

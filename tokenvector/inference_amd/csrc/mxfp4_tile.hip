@@ -27,8 +27,6 @@
 // in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros).  (The
 // 16x16x128 form reaches 6.9, its sums moved half as often, but took the same time
 // here, with twice the scales to read.)
-#include <math.h>
-
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -57,7 +55,6 @@ __device__ __forceinline__ void tile_of(int64_t block, int tiles_m, int tiles_n,
 // TM, TN: a wave's blocks of 32 tokens and of 32 weight rows.  ROWS: the scales come
 // as [rows][blocks] (of kRowSlices slices at most), and all of the tile's are laid
 // out in LDS first.
-constexpr int kRowSlices = 16;
 template <int TM, int TN, int STAGES, bool ROWS>
 struct Tile {
     static constexpr int BM = 64 * TM, BN = 64 * TN;
@@ -389,73 +386,18 @@ static int launch_tile(Ctx* c, const Product& p, int splits = 1) {
 
 }  // namespace mx
 
-// The kinds of tiles, and the times that choose among them, in us, as measured: of
-// a slice with 1 .. `held` workgroups of a CU at work, and of a workgroup besides.
-// What they stand for, 256 x 256, 128 x 128, 128 x 64, 64 x 64 and 64 x 64 with four
-// stages instead of two: 8192 x 8192 of 8192 263, 331, 393, 479, 515; 8192 x 2304 of
-// 768 (f32) 30, 24, 22, 25, 34; 1024 x 14336 of 4096 35, 40, 45, 55, 66; 512 x 4096
-// of 4096 26, 15, 12, 12, 11; 128 x 8192 of 8192 46, 25, 21, 19, 13; 333 x 1000 of
-// 2000 21, 9, 7, 5, 6.
-// K is split over up to four workgroups of the last kind where its tiles leave CUs
-// idle, 3.5 us for the join: 100 x 640 of 16000 20.6 -> 10.4 us (by eight 10.4), 200 x
-// 1000 of 9000 13.6 -> 9.4, 128 x 4096 of 16384 (128 tiles in three) 21.1 -> 14.8 (in
-// four 16.1); 300 x 300 of 3000 stays whole, 6.6 (7.2).
-enum { TILE_256, TILE_128, TILE_128_64, TILE_64, TILE_64_RING, TILE_KINDS };
-struct TilePlan {
-    int kind, splits;
-};
-static TilePlan tile_plan(const Ctx* c, const mx::Product& p) {
-    struct Kind {
-        int64_t m, n;
-        int held;
-        float slice[4], rest;
-    };
-    static constexpr Kind kinds[TILE_KINDS] = {{256, 256, 1, {1.7f}, 8.0f},
-                                               {128, 128, 2, {0.68f, 1.2f}, 3.0f},
-                                               {128, 64, 3, {0.6f, 0.7f, 1.0f}, 2.5f},
-                                               {64, 64, 4, {0.49f, 0.55f, 0.7f, 0.87f}, 1.0f},
-                                               {64, 64, 2, {0.28f, 0.48f}, 1.0f}};
-    const float slices = (float)((p.blocks + 7) >> 3);
-    int best = 0;
-    float least = 0.0f;
-    for (int i = 0; i < TILE_KINDS; i++) {
-        const Kind& k = kinds[i];
-        const int64_t tiles = ceil_div(p.m, k.m) * ceil_div(p.n, k.n), round = (int64_t)k.held * c->num_cus;
-        const int64_t full = tiles / round, left = ceil_div(tiles % round, c->num_cus);
-        float t = (float)full * (slices * k.slice[k.held - 1] + k.rest);
-        if (left) t += slices * k.slice[left - 1] + k.rest;
-        if (i == 0 || t < least) best = i, least = t;
-    }
-    const Kind& ring = kinds[TILE_64_RING];
-    const int64_t tiles = ceil_div(p.m, ring.m) * ceil_div(p.n, ring.n);
-    const int64_t splits = 3 * c->num_cus / 2 / tiles < 4 ? 3 * c->num_cus / 2 / tiles : 4;
-    if (splits > 1 && c->attn_arrivals) {
-        const float t = ceilf(slices / (float)splits) * ring.slice[tiles * splits > c->num_cus] + ring.rest + 3.5f;
-        if (t < least) return {TILE_64_RING, (int)splits};
-    }
-    return {best, 1};
-}
-
-// The few-row kernel and the smallest tiles take the scales as they come, a launch
-// less where a launch counts (333 x 1000 of 2000: 8 -> 6.4 us).
-bool mx_takes_rows(const Ctx* c, const mx::Product& p) {
-    const TilePlan plan = tile_plan(c, p);
-    const int64_t slices = ceil_div(ceil_div(p.blocks, 8), plan.splits);
-    return p.m <= kFewRows || (plan.kind >= TILE_64 && slices <= mx::kRowSlices);
-}
-
 int launch_mx_product(Ctx* c, const mx::Product& p) {
-    if (p.m <= kFewRows) return launch_mx_few(c, p);
-    const TilePlan plan = tile_plan(c, p);
+    if (p.m <= mx::kFewRows) return launch_mx_few(c, p);
+    const mx::TilePlan plan = mx::tile_plan(mx::shape_of(c, p));
     if (plan.splits > 1)
         return p.a_rows == 0 ? mx::launch_tile<1, 1, 4, true, true>(c, p, plan.splits)
                              : mx::launch_tile<1, 1, 4, false, true>(c, p, plan.splits);
     if (p.a_rows == 0) return mx::launch_tile<1, 1, 4, true>(c, p);
     switch (plan.kind) {
-        case TILE_256: return mx::launch_tile<4, 4, 2, false>(c, p);
-        case TILE_128: return mx::launch_tile<2, 2, 2, false>(c, p);
-        case TILE_128_64: return mx::launch_tile<2, 1, 2, false>(c, p);
-        case TILE_64: return mx::launch_tile<1, 1, 2, false>(c, p);
+        case mx::TILE_256: return mx::launch_tile<4, 4, 2, false>(c, p);
+        case mx::TILE_128: return mx::launch_tile<2, 2, 2, false>(c, p);
+        case mx::TILE_128_64: return mx::launch_tile<2, 1, 2, false>(c, p);
+        case mx::TILE_64: return mx::launch_tile<1, 1, 2, false>(c, p);
         default: return mx::launch_tile<1, 1, 4, false>(c, p);
     }
 }
