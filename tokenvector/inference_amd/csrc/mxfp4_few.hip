@@ -277,15 +277,17 @@ template <typename TI, int MT>
 static int launch_few(Ctx* c, FewArgs& a) {
     constexpr bool CODED = std::is_same<TI, Coded>::value || std::is_same<TI, CodedRows>::value;
     constexpr bool WIDE = CODED || MT == 1;
+    // (at most 1536 blocks a split are coded on the way, and 64 make one: 25 tokens)
+    constexpr bool JOINS = CODED || MT < 4;
     const FewPlan plan = few_plan(shape_of(c, a.p), CODED);
     const int64_t rows = ceil_div(a.p.n, 16);
-    a.splits = plan.splits;
+    a.splits = JOINS ? plan.splits : 1;
     if (a.splits > 1) {
         void* ws;
         TKV_RC_TRY(mx_room(c, 16, (size_t)(rows * a.splits * MT * 1024), &ws));
         a.sums = static_cast<unsigned long long*>(ws);
         a.arrivals = c->attn_arrivals;
-        start_few<TI, 1, MT, 8, true>(c, a, rows);
+        start_few<TI, 1, MT, 8, JOINS>(c, a, rows);
     } else if (plan.row_blocks == 4) {
         start_few<TI, WIDE && MT < 4 ? 4 : 1, MT>(c, a, rows);
     } else if (plan.row_blocks == 2) {
