@@ -72,3 +72,12 @@ def test_sizes_that_have_to_take_slabs(kernels):
     """A workspace that cannot be had is asked for before anything is launched, and
     slabs of more rows than a dimension of the grid holds are laid out."""
     assert kernels([((1 << 31) - 1, 70, 131040), ((1 << 29) + 77, 65, 288)], False) == ["tile 128 slabs"] * 2
+
+
+def test_scales_as_rows_where_the_launch_saved_pays(kernels):
+    """Many small tiles lay out their own scales more slowly than a launch before them
+    does."""
+    many = [(4096, 4100, 512), (12000, 1000, 64), (400, 6000, 4000), (16000, 300, 128), (5000, 611, 1542)]
+    few = [(333, 8192, 256), (1000, 2304, 256), (333, 1000, 2000), (65, 130, 511)]
+    assert kernels(many, False) == ["tile 64 slabs"] * len(many)
+    assert kernels(few, False) == ["tile 64 ring rows"] * len(few)

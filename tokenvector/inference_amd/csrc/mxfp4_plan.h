@@ -33,9 +33,16 @@ inline int64_t parts(int64_t all, int64_t of) { return (all + of - 1) / of; }
 // 1000 of 9000 13.6 -> 9.4, 128 x 4096 of 16384 (128 tiles in three) 21.1 -> 14.8 (in
 // four 16.1); 300 x 300 of 3000 stays whole, 6.6 (7.2).
 enum { TILE_256, TILE_128, TILE_128_64, TILE_64, TILE_64_RING, TILE_KINDS };
+//   The last kind also takes the scales as they come, of up to kRowSlices slices, and lays
+// them out itself, 0.5 us a workgroup more, where slabs cost a launch of 2.2 us: instead
+// of either kind of 64 x 64 tiles where it is no slower for that.  333 x 8192 of 256 7.0
+// us (slabs and two stages 6.7 to 7.8, by the host), 333 x 1000 of 2000 6.4 (8); 4096 x
+// 4100 of 512 33.7 (21.7), 12000 x 1000 of 64 20.3 (14.7), 400 x 6000 of 4000 21.5 (18.5).
 struct TilePlan {
     int kind, splits;
+    bool rows;
 };
+constexpr int kRowSlices = 16;
 inline TilePlan tile_plan(const Shape& p) {
     struct Kind {
         int64_t m, n;
@@ -48,14 +55,16 @@ inline TilePlan tile_plan(const Shape& p) {
                                                {64, 64, 4, {0.49f, 0.55f, 0.7f, 0.87f}, 1.0f},
                                                {64, 64, 2, {0.28f, 0.48f}, 1.0f}};
     const float slices = (float)((p.blocks + 7) >> 3);
+    const auto time = [&](const Kind& k, float rest) {
+        const int64_t tiles = parts(p.m, k.m) * parts(p.n, k.n), round = (int64_t)k.held * p.cus;
+        const int64_t full = tiles / round, left = parts(tiles % round, p.cus);
+        const float t = (float)full * (slices * k.slice[k.held - 1] + rest);
+        return left ? t + slices * k.slice[left - 1] + rest : t;
+    };
     int best = 0;
     float least = 0.0f;
     for (int i = 0; i < TILE_KINDS; i++) {
-        const Kind& k = kinds[i];
-        const int64_t tiles = parts(p.m, k.m) * parts(p.n, k.n), round = (int64_t)k.held * p.cus;
-        const int64_t full = tiles / round, left = parts(tiles % round, p.cus);
-        float t = (float)full * (slices * k.slice[k.held - 1] + k.rest);
-        if (left) t += slices * k.slice[left - 1] + k.rest;
+        const float t = time(kinds[i], kinds[i].rest);
         if (i == 0 || t < least) best = i, least = t;
     }
     const Kind& ring = kinds[TILE_64_RING];
@@ -63,26 +72,19 @@ inline TilePlan tile_plan(const Shape& p) {
     const int64_t splits = 3 * p.cus / 2 / tiles < 4 ? 3 * p.cus / 2 / tiles : 4;
     if (splits > 1 && p.joins) {
         const float t = ceilf(slices / (float)splits) * ring.slice[tiles * splits > p.cus] + ring.rest + 3.5f;
-        if (t < least) return {TILE_64_RING, (int)splits};
+        if (t < least) return {TILE_64_RING, (int)splits, parts(parts(p.blocks, 8), splits) <= kRowSlices};
     }
-    return {best, 1};
+    const bool rows = best >= TILE_64 && slices <= (float)kRowSlices && time(ring, ring.rest + 0.5f) <= least + 2.2f;
+    return {best, 1, rows};
 }
-
-// Slices of K whose scales the smallest tiles lay out themselves.
-constexpr int kRowSlices = 16;
 
 // ---- few rows: the weight streamed --------------------------------------------
 
 constexpr int kFewRows = 64;
 constexpr int kFewSplits = 8;
 
-// The few-row kernel and the smallest tiles take the scales as they come, a launch
-// less where a launch counts (333 x 1000 of 2000: 8 -> 6.4 us).
-inline bool takes_rows(const Shape& p) {
-    const TilePlan plan = tile_plan(p);
-    const int64_t slices = parts(parts(p.blocks, 8), plan.splits);
-    return p.m <= kFewRows || (plan.kind >= TILE_64 && slices <= kRowSlices);
-}
+// The few-row kernel takes the scales as they come too.
+inline bool takes_rows(const Shape& p) { return p.m <= kFewRows || tile_plan(p).rows; }
 
 // Workgroups of a row block.  A CU's loads in flight bound what it reads (0.08 us for
 // 256 elements of 16 rows, as long again for each 16 tokens more, and a row coded on the
