@@ -21,11 +21,12 @@
 // between two products stops them: copies and reads in one run, or a branch, past
 // which the compiler moves the products, cost 2.13 us a slice instead of 1.77.
 //
-// What bounds it: 8192 x 8192 x 8192 in bf16 247 us, 4.4 PFLOP/s.  A slice of a tile
-// alone on the card takes 1.14 us (2048 of its 2700 cycles the matrix units'), with
-// all CUs at work 1.77: power.  Of random codes the matrix units alone, all operands
-// in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros).  (The
-// 16x16x128 form reaches 6.9, its sums moved half as often, but took the same time
+// What bounds it: 8192 x 8192 x 8192 in bf16 247 to 257 us, 4.3 PFLOP/s.  A slice of
+// a tile alone on the card takes 1.14 us (2048 of its 2700 cycles the matrix units'),
+// 1.45 at the 1.87 GHz that power leaves with all CUs at work, and then 1.77: the other
+// 0.3 us is the copies' (without them 1.44).  Of random codes the matrix units alone,
+// all operands in registers, reach 6.2 PFLOP/s at 1.55 GHz (10 at 2.4 GHz of zeros),
+// 177 us.  (The 16x16x128 form reaches 6.9, its sums moved half as often, but took the same time
 // here, with twice the scales to read.)
 #include <type_traits>
 
